@@ -130,6 +130,19 @@ SIGNATURES = {
     "nsd_probe_gather_wave": (
         c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int, c_int,
                 c_void_p, c_void_p]),
+    "nsd_mx_bytes": (c_int, [c_int, c_int64, c_int64, POINTER(c_int64), POINTER(c_int64)]),
+    "nsd_mxfp4_quantize": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+    "nsd_mxfp4_pack": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+    "nsd_mxfp4_dequantize": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int, c_void_p]),
+    "nsd_mxfp8_quantize": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+    "nsd_mxfp8_dequantize": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int, c_void_p]),
+    "nsd_mx_workspace": (c_int, [c_int64, c_int64, c_int64, c_int, c_int, POINTER(c_int64)]),
+    "nsd_mxfp4_linear": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p,
+                c_int64, c_void_p]),
+    "nsd_mxfp4_up_gate_silu_and_mul": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p,
+                c_int64, c_void_p]),
     "nsd_prefill_attention": (
         c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
                 c_int64, c_int, c_int, c_int, c_float, c_void_p, c_void_p]),

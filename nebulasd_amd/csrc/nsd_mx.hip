@@ -1,0 +1,357 @@
+// Microscaled (OCP MX) blocks for gfx950: the quantisers of weights (E2M1) and
+// activations (E4M3), the packing of a checkpoint's codes, and the way back.
+//
+// A lane owns one block: row i of a 16-row tile, 32 consecutive k.  It reads
+// them as they lie, takes the largest magnitude as an unsigned maximum of bit
+// patterns (which puts a NaN above an infinity above every number), and from
+// its exponent the scale, so no block needs another lane.  Division by a power
+// of two is exact; the one rounding is the conversion's.
+//
+// All are bound by memory.
+#include <algorithm>
+
+#include "nsd_mx_device.h"
+
+namespace nsd {
+namespace {
+
+constexpr int kMxThreads = 256;
+
+__device__ inline float bf16_bits_to_float(uint32_t b) { return __builtin_bit_cast(float, b << 16); }
+__device__ inline float float_of_bits(uint32_t b) { return __builtin_bit_cast(float, b); }
+__device__ inline uint32_t bits_of(float f) { return __builtin_bit_cast(uint32_t, f); }
+
+// Block values in fp32.
+template <typename T>
+__device__ inline void load_block(const T* p, float (&v)[kMxBlock]);
+template <>
+__device__ inline void load_block<f16>(const f16* p, float (&v)[kMxBlock]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f16x8 h = reinterpret_cast<const f16x8*>(p)[i];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[8 * i + e] = (float)h[e];
+  }
+}
+template <>
+__device__ inline void load_block<uint16_t>(const uint16_t* p, float (&v)[kMxBlock]) {  // bf16
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const u32x4 h = reinterpret_cast<const u32x4*>(p)[i];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[8 * i + 2 * e] = bf16_bits_to_float(h[e] & 0xffffu);
+      v[8 * i + 2 * e + 1] = float_of_bits(h[e] & 0xffff0000u);
+    }
+  }
+}
+template <>
+__device__ inline void load_block<float>(const float* p, float (&v)[kMxBlock]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const f32x4 h = reinterpret_cast<const f32x4*>(p)[i];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[4 * i + e] = h[e];
+  }
+}
+
+__device__ inline int wave_unit() { return blockIdx.x * (kMxThreads / kWave) + (threadIdx.x >> 6); }
+
+__device__ inline uint32_t largest_bits(const float (&v)[kMxBlock]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int e = 0; e < kMxBlock; ++e) m = max(m, bits_of(v[e]) & 0x7fffffffu);
+  return m;
+}
+
+// One wave per (row tile, four tiles of k): the lane's four scale bytes go out
+// as one word.
+template <typename T>
+__global__ void __launch_bounds__(kMxThreads)
+mxfp4_quantize_kernel(const T* __restrict__ w, int64_t n_out, int n_in, int row_tiles, int k_tiles,
+                      u32x4* __restrict__ codes, uint32_t* __restrict__ scales) {
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int groups = (k_tiles + 3) / 4;
+  const int unit = wave_unit();
+  if (unit >= row_tiles * groups) return;
+  const int64_t tile = unit / groups, row = tile * 16 + i;
+  const int kg = unit % groups;
+  uint32_t word = 0;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const int kt = 4 * kg + t;
+    if (kt >= k_tiles) break;
+    const int k = kt * kMxTileK + g * kMxBlock;
+    u32x4 out = {0, 0, 0, 0};
+    uint32_t s = 0;
+    if (row < n_out && k < n_in) {
+      float v[kMxBlock];
+      load_block(w + row * n_in + k, v);
+      const uint32_t m = largest_bits(v);
+      if (m >= 0x7f800000u) {
+        s = kMxNanScale;
+      } else {
+        // floor(log2 m) - 2; below 2^-125 (the field of subnormals is 0) the
+        // smallest scale.  v 2^(127 - s): exact, or far below half a code
+        s = max((int)(m >> 23) - 2, 0);
+        const float inv = float_of_bits((254u - s) << 23);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t c = 0;
+          c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * q] * inv, v[8 * q + 1] * inv, 1.f, 0);
+          c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * q + 2] * inv, v[8 * q + 3] * inv, 1.f, 1);
+          c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * q + 4] * inv, v[8 * q + 5] * inv, 1.f, 2);
+          c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * q + 6] * inv, v[8 * q + 7] * inv, 1.f, 3);
+          out[q] = c;
+        }
+      }
+    }
+    codes[(tile * k_tiles + kt) * 64 + lane] = out;
+    word |= s << (8 * t);
+  }
+  scales[((int64_t)kg * row_tiles + tile) * 64 + lane] = word;
+}
+
+// The same cut over codes and scale bytes that exist.
+__global__ void __launch_bounds__(kMxThreads)
+mxfp4_pack_kernel(const u32x4* __restrict__ row_codes, const uint8_t* __restrict__ row_scales, int64_t n_out,
+                  int n_in, int row_tiles, int k_tiles, u32x4* __restrict__ codes,
+                  uint32_t* __restrict__ scales) {
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int groups = (k_tiles + 3) / 4, blocks = n_in / kMxBlock;
+  const int unit = wave_unit();
+  if (unit >= row_tiles * groups) return;
+  const int64_t tile = unit / groups, row = tile * 16 + i;
+  const int kg = unit % groups;
+  uint32_t word = 0;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const int kt = 4 * kg + t;
+    if (kt >= k_tiles) break;
+    const int b = kt * 4 + g;
+    u32x4 out = {0, 0, 0, 0};
+    uint32_t s = 0;
+    if (row < n_out && b < blocks) {
+      out = row_codes[row * blocks + b];
+      s = row_scales[row * blocks + b];
+    }
+    codes[(tile * k_tiles + kt) * 64 + lane] = out;
+    word |= s << (8 * t);
+  }
+  scales[((int64_t)kg * row_tiles + tile) * 64 + lane] = word;
+}
+
+// One lane per block, one wave per (row tile, tile of k).
+__global__ void __launch_bounds__(kMxThreads)
+mxfp8_quantize_kernel(const f16* __restrict__ x, int64_t n_rows, int n_in, int row_tiles, int k_tiles,
+                      u32x4* __restrict__ codes, uint8_t* __restrict__ scales) {
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int unit = wave_unit();
+  if (unit >= row_tiles * k_tiles) return;
+  const int64_t tile = unit / k_tiles, row = tile * 16 + i;
+  const int kt = unit % k_tiles, k = kt * kMxTileK + g * kMxBlock;
+  u32x4 out[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+  uint32_t s = 0;
+  if (row < n_rows && k < n_in) {
+    const f16x8* src = reinterpret_cast<const f16x8*>(x + row * n_in + k);
+    f16x8 h[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) h[q] = src[q];
+    s = mx8_block(h, out);
+  }
+  u32x4* dst = codes + (tile * k_tiles + kt) * 128 + 2 * g * 16 + i;
+  dst[0] = out[0];
+  dst[16] = out[1];
+  scales[((int64_t)(kt >> 2) * row_tiles + tile) * kMxScaleTile + lane * 4 + (kt & 3)] = (uint8_t)s;
+}
+
+// ---- the way back ----------------------------------------------------------
+
+// 2^(s - 127), NaN for 255.  2^-127 is subnormal: its bits are not s << 23.
+__device__ inline float scale_of(uint32_t s) {
+  return float_of_bits(s == kMxNanScale ? 0x7fc00000u : s == 0 ? 0x00400000u : s << 23);
+}
+__device__ inline float e2m1_value(uint32_t c) {
+  const uint32_t e = (c >> 1) & 3, m = c & 1;
+  const float a = e ? float_of_bits(((126 + e) << 23) | (m << 22)) : 0.5f * (float)m;
+  return c & 8 ? -a : a;
+}
+__device__ inline float e4m3_value(uint32_t c) {
+  const uint32_t e = (c >> 3) & 15, m = c & 7;
+  const float a = (c & 127) == 127 ? float_of_bits(0x7fc00000u)
+                  : e ? float_of_bits(((120 + e) << 23) | (m << 20)) : (float)m * 0.001953125f;
+  return c & 128 ? -a : a;
+}
+
+template <typename T>
+__device__ inline void store8(T* p, const float (&v)[8]);
+template <>
+__device__ inline void store8<f16>(f16* p, const float (&v)[8]) {
+  f16x8 h;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) h[e] = (f16)v[e];
+  *reinterpret_cast<f16x8*>(p) = h;
+}
+// bf16: the values have at most four significant bits, so the upper half of the
+// word is the value (the smallest subnormals of E4M3 excepted: 2^-127 2^-9,
+// below bf16's; they truncate to zero)
+template <>
+__device__ inline void store8<uint16_t>(uint16_t* p, const float (&v)[8]) {
+  u32x4 h;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) h[e] = (bits_of(v[2 * e]) >> 16) | (bits_of(v[2 * e + 1]) & 0xffff0000u);
+  *reinterpret_cast<u32x4*>(p) = h;
+}
+template <>
+__device__ inline void store8<float>(float* p, const float (&v)[8]) {
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    reinterpret_cast<f32x4*>(p)[e] = f32x4{v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]};
+}
+
+template <int BITS, typename T>
+__global__ void __launch_bounds__(kMxThreads)
+mx_dequantize_kernel(const u32x4* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t n_rows, int n_in,
+                     int row_tiles, int k_tiles, T* __restrict__ out) {
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int unit = wave_unit();
+  if (unit >= row_tiles * k_tiles) return;
+  const int64_t tile = unit / k_tiles, row = tile * 16 + i;
+  const int kt = unit % k_tiles, k = kt * kMxTileK + g * kMxBlock;
+  if (row >= n_rows || k >= n_in) return;
+  const float s = scale_of(scales[((int64_t)(kt >> 2) * row_tiles + tile) * kMxScaleTile + lane * 4 + (kt & 3)]);
+  T* dst = out + row * n_in + k;
+  u32x4 c[BITS / 4];
+  if constexpr (BITS == 4) {
+    c[0] = codes[(tile * k_tiles + kt) * 64 + lane];
+  } else {
+    c[0] = codes[(tile * k_tiles + kt) * 128 + 2 * g * 16 + i];
+    c[1] = codes[(tile * k_tiles + kt) * 128 + 2 * g * 16 + i + 16];
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (BITS == 4) v[e] = e2m1_value(c[0][q] >> (4 * e)) * s;
+      else v[e] = e4m3_value(c[q / 2][q % 2 * 2 + e / 4] >> (8 * (e % 4))) * s;
+    }
+    store8(dst + 8 * q, v);
+  }
+}
+
+int check_mx(const char* who, int64_t n_rows, int64_t n_in) {
+  if (n_rows < 0 || n_rows > INT32_MAX || n_in < kMxBlock || n_in % kMxBlock || n_in > INT32_MAX)
+    return fail(NSD_ERR_UNSUPPORTED, "%s: %lld rows of n_in=%lld (a multiple of 32)", who, (long long)n_rows,
+                (long long)n_in);
+  // a launch has at most one unit per (row tile, tile of k), counted in 32 bits
+  if (mx_row_tiles(n_rows) * mx_k_tiles(n_in) > INT32_MAX - kMxThreads)
+    return fail(NSD_ERR_UNSUPPORTED, "%s: %lld x %lld values are too many", who, (long long)n_rows, (long long)n_in);
+  return NSD_OK;
+}
+int check_dtype(const char* who, int dtype) {
+  if (dtype != NSD_DTYPE_F16 && dtype != NSD_DTYPE_BF16 && dtype != NSD_DTYPE_F32)
+    return fail(NSD_ERR_UNSUPPORTED, "%s: dtype=%d", who, dtype);
+  return NSD_OK;
+}
+int check_pointers(const char* who, std::initializer_list<const void*> ps) {
+  for (const void* p : ps) {
+    if (p == nullptr) return fail(NSD_ERR_INVALID, "%s: null pointer", who);
+    if (!aligned16(p)) return fail(NSD_ERR_UNSUPPORTED, "%s: pointers must be 16-byte aligned", who);
+  }
+  return NSD_OK;
+}
+
+unsigned wave_grid(int64_t units) { return (unsigned)((units + kMxThreads / kWave - 1) / (kMxThreads / kWave)); }
+
+template <int BITS>
+int dequantize(const char* who, const void* codes, const void* scales, int64_t n_rows, int64_t n_in, void* out,
+               int dtype, void* stream) {
+  if (int rc = check_mx(who, n_rows, n_in)) return rc;
+  if (int rc = check_dtype(who, dtype)) return rc;
+  if (n_rows == 0) return NSD_OK;
+  if (int rc = check_pointers(who, {codes, scales, out})) return rc;
+  const int64_t rt = mx_row_tiles(n_rows), kt = mx_k_tiles(n_in);
+  auto go = [&](auto* p) {
+    hipLaunchKernelGGL((mx_dequantize_kernel<BITS, std::remove_pointer_t<decltype(p)>>), dim3(wave_grid(rt * kt)),
+                       dim3(kMxThreads), 0, as_stream(stream), static_cast<const u32x4*>(codes),
+                       static_cast<const uint8_t*>(scales), n_rows, (int)n_in, (int)rt, (int)kt, p);
+  };
+  if (dtype == NSD_DTYPE_F16) go(static_cast<f16*>(out));
+  else if (dtype == NSD_DTYPE_BF16) go(static_cast<uint16_t*>(out));
+  else go(static_cast<float*>(out));
+  return launch_status(who);
+}
+
+}  // namespace
+
+int mxfp8_quantize(const void* x, int64_t n_rows, int64_t n_in, void* codes, void* scales, void* stream) {
+  const int64_t rt = mx_row_tiles(n_rows), kt = mx_k_tiles(n_in);
+  hipLaunchKernelGGL(mxfp8_quantize_kernel, dim3(wave_grid(rt * kt)), dim3(kMxThreads), 0, as_stream(stream),
+                     static_cast<const f16*>(x), n_rows, (int)n_in, (int)rt, (int)kt, static_cast<u32x4*>(codes),
+                     static_cast<uint8_t*>(scales));
+  return launch_status("mxfp8_quantize");
+}
+
+}  // namespace nsd
+
+using namespace nsd;
+
+extern "C" int nsd_mx_bytes(int bits, int64_t n_rows, int64_t n_in, int64_t* codes, int64_t* scales) {
+  if (bits != 4 && bits != 8) return fail(NSD_ERR_INVALID, "mx_bytes: bits=%d", bits);
+  if (!codes || !scales) return fail(NSD_ERR_INVALID, "mx_bytes: null output");
+  if (int rc = check_mx("mx_bytes", n_rows, n_in)) return rc;
+  const int64_t rt = mx_row_tiles(n_rows), kt = mx_k_tiles(n_in);
+  *codes = rt * kt * (bits == 4 ? kMxTile4 : kMxTile8);
+  *scales = rt * ((kt + 3) / 4) * kMxScaleTile;
+  return NSD_OK;
+}
+
+extern "C" int nsd_mxfp4_quantize(const void* w, int dtype, int64_t n_out, int64_t n_in, void* codes, void* scales,
+                                  void* stream) {
+  if (int rc = check_mx("mxfp4_quantize", n_out, n_in)) return rc;
+  if (int rc = check_dtype("mxfp4_quantize", dtype)) return rc;
+  if (n_out == 0) return NSD_OK;
+  if (int rc = check_pointers("mxfp4_quantize", {w, codes, scales})) return rc;
+  const int64_t rt = mx_row_tiles(n_out), kt = mx_k_tiles(n_in);
+  auto go = [&](const auto* p) {
+    hipLaunchKernelGGL((mxfp4_quantize_kernel<std::remove_cv_t<std::remove_pointer_t<decltype(p)>>>),
+                       dim3(wave_grid(rt * ((kt + 3) / 4))), dim3(kMxThreads), 0, as_stream(stream), p, n_out, (int)n_in,
+                       (int)rt, (int)kt, static_cast<u32x4*>(codes), static_cast<uint32_t*>(scales));
+  };
+  if (dtype == NSD_DTYPE_F16) go(static_cast<const f16*>(w));
+  else if (dtype == NSD_DTYPE_BF16) go(static_cast<const uint16_t*>(w));
+  else go(static_cast<const float*>(w));
+  return launch_status("mxfp4_quantize");
+}
+
+extern "C" int nsd_mxfp4_pack(const void* row_codes, const void* row_scales, int64_t n_out, int64_t n_in, void* codes,
+                              void* scales, void* stream) {
+  if (int rc = check_mx("mxfp4_pack", n_out, n_in)) return rc;
+  if (n_out == 0) return NSD_OK;
+  if (!row_scales) return fail(NSD_ERR_INVALID, "mxfp4_pack: null pointer");
+  if (int rc = check_pointers("mxfp4_pack", {row_codes, codes, scales})) return rc;
+  const int64_t rt = mx_row_tiles(n_out), kt = mx_k_tiles(n_in);
+  hipLaunchKernelGGL(mxfp4_pack_kernel, dim3(wave_grid(rt * ((kt + 3) / 4))), dim3(kMxThreads), 0, as_stream(stream),
+                     static_cast<const u32x4*>(row_codes), static_cast<const uint8_t*>(row_scales), n_out, (int)n_in,
+                     (int)rt, (int)kt, static_cast<u32x4*>(codes), static_cast<uint32_t*>(scales));
+  return launch_status("mxfp4_pack");
+}
+
+extern "C" int nsd_mxfp4_dequantize(const void* codes, const void* scales, int64_t n_out, int64_t n_in, void* out,
+                                    int dtype, void* stream) {
+  return dequantize<4>("mxfp4_dequantize", codes, scales, n_out, n_in, out, dtype, stream);
+}
+
+extern "C" int nsd_mxfp8_quantize(const void* x, int64_t n_rows, int64_t n_in, void* codes, void* scales,
+                                  void* stream) {
+  if (int rc = check_mx("mxfp8_quantize", n_rows, n_in)) return rc;
+  if (n_rows == 0) return NSD_OK;
+  if (int rc = check_pointers("mxfp8_quantize", {x, codes, scales})) return rc;
+  return mxfp8_quantize(x, n_rows, n_in, codes, scales, stream);
+}
+
+extern "C" int nsd_mxfp8_dequantize(const void* codes, const void* scales, int64_t n_rows, int64_t n_in, void* out,
+                                    int dtype, void* stream) {
+  return dequantize<8>("mxfp8_dequantize", codes, scales, n_rows, n_in, out, dtype, stream);
+}

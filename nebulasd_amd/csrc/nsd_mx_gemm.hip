@@ -1,0 +1,278 @@
+// Products of microscaled weights (MXFP4) and activations (MXFP8) for gfx950:
+// y[r][n] = sum_k X[r][k] W[n][k], and the up/gate pair with its SiLU-and-mul.
+#include <algorithm>
+
+#include "nsd_mx_device.h"
+
+namespace nsd {
+namespace {
+
+constexpr int64_t kMaxMxRows = 1 << 21;  // rows of one call
+
+struct MxArgs {
+  const u32x4* xc;     // x codes [row tiles][T][128] of 16 bytes
+  const uint32_t* xs;  // x scales [ceil(T / 4)][row tiles][64]
+  const u32x4* wc;     // weight codes [column tiles][T][64]
+  const uint32_t* ws;  // weight scales [ceil(T / 4)][column tiles][64]
+  f16* y;
+  float* part;  // [splits][rows][n], when splits > 1
+  int rows, n;  // n: columns of y
+  int T;        // tiles of k
+  int row_tiles, w_tiles;
+  int splits;
+};
+
+// Waves of a workgroup share its column tiles and split k: each streams its
+// range's weight tiles and x tiles straight into registers, D steps ahead, and
+// the sums meet in LDS at the end, in wave order.
+template <int MT, int JW, int NWV, int D, bool GATED>
+__global__ void __launch_bounds__(NWV* kWave) mx_stream_kernel(MxArgs a) {
+  constexpr int P = GATED ? JW / 2 : JW;  // column tiles of y
+  constexpr int NT = JW * MT;
+  constexpr int TPR = 64 / NWV < NT ? 64 / NWV : NT;  // tiles summed in one round through 64 KB of LDS
+  __shared__ f32x4 s_red[NWV * TPR * kWave];
+  const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int out_tiles = (a.n + 15) / 16;
+  const int groups = (out_tiles + P - 1) / P;
+  const int group = blockIdx.x % groups, split = blockIdx.x / groups;
+  const int rt0 = blockIdx.y * MT;
+  const int parts = a.splits * NWV, part = split * NWV + wave;
+  const int t0 = (int)((int64_t)part * a.T / parts), t1 = (int)((int64_t)(part + 1) * a.T / parts);
+
+  const u32x4* wp[JW];
+  const uint32_t* wsp[JW];
+#pragma unroll
+  for (int j = 0; j < JW; ++j) {
+    int tile = min(group * P + j % P, out_tiles - 1);
+    if (GATED && j >= P) tile += out_tiles;
+    wp[j] = a.wc + (int64_t)tile * a.T * 64 + lane;
+    wsp[j] = a.ws + (int64_t)tile * 64 + lane;
+  }
+  const u32x4* xp[MT];
+  const uint32_t* xsp[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int tile = min(rt0 + i, a.row_tiles - 1);
+    xp[i] = a.xc + (int64_t)tile * a.T * 128 + lane;
+    xsp[i] = a.xs + (int64_t)tile * 64 + lane;
+  }
+  f32x4 acc[JW][MT];
+#pragma unroll
+  for (int j = 0; j < JW; ++j)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  u32x4 w[D][JW], x[D][MT][2];
+  uint32_t sw[D][JW], sx[D][MT];
+  auto load = [&](int u, int t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < JW; ++j) {
+      w[u][j] = wp[j][(int64_t)t * 64];
+      sw[u][j] = wsp[j][(int64_t)(t >> 2) * a.w_tiles * 64];
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      x[u][i][0] = xp[i][(int64_t)t * 128];
+      x[u][i][1] = xp[i][(int64_t)t * 128 + 64];
+      sx[u][i] = xsp[i][(int64_t)(t >> 2) * a.row_tiles * 64];
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < D; ++u)
+    if (t0 + u < t1) load(u, t0 + u);
+  for (int t = t0; t < t1; t += D) {
+#pragma unroll
+    for (int u = 0; u < D; ++u) {
+      if (t + u < t1) {
+        const int sh = 8 * ((t + u) & 3);
+#pragma unroll
+        for (int j = 0; j < JW; ++j)
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+            acc[j][i] = mx_mfma(__builtin_bit_cast(i32x4, w[u][j]), __builtin_bit_cast(i32x4, x[u][i][0]),
+                                __builtin_bit_cast(i32x4, x[u][i][1]), acc[j][i], sw[u][j] >> sh, sx[u][i] >> sh);
+        if (t + u + D < t1) load(u, t + u + D);
+      }
+    }
+  }
+
+  // lane (li, lg) holds columns 4 lg .. 4 lg + 3 of a tile for row li
+  auto store = [&](int j, int i, f32x4 v, f32x4 gate) {
+    const int m = 16 * (rt0 + i) + li, n0 = 16 * (group * P + j) + 4 * lg;
+    if (m >= a.rows || n0 >= a.n) return;
+    if constexpr (GATED) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] *= gate[e] / (1.f + expf(-gate[e]));
+    }
+    if (!GATED && a.splits > 1) {  // n a multiple of 8
+      *reinterpret_cast<f32x4*>(a.part + ((int64_t)split * a.rows + m) * a.n + n0) = v;
+      return;
+    }
+    f16* y = a.y + (int64_t)m * a.n + n0;
+    const f16x4 h = {(f16)v[0], (f16)v[1], (f16)v[2], (f16)v[3]};
+    if (a.n % 4 == 0) {
+      *reinterpret_cast<f16x4*>(y) = h;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n0 + e < a.n) y[e] = h[e];
+    }
+  };
+  // rounds of whole y tiles: a gated one's up and gate sums in the same round
+  constexpr int PER = GATED ? 2 : 1, YT = P * MT, YPR = TPR / PER;
+#pragma unroll
+  for (int r = 0; r < YT; r += YPR) {
+    if (r) __syncthreads();
+#pragma unroll
+    for (int q = 0; q < YPR; ++q) {
+      if (r + q < YT) {
+        const int j = (r + q) / MT, i = (r + q) % MT;
+        s_red[(wave * TPR + q * PER) * kWave + lane] = acc[j][i];
+        if constexpr (GATED) s_red[(wave * TPR + q * PER + 1) * kWave + lane] = acc[j + P][i];
+      }
+    }
+    __syncthreads();
+    for (int q = wave; q < YPR && r + q < YT; q += NWV) {
+      f32x4 v = s_red[q * PER * kWave + lane], g = v;
+      if constexpr (GATED) g = s_red[(q * PER + 1) * kWave + lane];
+#pragma unroll
+      for (int o = 1; o < NWV; ++o) {
+        v += s_red[(o * TPR + q * PER) * kWave + lane];
+        if constexpr (GATED) g += s_red[(o * TPR + q * PER + 1) * kWave + lane];
+      }
+      store((r + q) / MT, (r + q) % MT, v, g);
+    }
+  }
+}
+
+struct MxConfig {
+  int jw = 2, splits = 1;
+};
+
+MxConfig choose_mx(int64_t n_rows, int64_t n, int64_t T, bool gated, int cus) {
+  (void)n_rows;
+  (void)T;
+  (void)cus;
+  (void)n;
+  MxConfig c;
+  c.jw = gated ? 2 : 1;
+  return c;
+}
+
+template <int MT, int JW, bool GATED>
+int launch_mx_stream(const MxArgs& a, hipStream_t st) {
+  constexpr int P = GATED ? JW / 2 : JW;
+  const int groups = ((a.n + 15) / 16 + P - 1) / P;
+  hipLaunchKernelGGL((mx_stream_kernel<MT, JW, 4, 2, GATED>), dim3(groups * a.splits, (a.row_tiles + MT - 1) / MT),
+                     dim3(4 * kWave), 0, st, a);
+  return launch_status(GATED ? "mxfp4_up_gate_silu_and_mul" : "mxfp4_linear");
+}
+
+template <bool GATED>
+int launch_mx(const MxArgs& a, const MxConfig& c, hipStream_t st) {
+  (void)c;
+  switch (std::min(a.row_tiles, 4)) {
+    case 1: return launch_mx_stream<1, GATED ? 2 : 1, GATED>(a, st);
+    case 2: return launch_mx_stream<2, GATED ? 2 : 1, GATED>(a, st);
+    case 3: return launch_mx_stream<3, GATED ? 2 : 1, GATED>(a, st);
+    default: return launch_mx_stream<4, GATED ? 2 : 1, GATED>(a, st);
+  }
+}
+
+int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
+
+int check_product(const char* who, int64_t n_rows, int64_t n, int64_t n_in) {
+  int64_t c, s;
+  if (n_rows < 0 || n < 1 || n > INT32_MAX || n_rows > kMaxMxRows)
+    return fail(NSD_ERR_UNSUPPORTED, "%s: n_rows=%lld, n_out=%lld", who, (long long)n_rows, (long long)n);
+  if (int rc = nsd_mx_bytes(4, n, n_in, &c, &s)) return rc;
+  return nsd_mx_bytes(8, n_rows, n_in, &c, &s);
+}
+
+// The workspace: the rows' codes and scales, when x is fp16, then the partials.
+struct MxWorkspace {
+  int64_t codes = 0, scales = 0, partials = 0;
+  int64_t total() const { return align256(codes) + align256(scales) + partials; }
+};
+MxWorkspace mx_workspace(int64_t n_rows, int64_t n, int64_t n_in, bool quantised, const MxConfig& c) {
+  MxWorkspace w;
+  if (!quantised) (void)nsd_mx_bytes(8, n_rows, n_in, &w.codes, &w.scales);
+  if (c.splits > 1) w.partials = c.splits * n_rows * n * (int64_t)sizeof(float);
+  return w;
+}
+
+template <bool GATED>
+int product(const char* who, const void* x, const void* x_codes, const void* x_scales, const void* w_codes,
+            const void* w_scales, void* y, int64_t n_rows, int64_t n, int64_t n_in, void* workspace,
+            int64_t workspace_bytes, void* stream) {
+  if (int rc = check_product(who, n_rows, GATED ? 2 * n : n, n_in)) return rc;
+  if (GATED && n % 16) return fail(NSD_ERR_UNSUPPORTED, "%s: inter=%lld (a multiple of 16)", who, (long long)n);
+  if (n_rows == 0) return NSD_OK;
+  if ((!x && (!x_codes || !x_scales)) || !w_codes || !w_scales || !y)
+    return fail(NSD_ERR_INVALID, "%s: null pointer", who);
+  for (const void* p : {x, x_codes, x_scales, w_codes, w_scales, (const void*)y, (const void*)workspace})
+    if (!aligned16(p)) return fail(NSD_ERR_UNSUPPORTED, "%s: pointers must be 16-byte aligned", who);
+  int cus = 0;
+  if (int rc = device_cus(&cus)) return rc;
+  const int64_t T = mx_k_tiles(n_in);
+  const MxConfig c = choose_mx(n_rows, n, T, GATED, cus);
+  const MxWorkspace need = mx_workspace(n_rows, n, n_in, x == nullptr, c);
+  if (workspace_bytes < need.total() || (need.total() > 0 && !workspace))
+    return fail(NSD_ERR_WORKSPACE, "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes,
+                (long long)need.total());
+  char* ws = static_cast<char*>(workspace);
+  if (x) {
+    void *codes = ws, *scales = ws + align256(need.codes);
+    if (int rc = mxfp8_quantize(x, n_rows, n_in, codes, scales, stream)) return rc;
+    x_codes = codes;
+    x_scales = scales;
+  }
+  MxArgs a{};
+  a.xc = static_cast<const u32x4*>(x_codes);
+  a.xs = static_cast<const uint32_t*>(x_scales);
+  a.wc = static_cast<const u32x4*>(w_codes);
+  a.ws = static_cast<const uint32_t*>(w_scales);
+  a.y = static_cast<f16*>(y);
+  a.part = reinterpret_cast<float*>(ws + align256(need.codes) + align256(need.scales));
+  a.rows = (int)n_rows;
+  a.n = (int)n;
+  a.T = (int)T;
+  a.row_tiles = (int)mx_row_tiles(n_rows);
+  a.w_tiles = (int)mx_row_tiles(GATED ? 2 * n : n);
+  a.splits = c.splits;
+  if (int rc = launch_mx<GATED>(a, c, as_stream(stream))) return rc;
+  if (c.splits > 1) return nsd_sum_partials(a.part, c.splits, y, n_rows, n, stream);
+  return NSD_OK;
+}
+
+}  // namespace
+}  // namespace nsd
+
+using namespace nsd;
+
+extern "C" int nsd_mx_workspace(int64_t n_rows, int64_t n_out, int64_t n_in, int gated, int quantised,
+                                int64_t* bytes) {
+  if (!bytes) return fail(NSD_ERR_INVALID, "mx_workspace: null output");
+  if (int rc = check_product("mx_workspace", n_rows, n_out, n_in)) return rc;
+  int cus = 0;
+  if (int rc = device_cus(&cus)) return rc;
+  const int64_t n = gated ? n_out / 2 : n_out;
+  *bytes = mx_workspace(n_rows, n, n_in, quantised != 0, choose_mx(n_rows, n, mx_k_tiles(n_in), gated != 0, cus)).total();
+  return NSD_OK;
+}
+
+extern "C" int nsd_mxfp4_linear(const void* x, const void* x_codes, const void* x_scales, const void* w_codes,
+                                const void* w_scales, void* y, int64_t n_rows, int64_t n_out, int64_t n_in,
+                                void* workspace, int64_t workspace_bytes, void* stream) {
+  return product<false>("mxfp4_linear", x, x_codes, x_scales, w_codes, w_scales, y, n_rows, n_out, n_in, workspace,
+                        workspace_bytes, stream);
+}
+
+extern "C" int nsd_mxfp4_up_gate_silu_and_mul(const void* x, const void* x_codes, const void* x_scales,
+                                              const void* w_codes, const void* w_scales, void* y, int64_t n_rows,
+                                              int64_t inter, int64_t n_in, void* workspace, int64_t workspace_bytes,
+                                              void* stream) {
+  return product<true>("mxfp4_up_gate_silu_and_mul", x, x_codes, x_scales, w_codes, w_scales, y, n_rows, inter, n_in,
+                       workspace, workspace_bytes, stream);
+}

@@ -4,6 +4,8 @@ from .block_mgmt import (gather_allocated_blocks_and_unset, set_block_table_and_
                          unset_block_table_and_num_seq_alloc_blocks, write_block_table_ranges)
 from .kvcache_mgmt import store_kvcache
 from .linear import fused_add_rmsnorm_partials, linear, linear_partials, linear_splits, sum_partials
+from .mxfp4 import (MXFP4Weight, MXFP8Rows, mxfp4_dequantize, mxfp4_linear, mxfp4_pack, mxfp4_quantize,
+                    mxfp4_up_gate_silu_and_mul, mxfp8_dequantize, mxfp8_quantize)
 from .paged_attn import paged_attention, paged_attention_fused
 from .post_layer import argmax_rows, lm_head_argmax, post_layer_forward
 from .prefill_attn import flash_attn_varlen_func, prefill_attention
@@ -18,4 +20,6 @@ __all__ = ["paged_attention", "paged_attention_fused", "store_kvcache", "rotary_
            "gather_allocated_blocks_and_unset", "write_block_table_ranges", "fused_add_rmsnorm_inplace",
            "silu_and_mul_inplace", "up_gate_silu_and_mul", "FUSED_UP_GATE_MAX_ROWS", "lm_head_argmax",
            "argmax_rows", "post_layer_forward", "linear", "linear_partials", "linear_splits", "sum_partials",
-           "fused_add_rmsnorm_partials", "qk_norm_rope_store_partials"]
+           "fused_add_rmsnorm_partials", "qk_norm_rope_store_partials", "MXFP4Weight", "MXFP8Rows", "mxfp4_quantize",
+           "mxfp4_pack", "mxfp4_dequantize", "mxfp4_linear", "mxfp4_up_gate_silu_and_mul", "mxfp8_quantize",
+           "mxfp8_dequantize"]

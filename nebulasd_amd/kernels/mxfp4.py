@@ -1,0 +1,206 @@
+"""Microscaled (OCP MX) projections: 4-bit weights, 8-bit activations.
+
+The decode and verify layers are bound by their weights' stream from memory.
+``mxfp4_linear`` and ``mxfp4_up_gate_silu_and_mul`` are ``linear`` and
+``up_gate_silu_and_mul`` over weights of 4.25 bits a value instead of 16 (the
+reference has only fp16 projections: swiftLLM/swiftllm/worker/kernels/linear.py:3-12),
+for any number of rows.  A row is cut into blocks of 32 values: one power of
+two and 32 codes, E2M1 for the weight (``MXFP4Weight``) and E4M3 for the rows it
+is multiplied with (``MXFP8Rows``), which gfx950's scaled matrix instructions
+multiply as they are, with fp32 sums.  ``include/nsd_mx.h`` states the formats,
+the roundings and the layouts.
+
+A weight comes from ``mxfp4_quantize`` (from fp16, bf16 or fp32) or
+``mxfp4_pack`` (from a checkpoint's codes and scales), once.  The products
+quantise fp16 rows themselves; rows that several projections read are
+quantised once with ``mxfp8_quantize`` and given instead.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import dataclasses
+import functools
+
+import torch
+
+from .. import _lib
+from ._util import require, require_cuda, stream_of
+
+BLOCK = 32
+_DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+@dataclasses.dataclass(frozen=True)
+class MXFP4Weight:
+    """A weight [n_out, n_in] in MXFP4: codes and scales (uint8) in the kernels' layout."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    n_out: int
+    n_in: int
+
+
+@dataclasses.dataclass(frozen=True)
+class MXFP8Rows:
+    """Rows [rows, n_in] in MXFP8: codes and scales (uint8) in the kernels' layout."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    rows: int
+    n_in: int
+
+
+@functools.lru_cache(maxsize=4096)
+def _bytes(bits: int, rows: int, n_in: int):
+    c, s = ctypes.c_int64(), ctypes.c_int64()
+    _lib.call("nsd_mx_bytes", bits, rows, n_in, ctypes.byref(c), ctypes.byref(s))
+    return c.value, s.value
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(device: int, rows: int, n_out: int, n_in: int, gated: bool, quantised: bool) -> int:
+    b = ctypes.c_int64()
+    _lib.call("nsd_mx_workspace", rows, n_out, n_in, gated, quantised, ctypes.byref(b))
+    return b.value
+
+
+def _call(t: torch.Tensor, name: str, *args) -> None:
+    """``name`` on ``t``'s device and its current stream."""
+    if t.get_device() == torch.cuda.current_device():
+        _lib.call(name, *args, stream_of(t))
+    else:
+        with torch.cuda.device(t.device):
+            _lib.call(name, *args, stream_of(t))
+
+
+def _same_device(*tensors: torch.Tensor) -> None:
+    if any(t.device != tensors[0].device for t in tensors[1:]):
+        raise ValueError("all tensors must be on one device")
+
+
+def _matrix(t: torch.Tensor, name: str) -> None:
+    if t.dim() != 2 or t.shape[1] < BLOCK or t.shape[1] % BLOCK:
+        raise ValueError(f"{name} must be [rows, n_in] with n_in a multiple of {BLOCK}, got {tuple(t.shape)}")
+
+
+def _empty(bits: int, rows: int, n_in: int, device):
+    c, s = _bytes(bits, rows, n_in)
+    return (torch.empty(c, dtype=torch.uint8, device=device), torch.empty(s, dtype=torch.uint8, device=device))
+
+
+def _check_blocks(b, bits: int, rows: int, what: str) -> None:
+    c, s = _bytes(bits, rows, b.n_in)
+    for t, n in ((b.codes, c), (b.scales, s)):
+        if t.dtype != torch.uint8 or not t.is_contiguous() or t.numel() != n:
+            raise ValueError(f"{what} [{rows}, {b.n_in}] must hold {c} bytes of codes and {s} of scales")
+    require_cuda(b.codes, b.scales)
+    _same_device(b.codes, b.scales)
+
+
+def mxfp4_quantize(w: torch.Tensor) -> MXFP4Weight:
+    """w [n_out, n_in] (fp16, bf16 or fp32) in MXFP4.  A block with an infinity or a NaN becomes NaN."""
+    require_cuda(w)
+    _matrix(w, "w")
+    if w.dtype not in _DTYPES:
+        raise TypeError(f"w must be fp16, bf16 or fp32, got {w.dtype}")
+    require(w, w.dtype, "w")
+    n_out, n_in = w.shape
+    codes, scales = _empty(4, n_out, n_in, w.device)
+    _call(w, "nsd_mxfp4_quantize", w.data_ptr(), _DTYPES[w.dtype], n_out, n_in, codes.data_ptr(), scales.data_ptr())
+    return MXFP4Weight(codes, scales, n_out, n_in)
+
+
+def mxfp4_pack(codes: torch.Tensor, scales: torch.Tensor) -> MXFP4Weight:
+    """A checkpoint's MXFP4 weight: uint8 codes [n_out, n_in / 2] (the even value in the low half) and uint8
+    scales [n_out, n_in / 32]."""
+    require_cuda(codes, scales)
+    require(codes, torch.uint8, "codes")
+    require(scales, torch.uint8, "scales")
+    if codes.dim() != 2 or scales.dim() != 2 or scales.shape[1] < 1 or \
+            tuple(codes.shape) != (scales.shape[0], scales.shape[1] * BLOCK // 2):
+        raise ValueError(f"codes must be [n_out, n_in / 2] and scales [n_out, n_in / {BLOCK}], got "
+                         f"{tuple(codes.shape)} and {tuple(scales.shape)}")
+    _same_device(codes, scales)
+    n_out, n_in = codes.shape[0], 2 * codes.shape[1]
+    out = _empty(4, n_out, n_in, codes.device)
+    _call(codes, "nsd_mxfp4_pack", codes.data_ptr(), scales.data_ptr(), n_out, n_in, *(t.data_ptr() for t in out))
+    return MXFP4Weight(*out, n_out, n_in)
+
+
+def mxfp8_quantize(x: torch.Tensor) -> MXFP8Rows:
+    """x [rows, n_in] fp16 in MXFP8.  A block with an infinity or a NaN becomes NaN."""
+    require_cuda(x)
+    _matrix(x, "x")
+    require(x, torch.float16, "x")
+    rows, n_in = x.shape
+    codes, scales = _empty(8, rows, n_in, x.device)
+    _call(x, "nsd_mxfp8_quantize", x.data_ptr(), rows, n_in, codes.data_ptr(), scales.data_ptr())
+    return MXFP8Rows(codes, scales, rows, n_in)
+
+
+def _dequantize(b, bits: int, rows: int, dtype: torch.dtype, name: str) -> torch.Tensor:
+    if dtype not in _DTYPES:
+        raise TypeError(f"dtype must be fp16, bf16 or fp32, got {dtype}")
+    _check_blocks(b, bits, rows, "the blocks of")
+    out = torch.empty((rows, b.n_in), dtype=dtype, device=b.codes.device)
+    _call(out, name, b.codes.data_ptr(), b.scales.data_ptr(), rows, b.n_in, out.data_ptr(), _DTYPES[dtype])
+    return out
+
+
+def mxfp4_dequantize(w: MXFP4Weight, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values [n_out, n_in] that ``w`` stands for; exact in bf16 and fp32."""
+    return _dequantize(w, 4, w.n_out, dtype, "nsd_mxfp4_dequantize")
+
+
+def mxfp8_dequantize(x: MXFP8Rows, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values [rows, n_in] that ``x`` stands for; exact in bf16 and fp32."""
+    return _dequantize(x, 8, x.rows, dtype, "nsd_mxfp8_dequantize")
+
+
+def _product(x, w: MXFP4Weight, out, gated: bool, name: str) -> torch.Tensor:
+    quantised = isinstance(x, MXFP8Rows)
+    if quantised:
+        rows, n_in, on = x.rows, x.n_in, x.codes
+        _check_blocks(x, 8, rows, "x")
+    else:
+        require_cuda(x)
+        _matrix(x, "x")
+        require(x, torch.float16, "x")
+        (rows, n_in), on = x.shape, x
+    if n_in != w.n_in:
+        raise ValueError(f"x has {n_in} columns, the weight is [{w.n_out}, {w.n_in}]")
+    _check_blocks(w, 4, w.n_out, "the weight")
+    n = w.n_out
+    if gated:
+        if n % 32:
+            raise ValueError(f"an up/gate weight has 2 * inter rows, inter a multiple of 16; got {n}")
+        n //= 2
+    if out is None:
+        out = torch.empty((rows, n), dtype=torch.float16, device=on.device)
+    else:
+        require_cuda(out)
+        require(out, torch.float16, "out")
+        if tuple(out.shape) != (rows, n):
+            raise ValueError(f"out must be [{rows}, {n}]")
+    _same_device(on, w.codes, out)
+    if rows == 0:
+        return out
+    ws = torch.empty(_workspace_bytes(on.get_device(), rows, w.n_out, n_in, gated, quantised), dtype=torch.uint8,
+                     device=on.device)
+    _call(on, name, *((None, x.codes.data_ptr(), x.scales.data_ptr()) if quantised else (x.data_ptr(), None, None)),
+          w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), rows, n, n_in, ws.data_ptr(), ws.numel())
+    return out
+
+
+def mxfp4_linear(x: torch.Tensor | MXFP8Rows, w: MXFP4Weight, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``linear`` with an MXFP4 weight: fp16 [rows, n_out] = fp16(X . W^T), X the MXFP8 values of x [rows, n_in]
+    (fp16, or quantised already), fp32 sums."""
+    return _product(x, w, out, False, "nsd_mxfp4_linear")
+
+
+def mxfp4_up_gate_silu_and_mul(x: torch.Tensor | MXFP8Rows, w: MXFP4Weight,
+                               out: torch.Tensor | None = None) -> torch.Tensor:
+    """``up_gate_silu_and_mul`` with an MXFP4 weight [2 * inter, n_in] (up rows first): fp16 [rows, inter] =
+    fp16(up * silu(gate)), the products and the SiLU-and-mul in fp32, rounded once."""
+    return _product(x, w, out, True, "nsd_mxfp4_up_gate_silu_and_mul")

@@ -1,0 +1,101 @@
+"""numpy restatement of the microscaled (OCP MX) formats and products, in 64
+bits (the oracle for ``nebulasd_amd.kernels.mxfp4``).
+
+TEST INFRASTRUCTURE ONLY: imported by ``tests/``; never by the product package.
+The reference has no counterpart (its projections are fp16).
+
+How each function is pinned (``tests/test_oracle_mx.py``):
+
+* ``mx_quantize`` -- the formats' value tables counted by hand; torch's own
+  ``float8_e4m3fn`` conversion for the 8-bit codes; brute force over every code
+  (no code is nearer, ties to the even code); closed forms for powers of two,
+  zeros, saturation and NaN; a planted mistake (the scale one step up).
+* ``mx_values`` -- quantising the values gives the codes back.
+* ``mx_linear`` / ``mx_up_gate`` -- one-hot rows, and torch in float64.
+"""
+
+from __future__ import annotations
+
+import numpy as np
+
+__all__ = ["MX_BLOCK", "E2M1", "E4M3", "mx_quantize", "mx_values", "mx_pack_nibbles", "mx_unpack_nibbles", "mx_linear",
+           "mx_up_gate", "mx_linear_bound"]
+
+MX_BLOCK = 32
+# The non-negative values of the codes, in code order.
+E2M1 = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6])
+E4M3 = np.array([m * 2.0 ** -9 for m in range(8)]
+                + [(8 + m) * 2.0 ** (p - 3) for p in range(-6, 9) for m in range(8)][:-1])
+
+
+def mx_quantize(x, bits):
+    """Codes [n, k] (4 or 8 bits, one a byte, the sign in the code's top bit) and scale bytes [n, k / 32].
+
+    4 bits: scale 2^(floor(log2 m) - 2), m the block's largest magnitude; 8 bits: the smallest power of two
+    with m <= 448 times it.  Scales start at 2^-127.  Nearest code, ties to the even one, past the largest to
+    the largest.  An infinity or NaN: scale byte 255 (codes 0; with 8 bits the NaN code 127)."""
+    x = np.asarray(x, np.float64)
+    n, k = x.shape
+    b = x.reshape(n, k // MX_BLOCK, MX_BLOCK)
+    bad = ~np.isfinite(b).all(-1)
+    b = np.where(bad[..., None], 0.0, b)
+    m = np.abs(b).max(-1)
+    f, p = np.frexp(m)  # m = f 2^p, 0.5 <= f < 1
+    e = p - 1 - 2 if bits == 4 else p - 1 - 8 + (f > 0.875)
+    e = np.where(m > 0, np.maximum(e, -127), -127)
+    table = E2M1 if bits == 4 else E4M3
+    a = np.ldexp(np.abs(b), -e[..., None])  # exact: a power of two
+    hi = np.clip(np.searchsorted(table, a), 1, len(table) - 1)  # table[hi - 1] <= a <= table[hi] within the table
+    d_lo, d_hi = a - table[hi - 1], table[hi] - a
+    code = np.where((d_hi < d_lo) | ((d_hi == d_lo) & (hi % 2 == 0)), hi, hi - 1).astype(np.uint8)
+    code = code | (np.signbit(b).astype(np.uint8) << (bits - 1))
+    if bits == 8:
+        code[bad] = 127
+    return code.reshape(n, k), np.where(bad, 255, e + 127).astype(np.uint8)
+
+
+def mx_values(codes, scales, bits):
+    """float64 [n, k] that codes and scale bytes stand for."""
+    table = (E2M1 if bits == 4 else np.append(E4M3, np.nan))
+    mag = table[codes & (2 ** (bits - 1) - 1)]
+    v = np.where(codes >> (bits - 1), -mag, mag).reshape(len(codes), -1, MX_BLOCK)
+    s = np.where(scales == 255, np.nan, np.ldexp(1.0, scales.astype(np.int64) - 127))
+    return (v * s[..., None]).reshape(codes.shape)
+
+
+def mx_pack_nibbles(codes):
+    """4-bit codes [n, k] by two, the even one in the low half: [n, k / 2]."""
+    return (codes[:, 0::2] | (codes[:, 1::2] << 4)).astype(np.uint8)
+
+
+def mx_unpack_nibbles(packed):
+    return np.stack((packed & 15, packed >> 4), -1).reshape(len(packed), -1)
+
+
+def mx_linear(x, w_values):
+    """float64 [rows, n_out]: the MXFP8 values of fp16 x times w_values [n_out, n_in] (the products' definition
+    before its one rounding)."""
+    return mx_values(*mx_quantize(x, 8), 8) @ w_values.T
+
+
+def mx_up_gate(x, w_values):
+    """float64 [rows, inter]: up * gate / (1 + exp(-gate)) over the halves of the product."""
+    y = mx_linear(x, w_values)
+    up, gate = np.split(y, 2, axis=1)
+    with np.errstate(over="ignore"):
+        return up * (gate / (1 + np.exp(-gate)))
+
+
+def mx_linear_bound(x, w_values):
+    """How far a product's fp32 sum may be off before its rounding, [rows, n_out].
+
+    The instruction adds a block's 32 products aligned to the largest of them and keeps 15 bits below it
+    (measured: a product under 2^-15 of the largest is lost, one above is not), so a block adds at most 32 of
+    those last places; sums of blocks are fp32: another 2^-24 of the absolute sum for each of the n_in / 32 + 16
+    additions (16 waves' sums and splits joined at most)."""
+    xv, wv = np.abs(mx_values(*mx_quantize(x, 8), 8)), np.abs(w_values)
+    r, k = xv.shape
+    top = np.zeros((r, len(wv)))
+    for b in range(0, k, MX_BLOCK):  # the largest product is at most the product of the largest
+        top += xv[:, b:b + MX_BLOCK].max(1)[:, None] * wv[:, b:b + MX_BLOCK].max(1)[None]
+    return 32 * 2.0 ** -15 * top + (k // MX_BLOCK + 16) * 2.0 ** -24 * (xv @ wv.T)

@@ -1,0 +1,318 @@
+"""GPU parity of the microscaled quantisers and products (kernels/mxfp4.py)
+against the 64-bit oracle (``oracle.mx``).
+
+- Codes and scales, the kernels' layout undone, equal the oracle's bit for
+  bit; dequantised values equal the oracle's exactly (bf16 and fp32).
+- Products: within half an fp16 step (2^-11 relative, 2^-25 among the
+  subnormals) of the float64 result moved by at most the fp32 sum's bound
+  (``oracle.mx_linear_bound``); and as a whole, in norm, within 2^-11 (the
+  rounding alone gives at most 2^-11 / sqrt(3) = 2.8e-4).  With the SiLU-and-mul, 8
+  fp32 roundings more (2^-21) and the sums' bounds carried through the
+  product: |silu(g)| du + |up| 1.1 dg (the SiLU's slope is at most 1.1).
+
+Every case prints its name first.
+"""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import oracle
+from nebulasd_amd import _lib
+from nebulasd_amd import kernels as K
+
+pytestmark = pytest.mark.gpu
+
+
+def _rows(rows, k, seed=0, std=1.0):
+    """Hidden states: a few channels far larger, a zero row at the end of a batch."""
+    rng = np.random.default_rng(seed)
+    x = rng.standard_normal((rows, k)) * std
+    x[:, rng.random(k) < 1 / 64] *= 24
+    if rows > 8:
+        x[-1] = 0
+    return x.astype(np.float16)
+
+
+def _weight(gpu, n, k, seed=0):
+    """An MXFP4 weight on the GPU and its float64 values."""
+    rng = np.random.default_rng(seed + 1000)
+    w = rng.standard_normal((n, k)) * (0.5 + rng.random((n, 1))) * k ** -0.5
+    codes, scales = oracle.mx_quantize(w, 4)
+    packed = torch.from_numpy(oracle.mx_pack_nibbles(codes)).to(gpu)
+    return K.mxfp4_pack(packed, torch.from_numpy(scales).to(gpu)), oracle.mx_values(codes, scales, 4)
+
+
+def _natural(b, bits, rows):
+    """(codes [rows, k], scales [rows, k / 32]) of a kernel-layout tensor pair; the padding's codes must be zero."""
+    k = b.n_in
+    rt, kt = -(-rows // 16), -(-k // 128)
+    c = b.codes.cpu().numpy()
+    if bits == 4:
+        c = c.reshape(rt, kt, 4, 16, 16).transpose(0, 3, 1, 2, 4).reshape(rt * 16, kt * 64)
+        c = oracle.mx_unpack_nibbles(c)
+    else:
+        c = c.reshape(rt, kt, 8, 16, 16).transpose(0, 3, 1, 2, 4).reshape(rt * 16, kt * 128)
+    kg = -(-kt // 4)
+    s = b.scales.cpu().numpy().reshape(kg, rt, 4, 16, 4).transpose(1, 3, 0, 4, 2).reshape(rt * 16, kg * 16)
+    assert not c[rows:].any() and not c[:, k:].any()
+    return c[:rows, :k], s[:rows, :k // 32]
+
+
+def _special(n, k, dtype, seed):
+    """Values over the type's whole range, on middles, zeros of both signs, a zero block, subnormals, and (in the
+    blocks before the last) infinities and NaN."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(n, k, generator=g, dtype=torch.float64)
+    span = {torch.float16: (-26, 14), torch.bfloat16: (-140, 125), torch.float32: (-150, 125)}[dtype]
+    x *= torch.exp2(torch.randint(*span, (n, k // 32), generator=g).double()).repeat_interleave(32, 1)
+    x[0, :32] = 0
+    x[0, 3] = -0.0
+    m = torch.tensor([.25, .75, 1.25, 1.75, 2.5, 3.5, 5, 7, 6, 4, 17, 1.0625, 448, 440, 7.75, 7.5])
+    x[-1, :16], x[-1, 16:32] = m, -m
+    x[n // 2, :32] = torch.finfo(dtype).smallest_normal * torch.rand(32, generator=g).double() * 0.5
+    x[n // 3, 0] = torch.finfo(dtype).max
+    if k > 32:
+        x[1, k - 32], x[2 % n, k - 1] = float("inf"), float("nan")
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,k", [(5, 64), (1, 32), (16, 128), (33, 160), (130, 544), (16, 2048), (257, 4096)])
+def test_quantize_weight_bits(gpu, dtype, n, k):
+    print(f"mxfp4_quantize {n} x {k} {dtype}", flush=True)
+    w = _special(n, k, dtype, n + k) if n > 2 else torch.randn(n, k).to(dtype)
+    q = K.mxfp4_quantize(w.to(gpu))
+    codes, scales = oracle.mx_quantize(w.double().numpy(), 4)
+    got_c, got_s = _natural(q, 4, n)
+    assert np.array_equal(got_s, scales)
+    live = np.repeat(scales != 255, 32, axis=1)
+    same = (got_c == codes) | ((got_c & 7 == 0) & (codes & 7 == 0))  # the sign of a zero
+    assert same[live].all()
+    want = oracle.mx_values(codes, scales, 4)
+    for out in (torch.bfloat16, torch.float32):
+        got = K.mxfp4_dequantize(q, out).double().cpu().numpy()
+        assert np.array_equal(got, want, equal_nan=True), out
+    got = K.mxfp4_dequantize(q, torch.float16).cpu().numpy()
+    with np.errstate(over="ignore"):
+        assert np.array_equal(got, want.astype(np.float16), equal_nan=True)
+
+
+@pytest.mark.parametrize("n,k", [(5, 64), (1, 32), (48, 1056), (4097, 128), (16, 12288)])
+def test_quantize_rows_bits(gpu, n, k):
+    print(f"mxfp8_quantize {n} x {k}", flush=True)
+    x = _special(n, k, torch.float16, n + k) if n > 2 else torch.randn(n, k).half()
+    q = K.mxfp8_quantize(x.to(gpu))
+    codes, scales = oracle.mx_quantize(x.double().numpy(), 8)
+    got_c, got_s = _natural(q, 8, n)
+    assert np.array_equal(got_s, scales)
+    same = (got_c == codes) | ((got_c & 127 == 0) & (codes & 127 == 0)) | ((got_c & 127 == 127) & (codes & 127 == 127))
+    assert same.all()
+    want = oracle.mx_values(codes, scales, 8)
+    for out in (torch.bfloat16, torch.float32):
+        assert np.array_equal(K.mxfp8_dequantize(q, out).double().cpu().numpy(), want, equal_nan=True), out
+
+
+def test_pack_equals_quantize(gpu):
+    w = torch.randn(83, 416)
+    q = K.mxfp4_quantize(w.to(gpu))
+    codes, scales = oracle.mx_quantize(w.double().numpy(), 4)
+    p = K.mxfp4_pack(torch.from_numpy(oracle.mx_pack_nibbles(codes)).to(gpu), torch.from_numpy(scales).to(gpu))
+    assert torch.equal(q.codes, p.codes) and torch.equal(q.scales, p.scales) and (p.n_out, p.n_in) == (83, 416)
+
+
+def _check(got, want, bound, extra=0.0):
+    got = got.double().cpu().numpy()
+    tol = 2.0 ** -11 * (np.abs(want) + bound) + 2.0 ** -25 + bound + extra * np.abs(want)
+    off = np.abs(got - want)
+    worst = np.unravel_index(np.argmax(off - tol), off.shape)
+    assert (off <= tol).all(), f"{(off > tol).sum()} of {off.size}; worst at {worst}: {got[worst]} {want[worst]}"
+    rel = np.linalg.norm(got - want) / max(np.linalg.norm(want), 1e-30)
+    print(f"  rel {rel:.2e}", flush=True)
+    assert rel <= 2.0 ** -11
+
+
+# (rows, n_out, n_in): one token; row counts at both sides of every tile count; odd widths and inner lengths;
+# one block, one tile, ragged tiles of k; more rows than one pass; wide and long ones.
+SHAPES = [(1, 16, 32), (1, 1024, 1024), (3, 17, 96), (16, 33, 128), (17, 1, 160), (32, 64, 512), (33, 1000, 544),
+          (48, 250, 2080), (49, 4096, 256), (64, 6144, 1024), (65, 515, 4096), (80, 4096, 4096), (81, 96, 12288),
+          (97, 2048, 2048), (112, 48, 8192), (113, 1001, 640), (128, 1024, 4096), (129, 300, 1024), (200, 1536, 608),
+          (257, 255, 2048), (513, 130, 1056), (1000, 1040, 512), (16, 20001, 256)]
+
+
+@pytest.mark.parametrize("rows,n,k", SHAPES, ids=[f"{r}x{n}x{k}" for r, n, k in SHAPES])
+def test_linear_matches_oracle(gpu, rows, n, k):
+    print(f"mxfp4_linear {rows} x {n} x {k}", flush=True)
+    x = _rows(rows, k, seed=n)
+    w, values = _weight(gpu, n, k, seed=rows)
+    buf = torch.full((rows * n + 512,), 7.0, dtype=torch.float16, device=gpu)
+    out = K.mxfp4_linear(torch.from_numpy(x).to(gpu), w, out=buf[:rows * n].view(rows, n))
+    assert bool((buf[rows * n:] == 7.0).all()), "the kernel wrote past the output"
+    _check(out, oracle.mx_linear(x, values), oracle.mx_linear_bound(x, values))
+    # the rows quantised beforehand: the same bits
+    assert torch.equal(K.mxfp4_linear(K.mxfp8_quantize(torch.from_numpy(x).to(gpu)), w), out)
+
+
+GATED = [(1, 16, 32), (1, 2816, 1024), (5, 48, 544), (16, 12288, 256), (33, 1024, 1056), (64, 2816, 1024),
+         (80, 1600, 4096), (100, 32, 8192), (128, 4096, 512), (129, 160, 1024), (300, 1040, 288), (700, 528, 2048)]
+
+
+@pytest.mark.parametrize("rows,inter,k", GATED, ids=[f"{r}x{n}x{k}" for r, n, k in GATED])
+def test_gated_matches_oracle(gpu, rows, inter, k):
+    print(f"mxfp4_up_gate_silu_and_mul {rows} x {inter} x {k}", flush=True)
+    x = _rows(rows, k, seed=inter)
+    w, values = _weight(gpu, 2 * inter, k, seed=rows)
+    buf = torch.full((rows * inter + 512,), 7.0, dtype=torch.float16, device=gpu)
+    out = K.mxfp4_up_gate_silu_and_mul(torch.from_numpy(x).to(gpu), w, out=buf[:rows * inter].view(rows, inter))
+    assert bool((buf[rows * inter:] == 7.0).all()), "the kernel wrote past the output"
+    up, gate = np.split(oracle.mx_linear(x, values), 2, axis=1)
+    du, dg = np.split(oracle.mx_linear_bound(x, values), 2, axis=1)
+    bound = np.abs(gate / (1 + np.exp(-gate))) * du + 1.1 * (np.abs(up) + du) * dg
+    _check(out, oracle.mx_up_gate(x, values), bound, extra=2.0 ** -21)
+    assert torch.equal(K.mxfp4_up_gate_silu_and_mul(K.mxfp8_quantize(torch.from_numpy(x).to(gpu)), w), out)
+
+
+@pytest.mark.parametrize("rows", [5, 40, 128, 300])
+def test_infinities_and_nan_stay_in_their_rows_and_columns(gpu, rows):
+    """A NaN block makes its row, or its weight's column, NaN, and nothing else."""
+    n, k = 72, 416
+    x = _rows(rows, k, seed=1)
+    x[1, 7], x[3, 200] = np.inf, np.nan
+    values = oracle.mx_quantize(np.random.default_rng(2).standard_normal((n, k)), 4)
+    values[1][11, 4] = 255
+    w = K.mxfp4_pack(torch.from_numpy(oracle.mx_pack_nibbles(values[0])).to(gpu), torch.from_numpy(values[1]).to(gpu))
+    got = K.mxfp4_linear(torch.from_numpy(x).to(gpu), w).isnan().cpu()
+    want = torch.zeros(rows, n, dtype=torch.bool)
+    want[1] = want[3] = True
+    want[:, 11] = True
+    assert torch.equal(got, want)
+
+
+def test_large_and_small_scales(gpu):
+    """Scales at both ends of the byte: products that only meet in range, overflow to infinity, and vanish."""
+    rng = np.random.default_rng(3)
+    codes = rng.integers(0, 16, (32, 64)).astype(np.uint8)
+    codes[:, 0] = 5
+    for byte, x_scale in ((1, 2.0 ** 9), (20, 1.0), (120, 2.0 ** -14), (150, 2.0 ** -20), (250, 1.0)):
+        scales = np.full((32, 2), byte, np.uint8)
+        w = K.mxfp4_pack(torch.from_numpy(oracle.mx_pack_nibbles(codes)).to(gpu), torch.from_numpy(scales).to(gpu))
+        x = (rng.random((3, 64)) * x_scale).astype(np.float16)
+        values = oracle.mx_values(codes, scales, 4)
+        with np.errstate(over="ignore"):
+            got = K.mxfp4_linear(torch.from_numpy(x).to(gpu), w).cpu().numpy()
+            want = oracle.mx_linear(x, values)
+            tol = 2.0 ** -11 * np.abs(want) + 2.0 ** -25 + 1.01 * oracle.mx_linear_bound(x, values)
+            inside = np.abs(want) < 65000
+            assert (np.abs(got - want)[inside] <= tol[inside]).all(), byte
+            over = np.abs(want) > 66000
+            assert np.array_equal(got[over], np.sign(want[over]) * np.inf), byte
+
+
+def test_no_rows_and_one_row(gpu):
+    w, _ = _weight(gpu, 64, 256)
+    assert K.mxfp4_linear(torch.empty(0, 256, dtype=torch.float16, device=gpu), w).shape == (0, 64)
+    assert K.mxfp4_up_gate_silu_and_mul(torch.empty(0, 256, dtype=torch.float16, device=gpu), w).shape == (0, 32)
+    assert K.mxfp8_dequantize(K.mxfp8_quantize(torch.empty(0, 64, dtype=torch.float16, device=gpu))).shape == (0, 64)
+
+
+def test_refusals(gpu):
+    w, _ = _weight(gpu, 64, 256)
+    x = torch.zeros(2, 256, dtype=torch.float16, device=gpu)
+    with pytest.raises(ValueError, match="256 columns|128 columns"):
+        K.mxfp4_linear(x[:, :128].contiguous(), w)
+    with pytest.raises(TypeError, match="float16"):
+        K.mxfp4_linear(x.float(), w)
+    with pytest.raises(ValueError, match="contiguous"):
+        K.mxfp4_linear(torch.zeros(2, 512, dtype=torch.float16, device=gpu)[:, ::2], w)
+    with pytest.raises(ValueError, match="multiple of 32"):
+        K.mxfp8_quantize(torch.zeros(2, 40, dtype=torch.float16, device=gpu))
+    with pytest.raises(TypeError, match="fp16, bf16 or fp32"):
+        K.mxfp4_quantize(torch.zeros(2, 64, dtype=torch.int8, device=gpu))
+    with pytest.raises(ValueError, match=r"out must be \[2, 64\]"):
+        K.mxfp4_linear(x, w, out=torch.empty(2, 65, dtype=torch.float16, device=gpu))
+    odd, _ = _weight(gpu, 24, 256)
+    with pytest.raises(ValueError, match="multiple of 16"):
+        K.mxfp4_up_gate_silu_and_mul(x, odd)
+    with pytest.raises(ValueError, match="codes must be"):
+        K.mxfp4_pack(torch.zeros(4, 16, dtype=torch.uint8, device=gpu), torch.zeros(4, 2, dtype=torch.uint8, device=gpu))
+    with pytest.raises(ValueError, match="must hold"):
+        K.mxfp4_linear(x, K.MXFP4Weight(w.codes[:-16], w.scales, 64, 256))
+    with pytest.raises(ValueError, match="GPU tensors"):
+        K.mxfp4_linear(x.cpu(), w)
+    buf = torch.zeros(2 * 256 + 4, dtype=torch.float16, device=gpu)
+    with pytest.raises(_lib.NativeLibraryError, match="aligned"):
+        K.mxfp4_linear(buf[4:].view(2, 256), w)
+
+
+@pytest.mark.parametrize("rows", [4, 80, 300])
+def test_graph_replays(gpu, rows):
+    """An FFN in a captured graph: every replay, with eager work between, gives the eager bits."""
+    wug, _ = _weight(gpu, 2 * 512, 1024, seed=1)
+    wd, _ = _weight(gpu, 1024, 512, seed=2)
+    x = torch.from_numpy(_rows(rows, 1024)).to(gpu)
+
+    def ffn():
+        return K.mxfp4_linear(K.mxfp4_up_gate_silu_and_mul(x, wug), wd)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ffn()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = ffn()
+        graphs.append((g, y))
+    for seed in range(4):
+        x.copy_(torch.from_numpy(_rows(rows, 1024, seed=seed)))
+        want = ffn()
+        for g, y in graphs:
+            y.zero_()
+            g.replay()
+        torch.cuda.synchronize()
+        for _, y in graphs:
+            assert torch.equal(y, want)
+
+
+def test_streams_do_not_share_scratch(gpu):
+    """The same shape on two streams at once: each call's own workspace."""
+    w, _ = _weight(gpu, 4096, 4096)
+    xs = [torch.from_numpy(_rows(80, 4096, seed=s)).to(gpu) for s in range(2)]
+    want = [K.mxfp4_linear(x, w) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(K.mxfp4_linear(xs[i], w))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(y, want[i]) for y in got[i])
+
+
+@pytest.mark.parametrize("rows", [1, 64, 200])
+def test_ffn_together(gpu, rows):
+    """Quantised weights from fp16 ones, then up/gate and down as a layer runs them: each step against the oracle
+    on the step's own input."""
+    g = torch.Generator(device=gpu).manual_seed(5)
+    hidden, inter = 1024, 1536
+    wug = torch.randn(2 * inter, hidden, device=gpu, generator=g).mul_(hidden ** -0.5).half()
+    wd = torch.randn(hidden, inter, device=gpu, generator=g).mul_(inter ** -0.5).half()
+    qug, qd = K.mxfp4_quantize(wug), K.mxfp4_quantize(wd)
+    x = torch.from_numpy(_rows(rows, hidden)).to(gpu)
+    h = K.mxfp4_up_gate_silu_and_mul(x, qug)
+    y = K.mxfp4_linear(h, qd)
+    vug, vd = (K.mxfp4_dequantize(q, torch.float32).double().cpu().numpy() for q in (qug, qd))
+    assert np.array_equal(vd, oracle.mx_values(*oracle.mx_quantize(wd.cpu().numpy(), 4), 4))
+    xn, hn = x.cpu().numpy(), h.cpu().numpy()
+    up, gate = np.split(oracle.mx_linear(xn, vug), 2, axis=1)
+    du, dg = np.split(oracle.mx_linear_bound(xn, vug), 2, axis=1)
+    _check(h, oracle.mx_up_gate(xn, vug), np.abs(gate / (1 + np.exp(-gate))) * du + 1.1 * (np.abs(up) + du) * dg,
+           extra=2.0 ** -21)
+    _check(y, oracle.mx_linear(hn, vd), oracle.mx_linear_bound(hn, vd))

@@ -1,0 +1,187 @@
+"""Pins of the microscaled oracle (no GPU), and the refusals that need none."""
+
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import oracle
+from oracle import E2M1, E4M3, mx_linear, mx_pack_nibbles, mx_quantize, mx_unpack_nibbles, mx_up_gate, mx_values
+
+
+def test_value_tables():
+    assert E2M1.tolist() == [0, .5, 1, 1.5, 2, 3, 4, 6]
+    every = torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).double().numpy()
+    assert np.array_equal(every, E4M3) and E4M3[-1] == 448
+
+
+def _blocks(seed, n=64, k=96):
+    rng = np.random.default_rng(seed)
+    return rng.standard_normal((n, k)) * 2.0 ** rng.integers(-12, 9, (n, 1))
+
+
+@pytest.mark.parametrize("bits,table", [(4, E2M1), (8, E4M3)])
+def test_nearest_code_ties_to_even(bits, table):
+    x = _blocks(1).astype(np.float16).astype(np.float64)
+    x[:, ::7] = np.round(x[:, ::7] * 64) / 64  # some on middles
+    codes, scales = mx_quantize(x, bits)
+    s = np.ldexp(1.0, np.repeat(scales.astype(np.int64) - 127, 32, axis=1))
+    a, mag = np.abs(x) / s, codes & (2 ** (bits - 1) - 1)
+    off = np.abs(a - table[mag])
+    every = np.abs(a[..., None] - table)
+    assert np.array_equal(off, every.min(-1))  # no code is nearer, saturation included
+    ties = (every == off[..., None]).sum(-1) == 2
+    assert (mag[ties] % 2 == 0).all()
+    assert np.array_equal(codes >> (bits - 1), np.signbit(x))
+
+
+def test_scale_rules():
+    m = np.abs(_blocks(2).reshape(64, 3, 32)).max(-1)
+    s4 = mx_quantize(_blocks(2), 4)[1].astype(np.int64) - 127
+    s8 = mx_quantize(_blocks(2), 8)[1].astype(np.int64) - 127
+    assert (np.ldexp(4.0, s4) <= m).all() and (m < np.ldexp(8.0, s4)).all()
+    assert (m <= np.ldexp(448.0, s8)).all() and (m > np.ldexp(448.0, s8 - 1)).all()
+
+
+def test_codes_match_torch_e4m3():
+    x = _blocks(3).astype(np.float16)
+    codes, scales = mx_quantize(x, 8)
+    s = np.ldexp(1.0, -np.repeat(scales.astype(np.int64) - 127, 32, axis=1))
+    want = torch.from_numpy(x.astype(np.float64) * s).float().to(torch.float8_e4m3fn).view(torch.uint8).numpy()
+    assert np.array_equal(codes, want)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_closed_forms(bits):
+    x = np.zeros((6, 32))
+    x[1, 3] = -1.0
+    x[2] = 7.0 if bits == 4 else 448.0   # 7: past 6 at the scale 1
+    x[3, 0], x[4, 5] = np.inf, np.nan
+    x[5, 0] = 2.0 ** -140
+    codes, scales = mx_quantize(x, bits)
+    v = mx_values(codes, scales, bits)
+    assert scales[0, 0] == 0 and not v[0].any()
+    assert v[1, 3] == -1 and np.count_nonzero(v[1]) == 1
+    assert int(scales[1, 0]) - 127 == (-2 if bits == 4 else -8)
+    assert (v[2] == (6.0 if bits == 4 else 448.0)).all()
+    assert (scales[3:5] == 255).all() and np.isnan(v[3:5]).all()
+    assert scales[5, 0] == 0 and v[5, 0] == 0
+    if bits == 8:
+        x = np.full((1, 32), np.nextafter(448.0, 449))  # just past the top: the next scale, no saturation
+        assert mx_quantize(x, 8)[1][0, 0] == 128
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_values_quantise_to_themselves(bits):
+    codes, scales = mx_quantize(_blocks(4), bits)
+    v = mx_values(codes, scales, bits)
+    again = mx_values(*mx_quantize(v, bits), bits)
+    assert np.array_equal(v, again)
+
+
+def test_nibbles():
+    c = np.arange(64, dtype=np.uint8).reshape(2, 32) % 16
+    p = mx_pack_nibbles(c)
+    assert p.shape == (2, 16) and p[0, 0] == 0x10 and np.array_equal(mx_unpack_nibbles(p), c)
+
+
+def test_products():
+    w = mx_values(*mx_quantize(_blocks(5, 20, 64), 4), 4)
+    one = np.zeros((64, 64), np.float16)
+    one[np.arange(64), np.arange(64)] = 1
+    assert np.array_equal(mx_linear(one, w), w.T)
+    x = _blocks(6, 9, 64).astype(np.float16)
+    xv = torch.from_numpy(mx_values(*mx_quantize(x, 8), 8))
+    y = torch.nn.functional.linear(xv, torch.from_numpy(w))
+    np.testing.assert_allclose(mx_linear(x, w), y.numpy(), rtol=1e-12, atol=1e-12)
+    up, gate = y.chunk(2, 1)
+    np.testing.assert_allclose(mx_up_gate(x, w), (up * torch.nn.functional.silu(gate)).numpy(), rtol=1e-12, atol=1e-12)
+    assert not np.allclose(mx_up_gate(x, np.roll(w, 10, 0)), mx_up_gate(x, w))  # the halves swapped
+
+
+def test_a_wrong_scale_is_seen():
+    x = _blocks(7)
+    codes, scales = mx_quantize(x, 4)
+    assert not np.allclose(mx_values(codes, scales + 1, 4), mx_values(codes, scales, 4))
+
+
+# ---- the C entries, short of a GPU ------------------------------------------------
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from nebulasd_amd import _lib
+    from nebulasd_amd.build import build
+
+    if not _lib.LIB_PATH.exists():
+        build()
+    return _lib.load()
+
+
+def _sizes(lib, bits, rows, n_in):
+    c, s = ctypes.c_int64(-1), ctypes.c_int64(-1)
+    return lib.nsd_mx_bytes(bits, rows, n_in, ctypes.byref(c), ctypes.byref(s)), c.value, s.value
+
+
+def test_bytes(lib):
+    assert _sizes(lib, 4, 16, 128) == (0, 1024, 256)
+    assert _sizes(lib, 8, 16, 128) == (0, 2048, 256)
+    assert _sizes(lib, 4, 17, 544) == (0, 2 * 5 * 1024, 2 * 2 * 256)
+    assert _sizes(lib, 8, 0, 32) == (0, 0, 0)
+    assert _sizes(lib, 4, 151936, 4096) == (0, 151936 * 2048, 9496 * 8 * 256)
+
+
+@pytest.mark.parametrize("bits,rows,n_in,rc", [(4, 16, 48, 2), (4, 16, 0, 2), (8, -1, 32, 2), (5, 16, 32, 1),
+                                               (4, 2 ** 31, 32, 2), (8, 2 ** 31 - 1, 2 ** 31 - 32, 2)])
+def test_bytes_refuses(lib, bits, rows, n_in, rc):
+    from nebulasd_amd import _lib
+
+    assert _sizes(lib, bits, rows, n_in)[0] == rc and "mx_bytes" in _lib.last_error()
+
+
+def test_entries_refuse_before_any_launch(lib):
+    from nebulasd_amd import _lib
+
+    def refused(rc, got, text):
+        assert got == rc and text in _lib.last_error(), (got, _lib.last_error())
+
+    ok, odd = 4096, 4098  # never read: every call below is refused first
+    refused(1, lib.nsd_mxfp4_quantize(None, 0, 16, 32, ok, ok, None), "null")
+    refused(2, lib.nsd_mxfp4_quantize(ok, 7, 16, 32, ok, ok, None), "dtype=7")
+    refused(2, lib.nsd_mxfp4_quantize(ok, 0, 16, 33, ok, ok, None), "n_in=33")
+    refused(2, lib.nsd_mxfp4_quantize(odd, 0, 16, 32, ok, ok, None), "aligned")
+    refused(1, lib.nsd_mxfp4_pack(ok, None, 16, 32, ok, ok, None), "null")
+    refused(2, lib.nsd_mxfp8_quantize(ok, 16, 40, ok, ok, None), "n_in=40")
+    refused(2, lib.nsd_mxfp8_dequantize(ok, ok, 16, 32, ok, 3, None), "dtype=3")
+    refused(1, lib.nsd_mxfp4_linear(None, None, None, ok, ok, ok, 1, 16, 32, None, 0, None), "null")
+    refused(2, lib.nsd_mxfp4_linear(ok, None, None, ok, ok, odd, 1, 16, 32, None, 0, None), "aligned")
+    refused(2, lib.nsd_mxfp4_linear(ok, None, None, ok, ok, ok, 1, 0, 32, None, 0, None), "n_out=0")
+    refused(2, lib.nsd_mxfp4_linear(ok, None, None, ok, ok, ok, 2 ** 22, 16, 32, None, 0, None), "n_rows")
+    refused(2, lib.nsd_mxfp4_up_gate_silu_and_mul(ok, None, None, ok, ok, ok, 1, 24, 32, None, 0, None), "inter=24")
+    # no rows: nothing to launch
+    assert lib.nsd_mxfp4_linear(None, None, None, None, None, None, 0, 16, 32, None, 0, None) == 0
+    assert lib.nsd_mxfp4_quantize(None, 0, 0, 32, None, None, None) == 0
+
+
+def test_wrappers_refuse(lib):
+    from nebulasd_amd import kernels as K
+
+    x = torch.zeros(4, 64, dtype=torch.float16)
+    for f in (K.mxfp4_quantize, K.mxfp8_quantize):
+        with pytest.raises(ValueError, match="GPU tensors"):
+            f(x)
+    with pytest.raises(ValueError, match="GPU tensors"):
+        K.mxfp4_pack(torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8))
+
+
+def test_bound_covers_lost_products():
+    """A block whose largest product hides 31 others under 2^-15 of it: the bound allows all of them to be lost."""
+    x = np.full((1, 32), 2.0 ** -9, np.float16)
+    x[0, 0] = 448.0
+    w = np.full((1, 32), 0.5)
+    w[0, 0] = 6.0
+    lost = mx_linear(x, w)[0, 0] - 448.0 * 6
+    assert 0 < lost <= oracle.mx_linear_bound(x, w)[0, 0]
