@@ -11,6 +11,7 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef f16 f16x2 __attribute__((ext_vector_type(2)));
 typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kMxBlock = 32;         // values under one scale
@@ -66,6 +67,17 @@ __device__ inline f32x4 mx_mfma(i32x4 a, i32x4 b0, i32x4 b1, f32x4 c, int sa, in
   const i32x8 av = {a[0], a[1], a[2], a[3], 0, 0, 0, 0};
   const i32x8 bv = {b0[0], b0[1], b0[2], b0[3], b1[0], b1[1], b1[2], b1[3]};
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 0, 0, sa, 0, sb);
+}
+
+// v_mfma_scale_f32_32x32x64_f8f6f4 likewise: lane (i = lane % 32, g = lane / 32)
+// holds A[i][32g .. 32g+31], B's runs [16g .. 16g+15] and [32+16g .. 32+16g+15]
+// of column i, the scales (byte BYTE of sa and sb) of block g of row and column
+// i, and receives C[8q + 4g .. 8q + 4g + 3][i] in registers 4q .. 4q+3.
+template <int BYTE>
+__device__ inline f32x16 mx_mfma32(i32x4 a, i32x4 b0, i32x4 b1, f32x16 c, int sa, int sb) {
+  const i32x8 av = {a[0], a[1], a[2], a[3], 0, 0, 0, 0};
+  const i32x8 bv = {b0[0], b0[1], b0[2], b0[3], b1[0], b1[1], b1[2], b1[3]};
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c, 4, 0, BYTE, sa, BYTE, sb);
 }
 
 // Activations to MXFP8 (arguments checked by the caller); in nsd_mx.hip.

@@ -7,7 +7,9 @@
 namespace nsd {
 namespace {
 
-constexpr int64_t kMaxMxRows = 1 << 21;  // rows of one call
+// Rows and columns of one call, and values of its output: the kernels count
+// tiles and a tile's scale bytes in 32 bits.
+constexpr int64_t kMaxMxRows = 1 << 21, kMaxMxColumns = 1 << 27, kMaxMxOut = (int64_t)1 << 40;
 
 struct MxArgs {
   const u32x4* xc;     // x codes [row tiles][T][128] of 16 bytes
@@ -146,18 +148,219 @@ __global__ void __launch_bounds__(NWV* kWave) mx_stream_kernel(MxArgs a) {
   }
 }
 
+
+// ---- prompts ---------------------------------------------------------------
+
+template <int N>
+__device__ inline void mx_wait() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// 16 bytes a lane from base + 16 lane to LDS.
+__device__ inline void mx_dma(uint32_t lds_addr, const char* base, uint32_t offset) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(lds_addr), "v"(offset), "s"(base)
+               : "memory", "m0");
+}
+
+template <int WR_, int WC_, int FR_, int FC_, bool GATED_>
+struct MxTile {
+  static constexpr int WR = WR_, WC = WC_, FR = FR_, FC = FC_;  // waves and 32-wide fragments a wave, over rows and columns
+  static constexpr bool GATED = GATED_;
+  static constexpr int NW = WR * WC, XT = WR * FR * 2, WT = WC * FC * 2;  // 16-row tiles of x and of the weight
+  static constexpr int TM = XT * 16, TN = WT * 16, OUT = GATED ? TN / 2 : TN;
+  static constexpr int XI = 2 * XT / NW, WI = WT / NW;  // loads a wave of a step's codes, 1 KB each
+  static constexpr int R = 3, kStep = XT * kMxTile8 + WT * kMxTile4, kScales = (XT + WT) * kMxScaleTile;
+  static constexpr int kLds = R * kStep + 2 * kScales;
+  static_assert(XI * NW == 2 * XT && WI * NW == WT && (XT + WT) / 4 == NW && XT % 4 == 0 && kLds <= 160 * 1024);
+};
+
+template <class S>
+__global__ void __launch_bounds__(S::NW* kWave) mx_tile_kernel(MxArgs a, int m_tiles, int n_tiles) {
+  constexpr int FR = S::FR, FC = S::FC, NW = S::NW, XT = S::XT, WT = S::WT;
+  extern __shared__ __attribute__((aligned(16))) char lds_raw[];
+  lds_char* ring = (lds_char*)lds_raw;
+  lds_char* scales = ring + S::R * S::kStep;
+  const int lane = threadIdx.x & 63, l32 = lane & 31, lg = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wr = wave / S::WC, wc = wave % S::WC;
+  // workgroup i runs on XCD i % 8: each XCD a contiguous run of tiles, in bands
+  // of eight row tiles
+  const int total = m_tiles * n_tiles;
+  int id = blockIdx.x;
+  {
+    const int q = total / kXcds, r = total % kXcds, xcd = id % kXcds, at = id / kXcds;
+    id = xcd * q + min(xcd, r) + at;
+  }
+  constexpr int kBand = 8;
+  const int band = id / (kBand * n_tiles), rows_in = min(kBand, m_tiles - band * kBand);
+  const int in_band = id - band * kBand * n_tiles;
+  const int bm = band * kBand + in_band % rows_in, bn = in_band / rows_in;
+  const int T = a.T, out_tiles = (a.n + 15) / 16;
+
+  // this wave's loads of a step: chunks i NW + wave of x (two a tile) and of the weight
+  auto w_tile = [&](int j) {
+    if constexpr (!S::GATED) return min(bn * WT + j, out_tiles - 1);
+    constexpr int H = FC / 2;
+    const int c = j / (2 * FC), f = j / 2 % FC;
+    const int out = min(bn * (WT / 2) + (c * H + f % H) * 2 + j % 2, out_tiles - 1);
+    return f < H ? out : out + out_tiles;
+  };
+  const char* xsrc[S::XI];
+  const char* wsrc[S::WI];
+#pragma unroll
+  for (int i = 0; i < S::XI; ++i) {
+    const int q = i * NW + wave, tile = min(bm * XT + q / 2, a.row_tiles - 1);
+    xsrc[i] = reinterpret_cast<const char*>(a.xc) + (int64_t)tile * T * kMxTile8 + q % 2 * 1024;
+  }
+#pragma unroll
+  for (int i = 0; i < S::WI; ++i)
+    wsrc[i] = reinterpret_cast<const char*>(a.wc) + (int64_t)w_tile(i * NW + wave) * T * kMxTile4;
+  // scales of four steps: this wave's 1 KB is four tiles of x or of the weight
+  const bool sx = wave < XT / 4;
+  const int s_tile = sx ? min(bm * XT + wave * 4 + (lane >> 4), a.row_tiles - 1)
+                        : w_tile((wave - XT / 4) * 4 + (lane >> 4));
+  const char* ssrc = reinterpret_cast<const char*>(sx ? a.xs : a.ws);
+  const int64_t s_stride = (int64_t)(sx ? a.row_tiles : a.w_tiles) * kMxScaleTile;
+  const uint32_t s_off = (uint32_t)s_tile * kMxScaleTile + (lane & 15) * 16;
+
+  auto issue = [&](int t, int slot, auto with_scales) __attribute__((always_inline)) {
+    const uint32_t base = (uint32_t)(uintptr_t)(ring + slot * S::kStep);
+#pragma unroll
+    for (int i = 0; i < S::XI; ++i) mx_dma(base + (i * NW + wave) * 1024, xsrc[i] + (int64_t)t * kMxTile8, lane * 16);
+#pragma unroll
+    for (int i = 0; i < S::WI; ++i)
+      mx_dma(base + XT * kMxTile8 + (i * NW + wave) * 1024, wsrc[i] + (int64_t)t * kMxTile4, lane * 16);
+    if constexpr (decltype(with_scales)::value)
+      mx_dma((uint32_t)(uintptr_t)(scales + (t >> 2 & 1) * S::kScales + wave * 1024), ssrc + (t >> 2) * s_stride, s_off);
+  };
+
+  f32x16 acc[FC][FR];
+#pragma unroll
+  for (int j = 0; j < FC; ++j)
+#pragma unroll
+    for (int i = 0; i < FR; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[j][i][e] = 0.f;
+  uint32_t sw[FC][2], sxv[FR][2];  // scales of the wave's fragments, blocks lg and 2 + lg, four steps a word
+  // lane's place in a fragment: its row's 16-byte run in tile l32 / 16
+  const int row16 = (l32 & 15) * 16;
+  const int x_at = (l32 >> 4) * kMxTile8 + lg * 256 + row16, w_at = (l32 >> 4) * kMxTile4 + lg * 256 + row16;
+  const int s_at = (l32 >> 4) * kMxScaleTile + lg * 64 + (l32 & 15) * 4;
+
+  issue(0, 0, std::true_type{});
+  if (T > 1) issue(1, 1, std::false_type{});
+  int slot = 0, slot2 = 2;
+  for (int t0 = 0; t0 < T; t0 += 4) {
+    static_for<4>([&](auto uc) __attribute__((always_inline)) {
+      constexpr int u = decltype(uc)::value;
+      const int t = t0 + u;
+      if (t >= T) return;
+      // step t has landed: all but this wave's loads of step t + 1; then
+      // everybody's, and everybody is done with step t - 1
+      if (t + 1 < T) mx_wait<S::XI + S::WI + (u == 3 ? 1 : 0)>();
+      else mx_wait<0>();
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (t + 2 < T) issue(t + 2, slot2, std::bool_constant<u == 2>{});
+      const lds_char* xs = ring + slot * S::kStep + wr * FR * 2 * kMxTile8 + x_at;
+      const lds_char* wsl = ring + slot * S::kStep + XT * kMxTile8 + wc * FC * 2 * kMxTile4 + w_at;
+      slot = slot == 2 ? 0 : slot + 1;
+      slot2 = slot2 == 2 ? 0 : slot2 + 1;
+      if constexpr (u == 0) {
+        const lds_char* sc = scales + (t >> 2 & 1) * S::kScales + s_at;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+#pragma unroll
+          for (int i = 0; i < FR; ++i)
+            sxv[i][q] = *(const __attribute__((address_space(3))) uint32_t*)(sc + (wr * FR + i) * 2 * kMxScaleTile + q * 128);
+#pragma unroll
+          for (int j = 0; j < FC; ++j)
+            sw[j][q] = *(const __attribute__((address_space(3))) uint32_t*)(sc + (XT + (wc * FC + j) * 2) * kMxScaleTile + q * 128);
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {  // 64 k each
+        i32x4 x[FR][2], w[FC];
+#pragma unroll
+        for (int j = 0; j < FC; ++j)
+          w[j] = *(const __attribute__((address_space(3))) i32x4*)(wsl + j * 2 * kMxTile4 + q * 512);
+#pragma unroll
+        for (int i = 0; i < FR; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            x[i][h] = *(const __attribute__((address_space(3))) i32x4*)(xs + i * 2 * kMxTile8 + q * 1024 + h * 512);
+#pragma unroll
+        for (int i = 0; i < FR; ++i)
+#pragma unroll
+          for (int j = 0; j < FC; ++j)
+            acc[j][i] = mx_mfma32<u>(w[j], x[i][0], x[i][1], acc[j][i], sw[j][q], sxv[i][q]);
+      }
+    });
+  }
+
+  // lane (l32, lg): columns 8 q + 4 lg .. + 3 of a fragment, row l32
+  constexpr int H = S::GATED ? FC / 2 : FC;
+#pragma unroll
+  for (int i = 0; i < FR; ++i) {
+    const int m = bm * S::TM + (wr * FR + i) * 32 + l32;
+#pragma unroll
+    for (int j = 0; j < H; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int n0 = bn * S::OUT + (wc * H + j) * 32 + 8 * q + 4 * lg;
+        if (m >= a.rows || n0 >= a.n) continue;
+        f16x4 h;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float v = acc[j][i][4 * q + e];
+          if constexpr (S::GATED) {
+            const float g = acc[j + H][i][4 * q + e];
+            v *= g / (1.f + expf(-g));
+          }
+          h[e] = (f16)v;
+        }
+        f16* y = a.y + (int64_t)m * a.n + n0;
+        if (a.n % 4 == 0) {
+          *reinterpret_cast<f16x4*>(y) = h;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (n0 + e < a.n) y[e] = h[e];
+        }
+      }
+  }
+}
+
 struct MxConfig {
-  int jw = 2, splits = 1;
+  bool tile = false;  // mx_tile_kernel
+  int splits = 1;
 };
 
 MxConfig choose_mx(int64_t n_rows, int64_t n, int64_t T, bool gated, int cus) {
-  (void)n_rows;
+  (void)gated;
   (void)T;
   (void)cus;
   (void)n;
   MxConfig c;
-  c.jw = gated ? 2 : 1;
+  c.tile = n_rows > 128;
   return c;
+}
+
+// Raises a kernel's dynamic-LDS limit once per process.
+template <auto Kernel, int kLds>
+int allow_mx_lds() {
+  static const hipError_t attr =
+      hipFuncSetAttribute(reinterpret_cast<const void*>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+  return attr == hipSuccess ? NSD_OK : fail(NSD_ERR_HIP, "mxfp4: LDS attribute: %s", hipGetErrorString(attr));
+}
+
+template <class S>
+int launch_mx_tile(const MxArgs& a, hipStream_t st) {
+  if (int rc = allow_mx_lds<&mx_tile_kernel<S>, S::kLds>()) return rc;
+  const int m_tiles = (a.rows + S::TM - 1) / S::TM, n_tiles = (a.n + S::OUT - 1) / S::OUT;
+  hipLaunchKernelGGL(mx_tile_kernel<S>, dim3((unsigned)m_tiles * n_tiles), dim3(S::NW * kWave), S::kLds, st, a, m_tiles,
+                     n_tiles);
+  return launch_status(S::GATED ? "mxfp4_up_gate_silu_and_mul" : "mxfp4_linear");
 }
 
 template <int MT, int JW, bool GATED>
@@ -171,7 +374,11 @@ int launch_mx_stream(const MxArgs& a, hipStream_t st) {
 
 template <bool GATED>
 int launch_mx(const MxArgs& a, const MxConfig& c, hipStream_t st) {
-  (void)c;
+  if (c.tile) {
+    const int64_t big = (int64_t)((a.rows + 255) / 256) * ((a.n + (GATED ? 127 : 255)) / (GATED ? 128 : 256));
+    if (big >= 200) return launch_mx_tile<MxTile<4, 2, 2, 4, GATED>>(a, st);
+    return launch_mx_tile<MxTile<2, 2, 2, 2, GATED>>(a, st);
+  }
   switch (std::min(a.row_tiles, 4)) {
     case 1: return launch_mx_stream<1, GATED ? 2 : 1, GATED>(a, st);
     case 2: return launch_mx_stream<2, GATED ? 2 : 1, GATED>(a, st);
@@ -184,7 +391,7 @@ int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 
 int check_product(const char* who, int64_t n_rows, int64_t n, int64_t n_in) {
   int64_t c, s;
-  if (n_rows < 0 || n < 1 || n > INT32_MAX || n_rows > kMaxMxRows)
+  if (n_rows < 0 || n < 1 || n > kMaxMxColumns || n_rows > kMaxMxRows || n_rows * n > kMaxMxOut)
     return fail(NSD_ERR_UNSUPPORTED, "%s: n_rows=%lld, n_out=%lld", who, (long long)n_rows, (long long)n);
   if (int rc = nsd_mx_bytes(4, n, n_in, &c, &s)) return rc;
   return nsd_mx_bytes(8, n_rows, n_in, &c, &s);

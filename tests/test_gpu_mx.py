@@ -139,7 +139,8 @@ def _check(got, want, bound, extra=0.0):
 SHAPES = [(1, 16, 32), (1, 1024, 1024), (3, 17, 96), (16, 33, 128), (17, 1, 160), (32, 64, 512), (33, 1000, 544),
           (48, 250, 2080), (49, 4096, 256), (64, 6144, 1024), (65, 515, 4096), (80, 4096, 4096), (81, 96, 12288),
           (97, 2048, 2048), (112, 48, 8192), (113, 1001, 640), (128, 1024, 4096), (129, 300, 1024), (200, 1536, 608),
-          (257, 255, 2048), (513, 130, 1056), (1000, 1040, 512), (16, 20001, 256)]
+          (257, 255, 2048), (513, 130, 1056), (1000, 1040, 512), (16, 20001, 256),
+          (2049, 6500, 416), (1030, 13001, 96)]
 
 
 @pytest.mark.parametrize("rows,n,k", SHAPES, ids=[f"{r}x{n}x{k}" for r, n, k in SHAPES])
@@ -156,7 +157,8 @@ def test_linear_matches_oracle(gpu, rows, n, k):
 
 
 GATED = [(1, 16, 32), (1, 2816, 1024), (5, 48, 544), (16, 12288, 256), (33, 1024, 1056), (64, 2816, 1024),
-         (80, 1600, 4096), (100, 32, 8192), (128, 4096, 512), (129, 160, 1024), (300, 1040, 288), (700, 528, 2048)]
+         (80, 1600, 4096), (100, 32, 8192), (128, 4096, 512), (129, 160, 1024), (300, 1040, 288), (700, 528, 2048),
+         (1100, 6416, 288)]
 
 
 @pytest.mark.parametrize("rows,inter,k", GATED, ids=[f"{r}x{n}x{k}" for r, n, k in GATED])
