@@ -61,12 +61,17 @@ __device__ inline uint32_t mx8_block(const f16x8 (&h)[4], u32x4 (&out)[2]) {
 // v_mfma_scale_f32_16x16x128_f8f6f4 with A = E2M1, B = E4M3: lane (i = lane %
 // 16, g = lane / 16) holds A[i][32g .. 32g+31] in the first four registers,
 // and of B the two runs [16g .. 16g+15] and [64+16g .. 64+16g+15] of column i;
-// byte 0 of sa and sb is the scale of block g of row i and of column i.  It
+// byte BYTE of sa and sb is the scale of block g of row i and of column i.  It
 // receives C[4g .. 4g+3][i].
+//
+// The 32 products of a block are added aligned to the largest of them, whose
+// last kept place is 2^-15 of it (measured; a library product in fp16 rounds
+// its inputs no finer), blocks to each other and to C in fp32.
+template <int BYTE>
 __device__ inline f32x4 mx_mfma(i32x4 a, i32x4 b0, i32x4 b1, f32x4 c, int sa, int sb) {
   const i32x8 av = {a[0], a[1], a[2], a[3], 0, 0, 0, 0};
   const i32x8 bv = {b0[0], b0[1], b0[2], b0[3], b1[0], b1[1], b1[2], b1[3]};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 0, 0, sa, 0, sb);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 0, BYTE, sa, BYTE, sb);
 }
 
 // v_mfma_scale_f32_32x32x64_f8f6f4 likewise: lane (i = lane % 32, g = lane / 32)

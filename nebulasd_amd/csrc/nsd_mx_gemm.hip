@@ -10,6 +10,7 @@ namespace {
 // Rows and columns of one call, and values of its output: the kernels count
 // tiles and a tile's scale bytes in 32 bits.
 constexpr int64_t kMaxMxRows = 1 << 21, kMaxMxColumns = 1 << 27, kMaxMxOut = (int64_t)1 << 40;
+constexpr int64_t kMaxMxIn = 1 << 20;  // and a row tile's bytes
 
 struct MxArgs {
   const u32x4* xc;     // x codes [row tiles][T][128] of 16 bytes
@@ -24,40 +25,68 @@ struct MxArgs {
   int splits;
 };
 
-// Waves of a workgroup share its column tiles and split k: each streams its
-// range's weight tiles and x tiles straight into registers, D steps ahead, and
-// the sums meet in LDS at the end, in wave order.
-template <int MT, int JW, int NWV, int D, bool GATED>
-__global__ void __launch_bounds__(NWV* kWave) mx_stream_kernel(MxArgs a) {
-  constexpr int P = GATED ? JW / 2 : JW;  // column tiles of y
-  constexpr int NT = JW * MT;
-  constexpr int TPR = 64 / NWV < NT ? 64 / NWV : NT;  // tiles summed in one round through 64 KB of LDS
-  __shared__ f32x4 s_red[NWV * TPR * kWave];
+// ---- decode and verify batches -----------------------------------------------
+
+// A buffer whose loads past `bytes` give zeros: the streams below run ahead of
+// their range without a branch, so the loop's waits stay exact.
+__device__ inline __amdgpu_buffer_rsrc_t mx_buffer(const void* p, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00027000);
+}
+template <bool NT>
+__device__ inline i32x4 mx_load16(__amdgpu_buffer_rsrc_t r, int off) {
+  return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, NT ? 2 : 0));
+}
+
+constexpr int kMxWaves = 4;  // of a workgroup
+
+// MT row tiles by JW column tiles a workgroup (gated: the first half up tiles,
+// then their gate tiles).  Its four waves split k: each streams its range's
+// weight and x tiles straight into registers, two steps ahead, and multiplies
+// all MT x JW pairs, so no wave loads what another one has and no step waits
+// for another wave.  The sums meet in LDS at the end, added in wave order.
+template <int MT, int JW, bool GATED>
+struct MxStream {
+  static constexpr int P = GATED ? JW / 2 : JW, PER = GATED ? 2 : 1;  // column tiles of y, sums of one
+  static constexpr int YT = P * MT;
+  static constexpr int kLds = YT * (kMxWaves - 1) * PER * 1024;
+  static_assert(P * PER == JW && kLds <= 160 * 1024);
+};
+
+template <int MT, int JW, bool GATED>
+__global__ void __launch_bounds__(kMxWaves* kWave, 1) mx_stream_kernel(MxArgs a) {
+  using S = MxStream<MT, JW, GATED>;
+  constexpr int P = S::P, D = 2;
+  extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int out_tiles = (a.n + 15) / 16;
   const int groups = (out_tiles + P - 1) / P;
   const int group = blockIdx.x % groups, split = blockIdx.x / groups;
   const int rt0 = blockIdx.y * MT;
-  const int parts = a.splits * NWV, part = split * NWV + wave;
-  const int t0 = (int)((int64_t)part * a.T / parts), t1 = (int)((int64_t)(part + 1) * a.T / parts);
+  const int parts = a.splits * kMxWaves, part = split * kMxWaves + wave;
+  // a wave's steps [t0, t1), in whole fours (a scale word's tiles of k) where
+  // they come out even; ta: the four that t0 lies in, whose other steps are
+  // loaded and not multiplied
+  const int kgs = (a.T + 3) / 4;
+  const bool fours = kgs % parts == 0 || kgs >= 4 * parts;
+  const int units = fours ? kgs : a.T, per = fours ? 4 : 1;
+  const int t0 = (int)((int64_t)part * units / parts) * per;
+  const int t1 = min((int)((int64_t)(part + 1) * units / parts) * per, a.T);
+  const int ta = t0 & ~3;
 
-  const u32x4* wp[JW];
-  const uint32_t* wsp[JW];
+  __amdgpu_buffer_rsrc_t wb[JW], wsb[JW], xb[MT], xsb[MT];
 #pragma unroll
   for (int j = 0; j < JW; ++j) {
     int tile = min(group * P + j % P, out_tiles - 1);
     if (GATED && j >= P) tile += out_tiles;
-    wp[j] = a.wc + (int64_t)tile * a.T * 64 + lane;
-    wsp[j] = a.ws + (int64_t)tile * 64 + lane;
+    wb[j] = mx_buffer(a.wc + ((int64_t)tile * a.T + ta) * 64, (t1 - ta) * kMxTile4);
+    wsb[j] = mx_buffer(a.ws + (int64_t)tile * 64, ((kgs - 1) * a.w_tiles + 1) * kMxScaleTile);
   }
-  const u32x4* xp[MT];
-  const uint32_t* xsp[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
     const int tile = min(rt0 + i, a.row_tiles - 1);
-    xp[i] = a.xc + (int64_t)tile * a.T * 128 + lane;
-    xsp[i] = a.xs + (int64_t)tile * 64 + lane;
+    xb[i] = mx_buffer(a.xc + ((int64_t)tile * a.T + ta) * 128, (t1 - ta) * kMxTile8);
+    xsb[i] = mx_buffer(a.xs + (int64_t)tile * 64, ((kgs - 1) * a.row_tiles + 1) * kMxScaleTile);
   }
   f32x4 acc[JW][MT];
 #pragma unroll
@@ -65,42 +94,49 @@ __global__ void __launch_bounds__(NWV* kWave) mx_stream_kernel(MxArgs a) {
 #pragma unroll
     for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  u32x4 w[D][JW], x[D][MT][2];
-  uint32_t sw[D][JW], sx[D][MT];
+  i32x4 w[D][JW], x[D][MT][2];
+  int sw[2][JW], sx[2][MT];  // scales of this four tiles of k, and of the next
   auto load = [&](int u, int t) __attribute__((always_inline)) {
+    const int wo = (t - ta) * kMxTile4 + lane * 16, xo = (t - ta) * kMxTile8 + lane * 16;
 #pragma unroll
-    for (int j = 0; j < JW; ++j) {
-      w[u][j] = wp[j][(int64_t)t * 64];
-      sw[u][j] = wsp[j][(int64_t)(t >> 2) * a.w_tiles * 64];
-    }
+    for (int j = 0; j < JW; ++j) w[u][j] = mx_load16<true>(wb[j], wo);
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      x[u][i][0] = xp[i][(int64_t)t * 128];
-      x[u][i][1] = xp[i][(int64_t)t * 128 + 64];
-      sx[u][i] = xsp[i][(int64_t)(t >> 2) * a.row_tiles * 64];
+      x[u][i][0] = mx_load16<false>(xb[i], xo);
+      x[u][i][1] = mx_load16<false>(xb[i], xo + 1024);
     }
   };
+  auto load_scales = [&](int u, int kg) __attribute__((always_inline)) {
+    const int wo = kg * a.w_tiles * kMxScaleTile + lane * 4, xo = kg * a.row_tiles * kMxScaleTile + lane * 4;
 #pragma unroll
-  for (int u = 0; u < D; ++u)
-    if (t0 + u < t1) load(u, t0 + u);
-  for (int t = t0; t < t1; t += D) {
+    for (int j = 0; j < JW; ++j) sw[u][j] = __builtin_amdgcn_raw_buffer_load_b32(wsb[j], wo, 0, 0);
 #pragma unroll
-    for (int u = 0; u < D; ++u) {
-      if (t + u < t1) {
-        const int sh = 8 * ((t + u) & 3);
+    for (int i = 0; i < MT; ++i) sx[u][i] = __builtin_amdgcn_raw_buffer_load_b32(xsb[i], xo, 0, 0);
+  };
+  load_scales(0, ta >> 2);
+#pragma unroll
+  for (int u = 0; u < D; ++u) load(u, ta + u);
+  for (int t = ta; t < t1; t += 4) {
+    load_scales(1, (t >> 2) + 1);
+    static_for<4>([&](auto uc) __attribute__((always_inline)) {
+      constexpr int u = decltype(uc)::value, r = u % D;
+      if (t + u >= t0 && t + u < t1) {
 #pragma unroll
         for (int j = 0; j < JW; ++j)
 #pragma unroll
           for (int i = 0; i < MT; ++i)
-            acc[j][i] = mx_mfma(__builtin_bit_cast(i32x4, w[u][j]), __builtin_bit_cast(i32x4, x[u][i][0]),
-                                __builtin_bit_cast(i32x4, x[u][i][1]), acc[j][i], sw[u][j] >> sh, sx[u][i] >> sh);
-        if (t + u + D < t1) load(u, t + u + D);
+            acc[j][i] = mx_mfma<u>(w[r][j], x[r][i][0], x[r][i][1], acc[j][i], sw[0][j], sx[0][i]);
       }
-    }
+      load(r, t + u + D);
+    });
+#pragma unroll
+    for (int j = 0; j < JW; ++j) sw[0][j] = sw[1][j];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) sx[0][i] = sx[1][i];
   }
 
   // lane (li, lg) holds columns 4 lg .. 4 lg + 3 of a tile for row li
-  auto store = [&](int j, int i, f32x4 v, f32x4 gate) {
+  auto store = [&](int j, int i, f32x4 v, f32x4 gate) __attribute__((always_inline)) {
     const int m = 16 * (rt0 + i) + li, n0 = 16 * (group * P + j) + 4 * lg;
     if (m >= a.rows || n0 >= a.n) return;
     if constexpr (GATED) {
@@ -121,33 +157,39 @@ __global__ void __launch_bounds__(NWV* kWave) mx_stream_kernel(MxArgs a) {
         if (n0 + e < a.n) y[e] = h[e];
     }
   };
-  // rounds of whole y tiles: a gated one's up and gate sums in the same round
-  constexpr int PER = GATED ? 2 : 1, YT = P * MT, YPR = TPR / PER;
-#pragma unroll
-  for (int r = 0; r < YT; r += YPR) {
-    if (r) __syncthreads();
-#pragma unroll
-    for (int q = 0; q < YPR; ++q) {
-      if (r + q < YT) {
-        const int j = (r + q) / MT, i = (r + q) % MT;
-        s_red[(wave * TPR + q * PER) * kWave + lane] = acc[j][i];
-        if constexpr (GATED) s_red[(wave * TPR + q * PER + 1) * kWave + lane] = acc[j + P][i];
-      }
+  // y tile q is wave q % 4's to finish: it gets the others' sums through LDS
+  f32x4* red = reinterpret_cast<f32x4*>(lds_raw) + lane;
+  static_for<S::YT>([&](auto qc) __attribute__((always_inline)) {
+    constexpr int q = decltype(qc)::value, owner = q % kMxWaves;
+    if (wave != owner) {
+      f32x4* at = red + (q * (kMxWaves - 1) + wave - (wave > owner)) * S::PER * kWave;
+      at[0] = acc[q / MT][q % MT];
+      if constexpr (GATED) at[kWave] = acc[q / MT + P][q % MT];
     }
-    __syncthreads();
-    for (int q = wave; q < YPR && r + q < YT; q += NWV) {
-      f32x4 v = s_red[q * PER * kWave + lane], g = v;
-      if constexpr (GATED) g = s_red[(q * PER + 1) * kWave + lane];
-#pragma unroll
-      for (int o = 1; o < NWV; ++o) {
-        v += s_red[(o * TPR + q * PER) * kWave + lane];
-        if constexpr (GATED) g += s_red[(o * TPR + q * PER + 1) * kWave + lane];
-      }
-      store((r + q) / MT, (r + q) % MT, v, g);
+  });
+  __syncthreads();
+  static_for<S::YT>([&](auto qc) __attribute__((always_inline)) {
+    constexpr int q = decltype(qc)::value, owner = q % kMxWaves;
+    if (wave == owner) {
+      auto sum = [&](int per, f32x4 mine) __attribute__((always_inline)) {
+        f32x4 v;
+        static_for<kMxWaves>([&](auto oc) __attribute__((always_inline)) {
+          constexpr int o = decltype(oc)::value;
+          f32x4 part = mine;
+          if constexpr (o != owner)
+            part = red[((q * (kMxWaves - 1) + o - (o > owner ? 1 : 0)) * S::PER + per) * kWave];
+          if constexpr (o == 0) v = part;
+          else v += part;
+        });
+        return v;
+      };
+      const f32x4 v = sum(0, acc[q / MT][q % MT]);
+      f32x4 gate = v;
+      if constexpr (GATED) gate = sum(1, acc[q / MT + P][q % MT]);
+      store(q / MT, q % MT, v, gate);
     }
-  }
+  });
 }
-
 
 // ---- prompts ---------------------------------------------------------------
 
@@ -331,27 +373,59 @@ __global__ void __launch_bounds__(S::NW* kWave) mx_tile_kernel(MxArgs a, int m_t
   }
 }
 
-struct MxConfig {
-  bool tile = false;  // mx_tile_kernel
-  int splits = 1;
-};
-
-MxConfig choose_mx(int64_t n_rows, int64_t n, int64_t T, bool gated, int cus) {
-  (void)gated;
-  (void)T;
-  (void)cus;
-  (void)n;
-  MxConfig c;
-  c.tile = n_rows > 128;
-  return c;
-}
-
 // Raises a kernel's dynamic-LDS limit once per process.
 template <auto Kernel, int kLds>
 int allow_mx_lds() {
   static const hipError_t attr =
       hipFuncSetAttribute(reinterpret_cast<const void*>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
   return attr == hipSuccess ? NSD_OK : fail(NSD_ERR_HIP, "mxfp4: LDS attribute: %s", hipGetErrorString(attr));
+}
+
+struct MxConfig {
+  bool tile = false;  // mx_tile_kernel, else mx_stream_kernel with
+  int mt = 1, jw = 1, splits = 1;
+};
+
+// Column tiles a workgroup and splits of k over workgroups for the stream
+// kernel: the cheapest by a model of its time in ns.  A compute unit takes in
+// about 20 bytes a cycle of weight and x together while the weight comes from
+// memory, 21 ns a KB, however they mix, and all of them 6.1 TB/s of weight;
+// splits cost a pass that adds them, 2.5 us and their bytes.
+MxConfig choose_stream(int64_t n_rows, int64_t n, int64_t T, bool gated, int cus) {
+  MxConfig best;
+  const int64_t row_tiles = mx_row_tiles(n_rows), chunks = (row_tiles + 7) / 8;
+  best.mt = (int)((row_tiles + chunks - 1) / chunks);
+  const int64_t out_tiles = (n + 15) / 16;
+  double least = 1e300;
+  for (int jw : {1, 2, 3, 4, 6}) {
+    if (gated && jw % 2) continue;
+    const int p = gated ? jw / 2 : jw;
+    const int64_t groups = (out_tiles + p - 1) / p * chunks;
+    for (int splits : {1, 2, 3, 4, 6, 8}) {
+      // a wave has a step at least; sum_partials takes rows of whole vectors
+      if (splits > 1 && (gated || n % 8 || T < kMxWaves * splits)) break;
+      const int64_t wgs = groups * splits;
+      const double rounds = wgs <= 2 * cus ? (double)((wgs + cus - 1) / cus) : (double)wgs / cus + 0.5;
+      const double steps = (double)((T + splits - 1) / splits);
+      double t = std::max(rounds * steps * (jw + 2 * best.mt) * 21.0,
+                          (double)out_tiles * (gated ? 2 : 1) * T * chunks * kMxTile4 / 6100.0) +
+                 rounds * jw * best.mt * 50.0;
+      if (splits > 1) t += 2500.0 + (double)splits * n_rows * n * 8 / 5000.0;
+      if (t < least) {
+        least = t;
+        best.jw = jw;
+        best.splits = splits;
+      }
+    }
+  }
+  return best;
+}
+
+MxConfig choose_mx(int64_t n_rows, int64_t n, int64_t T, bool gated, int cus) {
+  if (n_rows <= 128) return choose_stream(n_rows, n, T, gated, cus);
+  MxConfig c;
+  c.tile = true;
+  return c;
 }
 
 template <class S>
@@ -365,26 +439,37 @@ int launch_mx_tile(const MxArgs& a, hipStream_t st) {
 
 template <int MT, int JW, bool GATED>
 int launch_mx_stream(const MxArgs& a, hipStream_t st) {
-  constexpr int P = GATED ? JW / 2 : JW;
-  const int groups = ((a.n + 15) / 16 + P - 1) / P;
-  hipLaunchKernelGGL((mx_stream_kernel<MT, JW, 4, 2, GATED>), dim3(groups * a.splits, (a.row_tiles + MT - 1) / MT),
-                     dim3(4 * kWave), 0, st, a);
+  using S = MxStream<MT, JW, GATED>;
+  if (int rc = allow_mx_lds<&mx_stream_kernel<MT, JW, GATED>, S::kLds>()) return rc;
+  const int groups = ((a.n + 15) / 16 + S::P - 1) / S::P;
+  hipLaunchKernelGGL((mx_stream_kernel<MT, JW, GATED>), dim3(groups * a.splits, (a.row_tiles + MT - 1) / MT),
+                     dim3(kMxWaves * kWave), S::kLds, st, a);
   return launch_status(GATED ? "mxfp4_up_gate_silu_and_mul" : "mxfp4_linear");
+}
+
+template <bool GATED, int... I>
+int launch_mx_rows(std::integer_sequence<int, I...>, const MxArgs& a, const MxConfig& c, hipStream_t st) {
+  int rc = NSD_ERR_UNSUPPORTED;
+  auto with = [&](auto mt) {
+    constexpr int MT = decltype(mt)::value;
+    if constexpr (!GATED) {
+      if (c.jw == 1) return launch_mx_stream<MT, 1, GATED>(a, st);
+      if (c.jw == 3) return launch_mx_stream<MT, 3, GATED>(a, st);
+    }
+    if (c.jw == 2) return launch_mx_stream<MT, 2, GATED>(a, st);
+    if (c.jw == 4) return launch_mx_stream<MT, 4, GATED>(a, st);
+    return launch_mx_stream<MT, 6, GATED>(a, st);
+  };
+  ((c.mt == I + 1 ? (rc = with(std::integral_constant<int, I + 1>{}), 0) : 0), ...);
+  return rc;
 }
 
 template <bool GATED>
 int launch_mx(const MxArgs& a, const MxConfig& c, hipStream_t st) {
-  if (c.tile) {
-    const int64_t big = (int64_t)((a.rows + 255) / 256) * ((a.n + (GATED ? 127 : 255)) / (GATED ? 128 : 256));
-    if (big >= 200) return launch_mx_tile<MxTile<4, 2, 2, 4, GATED>>(a, st);
-    return launch_mx_tile<MxTile<2, 2, 2, 2, GATED>>(a, st);
-  }
-  switch (std::min(a.row_tiles, 4)) {
-    case 1: return launch_mx_stream<1, GATED ? 2 : 1, GATED>(a, st);
-    case 2: return launch_mx_stream<2, GATED ? 2 : 1, GATED>(a, st);
-    case 3: return launch_mx_stream<3, GATED ? 2 : 1, GATED>(a, st);
-    default: return launch_mx_stream<4, GATED ? 2 : 1, GATED>(a, st);
-  }
+  if (!c.tile) return launch_mx_rows<GATED>(std::make_integer_sequence<int, 8>{}, a, c, st);
+  const int64_t big = (int64_t)((a.rows + 255) / 256) * ((a.n + (GATED ? 127 : 255)) / (GATED ? 128 : 256));
+  if (big >= 200) return launch_mx_tile<MxTile<4, 2, 2, 4, GATED>>(a, st);
+  return launch_mx_tile<MxTile<2, 2, 2, 2, GATED>>(a, st);
 }
 
 int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
@@ -393,8 +478,12 @@ int check_product(const char* who, int64_t n_rows, int64_t n, int64_t n_in) {
   int64_t c, s;
   if (n_rows < 0 || n < 1 || n > kMaxMxColumns || n_rows > kMaxMxRows || n_rows * n > kMaxMxOut)
     return fail(NSD_ERR_UNSUPPORTED, "%s: n_rows=%lld, n_out=%lld", who, (long long)n_rows, (long long)n);
-  if (int rc = nsd_mx_bytes(4, n, n_in, &c, &s)) return rc;
-  return nsd_mx_bytes(8, n_rows, n_in, &c, &s);
+  if (n_in > kMaxMxIn) return fail(NSD_ERR_UNSUPPORTED, "%s: n_in=%lld > %lld", who, (long long)n_in, (long long)kMaxMxIn);
+  for (auto [bits, rows] : {std::pair<int, int64_t>{4, n}, {8, n_rows}}) {
+    if (int rc = nsd_mx_bytes(bits, rows, n_in, &c, &s)) return rc;
+    if (s > INT32_MAX) return fail(NSD_ERR_UNSUPPORTED, "%s: %lld bytes of scales", who, (long long)s);
+  }
+  return NSD_OK;
 }
 
 // The workspace: the rows' codes and scales, when x is fp16, then the partials.
