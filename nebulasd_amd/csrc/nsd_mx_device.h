@@ -24,38 +24,79 @@ constexpr uint8_t kMxNanScale = 255;
 inline __host__ __device__ int64_t mx_row_tiles(int64_t rows) { return (rows + 15) / 16; }
 inline __host__ __device__ int64_t mx_k_tiles(int64_t n_in) { return (n_in + kMxTileK - 1) / kMxTileK; }
 
-// The 32 fp16 values h as one E4M3 block: its codes, 16 a register quad, and
-// its scale byte.  The largest magnitude m = f 2^p (1 <= f < 2) takes 2^(p-8) up
-// to f = 1.75 = 448 / 256 and 2^(p-7) above, so no value saturates.
-__device__ inline uint32_t mx8_block(const f16x8 (&h)[4], u32x4 (&out)[2]) {
-  u16x8 most = __builtin_bit_cast(u16x8, h[0]) & (uint16_t)0x7fff;
+// Scale byte of an E4M3 block whose largest magnitude has the fp16 bits m, and
+// its power of two: m = f 2^p (1 <= f < 2) takes 2^(p-8) up to f = 1.75 = 448 /
+// 256 and 2^(p-7) above, so no value saturates.  Of a block of zeros the byte
+// is 0, of one with an infinity or a NaN 255 (its codes mean nothing).
+__device__ inline uint32_t mx8_scale(uint32_t m, float* power) {
+  const uint32_t f = __builtin_bit_cast(uint32_t, (float)__builtin_bit_cast(f16, (uint16_t)m));
+  const uint32_t s = (f >> 23) - 8 + ((f & 0x7fffffu) > 0x600000u);
+  const bool plain = m != 0 && m < 0x7c00u;
+  *power = plain ? __builtin_bit_cast(float, s << 23) : 1.f;
+  return plain ? s : m ? kMxNanScale : 0;
+}
+// Eight values over 2^power as codes.
+__device__ inline u32x2 mx8_codes(f16x8 h, float power) {
+  u32x2 out;
 #pragma unroll
-  for (int q = 1; q < 4; ++q) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x8, h[q]) & (uint16_t)0x7fff);
+  for (int q = 0; q < 2; ++q) {
+    s16x2 c = {0, 0};
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(c, f16x2{h[4 * q], h[4 * q + 1]}, power, false);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(c, f16x2{h[4 * q + 2], h[4 * q + 3]}, power, true);
+    out[q] = __builtin_bit_cast(uint32_t, c);
+  }
+  return out;
+}
+// |bits| of eight values; the largest of eight.
+__device__ inline u16x8 mx_abs_bits(f16x8 h) { return __builtin_bit_cast(u16x8, h) & (uint16_t)0x7fff; }
+__device__ inline uint32_t mx_largest(u16x8 v) {
   uint32_t m = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) m = max(m, (uint32_t)most[e]);
-  uint32_t s = 0;
-  float scale = 1.f;  // of a block of zeros, whose scale byte is 0
-  if (m != 0) {
-    const uint32_t f = __builtin_bit_cast(uint32_t, (float)__builtin_bit_cast(f16, (uint16_t)m));
-    s = (f >> 23) - 8 + ((f & 0x7fffffu) > 0x600000u);
-    scale = __builtin_bit_cast(float, s << 23);
-  }
-  if (m >= 0x7c00u) {
-    s = kMxNanScale;
-    out[0] = out[1] = u32x4{0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu};
-    return s;
-  }
+  for (int e = 0; e < 8; ++e) m = max(m, (uint32_t)v[e]);
+  return m;
+}
+
+// The 32 fp16 values h as one E4M3 block: its codes, 16 a register quad, and
+// its scale byte.
+__device__ inline uint32_t mx8_block(const f16x8 (&h)[4], u32x4 (&out)[2]) {
+  u16x8 most = mx_abs_bits(h[0]);
 #pragma unroll
-  for (int q = 0; q < 8; ++q) {
-    const f16x2 a = {h[q / 2][q % 2 * 4], h[q / 2][q % 2 * 4 + 1]};
-    const f16x2 b = {h[q / 2][q % 2 * 4 + 2], h[q / 2][q % 2 * 4 + 3]};
-    s16x2 c = {0, 0};
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(c, a, scale, false);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(c, b, scale, true);
-    out[q / 4][q % 4] = __builtin_bit_cast(uint32_t, c);
+  for (int q = 1; q < 4; ++q) most = __builtin_elementwise_max(most, mx_abs_bits(h[q]));
+  float power;
+  const uint32_t s = mx8_scale(mx_largest(most), &power);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const u32x2 c = mx8_codes(h[q], power);
+    out[q / 2][q % 2 * 2] = s == kMxNanScale ? 0x7f7f7f7fu : c[0];
+    out[q / 2][q % 2 * 2 + 1] = s == kMxNanScale ? 0x7f7f7f7fu : c[1];
   }
   return s;
+}
+
+// A lane's share of a 16 x 128 tile of fp16 rows as the MFMA's B operand: h[0],
+// h[1] the run of 16 k at 16 g, h[2], h[3] the one at 64 + 16 g (g = lane /
+// 16).  A block is such a run in each of two neighbouring groups, so its
+// largest value needs one exchange (of rows of 16 lanes); the first halves hold
+// the blocks 0, 0, 1, 1 and the second 2, 2, 3, 3, and the scale operand wants
+// block g from group g: one exchange of half waves.
+__device__ inline int mx8_operand(const f16x8 (&h)[4], int lane, i32x4& b0, i32x4& b1) {
+  const uint32_t lo = mx_largest(__builtin_elementwise_max(mx_abs_bits(h[0]), mx_abs_bits(h[1])));
+  const uint32_t hi = mx_largest(__builtin_elementwise_max(mx_abs_bits(h[2]), mx_abs_bits(h[3])));
+  const uint32_t both = lo | hi << 16;
+  const auto sw = __builtin_amdgcn_permlane16_swap(both, both, false, false);  // each group and its neighbour
+  float p0, p1;
+  const uint32_t s0 = mx8_scale(max(sw[0] & 0xffffu, sw[1] & 0xffffu), &p0);
+  const uint32_t s1 = mx8_scale(max(sw[0] >> 16, sw[1] >> 16), &p1);
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const u32x2 c = mx8_codes(h[q], p0), d = mx8_codes(h[q + 2], p1);
+    b0[2 * q] = (int)c[0];
+    b0[2 * q + 1] = (int)c[1];
+    b1[2 * q] = (int)d[0];
+    b1[2 * q + 1] = (int)d[1];
+  }
+  const auto ss = __builtin_amdgcn_permlane32_swap(s0, s1, false, false);
+  return (int)(lane & 16 ? ss[1] : ss[0]);
 }
 
 // v_mfma_scale_f32_16x16x128_f8f6f4 with A = E2M1, B = E4M3: lane (i = lane %

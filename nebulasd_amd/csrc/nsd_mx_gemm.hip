@@ -13,6 +13,7 @@ constexpr int64_t kMaxMxRows = 1 << 21, kMaxMxColumns = 1 << 27, kMaxMxOut = (in
 constexpr int64_t kMaxMxIn = 1 << 20;  // and a row tile's bytes
 
 struct MxArgs {
+  const f16* x;        // x [rows][n_in], or null with
   const u32x4* xc;     // x codes [row tiles][T][128] of 16 bytes
   const uint32_t* xs;  // x scales [ceil(T / 4)][row tiles][64]
   const u32x4* wc;     // weight codes [column tiles][T][64]
@@ -20,7 +21,7 @@ struct MxArgs {
   f16* y;
   float* part;  // [splits][rows][n], when splits > 1
   int rows, n;  // n: columns of y
-  int T;        // tiles of k
+  int n_in, T;  // T: tiles of k
   int row_tiles, w_tiles;
   int splits;
 };
@@ -37,13 +38,17 @@ __device__ inline i32x4 mx_load16(__amdgpu_buffer_rsrc_t r, int off) {
   return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, NT ? 2 : 0));
 }
 
-constexpr int kMxWaves = 4;  // of a workgroup
+constexpr int kMxWaves = 4;             // of a workgroup
+constexpr int kMxNowhere = 0x40000000;  // an offset past every buffer's end
+constexpr int kMxFp16Tiles = 2;         // row tiles of the fp16 form
 
 // MT row tiles by JW column tiles a workgroup (gated: the first half up tiles,
 // then their gate tiles).  Its four waves split k: each streams its range's
 // weight and x tiles straight into registers, two steps ahead, and multiplies
 // all MT x JW pairs, so no wave loads what another one has and no step waits
 // for another wave.  The sums meet in LDS at the end, added in wave order.
+// FP16: x as it is, cut into blocks between load and product.  NT: the weight
+// past the caches.
 template <int MT, int JW, bool GATED>
 struct MxStream {
   static constexpr int P = GATED ? JW / 2 : JW, PER = GATED ? 2 : 1;  // column tiles of y, sums of one
@@ -52,7 +57,7 @@ struct MxStream {
   static_assert(P * PER == JW && kLds <= 160 * 1024);
 };
 
-template <int MT, int JW, bool GATED>
+template <int MT, int JW, bool GATED, bool FP16, bool NT>
 __global__ void __launch_bounds__(kMxWaves* kWave, 1) mx_stream_kernel(MxArgs a) {
   using S = MxStream<MT, JW, GATED>;
   constexpr int P = S::P, D = 2;
@@ -73,6 +78,7 @@ __global__ void __launch_bounds__(kMxWaves* kWave, 1) mx_stream_kernel(MxArgs a)
   const int t0 = (int)((int64_t)part * units / parts) * per;
   const int t1 = min((int)((int64_t)(part + 1) * units / parts) * per, a.T);
   const int ta = t0 & ~3;
+  [[maybe_unused]] const int k_end = min(t1 * kMxTileK, a.n_in);
 
   __amdgpu_buffer_rsrc_t wb[JW], wsb[JW], xb[MT], xsb[MT];
 #pragma unroll
@@ -85,8 +91,12 @@ __global__ void __launch_bounds__(kMxWaves* kWave, 1) mx_stream_kernel(MxArgs a)
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
     const int tile = min(rt0 + i, a.row_tiles - 1);
-    xb[i] = mx_buffer(a.xc + ((int64_t)tile * a.T + ta) * 128, (t1 - ta) * kMxTile8);
-    xsb[i] = mx_buffer(a.xs + (int64_t)tile * 64, ((kgs - 1) * a.row_tiles + 1) * kMxScaleTile);
+    if constexpr (FP16) {  // rows past the last: zeros
+      xb[i] = mx_buffer(a.x + (int64_t)tile * 16 * a.n_in, min(a.rows - tile * 16, 16) * a.n_in * 2);
+    } else {
+      xb[i] = mx_buffer(a.xc + ((int64_t)tile * a.T + ta) * 128, (t1 - ta) * kMxTile8);
+      xsb[i] = mx_buffer(a.xs + (int64_t)tile * 64, ((kgs - 1) * a.row_tiles + 1) * kMxScaleTile);
+    }
   }
   f32x4 acc[JW][MT];
 #pragma unroll
@@ -94,24 +104,40 @@ __global__ void __launch_bounds__(kMxWaves* kWave, 1) mx_stream_kernel(MxArgs a)
 #pragma unroll
     for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  i32x4 w[D][JW], x[D][MT][2];
+  constexpr int XV = FP16 ? 4 : 2;
+  i32x4 w[D][JW], x[D][MT][XV];
   int sw[2][JW], sx[2][MT];  // scales of this four tiles of k, and of the next
   auto load = [&](int u, int t) __attribute__((always_inline)) {
     const int wo = (t - ta) * kMxTile4 + lane * 16, xo = (t - ta) * kMxTile8 + lane * 16;
 #pragma unroll
-    for (int j = 0; j < JW; ++j) w[u][j] = mx_load16<true>(wb[j], wo);
+    for (int j = 0; j < JW; ++j) w[u][j] = mx_load16<NT>(wb[j], wo);
+    if constexpr (FP16) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      x[u][i][0] = mx_load16<false>(xb[i], xo);
-      x[u][i][1] = mx_load16<false>(xb[i], xo + 1024);
+      for (int h = 0; h < 2; ++h) {  // the runs of 16 k at 16 lg and 64 + 16 lg; past the row or the range: zeros
+        const int k = t * kMxTileK + h * 64 + lg * 16;
+        const int off = k < k_end ? (li * a.n_in + k) * 2 : kMxNowhere;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          x[u][i][2 * h] = mx_load16<false>(xb[i], off);
+          x[u][i][2 * h + 1] = mx_load16<false>(xb[i], off + 16);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        x[u][i][0] = mx_load16<false>(xb[i], xo);
+        x[u][i][1] = mx_load16<false>(xb[i], xo + 1024);
+      }
     }
   };
   auto load_scales = [&](int u, int kg) __attribute__((always_inline)) {
     const int wo = kg * a.w_tiles * kMxScaleTile + lane * 4, xo = kg * a.row_tiles * kMxScaleTile + lane * 4;
 #pragma unroll
     for (int j = 0; j < JW; ++j) sw[u][j] = __builtin_amdgcn_raw_buffer_load_b32(wsb[j], wo, 0, 0);
+    if constexpr (!FP16) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i) sx[u][i] = __builtin_amdgcn_raw_buffer_load_b32(xsb[i], xo, 0, 0);
+      for (int i = 0; i < MT; ++i) sx[u][i] = __builtin_amdgcn_raw_buffer_load_b32(xsb[i], xo, 0, 0);
+    }
   };
   load_scales(0, ta >> 2);
 #pragma unroll
@@ -122,17 +148,30 @@ __global__ void __launch_bounds__(kMxWaves* kWave, 1) mx_stream_kernel(MxArgs a)
       constexpr int u = decltype(uc)::value, r = u % D;
       if (t + u >= t0 && t + u < t1) {
 #pragma unroll
-        for (int j = 0; j < JW; ++j)
+        for (int i = 0; i < MT; ++i) {
+          i32x4 b0, b1;
+          int sb;
+          if constexpr (FP16) {
+            const f16x8 h[4] = {__builtin_bit_cast(f16x8, x[r][i][0]), __builtin_bit_cast(f16x8, x[r][i][1]),
+                                __builtin_bit_cast(f16x8, x[r][i][2]), __builtin_bit_cast(f16x8, x[r][i][3])};
+            sb = mx8_operand(h, lane, b0, b1) << 8 * u;
+          } else {
+            b0 = x[r][i][0];
+            b1 = x[r][i][1];
+            sb = sx[0][i];
+          }
 #pragma unroll
-          for (int i = 0; i < MT; ++i)
-            acc[j][i] = mx_mfma<u>(w[r][j], x[r][i][0], x[r][i][1], acc[j][i], sw[0][j], sx[0][i]);
+          for (int j = 0; j < JW; ++j) acc[j][i] = mx_mfma<u>(w[r][j], b0, b1, acc[j][i], sw[0][j], sb);
+        }
       }
       load(r, t + u + D);
     });
 #pragma unroll
     for (int j = 0; j < JW; ++j) sw[0][j] = sw[1][j];
+    if constexpr (!FP16) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i) sx[0][i] = sx[1][i];
+      for (int i = 0; i < MT; ++i) sx[0][i] = sx[1][i];
+    }
   }
 
   // lane (li, lg) holds columns 4 lg .. 4 lg + 3 of a tile for row li
@@ -384,45 +423,64 @@ int allow_mx_lds() {
 struct MxConfig {
   bool tile = false;  // mx_tile_kernel, else mx_stream_kernel with
   int mt = 1, jw = 1, splits = 1;
+  bool fp16 = false;  // reads x as it is
+  bool nt = false;    // the weight past the caches
 };
 
-// Column tiles a workgroup and splits of k over workgroups for the stream
-// kernel: the cheapest by a model of its time in ns.  A compute unit takes in
-// about 20 bytes a cycle of weight and x together while the weight comes from
-// memory, 21 ns a KB, however they mix, and all of them 6.1 TB/s of weight;
-// splits cost a pass that adds them, 2.5 us and their bytes.
-MxConfig choose_stream(int64_t n_rows, int64_t n, int64_t T, bool gated, int cus) {
+// Column tiles a workgroup, splits of k over workgroups and the form of x for
+// the stream kernel: the cheapest by a model of its time in ns.
+//   - A compute unit takes in weight and x together, however they mix, a KB in
+//     21 ns where two workgroups share it or it has one to run, in 28 where
+//     one's registers leave no room for another; all of them take in 6.1 TB/s
+//     of weight at most.
+//   - A workgroup's end, its sums through LDS, takes 50 ns a tile.
+//   - Splits cost a pass that adds them: 2.5 us and their bytes.
+//   - x as fp16 is twice the bytes to every workgroup, and saves the pass that
+//     cuts it into blocks, 4 us with its launch.
+MxConfig choose_stream(int64_t n_rows, int64_t n, int64_t T, bool gated, bool quantised, int cus) {
   MxConfig best;
   const int64_t row_tiles = mx_row_tiles(n_rows), chunks = (row_tiles + 7) / 8;
-  best.mt = (int)((row_tiles + chunks - 1) / chunks);
+  const int mt = (int)((row_tiles + chunks - 1) / chunks);
   const int64_t out_tiles = (n + 15) / 16;
   double least = 1e300;
-  for (int jw : {1, 2, 3, 4, 6}) {
-    if (gated && jw % 2) continue;
-    const int p = gated ? jw / 2 : jw;
-    const int64_t groups = (out_tiles + p - 1) / p * chunks;
-    for (int splits : {1, 2, 3, 4, 6, 8}) {
-      // a wave has a step at least; sum_partials takes rows of whole vectors
-      if (splits > 1 && (gated || n % 8 || T < kMxWaves * splits)) break;
-      const int64_t wgs = groups * splits;
-      const double rounds = wgs <= 2 * cus ? (double)((wgs + cus - 1) / cus) : (double)wgs / cus + 0.5;
-      const double steps = (double)((T + splits - 1) / splits);
-      double t = std::max(rounds * steps * (jw + 2 * best.mt) * 21.0,
-                          (double)out_tiles * (gated ? 2 : 1) * T * chunks * kMxTile4 / 6100.0) +
-                 rounds * jw * best.mt * 50.0;
-      if (splits > 1) t += 2500.0 + (double)splits * n_rows * n * 8 / 5000.0;
-      if (t < least) {
-        least = t;
-        best.jw = jw;
-        best.splits = splits;
+  for (int fp16 = 0; fp16 <= (!quantised && row_tiles <= kMxFp16Tiles ? 1 : 0); ++fp16)
+    for (int jw : {1, 2, 3, 4, 6}) {
+      if (gated && jw % 2) continue;
+      const int p = gated ? jw / 2 : jw;
+      const int64_t groups = (out_tiles + p - 1) / p * chunks;
+      const bool two = 4 * jw * mt + (fp16 ? 34 : 18) * mt + 11 * jw + 12 <= 252;
+      for (int splits : {1, 2, 3, 4, 6, 8}) {
+        // a wave has a step at least; sum_partials takes rows of whole vectors
+        if (splits > 1 && (gated || n % 8 || T < kMxWaves * splits)) break;
+        const int64_t wgs = groups * splits;
+        const double rounds = wgs <= 2 * cus ? (double)((wgs + cus - 1) / cus) : (double)wgs / cus + 0.5;
+        const double steps = (double)((T + splits - 1) / splits);
+        // rows of x that exist: the others of a tile are not fetched as fp16
+        const double x_kb = fp16 ? n_rows * 0.25 : 2.0 * mt;
+        double t = std::max(rounds * steps * (jw + x_kb) * (wgs > cus && !two ? 28.0 : 21.0),
+                            (double)out_tiles * (gated ? 2 : 1) * T * chunks * kMxTile4 / 6100.0) +
+                   rounds * jw * mt * 50.0;
+        if (splits > 1) t += 2500.0 + (double)splits * n_rows * n * 8 / 5000.0;
+        if (!fp16 && !quantised) t += 4000.0;
+        if (t < least) {
+          least = t;
+          best.mt = mt;
+          best.jw = jw;
+          best.splits = splits;
+          best.fp16 = fp16 != 0;
+        }
       }
     }
-  }
+  // A weight that the 256 MB last-level cache cannot keep from call to call
+  // streams faster past it: 330 MB, 16 rows 64.9 -> 59.7 us; one that it keeps
+  // (13 to 53 MB, called again and again) slower, 3.7 -> 5.5 and 15.1 -> 16.9,
+  // and neither way among other weights.
+  best.nt = (double)out_tiles * (gated ? 2 : 1) * T * kMxTile4 > 192e6;
   return best;
 }
 
-MxConfig choose_mx(int64_t n_rows, int64_t n, int64_t T, bool gated, int cus) {
-  if (n_rows <= 128) return choose_stream(n_rows, n, T, gated, cus);
+MxConfig choose_mx(int64_t n_rows, int64_t n, int64_t T, bool gated, bool quantised, int cus) {
+  if (n_rows <= 128) return choose_stream(n_rows, n, T, gated, quantised, cus);
   MxConfig c;
   c.tile = true;
   return c;
@@ -437,14 +495,21 @@ int launch_mx_tile(const MxArgs& a, hipStream_t st) {
   return launch_status(S::GATED ? "mxfp4_up_gate_silu_and_mul" : "mxfp4_linear");
 }
 
-template <int MT, int JW, bool GATED>
+template <int MT, int JW, bool GATED, bool FP16, bool NT>
 int launch_mx_stream(const MxArgs& a, hipStream_t st) {
   using S = MxStream<MT, JW, GATED>;
-  if (int rc = allow_mx_lds<&mx_stream_kernel<MT, JW, GATED>, S::kLds>()) return rc;
+  if (int rc = allow_mx_lds<&mx_stream_kernel<MT, JW, GATED, FP16, NT>, S::kLds>()) return rc;
   const int groups = ((a.n + 15) / 16 + S::P - 1) / S::P;
-  hipLaunchKernelGGL((mx_stream_kernel<MT, JW, GATED>), dim3(groups * a.splits, (a.row_tiles + MT - 1) / MT),
+  hipLaunchKernelGGL((mx_stream_kernel<MT, JW, GATED, FP16, NT>), dim3(groups * a.splits, (a.row_tiles + MT - 1) / MT),
                      dim3(kMxWaves * kWave), S::kLds, st, a);
   return launch_status(GATED ? "mxfp4_up_gate_silu_and_mul" : "mxfp4_linear");
+}
+template <int MT, int JW, bool GATED>
+int launch_mx_stream(const MxArgs& a, const MxConfig& c, hipStream_t st) {
+  if constexpr (MT <= kMxFp16Tiles)
+    if (c.fp16)
+      return c.nt ? launch_mx_stream<MT, JW, GATED, true, true>(a, st) : launch_mx_stream<MT, JW, GATED, true, false>(a, st);
+  return c.nt ? launch_mx_stream<MT, JW, GATED, false, true>(a, st) : launch_mx_stream<MT, JW, GATED, false, false>(a, st);
 }
 
 template <bool GATED, int... I>
@@ -453,12 +518,12 @@ int launch_mx_rows(std::integer_sequence<int, I...>, const MxArgs& a, const MxCo
   auto with = [&](auto mt) {
     constexpr int MT = decltype(mt)::value;
     if constexpr (!GATED) {
-      if (c.jw == 1) return launch_mx_stream<MT, 1, GATED>(a, st);
-      if (c.jw == 3) return launch_mx_stream<MT, 3, GATED>(a, st);
+      if (c.jw == 1) return launch_mx_stream<MT, 1, GATED>(a, c, st);
+      if (c.jw == 3) return launch_mx_stream<MT, 3, GATED>(a, c, st);
     }
-    if (c.jw == 2) return launch_mx_stream<MT, 2, GATED>(a, st);
-    if (c.jw == 4) return launch_mx_stream<MT, 4, GATED>(a, st);
-    return launch_mx_stream<MT, 6, GATED>(a, st);
+    if (c.jw == 2) return launch_mx_stream<MT, 2, GATED>(a, c, st);
+    if (c.jw == 4) return launch_mx_stream<MT, 4, GATED>(a, c, st);
+    return launch_mx_stream<MT, 6, GATED>(a, c, st);
   };
   ((c.mt == I + 1 ? (rc = with(std::integral_constant<int, I + 1>{}), 0) : 0), ...);
   return rc;
@@ -493,7 +558,7 @@ struct MxWorkspace {
 };
 MxWorkspace mx_workspace(int64_t n_rows, int64_t n, int64_t n_in, bool quantised, const MxConfig& c) {
   MxWorkspace w;
-  if (!quantised) (void)nsd_mx_bytes(8, n_rows, n_in, &w.codes, &w.scales);
+  if (!quantised && !c.fp16) (void)nsd_mx_bytes(8, n_rows, n_in, &w.codes, &w.scales);
   if (c.splits > 1) w.partials = c.splits * n_rows * n * (int64_t)sizeof(float);
   return w;
 }
@@ -512,19 +577,21 @@ int product(const char* who, const void* x, const void* x_codes, const void* x_s
   int cus = 0;
   if (int rc = device_cus(&cus)) return rc;
   const int64_t T = mx_k_tiles(n_in);
-  const MxConfig c = choose_mx(n_rows, n, T, GATED, cus);
+  const MxConfig c = choose_mx(n_rows, n, T, GATED, x == nullptr, cus);
   const MxWorkspace need = mx_workspace(n_rows, n, n_in, x == nullptr, c);
   if (workspace_bytes < need.total() || (need.total() > 0 && !workspace))
     return fail(NSD_ERR_WORKSPACE, "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes,
                 (long long)need.total());
   char* ws = static_cast<char*>(workspace);
-  if (x) {
+  if (x && !c.fp16) {
     void *codes = ws, *scales = ws + align256(need.codes);
     if (int rc = mxfp8_quantize(x, n_rows, n_in, codes, scales, stream)) return rc;
     x_codes = codes;
     x_scales = scales;
   }
   MxArgs a{};
+  a.x = static_cast<const f16*>(x);
+  a.n_in = (int)n_in;
   a.xc = static_cast<const u32x4*>(x_codes);
   a.xs = static_cast<const uint32_t*>(x_scales);
   a.wc = static_cast<const u32x4*>(w_codes);
@@ -554,7 +621,7 @@ extern "C" int nsd_mx_workspace(int64_t n_rows, int64_t n_out, int64_t n_in, int
   int cus = 0;
   if (int rc = device_cus(&cus)) return rc;
   const int64_t n = gated ? n_out / 2 : n_out;
-  *bytes = mx_workspace(n_rows, n, n_in, quantised != 0, choose_mx(n_rows, n, mx_k_tiles(n_in), gated != 0, cus)).total();
+  *bytes = mx_workspace(n_rows, n, n_in, quantised != 0, choose_mx(n_rows, n, mx_k_tiles(n_in), gated != 0, quantised != 0, cus)).total();
   return NSD_OK;
 }
 

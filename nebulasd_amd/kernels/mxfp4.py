@@ -31,6 +31,15 @@ BLOCK = 32
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
 
+def _check_blocks(codes, scales, bits: int, rows: int, n_in: int) -> None:
+    c, s = _bytes(bits, rows, n_in)
+    for t, n in ((codes, c), (scales, s)):
+        if t.dtype != torch.uint8 or not t.is_contiguous() or t.numel() != n:
+            raise ValueError(f"[{rows}, {n_in}] in MXFP{bits} is {c} bytes of codes and {s} of scales")
+    require_cuda(codes, scales)
+    _same_device(codes, scales)
+
+
 @dataclasses.dataclass(frozen=True)
 class MXFP4Weight:
     """A weight [n_out, n_in] in MXFP4: codes and scales (uint8) in the kernels' layout."""
@@ -39,6 +48,9 @@ class MXFP4Weight:
     scales: torch.Tensor
     n_out: int
     n_in: int
+
+    def __post_init__(self):
+        _check_blocks(self.codes, self.scales, 4, self.n_out, self.n_in)
 
 
 @dataclasses.dataclass(frozen=True)
@@ -49,6 +61,9 @@ class MXFP8Rows:
     scales: torch.Tensor
     rows: int
     n_in: int
+
+    def __post_init__(self):
+        _check_blocks(self.codes, self.scales, 8, self.rows, self.n_in)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -61,7 +76,8 @@ def _bytes(bits: int, rows: int, n_in: int):
 @functools.lru_cache(maxsize=4096)
 def _workspace_bytes(device: int, rows: int, n_out: int, n_in: int, gated: bool, quantised: bool) -> int:
     b = ctypes.c_int64()
-    _lib.call("nsd_mx_workspace", rows, n_out, n_in, gated, quantised, ctypes.byref(b))
+    with torch.cuda.device(device):
+        _lib.call("nsd_mx_workspace", rows, n_out, n_in, gated, quantised, ctypes.byref(b))
     return b.value
 
 
@@ -74,9 +90,9 @@ def _call(t: torch.Tensor, name: str, *args) -> None:
             _lib.call(name, *args, stream_of(t))
 
 
-def _same_device(*tensors: torch.Tensor) -> None:
-    if any(t.device != tensors[0].device for t in tensors[1:]):
-        raise ValueError("all tensors must be on one device")
+def _same_device(a: torch.Tensor, b: torch.Tensor) -> None:
+    if a.get_device() != b.get_device():
+        raise ValueError(f"all tensors must be on one device, got {a.device} and {b.device}")
 
 
 def _matrix(t: torch.Tensor, name: str) -> None:
@@ -87,15 +103,6 @@ def _matrix(t: torch.Tensor, name: str) -> None:
 def _empty(bits: int, rows: int, n_in: int, device):
     c, s = _bytes(bits, rows, n_in)
     return (torch.empty(c, dtype=torch.uint8, device=device), torch.empty(s, dtype=torch.uint8, device=device))
-
-
-def _check_blocks(b, bits: int, rows: int, what: str) -> None:
-    c, s = _bytes(bits, rows, b.n_in)
-    for t, n in ((b.codes, c), (b.scales, s)):
-        if t.dtype != torch.uint8 or not t.is_contiguous() or t.numel() != n:
-            raise ValueError(f"{what} [{rows}, {b.n_in}] must hold {c} bytes of codes and {s} of scales")
-    require_cuda(b.codes, b.scales)
-    _same_device(b.codes, b.scales)
 
 
 def mxfp4_quantize(w: torch.Tensor) -> MXFP4Weight:
@@ -139,10 +146,9 @@ def mxfp8_quantize(x: torch.Tensor) -> MXFP8Rows:
     return MXFP8Rows(codes, scales, rows, n_in)
 
 
-def _dequantize(b, bits: int, rows: int, dtype: torch.dtype, name: str) -> torch.Tensor:
+def _dequantize(b, rows: int, dtype: torch.dtype, name: str) -> torch.Tensor:
     if dtype not in _DTYPES:
         raise TypeError(f"dtype must be fp16, bf16 or fp32, got {dtype}")
-    _check_blocks(b, bits, rows, "the blocks of")
     out = torch.empty((rows, b.n_in), dtype=dtype, device=b.codes.device)
     _call(out, name, b.codes.data_ptr(), b.scales.data_ptr(), rows, b.n_in, out.data_ptr(), _DTYPES[dtype])
     return out
@@ -150,57 +156,61 @@ def _dequantize(b, bits: int, rows: int, dtype: torch.dtype, name: str) -> torch
 
 def mxfp4_dequantize(w: MXFP4Weight, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values [n_out, n_in] that ``w`` stands for; exact in bf16 and fp32."""
-    return _dequantize(w, 4, w.n_out, dtype, "nsd_mxfp4_dequantize")
+    return _dequantize(w, w.n_out, dtype, "nsd_mxfp4_dequantize")
 
 
 def mxfp8_dequantize(x: MXFP8Rows, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values [rows, n_in] that ``x`` stands for; exact in bf16 and fp32."""
-    return _dequantize(x, 8, x.rows, dtype, "nsd_mxfp8_dequantize")
+    return _dequantize(x, x.rows, dtype, "nsd_mxfp8_dequantize")
 
 
-def _product(x, w: MXFP4Weight, out, gated: bool, name: str) -> torch.Tensor:
+def _product(x, w: MXFP4Weight, n: int, out, gated: bool, name: str) -> torch.Tensor:
+    # the checks of a decode step's call are kept short: at one row they and
+    # the launch are most of its time
+    codes = w.codes
     quantised = isinstance(x, MXFP8Rows)
     if quantised:
-        rows, n_in, on = x.rows, x.n_in, x.codes
-        _check_blocks(x, 8, rows, "x")
+        rows, n_in = x.rows, x.n_in
+        _same_device(x.codes, codes)
+        given = (None, x.codes.data_ptr(), x.scales.data_ptr())
     else:
         require_cuda(x)
-        _matrix(x, "x")
         require(x, torch.float16, "x")
-        (rows, n_in), on = x.shape, x
+        if x.dim() != 2:
+            raise ValueError(f"x must be [rows, n_in], got {tuple(x.shape)}")
+        rows, n_in = x.shape
+        _same_device(x, codes)
+        given = (x.data_ptr(), None, None)
     if n_in != w.n_in:
         raise ValueError(f"x has {n_in} columns, the weight is [{w.n_out}, {w.n_in}]")
-    _check_blocks(w, 4, w.n_out, "the weight")
-    n = w.n_out
-    if gated:
-        if n % 32:
-            raise ValueError(f"an up/gate weight has 2 * inter rows, inter a multiple of 16; got {n}")
-        n //= 2
     if out is None:
-        out = torch.empty((rows, n), dtype=torch.float16, device=on.device)
+        out = codes.new_empty((rows, n), dtype=torch.float16)
     else:
         require_cuda(out)
         require(out, torch.float16, "out")
+        _same_device(out, codes)
         if tuple(out.shape) != (rows, n):
             raise ValueError(f"out must be [{rows}, {n}]")
-    _same_device(on, w.codes, out)
     if rows == 0:
         return out
-    ws = torch.empty(_workspace_bytes(on.get_device(), rows, w.n_out, n_in, gated, quantised), dtype=torch.uint8,
-                     device=on.device)
-    _call(on, name, *((None, x.codes.data_ptr(), x.scales.data_ptr()) if quantised else (x.data_ptr(), None, None)),
-          w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), rows, n, n_in, ws.data_ptr(), ws.numel())
+    size = _workspace_bytes(codes.get_device(), rows, w.n_out, n_in, gated, quantised)
+    # the call's own, so calls on other streams and captured ones share nothing
+    ws = codes.new_empty(size) if size else None
+    _call(codes, name, *given, codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), rows, n, n_in,
+          ws.data_ptr() if size else None, size)
     return out
 
 
 def mxfp4_linear(x: torch.Tensor | MXFP8Rows, w: MXFP4Weight, out: torch.Tensor | None = None) -> torch.Tensor:
     """``linear`` with an MXFP4 weight: fp16 [rows, n_out] = fp16(X . W^T), X the MXFP8 values of x [rows, n_in]
     (fp16, or quantised already), fp32 sums."""
-    return _product(x, w, out, False, "nsd_mxfp4_linear")
+    return _product(x, w, w.n_out, out, False, "nsd_mxfp4_linear")
 
 
 def mxfp4_up_gate_silu_and_mul(x: torch.Tensor | MXFP8Rows, w: MXFP4Weight,
                                out: torch.Tensor | None = None) -> torch.Tensor:
     """``up_gate_silu_and_mul`` with an MXFP4 weight [2 * inter, n_in] (up rows first): fp16 [rows, inter] =
     fp16(up * silu(gate)), the products and the SiLU-and-mul in fp32, rounded once."""
-    return _product(x, w, out, True, "nsd_mxfp4_up_gate_silu_and_mul")
+    if w.n_out % 32:
+        raise ValueError(f"an up/gate weight has 2 * inter rows, inter a multiple of 16; got {w.n_out}")
+    return _product(x, w, w.n_out // 2, out, True, "nsd_mxfp4_up_gate_silu_and_mul")
