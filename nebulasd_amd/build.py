@@ -21,7 +21,7 @@ LIB_DIR = PKG / "_lib"
 LIB_PATH = LIB_DIR / "libnsd_attn.so"
 SOURCES = ["nsd_host.cpp", "nsd_prologue.hip", "nsd_attention.hip", "nsd_prefill.hip", "nsd_blocks.hip", "nsd_hostkv.hip",
            "nsd_layer.hip", "nsd_probe.hip", "nsd_decoder.hip", "nsd_gemm.hip",
-           "nsd_mx.hip", "nsd_mx_gemm.hip"]
+           "nsd_mx.hip", "nsd_mx_gemm.hip", "nsd_mx_stream_linear.hip", "nsd_mx_stream_gated.hip"]
 LIBS: list[str] = []  # the HIP runtime only
 ARCH = "gfx950"
 

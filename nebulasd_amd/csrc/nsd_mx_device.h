@@ -126,6 +126,53 @@ __device__ inline f32x16 mx_mfma32(i32x4 a, i32x4 b0, i32x4 b1, f32x16 c, int sa
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c, 4, 0, BYTE, sa, BYTE, sb);
 }
 
+// g / (1 + exp(-g)) in fp32, by the instructions for 2^x and 1 / x (an ulp
+// each): off by (|g| + 6) 2^-23 of the value at most, where fp16 keeps 2^-11.
+// The library's expf and division take 40 instructions more, a third of the
+// time of a 256 x 256 tile over 4096 k.  At g = -inf the product is NaN, as
+// is -inf * 0.
+__device__ inline float mx_silu(float g) {
+  return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.44269504088896341f));
+}
+
+// What a product reads and writes.
+struct MxArgs {
+  const f16* x;        // x [rows][n_in], or null with
+  const u32x4* xc;     // x codes [row tiles][T][128] of 16 bytes
+  const uint32_t* xs;  // x scales [ceil(T / 4)][row tiles][64]
+  const u32x4* wc;     // weight codes [column tiles][T][64]
+  const uint32_t* ws;  // weight scales [ceil(T / 4)][column tiles][64]
+  f16* y;
+  float* part;  // [splits][rows][n], when splits > 1
+  int rows, n;  // n: columns of y
+  int n_in, T;  // T: tiles of k
+  int row_tiles, w_tiles;
+  int splits;
+};
+
+// Which kernel serves it, chosen in nsd_mx_gemm.hip.
+struct MxConfig {
+  bool tile = false;  // mx_tile_kernel, else mx_stream_kernel with
+  int mt = 1, jw = 1, splits = 1;
+  bool fp16 = false;  // reads x as it is
+  bool nt = false;    // the weight past the caches
+};
+
+constexpr int kMxWaves = 4;      // of a workgroup of the stream kernel
+constexpr int kMxFp16Tiles = 2;  // row tiles that it takes as fp16
+
+// Up to 128 rows (nsd_mx_stream.h): y = x . W^T, and its gated form.
+int mx_stream_linear(const MxArgs& a, const MxConfig& c, hipStream_t st);
+int mx_stream_gated(const MxArgs& a, const MxConfig& c, hipStream_t st);
+
+// Raises a kernel's dynamic-LDS limit once per process.
+template <auto Kernel, int kLds>
+int allow_mx_lds() {
+  static const hipError_t attr =
+      hipFuncSetAttribute(reinterpret_cast<const void*>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+  return attr == hipSuccess ? NSD_OK : fail(NSD_ERR_HIP, "mxfp4: LDS attribute: %s", hipGetErrorString(attr));
+}
+
 // Activations to MXFP8 (arguments checked by the caller); in nsd_mx.hip.
 int mxfp8_quantize(const void* x, int64_t n_rows, int64_t n_in, void* codes, void* scales, void* stream);
 

@@ -12,223 +12,8 @@ namespace {
 constexpr int64_t kMaxMxRows = 1 << 21, kMaxMxColumns = 1 << 27, kMaxMxOut = (int64_t)1 << 40;
 constexpr int64_t kMaxMxIn = 1 << 20;  // and a row tile's bytes
 
-struct MxArgs {
-  const f16* x;        // x [rows][n_in], or null with
-  const u32x4* xc;     // x codes [row tiles][T][128] of 16 bytes
-  const uint32_t* xs;  // x scales [ceil(T / 4)][row tiles][64]
-  const u32x4* wc;     // weight codes [column tiles][T][64]
-  const uint32_t* ws;  // weight scales [ceil(T / 4)][column tiles][64]
-  f16* y;
-  float* part;  // [splits][rows][n], when splits > 1
-  int rows, n;  // n: columns of y
-  int n_in, T;  // T: tiles of k
-  int row_tiles, w_tiles;
-  int splits;
-};
-
-// ---- decode and verify batches -----------------------------------------------
-
-// A buffer whose loads past `bytes` give zeros: the streams below run ahead of
-// their range without a branch, so the loop's waits stay exact.
-__device__ inline __amdgpu_buffer_rsrc_t mx_buffer(const void* p, int bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00027000);
-}
-template <bool NT>
-__device__ inline i32x4 mx_load16(__amdgpu_buffer_rsrc_t r, int off) {
-  return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, NT ? 2 : 0));
-}
-
-constexpr int kMxWaves = 4;             // of a workgroup
-constexpr int kMxNowhere = 0x40000000;  // an offset past every buffer's end
-constexpr int kMxFp16Tiles = 2;         // row tiles of the fp16 form
-
-// MT row tiles by JW column tiles a workgroup (gated: the first half up tiles,
-// then their gate tiles).  Its four waves split k: each streams its range's
-// weight and x tiles straight into registers, two steps ahead, and multiplies
-// all MT x JW pairs, so no wave loads what another one has and no step waits
-// for another wave.  The sums meet in LDS at the end, added in wave order.
-// FP16: x as it is, cut into blocks between load and product.  NT: the weight
-// past the caches.
-template <int MT, int JW, bool GATED>
-struct MxStream {
-  static constexpr int P = GATED ? JW / 2 : JW, PER = GATED ? 2 : 1;  // column tiles of y, sums of one
-  static constexpr int YT = P * MT;
-  static constexpr int kLds = YT * (kMxWaves - 1) * PER * 1024;
-  static_assert(P * PER == JW && kLds <= 160 * 1024);
-};
-
-template <int MT, int JW, bool GATED, bool FP16, bool NT>
-__global__ void __launch_bounds__(kMxWaves* kWave, 1) mx_stream_kernel(MxArgs a) {
-  using S = MxStream<MT, JW, GATED>;
-  constexpr int P = S::P, D = 2;
-  extern __shared__ __attribute__((aligned(16))) char lds_raw[];
-  const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int out_tiles = (a.n + 15) / 16;
-  const int groups = (out_tiles + P - 1) / P;
-  const int group = blockIdx.x % groups, split = blockIdx.x / groups;
-  const int rt0 = blockIdx.y * MT;
-  const int parts = a.splits * kMxWaves, part = split * kMxWaves + wave;
-  // a wave's steps [t0, t1), in whole fours (a scale word's tiles of k) where
-  // they come out even; ta: the four that t0 lies in, whose other steps are
-  // loaded and not multiplied
-  const int kgs = (a.T + 3) / 4;
-  const bool fours = kgs % parts == 0 || kgs >= 4 * parts;
-  const int units = fours ? kgs : a.T, per = fours ? 4 : 1;
-  const int t0 = (int)((int64_t)part * units / parts) * per;
-  const int t1 = min((int)((int64_t)(part + 1) * units / parts) * per, a.T);
-  const int ta = t0 & ~3;
-  [[maybe_unused]] const int k_end = min(t1 * kMxTileK, a.n_in);
-
-  __amdgpu_buffer_rsrc_t wb[JW], wsb[JW], xb[MT], xsb[MT];
-#pragma unroll
-  for (int j = 0; j < JW; ++j) {
-    int tile = min(group * P + j % P, out_tiles - 1);
-    if (GATED && j >= P) tile += out_tiles;
-    wb[j] = mx_buffer(a.wc + ((int64_t)tile * a.T + ta) * 64, (t1 - ta) * kMxTile4);
-    wsb[j] = mx_buffer(a.ws + (int64_t)tile * 64, ((kgs - 1) * a.w_tiles + 1) * kMxScaleTile);
-  }
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int tile = min(rt0 + i, a.row_tiles - 1);
-    if constexpr (FP16) {  // rows past the last: zeros
-      xb[i] = mx_buffer(a.x + (int64_t)tile * 16 * a.n_in, min(a.rows - tile * 16, 16) * a.n_in * 2);
-    } else {
-      xb[i] = mx_buffer(a.xc + ((int64_t)tile * a.T + ta) * 128, (t1 - ta) * kMxTile8);
-      xsb[i] = mx_buffer(a.xs + (int64_t)tile * 64, ((kgs - 1) * a.row_tiles + 1) * kMxScaleTile);
-    }
-  }
-  f32x4 acc[JW][MT];
-#pragma unroll
-  for (int j = 0; j < JW; ++j)
-#pragma unroll
-    for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  constexpr int XV = FP16 ? 4 : 2;
-  i32x4 w[D][JW], x[D][MT][XV];
-  int sw[2][JW], sx[2][MT];  // scales of this four tiles of k, and of the next
-  auto load = [&](int u, int t) __attribute__((always_inline)) {
-    const int wo = (t - ta) * kMxTile4 + lane * 16, xo = (t - ta) * kMxTile8 + lane * 16;
-#pragma unroll
-    for (int j = 0; j < JW; ++j) w[u][j] = mx_load16<NT>(wb[j], wo);
-    if constexpr (FP16) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {  // the runs of 16 k at 16 lg and 64 + 16 lg; past the row or the range: zeros
-        const int k = t * kMxTileK + h * 64 + lg * 16;
-        const int off = k < k_end ? (li * a.n_in + k) * 2 : kMxNowhere;
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          x[u][i][2 * h] = mx_load16<false>(xb[i], off);
-          x[u][i][2 * h + 1] = mx_load16<false>(xb[i], off + 16);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        x[u][i][0] = mx_load16<false>(xb[i], xo);
-        x[u][i][1] = mx_load16<false>(xb[i], xo + 1024);
-      }
-    }
-  };
-  auto load_scales = [&](int u, int kg) __attribute__((always_inline)) {
-    const int wo = kg * a.w_tiles * kMxScaleTile + lane * 4, xo = kg * a.row_tiles * kMxScaleTile + lane * 4;
-#pragma unroll
-    for (int j = 0; j < JW; ++j) sw[u][j] = __builtin_amdgcn_raw_buffer_load_b32(wsb[j], wo, 0, 0);
-    if constexpr (!FP16) {
-#pragma unroll
-      for (int i = 0; i < MT; ++i) sx[u][i] = __builtin_amdgcn_raw_buffer_load_b32(xsb[i], xo, 0, 0);
-    }
-  };
-  load_scales(0, ta >> 2);
-#pragma unroll
-  for (int u = 0; u < D; ++u) load(u, ta + u);
-  for (int t = ta; t < t1; t += 4) {
-    load_scales(1, (t >> 2) + 1);
-    static_for<4>([&](auto uc) __attribute__((always_inline)) {
-      constexpr int u = decltype(uc)::value, r = u % D;
-      if (t + u >= t0 && t + u < t1) {
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          i32x4 b0, b1;
-          int sb;
-          if constexpr (FP16) {
-            const f16x8 h[4] = {__builtin_bit_cast(f16x8, x[r][i][0]), __builtin_bit_cast(f16x8, x[r][i][1]),
-                                __builtin_bit_cast(f16x8, x[r][i][2]), __builtin_bit_cast(f16x8, x[r][i][3])};
-            sb = mx8_operand(h, lane, b0, b1) << 8 * u;
-          } else {
-            b0 = x[r][i][0];
-            b1 = x[r][i][1];
-            sb = sx[0][i];
-          }
-#pragma unroll
-          for (int j = 0; j < JW; ++j) acc[j][i] = mx_mfma<u>(w[r][j], b0, b1, acc[j][i], sw[0][j], sb);
-        }
-      }
-      load(r, t + u + D);
-    });
-#pragma unroll
-    for (int j = 0; j < JW; ++j) sw[0][j] = sw[1][j];
-    if constexpr (!FP16) {
-#pragma unroll
-      for (int i = 0; i < MT; ++i) sx[0][i] = sx[1][i];
-    }
-  }
-
-  // lane (li, lg) holds columns 4 lg .. 4 lg + 3 of a tile for row li
-  auto store = [&](int j, int i, f32x4 v, f32x4 gate) __attribute__((always_inline)) {
-    const int m = 16 * (rt0 + i) + li, n0 = 16 * (group * P + j) + 4 * lg;
-    if (m >= a.rows || n0 >= a.n) return;
-    if constexpr (GATED) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] *= gate[e] / (1.f + expf(-gate[e]));
-    }
-    if (!GATED && a.splits > 1) {  // n a multiple of 8
-      *reinterpret_cast<f32x4*>(a.part + ((int64_t)split * a.rows + m) * a.n + n0) = v;
-      return;
-    }
-    f16* y = a.y + (int64_t)m * a.n + n0;
-    const f16x4 h = {(f16)v[0], (f16)v[1], (f16)v[2], (f16)v[3]};
-    if (a.n % 4 == 0) {
-      *reinterpret_cast<f16x4*>(y) = h;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (n0 + e < a.n) y[e] = h[e];
-    }
-  };
-  // y tile q is wave q % 4's to finish: it gets the others' sums through LDS
-  f32x4* red = reinterpret_cast<f32x4*>(lds_raw) + lane;
-  static_for<S::YT>([&](auto qc) __attribute__((always_inline)) {
-    constexpr int q = decltype(qc)::value, owner = q % kMxWaves;
-    if (wave != owner) {
-      f32x4* at = red + (q * (kMxWaves - 1) + wave - (wave > owner)) * S::PER * kWave;
-      at[0] = acc[q / MT][q % MT];
-      if constexpr (GATED) at[kWave] = acc[q / MT + P][q % MT];
-    }
-  });
-  __syncthreads();
-  static_for<S::YT>([&](auto qc) __attribute__((always_inline)) {
-    constexpr int q = decltype(qc)::value, owner = q % kMxWaves;
-    if (wave == owner) {
-      auto sum = [&](int per, f32x4 mine) __attribute__((always_inline)) {
-        f32x4 v;
-        static_for<kMxWaves>([&](auto oc) __attribute__((always_inline)) {
-          constexpr int o = decltype(oc)::value;
-          f32x4 part = mine;
-          if constexpr (o != owner)
-            part = red[((q * (kMxWaves - 1) + o - (o > owner ? 1 : 0)) * S::PER + per) * kWave];
-          if constexpr (o == 0) v = part;
-          else v += part;
-        });
-        return v;
-      };
-      const f32x4 v = sum(0, acc[q / MT][q % MT]);
-      f32x4 gate = v;
-      if constexpr (GATED) gate = sum(1, acc[q / MT + P][q % MT]);
-      store(q / MT, q % MT, v, gate);
-    }
-  });
-}
+typedef __attribute__((address_space(3))) i32x4 lds_i32x4;
+typedef __attribute__((address_space(3))) int lds_int;
 
 // ---- prompts ---------------------------------------------------------------
 
@@ -298,21 +83,23 @@ __global__ void __launch_bounds__(S::NW* kWave) mx_tile_kernel(MxArgs a, int m_t
   for (int i = 0; i < S::WI; ++i)
     wsrc[i] = reinterpret_cast<const char*>(a.wc) + (int64_t)w_tile(i * NW + wave) * T * kMxTile4;
   // scales of four steps: this wave's 1 KB is four tiles of x or of the weight
-  const bool sx = wave < XT / 4;
-  const int s_tile = sx ? min(bm * XT + wave * 4 + (lane >> 4), a.row_tiles - 1)
+  const bool of_x = wave < XT / 4;
+  const int s_tile = of_x ? min(bm * XT + wave * 4 + (lane >> 4), a.row_tiles - 1)
                         : w_tile((wave - XT / 4) * 4 + (lane >> 4));
-  const char* ssrc = reinterpret_cast<const char*>(sx ? a.xs : a.ws);
-  const int64_t s_stride = (int64_t)(sx ? a.row_tiles : a.w_tiles) * kMxScaleTile;
+  const char* ssrc = reinterpret_cast<const char*>(of_x ? a.xs : a.ws);
+  const int64_t s_stride = (int64_t)(of_x ? a.row_tiles : a.w_tiles) * kMxScaleTile;
   const uint32_t s_off = (uint32_t)s_tile * kMxScaleTile + (lane & 15) * 16;
 
-  auto issue = [&](int t, int slot, auto with_scales) __attribute__((always_inline)) {
+  // load i of a step: of x, of the weight, and of the scales with every fourth
+  constexpr int N = S::XI + S::WI;
+  auto issue = [&](auto ic, int t, int slot) __attribute__((always_inline)) {
+    constexpr int i = decltype(ic)::value;
     const uint32_t base = (uint32_t)(uintptr_t)(ring + slot * S::kStep);
-#pragma unroll
-    for (int i = 0; i < S::XI; ++i) mx_dma(base + (i * NW + wave) * 1024, xsrc[i] + (int64_t)t * kMxTile8, lane * 16);
-#pragma unroll
-    for (int i = 0; i < S::WI; ++i)
-      mx_dma(base + XT * kMxTile8 + (i * NW + wave) * 1024, wsrc[i] + (int64_t)t * kMxTile4, lane * 16);
-    if constexpr (decltype(with_scales)::value)
+    if constexpr (i < S::XI)
+      mx_dma(base + (i * NW + wave) * 1024, xsrc[i] + (int64_t)t * kMxTile8, lane * 16);
+    else if constexpr (i < N)
+      mx_dma(base + XT * kMxTile8 + ((i - S::XI) * NW + wave) * 1024, wsrc[i - S::XI] + (int64_t)t * kMxTile4, lane * 16);
+    else
       mx_dma((uint32_t)(uintptr_t)(scales + (t >> 2 & 1) * S::kScales + wave * 1024), ssrc + (t >> 2) * s_stride, s_off);
   };
 
@@ -323,120 +110,159 @@ __global__ void __launch_bounds__(S::NW* kWave) mx_tile_kernel(MxArgs a, int m_t
     for (int i = 0; i < FR; ++i)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[j][i][e] = 0.f;
-  uint32_t sw[FC][2], sxv[FR][2];  // scales of the wave's fragments, blocks lg and 2 + lg, four steps a word
   // lane's place in a fragment: its row's 16-byte run in tile l32 / 16
   const int row16 = (l32 & 15) * 16;
-  const int x_at = (l32 >> 4) * kMxTile8 + lg * 256 + row16, w_at = (l32 >> 4) * kMxTile4 + lg * 256 + row16;
+  const int x_at = (wr * FR * 2 + (l32 >> 4)) * kMxTile8 + lg * 256 + row16;
+  const int w_at = XT * kMxTile8 + (wc * FC * 2 + (l32 >> 4)) * kMxTile4 + lg * 256 + row16;
   const int s_at = (l32 >> 4) * kMxScaleTile + lg * 64 + (l32 & 15) * 4;
 
-  issue(0, 0, std::true_type{});
-  if (T > 1) issue(1, 1, std::false_type{});
-  int slot = 0, slot2 = 2;
+  // A step is two halves of 64 k, each a set of fragments in registers: one is
+  // multiplied while the other is read.  Scales of the wave's fragments, blocks
+  // lg and 2 + lg: a word holds four steps.
+  i32x4 x[2][FR][2], w[2][FC];
+  int sw[FC][2], sx[FR][2], sw_next[FC][2], sx_next[FR][2];
+  constexpr int M = FR * FC, F = 2 * FR + FC;  // products and reads of a half
+  auto read = [&](auto qc, auto rc, int slot) __attribute__((always_inline)) {
+    constexpr int q = decltype(qc)::value, r = decltype(rc)::value;
+    const lds_char* step = ring + slot * S::kStep;
+    if constexpr (r < 2 * FR)
+      x[q][r / 2][r % 2] = *(const lds_i32x4*)(step + x_at + r / 2 * 2 * kMxTile8 + q * 1024 + r % 2 * 512);
+    else
+      w[q][r - 2 * FR] = *(const lds_i32x4*)(step + w_at + (r - 2 * FR) * 2 * kMxTile4 + q * 512);
+  };
+  auto read_scales = [&](int kg) __attribute__((always_inline)) {
+    const lds_char* sc = scales + (kg & 1) * S::kScales + s_at;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+#pragma unroll
+      for (int i = 0; i < FR; ++i) sx_next[i][q] = *(const lds_int*)(sc + (wr * FR + i) * 2 * kMxScaleTile + q * 128);
+#pragma unroll
+      for (int j = 0; j < FC; ++j)
+        sw_next[j][q] = *(const lds_int*)(sc + (XT + (wc * FC + j) * 2) * kMxScaleTile + q * 128);
+    }
+  };
+  // The products of a half in order, after(i) behind product i.  The matrix
+  // pipe takes a product every 64 cycles and a wave issues in order: reads and
+  // loads in a bunch, eight waves at once, would fill their queues and hold the
+  // products up behind them.
+  auto multiply = [&](auto qc, auto uc, auto after) __attribute__((always_inline)) {
+    constexpr int q = decltype(qc)::value, u = decltype(uc)::value;
+    static_for<M>([&](auto mc) __attribute__((always_inline)) {
+      constexpr int i = decltype(mc)::value / FC, j = decltype(mc)::value % FC;
+      acc[j][i] = mx_mfma32<u>(w[q][j], x[q][i][0], x[q][i][1], acc[j][i], sw[j][q], sx[i][q]);
+      after(mc);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  using Q0 = std::integral_constant<int, 0>;
+  using Q1 = std::integral_constant<int, 1>;
+  // reads 2 m and 2 m + 1 of a half behind product m of the other
+  auto read_two = [&](auto qc, auto mc, int slot) __attribute__((always_inline)) {
+    constexpr int r = 2 * decltype(mc)::value;
+    if constexpr (r < F) read(qc, std::integral_constant<int, r>{}, slot);
+    if constexpr (r + 1 < F) read(qc, std::integral_constant<int, r + 1>{}, slot);
+  };
+  static_assert(2 * M >= F);
+
+  static_for<N + 1>([&](auto i) { issue(i, 0, 0); });
+  if (T > 1) static_for<N>([&](auto i) { issue(i, 1, 1); });
+  if (T > 2) static_for<N>([&](auto i) { issue(i, 2, 2); });
+  if (T > 2) mx_wait<2 * N>();
+  else if (T > 1) mx_wait<N>();
+  else mx_wait<0>();
+  asm volatile("s_barrier" ::: "memory");
+  read_scales(0);
+  static_for<F>([&](auto r) { read(Q0{}, r, 0); });
+  int slot = 0;
   for (int t0 = 0; t0 < T; t0 += 4) {
     static_for<4>([&](auto uc) __attribute__((always_inline)) {
       constexpr int u = decltype(uc)::value;
       const int t = t0 + u;
       if (t >= T) return;
-      // step t has landed: all but this wave's loads of step t + 1; then
-      // everybody's, and everybody is done with step t - 1
-      if (t + 1 < T) mx_wait<S::XI + S::WI + (u == 3 ? 1 : 0)>();
-      else mx_wait<0>();
-      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (t + 2 < T) issue(t + 2, slot2, std::bool_constant<u == 2>{});
-      const lds_char* xs = ring + slot * S::kStep + wr * FR * 2 * kMxTile8 + x_at;
-      const lds_char* wsl = ring + slot * S::kStep + XT * kMxTile8 + wc * FC * 2 * kMxTile4 + w_at;
-      slot = slot == 2 ? 0 : slot + 1;
-      slot2 = slot2 == 2 ? 0 : slot2 + 1;
       if constexpr (u == 0) {
-        const lds_char* sc = scales + (t >> 2 & 1) * S::kScales + s_at;
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
 #pragma unroll
-          for (int i = 0; i < FR; ++i)
-            sxv[i][q] = *(const __attribute__((address_space(3))) uint32_t*)(sc + (wr * FR + i) * 2 * kMxScaleTile + q * 128);
+          for (int i = 0; i < FR; ++i) sx[i][q] = sx_next[i][q];
 #pragma unroll
-          for (int j = 0; j < FC; ++j)
-            sw[j][q] = *(const __attribute__((address_space(3))) uint32_t*)(sc + (XT + (wc * FC + j) * 2) * kMxScaleTile + q * 128);
+          for (int j = 0; j < FC; ++j) sw[j][q] = sw_next[j][q];
         }
       }
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {  // 64 k each
-        i32x4 x[FR][2], w[FC];
-#pragma unroll
-        for (int j = 0; j < FC; ++j)
-          w[j] = *(const __attribute__((address_space(3))) i32x4*)(wsl + j * 2 * kMxTile4 + q * 512);
-#pragma unroll
-        for (int i = 0; i < FR; ++i)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            x[i][h] = *(const __attribute__((address_space(3))) i32x4*)(xs + i * 2 * kMxTile8 + q * 1024 + h * 512);
-#pragma unroll
-        for (int i = 0; i < FR; ++i)
-#pragma unroll
-          for (int j = 0; j < FC; ++j)
-            acc[j][i] = mx_mfma32<u>(w[j], x[i][0], x[i][1], acc[j][i], sw[j][q], sxv[i][q]);
+      multiply(Q0{}, uc, [&](auto m) __attribute__((always_inline)) { read_two(Q1{}, m, slot); });
+      const int free = slot;
+      if (t + 1 < T) {
+        // step t is in registers and step t + 1 has landed, but for this wave's
+        // loads of step t + 2; then the same of everybody
+        if (t + 2 < T) mx_wait<N + (u == 2 ? 1 : 0)>();
+        else mx_wait<0>();
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        slot = slot == 2 ? 0 : slot + 1;
+        if constexpr (u == 3) read_scales((t + 1) >> 2);
       }
+      const bool more = t + 3 < T;
+      multiply(Q1{}, uc, [&](auto m) __attribute__((always_inline)) {
+        read_two(Q0{}, m, slot);  // past the last step: read and not used
+        constexpr int i = decltype(m)::value, n = N + (u == 1 ? 1 : 0), per = (n + M - 1) / M;  // loads of step t + 3
+        if (more)
+          static_for<per>([&](auto e) __attribute__((always_inline)) {
+            if constexpr (i * per + decltype(e)::value < n)
+              issue(std::integral_constant<int, i * per + decltype(e)::value>{}, t + 3, free);
+          });
+      });
     });
   }
 
-  // lane (l32, lg): columns 8 q + 4 lg .. + 3 of a fragment, row l32
-  constexpr int H = S::GATED ? FC / 2 : FC;
+  // The output goes out in whole rows of the wave's columns, by way of LDS (the
+  // ring's: every wave is done with it).  Lane (l32, lg) holds columns 8 q + 4 lg
+  // .. + 3 of a fragment, row l32.
+  constexpr int H = S::GATED ? FC / 2 : FC, C = H * 32, kPitch = C + 8, ROWS = FR * 32;
+  static_assert(NW * ROWS * kPitch * 2 <= S::kLds);
+  __syncthreads();
+  f16* own = reinterpret_cast<f16*>(lds_raw) + wave * ROWS * kPitch;
 #pragma unroll
-  for (int i = 0; i < FR; ++i) {
-    const int m = bm * S::TM + (wr * FR + i) * 32 + l32;
+  for (int i = 0; i < FR; ++i)
 #pragma unroll
     for (int j = 0; j < H; ++j)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int n0 = bn * S::OUT + (wc * H + j) * 32 + 8 * q + 4 * lg;
-        if (m >= a.rows || n0 >= a.n) continue;
         f16x4 h;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float v = acc[j][i][4 * q + e];
-          if constexpr (S::GATED) {
-            const float g = acc[j + H][i][4 * q + e];
-            v *= g / (1.f + expf(-g));
-          }
+          if constexpr (S::GATED) v *= mx_silu(acc[j + H][i][4 * q + e]);
           h[e] = (f16)v;
         }
-        f16* y = a.y + (int64_t)m * a.n + n0;
-        if (a.n % 4 == 0) {
-          *reinterpret_cast<f16x4*>(y) = h;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (n0 + e < a.n) y[e] = h[e];
-        }
+        *reinterpret_cast<f16x4*>(own + (i * 32 + l32) * kPitch + j * 32 + 8 * q + 4 * lg) = h;
       }
-  }
+  const int m0 = bm * S::TM + wr * ROWS, n0 = bn * S::OUT + wc * C;
+  const int rows = min(ROWS, a.rows - m0), cols = min(C, a.n - n0);
+  f16* y = a.y + (int64_t)m0 * a.n + n0;
+  auto rows_of = [&](auto v) __attribute__((always_inline)) {  // vectors of decltype(v), where rows start at whole ones
+    using V = decltype(v);
+    constexpr int E = sizeof(V) / 2, PER = C / E;  // a row's vectors
+    for (int r = lane; r < ROWS * PER; r += kWave) {
+      const int m = r / PER, c = r % PER * E;
+      if (m < rows && c < cols) *reinterpret_cast<V*>(y + (int64_t)m * a.n + c) = *reinterpret_cast<const V*>(own + m * kPitch + c);
+    }
+  };
+  if (a.n % 8 == 0) rows_of(f16x8{});
+  else if (a.n % 2 == 0) rows_of(f16x2{});
+  else rows_of(f16{});
 }
 
-// Raises a kernel's dynamic-LDS limit once per process.
-template <auto Kernel, int kLds>
-int allow_mx_lds() {
-  static const hipError_t attr =
-      hipFuncSetAttribute(reinterpret_cast<const void*>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
-  return attr == hipSuccess ? NSD_OK : fail(NSD_ERR_HIP, "mxfp4: LDS attribute: %s", hipGetErrorString(attr));
-}
-
-struct MxConfig {
-  bool tile = false;  // mx_tile_kernel, else mx_stream_kernel with
-  int mt = 1, jw = 1, splits = 1;
-  bool fp16 = false;  // reads x as it is
-  bool nt = false;    // the weight past the caches
-};
 
 // Column tiles a workgroup, splits of k over workgroups and the form of x for
-// the stream kernel: the cheapest by a model of its time in ns.
+// the stream kernel: the cheapest by a model of its time in ns, whose constants
+// are fitted to every choice at 116 shapes (1 to 128 rows, 1024 x 1024 to
+// 151936 x 4096); the chosen one is within 1% of the best on the average and 14%
+// at worst.
 //   - A compute unit takes in weight and x together, however they mix, a KB in
-//     21 ns where two workgroups share it or it has one to run, in 28 where
-//     one's registers leave no room for another; all of them take in 6.1 TB/s
-//     of weight at most.
-//   - A workgroup's end, its sums through LDS, takes 50 ns a tile.
-//   - Splits cost a pass that adds them: 2.5 us and their bytes.
-//   - x as fp16 is twice the bytes to every workgroup, and saves the pass that
-//     cuts it into blocks, 4 us with its launch.
+//     12 ns where two workgroups share it or it has one to run, in 18 where
+//     one's registers leave no room for another.
+//   - A workgroup's end, its sums through LDS, takes 145 ns a tile.
+//   - Splits cost a pass that adds them: 2 us and their bytes.
+//   - x as fp16 is more bytes to every workgroup and 36 ns of cutting a step
+//     and row tile, and saves the pass that cuts it once, 2.4 us.
 MxConfig choose_stream(int64_t n_rows, int64_t n, int64_t T, bool gated, bool quantised, int cus) {
   MxConfig best;
   const int64_t row_tiles = mx_row_tiles(n_rows), chunks = (row_tiles + 7) / 8;
@@ -457,11 +283,10 @@ MxConfig choose_stream(int64_t n_rows, int64_t n, int64_t T, bool gated, bool qu
         const double steps = (double)((T + splits - 1) / splits);
         // rows of x that exist: the others of a tile are not fetched as fp16
         const double x_kb = fp16 ? n_rows * 0.25 : 2.0 * mt;
-        double t = std::max(rounds * steps * (jw + x_kb) * (wgs > cus && !two ? 28.0 : 21.0),
-                            (double)out_tiles * (gated ? 2 : 1) * T * chunks * kMxTile4 / 6100.0) +
-                   rounds * jw * mt * 50.0;
-        if (splits > 1) t += 2500.0 + (double)splits * n_rows * n * 8 / 5000.0;
-        if (!fp16 && !quantised) t += 4000.0;
+        double t = rounds * (steps * (jw + x_kb) * (wgs > cus && !two ? 18.0 : 12.0) + jw * mt * 145.0);
+        if (splits > 1) t += 2000.0 + (double)splits * n_rows * n * 8 / 1830.0;
+        if (fp16) t += rounds * steps * mt * 36.0;
+        else if (!quantised) t += 2400.0;
         if (t < least) {
           least = t;
           best.mt = mt;
@@ -495,43 +320,9 @@ int launch_mx_tile(const MxArgs& a, hipStream_t st) {
   return launch_status(S::GATED ? "mxfp4_up_gate_silu_and_mul" : "mxfp4_linear");
 }
 
-template <int MT, int JW, bool GATED, bool FP16, bool NT>
-int launch_mx_stream(const MxArgs& a, hipStream_t st) {
-  using S = MxStream<MT, JW, GATED>;
-  if (int rc = allow_mx_lds<&mx_stream_kernel<MT, JW, GATED, FP16, NT>, S::kLds>()) return rc;
-  const int groups = ((a.n + 15) / 16 + S::P - 1) / S::P;
-  hipLaunchKernelGGL((mx_stream_kernel<MT, JW, GATED, FP16, NT>), dim3(groups * a.splits, (a.row_tiles + MT - 1) / MT),
-                     dim3(kMxWaves * kWave), S::kLds, st, a);
-  return launch_status(GATED ? "mxfp4_up_gate_silu_and_mul" : "mxfp4_linear");
-}
-template <int MT, int JW, bool GATED>
-int launch_mx_stream(const MxArgs& a, const MxConfig& c, hipStream_t st) {
-  if constexpr (MT <= kMxFp16Tiles)
-    if (c.fp16)
-      return c.nt ? launch_mx_stream<MT, JW, GATED, true, true>(a, st) : launch_mx_stream<MT, JW, GATED, true, false>(a, st);
-  return c.nt ? launch_mx_stream<MT, JW, GATED, false, true>(a, st) : launch_mx_stream<MT, JW, GATED, false, false>(a, st);
-}
-
-template <bool GATED, int... I>
-int launch_mx_rows(std::integer_sequence<int, I...>, const MxArgs& a, const MxConfig& c, hipStream_t st) {
-  int rc = NSD_ERR_UNSUPPORTED;
-  auto with = [&](auto mt) {
-    constexpr int MT = decltype(mt)::value;
-    if constexpr (!GATED) {
-      if (c.jw == 1) return launch_mx_stream<MT, 1, GATED>(a, c, st);
-      if (c.jw == 3) return launch_mx_stream<MT, 3, GATED>(a, c, st);
-    }
-    if (c.jw == 2) return launch_mx_stream<MT, 2, GATED>(a, c, st);
-    if (c.jw == 4) return launch_mx_stream<MT, 4, GATED>(a, c, st);
-    return launch_mx_stream<MT, 6, GATED>(a, c, st);
-  };
-  ((c.mt == I + 1 ? (rc = with(std::integral_constant<int, I + 1>{}), 0) : 0), ...);
-  return rc;
-}
-
 template <bool GATED>
 int launch_mx(const MxArgs& a, const MxConfig& c, hipStream_t st) {
-  if (!c.tile) return launch_mx_rows<GATED>(std::make_integer_sequence<int, 8>{}, a, c, st);
+  if (!c.tile) return GATED ? mx_stream_gated(a, c, st) : mx_stream_linear(a, c, st);
   const int64_t big = (int64_t)((a.rows + 255) / 256) * ((a.n + (GATED ? 127 : 255)) / (GATED ? 128 : 256));
   if (big >= 200) return launch_mx_tile<MxTile<4, 2, 2, 4, GATED>>(a, st);
   return launch_mx_tile<MxTile<2, 2, 2, 2, GATED>>(a, st);
