@@ -151,8 +151,9 @@ struct MxArgs {
 };
 
 // Which kernel serves it, chosen in nsd_mx_gemm.hip.
+enum MxKernel { kMxStream, kMxTile128x256, kMxTile128 };
 struct MxConfig {
-  bool tile = false;  // mx_tile_kernel, else mx_stream_kernel with
+  MxKernel kernel = kMxStream;  // a shape of mx_tile_kernel, or mx_stream_kernel with
   int mt = 1, jw = 1, splits = 1;
   bool fp16 = false;  // reads x as it is
   bool nt = false;    // the weight past the caches

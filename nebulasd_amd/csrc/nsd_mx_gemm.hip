@@ -21,28 +21,33 @@ template <int N>
 __device__ inline void mx_wait() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
-// 16 bytes a lane from base + 16 lane to LDS.
+// 16 bytes a lane from base + offset to LDS.  The wait states are the ones the
+// compiler would put between a write of m0, or a VALU's write of the base's
+// registers, and the load; it does not look into the asm.
 __device__ inline void mx_dma(uint32_t lds_addr, const char* base, uint32_t offset) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2"
                :
                : "s"(lds_addr), "v"(offset), "s"(base)
                : "memory", "m0");
 }
 
-template <int WR_, int WC_, int FR_, int FC_, bool GATED_>
+template <int WR_, int WC_, int FR_, int FC_, int R_, bool GATED_>
 struct MxTile {
   static constexpr int WR = WR_, WC = WC_, FR = FR_, FC = FC_;  // waves and 32-wide fragments a wave, over rows and columns
+  static constexpr int R = R_;                                  // steps in the ring
   static constexpr bool GATED = GATED_;
   static constexpr int NW = WR * WC, XT = WR * FR * 2, WT = WC * FC * 2;  // 16-row tiles of x and of the weight
   static constexpr int TM = XT * 16, TN = WT * 16, OUT = GATED ? TN / 2 : TN;
-  static constexpr int XI = 2 * XT / NW, WI = WT / NW;  // loads a wave of a step's codes, 1 KB each
-  static constexpr int R = 3, kStep = XT * kMxTile8 + WT * kMxTile4, kScales = (XT + WT) * kMxScaleTile;
+  static constexpr int SK = (XT + WT) / 4;  // KB of scales of four steps
+  // loads a wave, 1 KB each: a step's x and weight, four steps' scales
+  static constexpr int XI = 2 * XT / NW, WI = WT / NW, SI = (SK + NW - 1) / NW;
+  static constexpr int kStep = XT * kMxTile8 + WT * kMxTile4, kScales = SK * 1024;
   static constexpr int kLds = R * kStep + 2 * kScales;
-  static_assert(XI * NW == 2 * XT && WI * NW == WT && (XT + WT) / 4 == NW && XT % 4 == 0 && kLds <= 160 * 1024);
+  static_assert(XI * NW == 2 * XT && WI * NW == WT && XT % 4 == 0 && WT % 4 == 0 && R >= 2 && kLds <= 160 * 1024);
 };
 
 template <class S>
-__global__ void __launch_bounds__(S::NW* kWave) mx_tile_kernel(MxArgs a, int m_tiles, int n_tiles) {
+__global__ void __launch_bounds__(S::NW* kWave, 2) mx_tile_kernel(MxArgs a, int m_tiles, int n_tiles) {
   constexpr int FR = S::FR, FC = S::FC, NW = S::NW, XT = S::XT, WT = S::WT;
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   lds_char* ring = (lds_char*)lds_raw;
@@ -52,8 +57,8 @@ __global__ void __launch_bounds__(S::NW* kWave) mx_tile_kernel(MxArgs a, int m_t
   const int wr = wave / S::WC, wc = wave % S::WC;
   // workgroup i runs on XCD i % 8: each XCD a contiguous run of tiles, in bands
   // of eight row tiles
-  const int total = m_tiles * n_tiles;
-  int id = blockIdx.x;
+  const int total = m_tiles * n_tiles, split = blockIdx.x / total;
+  int id = blockIdx.x - split * total;
   {
     const int q = total / kXcds, r = total % kXcds, xcd = id % kXcds, at = id / kXcds;
     id = xcd * q + min(xcd, r) + at;
@@ -62,7 +67,10 @@ __global__ void __launch_bounds__(S::NW* kWave) mx_tile_kernel(MxArgs a, int m_t
   const int band = id / (kBand * n_tiles), rows_in = min(kBand, m_tiles - band * kBand);
   const int in_band = id - band * kBand * n_tiles;
   const int bm = band * kBand + in_band % rows_in, bn = in_band / rows_in;
-  const int T = a.T, out_tiles = (a.n + 15) / 16;
+  const int out_tiles = (a.n + 15) / 16;
+  // this split's steps: whole fours, so that a scale word is one split's
+  const int fours = (a.T + 3) / 4, four0 = (int)((int64_t)split * fours / a.splits);
+  const int T = min(4 * (int)((int64_t)(split + 1) * fours / a.splits), a.T) - 4 * four0;
 
   // this wave's loads of a step: chunks i NW + wave of x (two a tile) and of the weight
   auto w_tile = [&](int j) {
@@ -77,18 +85,27 @@ __global__ void __launch_bounds__(S::NW* kWave) mx_tile_kernel(MxArgs a, int m_t
 #pragma unroll
   for (int i = 0; i < S::XI; ++i) {
     const int q = i * NW + wave, tile = min(bm * XT + q / 2, a.row_tiles - 1);
-    xsrc[i] = reinterpret_cast<const char*>(a.xc) + (int64_t)tile * T * kMxTile8 + q % 2 * 1024;
+    xsrc[i] = reinterpret_cast<const char*>(a.xc) + ((int64_t)tile * a.T + 4 * four0) * kMxTile8 + q % 2 * 1024;
   }
 #pragma unroll
   for (int i = 0; i < S::WI; ++i)
-    wsrc[i] = reinterpret_cast<const char*>(a.wc) + (int64_t)w_tile(i * NW + wave) * T * kMxTile4;
-  // scales of four steps: this wave's 1 KB is four tiles of x or of the weight
-  const bool of_x = wave < XT / 4;
-  const int s_tile = of_x ? min(bm * XT + wave * 4 + (lane >> 4), a.row_tiles - 1)
-                        : w_tile((wave - XT / 4) * 4 + (lane >> 4));
-  const char* ssrc = reinterpret_cast<const char*>(of_x ? a.xs : a.ws);
-  const int64_t s_stride = (int64_t)(of_x ? a.row_tiles : a.w_tiles) * kMxScaleTile;
-  const uint32_t s_off = (uint32_t)s_tile * kMxScaleTile + (lane & 15) * 16;
+    wsrc[i] = reinterpret_cast<const char*>(a.wc) + ((int64_t)w_tile(i * NW + wave) * a.T + 4 * four0) * kMxTile4;
+  // scales of four steps: a KB is four tiles of x or of the weight; where they
+  // do not come out even, a wave brings the last one again
+  const char* ssrc[S::SI];
+  int64_t s_stride[S::SI];
+  uint32_t s_off[S::SI];
+  int s_kb[S::SI];
+#pragma unroll
+  for (int i = 0; i < S::SI; ++i) {
+    s_kb[i] = min(i * NW + wave, S::SK - 1);
+    const bool of_x = s_kb[i] < XT / 4;
+    const int tile = of_x ? min(bm * XT + s_kb[i] * 4 + (lane >> 4), a.row_tiles - 1)
+                          : w_tile((s_kb[i] - XT / 4) * 4 + (lane >> 4));
+    s_stride[i] = (int64_t)(of_x ? a.row_tiles : a.w_tiles) * kMxScaleTile;
+    ssrc[i] = reinterpret_cast<const char*>(of_x ? a.xs : a.ws) + four0 * s_stride[i];
+    s_off[i] = (uint32_t)tile * kMxScaleTile + (lane & 15) * 16;
+  }
 
   // load i of a step: of x, of the weight, and of the scales with every fourth
   constexpr int N = S::XI + S::WI;
@@ -100,7 +117,8 @@ __global__ void __launch_bounds__(S::NW* kWave) mx_tile_kernel(MxArgs a, int m_t
     else if constexpr (i < N)
       mx_dma(base + XT * kMxTile8 + ((i - S::XI) * NW + wave) * 1024, wsrc[i - S::XI] + (int64_t)t * kMxTile4, lane * 16);
     else
-      mx_dma((uint32_t)(uintptr_t)(scales + (t >> 2 & 1) * S::kScales + wave * 1024), ssrc + (t >> 2) * s_stride, s_off);
+      mx_dma((uint32_t)(uintptr_t)(scales + (t >> 2 & 1) * S::kScales + s_kb[i - N] * 1024),
+             ssrc[i - N] + (t >> 2) * s_stride[i - N], s_off[i - N]);
   };
 
   f32x16 acc[FC][FR];
@@ -164,11 +182,13 @@ __global__ void __launch_bounds__(S::NW* kWave) mx_tile_kernel(MxArgs a, int m_t
   };
   static_assert(2 * M >= F);
 
-  static_for<N + 1>([&](auto i) { issue(i, 0, 0); });
-  if (T > 1) static_for<N>([&](auto i) { issue(i, 1, 1); });
-  if (T > 2) static_for<N>([&](auto i) { issue(i, 2, 2); });
-  if (T > 2) mx_wait<2 * N>();
-  else if (T > 1) mx_wait<N>();
+  // steps 0 .. R - 1, then step 0 has landed
+  constexpr int R = S::R;
+  static_for<R>([&](auto tc) __attribute__((always_inline)) {
+    constexpr int t = decltype(tc)::value;
+    if (t < T) static_for<N + (t % 4 == 0 ? S::SI : 0)>([&](auto i) { issue(i, t, t); });
+  });
+  if (T >= R) mx_wait<(R - 1) * N>();  // R <= 4: scales with step 0 alone
   else mx_wait<0>();
   asm volatile("s_barrier" ::: "memory");
   read_scales(0);
@@ -191,22 +211,24 @@ __global__ void __launch_bounds__(S::NW* kWave) mx_tile_kernel(MxArgs a, int m_t
       multiply(Q0{}, uc, [&](auto m) __attribute__((always_inline)) { read_two(Q1{}, m, slot); });
       const int free = slot;
       if (t + 1 < T) {
-        // step t is in registers and step t + 1 has landed, but for this wave's
-        // loads of step t + 2; then the same of everybody
-        if (t + 2 < T) mx_wait<N + (u == 2 ? 1 : 0)>();
+        // step t is in registers and step t + 1 has landed, all but this wave's
+        // loads of the R - 2 steps after it; then the same of everybody
+        constexpr int later = (R - 2) * N + (u + 2 <= 4 && 4 < u + R ? S::SI : 0);
+        if (t + R - 1 < T) mx_wait<later>();
         else mx_wait<0>();
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        slot = slot == 2 ? 0 : slot + 1;
+        slot = slot == R - 1 ? 0 : slot + 1;
         if constexpr (u == 3) read_scales((t + 1) >> 2);
       }
-      const bool more = t + 3 < T;
+      const bool more = t + R < T;
       multiply(Q1{}, uc, [&](auto m) __attribute__((always_inline)) {
         read_two(Q0{}, m, slot);  // past the last step: read and not used
-        constexpr int i = decltype(m)::value, n = N + (u == 1 ? 1 : 0), per = (n + M - 1) / M;  // loads of step t + 3
+        // loads of step t + R
+        constexpr int i = decltype(m)::value, n = N + ((u + R) % 4 == 0 ? S::SI : 0), per = (n + M - 1) / M;
         if (more)
           static_for<per>([&](auto e) __attribute__((always_inline)) {
             if constexpr (i * per + decltype(e)::value < n)
-              issue(std::integral_constant<int, i * per + decltype(e)::value>{}, t + 3, free);
+              issue(std::integral_constant<int, i * per + decltype(e)::value>{}, t + R, free);
           });
       });
     });
@@ -215,6 +237,22 @@ __global__ void __launch_bounds__(S::NW* kWave) mx_tile_kernel(MxArgs a, int m_t
   // The output goes out in whole rows of the wave's columns, by way of LDS (the
   // ring's: every wave is done with it).  Lane (l32, lg) holds columns 8 q + 4 lg
   // .. + 3 of a fragment, row l32.
+  if constexpr (!S::GATED) {
+    if (a.splits > 1) {  // fp32 sums as they lie; n a multiple of 8
+#pragma unroll
+      for (int i = 0; i < FR; ++i)
+#pragma unroll
+        for (int j = 0; j < FC; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int m = bm * S::TM + (wr * FR + i) * 32 + l32, c = bn * S::OUT + (wc * FC + j) * 32 + 8 * q + 4 * lg;
+            if (m < a.rows && c < a.n)
+              *reinterpret_cast<f32x4*>(a.part + ((int64_t)split * a.rows + m) * a.n + c) =
+                  f32x4{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
+          }
+      return;
+    }
+  }
   constexpr int H = S::GATED ? FC / 2 : FC, C = H * 32, kPitch = C + 8, ROWS = FR * 32;
   static_assert(NW * ROWS * kPitch * 2 <= S::kLds);
   __syncthreads();
@@ -251,24 +289,35 @@ __global__ void __launch_bounds__(S::NW* kWave) mx_tile_kernel(MxArgs a, int m_t
 }
 
 
-// Column tiles a workgroup, splits of k over workgroups and the form of x for
-// the stream kernel: the cheapest by a model of its time in ns, whose constants
-// are fitted to every choice at 116 shapes (1 to 128 rows, 1024 x 1024 to
-// 151936 x 4096); the chosen one is within 1% of the best on the average and 14%
-// at worst.
+// Which kernel serves a product, and how: the cheapest by a model of each one's
+// time in ns, whose constants are fitted to every choice at 222 shapes (1 to
+// 8192 rows, weights of 500 x 2048 to 151936 x 4096); the chosen one is within 1%
+// of the best on the average and 14% at worst.
+//
+// The stream kernel:
 //   - A compute unit takes in weight and x together, however they mix, a KB in
-//     12 ns where two workgroups share it or it has one to run, in 18 where
+//     11 ns where two workgroups share it or it has one to run, in 18 where
 //     one's registers leave no room for another.
-//   - A workgroup's end, its sums through LDS, takes 145 ns a tile.
-//   - Splits cost a pass that adds them: 2 us and their bytes.
-//   - x as fp16 is more bytes to every workgroup and 36 ns of cutting a step
-//     and row tile, and saves the pass that cuts it once, 2.4 us.
-MxConfig choose_stream(int64_t n_rows, int64_t n, int64_t T, bool gated, bool quantised, int cus) {
-  MxConfig best;
+//   - A workgroup's end, its sums through LDS, takes 155 ns a tile.
+//   - x as fp16 is more bytes to every workgroup and 40 ns of cutting a step
+//     and row tile, and saves the pass that cuts it once, 2.6 us.
+// The tile kernel: a step of 128 k takes a workgroup of 128 x 256 890 ns alone on
+// its compute unit, two of them 1430; of 128 x 128 430 and 780.  (One of 256 x
+// 256, eight waves, takes as long as two of 128 x 256 and was no faster where
+// its tiles come out even, 105 us for 8192 x 4096 -> 4096 either way.)
+// Splits of k cost a pass that adds them, 1.9 us and their bytes, and serve
+// rows of whole vectors.
+constexpr double kMxSplitNs = 1900.0, kMxSplitBytesPerNs = 1900.0, kMxCutNs = 2600.0;
+
+double mx_split_ns(int splits, int64_t n_rows, int64_t n) {
+  return splits == 1 ? 0.0 : kMxSplitNs + (double)splits * n_rows * n * 8 / kMxSplitBytesPerNs;
+}
+
+double choose_stream(MxConfig& best, double least, int64_t n_rows, int64_t n, int64_t T, bool gated, bool quantised,
+                     int cus) {
   const int64_t row_tiles = mx_row_tiles(n_rows), chunks = (row_tiles + 7) / 8;
   const int mt = (int)((row_tiles + chunks - 1) / chunks);
   const int64_t out_tiles = (n + 15) / 16;
-  double least = 1e300;
   for (int fp16 = 0; fp16 <= (!quantised && row_tiles <= kMxFp16Tiles ? 1 : 0); ++fp16)
     for (int jw : {1, 2, 3, 4, 6}) {
       if (gated && jw % 2) continue;
@@ -276,19 +325,17 @@ MxConfig choose_stream(int64_t n_rows, int64_t n, int64_t T, bool gated, bool qu
       const int64_t groups = (out_tiles + p - 1) / p * chunks;
       const bool two = 4 * jw * mt + (fp16 ? 34 : 18) * mt + 11 * jw + 12 <= 252;
       for (int splits : {1, 2, 3, 4, 6, 8}) {
-        // a wave has a step at least; sum_partials takes rows of whole vectors
-        if (splits > 1 && (gated || n % 8 || T < kMxWaves * splits)) break;
+        if (splits > 1 && (gated || n % 8 || T < kMxWaves * splits)) break;  // a wave has a step at least
         const int64_t wgs = groups * splits;
         const double rounds = wgs <= 2 * cus ? (double)((wgs + cus - 1) / cus) : (double)wgs / cus + 0.5;
         const double steps = (double)((T + splits - 1) / splits);
-        // rows of x that exist: the others of a tile are not fetched as fp16
-        const double x_kb = fp16 ? n_rows * 0.25 : 2.0 * mt;
-        double t = rounds * (steps * (jw + x_kb) * (wgs > cus && !two ? 18.0 : 12.0) + jw * mt * 145.0);
-        if (splits > 1) t += 2000.0 + (double)splits * n_rows * n * 8 / 1830.0;
-        if (fp16) t += rounds * steps * mt * 36.0;
-        else if (!quantised) t += 2400.0;
+        const double x_kb = fp16 ? n_rows * 0.25 : 2.0 * mt;  // rows of fp16 that do not exist are not fetched
+        const double t = 2700.0 + mx_split_ns(splits, n_rows, n) + (fp16 ? 0.0 : quantised ? 0.0 : kMxCutNs) +
+                         rounds * (steps * ((jw + x_kb) * (wgs > cus && !two ? 18.0 : 11.0) + (fp16 ? 40.0 * mt : 0.0)) +
+                                   jw * mt * 155.0);
         if (t < least) {
           least = t;
+          best = MxConfig{};
           best.mt = mt;
           best.jw = jw;
           best.splits = splits;
@@ -296,36 +343,74 @@ MxConfig choose_stream(int64_t n_rows, int64_t n, int64_t T, bool gated, bool qu
         }
       }
     }
+  return least;
+}
+
+double choose_tile(MxConfig& best, double least, int64_t n_rows, int64_t n, int64_t T, bool gated, bool quantised,
+                   int cus) {
+  for (MxKernel kernel : {kMxTile128x256, kMxTile128}) {
+    const bool wide = kernel == kMxTile128x256;
+    const int64_t columns = (wide ? 256 : 128) / (gated ? 2 : 1);
+    const int64_t tiles = (n_rows + 127) / 128 * ((n + columns - 1) / columns);
+    for (int splits : {1, 2, 3, 4, 6, 8}) {
+      if (splits > 1 && (gated || n % 8 || (T + 3) / 4 < splits)) break;
+      const int64_t wgs = tiles * splits, full = wgs / (2 * cus), rest = wgs - full * 2 * cus;
+      const double one = wide ? 890.0 : 430.0, two = wide ? 1430.0 : 780.0;
+      const double steps = splits == 1 ? (double)T : 4.0 * (((T + 3) / 4 + splits - 1) / splits);
+      const double t = 2800.0 + mx_split_ns(splits, n_rows, n) + (quantised ? 0.0 : kMxCutNs) +
+                       steps * (full * two + (rest == 0 ? 0.0 : rest <= cus ? one : two)) +
+                       (double)(full + (rest > 0)) * (wide ? 1500.0 : 840.0);
+      if (t < least) {
+        least = t;
+        best = MxConfig{};
+        best.kernel = kernel;
+        best.splits = splits;
+      }
+    }
+  }
+  return least;
+}
+
+MxConfig choose_mx(int64_t n_rows, int64_t n, int64_t T, bool gated, bool quantised, int cus) {
+  // The choice of a shape, not worked out anew every call (1.5 us of a decode
+  // step's 7): the last ones of this thread.
+  struct Chosen {
+    int64_t n_rows = -1, n = 0, T = 0;
+    int kind = 0, cus = 0;
+    MxConfig config;
+  };
+  static thread_local Chosen kept[64];
+  const int kind = gated * 2 + quantised;
+  Chosen& c = kept[(uint64_t)(n_rows * 31 + n * 7 + T * 3 + kind) % 64];
+  if (c.n_rows == n_rows && c.n == n && c.T == T && c.kind == kind && c.cus == cus) return c.config;
+  MxConfig best;
+  double least = choose_stream(best, 1e300, n_rows, n, T, gated, quantised, cus);
+  choose_tile(best, least, n_rows, n, T, gated, quantised, cus);
   // A weight that the 256 MB last-level cache cannot keep from call to call
   // streams faster past it: 330 MB, 16 rows 64.9 -> 59.7 us; one that it keeps
   // (13 to 53 MB, called again and again) slower, 3.7 -> 5.5 and 15.1 -> 16.9,
   // and neither way among other weights.
-  best.nt = (double)out_tiles * (gated ? 2 : 1) * T * kMxTile4 > 192e6;
+  best.nt = best.kernel == kMxStream && (double)((n + 15) / 16) * (gated ? 2 : 1) * T * kMxTile4 > 192e6;
+  c = Chosen{n_rows, n, T, kind, cus, best};
   return best;
-}
-
-MxConfig choose_mx(int64_t n_rows, int64_t n, int64_t T, bool gated, bool quantised, int cus) {
-  if (n_rows <= 128) return choose_stream(n_rows, n, T, gated, quantised, cus);
-  MxConfig c;
-  c.tile = true;
-  return c;
 }
 
 template <class S>
 int launch_mx_tile(const MxArgs& a, hipStream_t st) {
   if (int rc = allow_mx_lds<&mx_tile_kernel<S>, S::kLds>()) return rc;
   const int m_tiles = (a.rows + S::TM - 1) / S::TM, n_tiles = (a.n + S::OUT - 1) / S::OUT;
-  hipLaunchKernelGGL(mx_tile_kernel<S>, dim3((unsigned)m_tiles * n_tiles), dim3(S::NW * kWave), S::kLds, st, a, m_tiles,
+  hipLaunchKernelGGL(mx_tile_kernel<S>, dim3((unsigned)m_tiles * n_tiles * a.splits), dim3(S::NW * kWave), S::kLds, st, a, m_tiles,
                      n_tiles);
   return launch_status(S::GATED ? "mxfp4_up_gate_silu_and_mul" : "mxfp4_linear");
 }
 
 template <bool GATED>
 int launch_mx(const MxArgs& a, const MxConfig& c, hipStream_t st) {
-  if (!c.tile) return GATED ? mx_stream_gated(a, c, st) : mx_stream_linear(a, c, st);
-  const int64_t big = (int64_t)((a.rows + 255) / 256) * ((a.n + (GATED ? 127 : 255)) / (GATED ? 128 : 256));
-  if (big >= 200) return launch_mx_tile<MxTile<4, 2, 2, 4, GATED>>(a, st);
-  return launch_mx_tile<MxTile<2, 2, 2, 2, GATED>>(a, st);
+  switch (c.kernel) {
+    case kMxTile128x256: return launch_mx_tile<MxTile<2, 2, 2, 4, 2, GATED>>(a, st);
+    case kMxTile128: return launch_mx_tile<MxTile<2, 2, 2, 2, 3, GATED>>(a, st);
+    default: return GATED ? mx_stream_gated(a, c, st) : mx_stream_linear(a, c, st);
+  }
 }
 
 int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
