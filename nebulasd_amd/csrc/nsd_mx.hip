@@ -17,41 +17,42 @@ namespace {
 
 constexpr int kMxThreads = 256;
 
-__device__ inline float bf16_bits_to_float(uint32_t b) { return __builtin_bit_cast(float, b << 16); }
 __device__ inline float float_of_bits(uint32_t b) { return __builtin_bit_cast(float, b); }
 __device__ inline uint32_t bits_of(float f) { return __builtin_bit_cast(uint32_t, f); }
 
-// Block values in fp32.
+// A block as it lies, and its values in fp32.
 template <typename T>
-__device__ inline void load_block(const T* p, float (&v)[kMxBlock]);
-template <>
-__device__ inline void load_block<f16>(const f16* p, float (&v)[kMxBlock]) {
+struct MxRaw {
+  u32x4 v[sizeof(T) * kMxBlock / 16];
+  __device__ void load(const T* p) {
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(v) / 16; ++i) v[i] = reinterpret_cast<const u32x4*>(p)[i];
+  }
+};
+__device__ inline void values(const MxRaw<f16>& raw, float (&v)[kMxBlock]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const f16x8 h = reinterpret_cast<const f16x8*>(p)[i];
+    const f16x8 h = __builtin_bit_cast(f16x8, raw.v[i]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[8 * i + e] = (float)h[e];
   }
 }
-template <>
-__device__ inline void load_block<uint16_t>(const uint16_t* p, float (&v)[kMxBlock]) {  // bf16
+__device__ inline void values(const MxRaw<uint16_t>& raw, float (&v)[kMxBlock]) {  // bf16
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const u32x4 h = reinterpret_cast<const u32x4*>(p)[i];
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      v[8 * i + 2 * e] = bf16_bits_to_float(h[e] & 0xffffu);
-      v[8 * i + 2 * e + 1] = float_of_bits(h[e] & 0xffff0000u);
+      const uint32_t two = raw.v[i][e];
+      v[8 * i + 2 * e] = float_of_bits(two << 16);
+      v[8 * i + 2 * e + 1] = float_of_bits(two & 0xffff0000u);
     }
-  }
 }
-template <>
-__device__ inline void load_block<float>(const float* p, float (&v)[kMxBlock]) {
+__device__ inline void values(const MxRaw<float>& raw, float (&v)[kMxBlock]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const f32x4 h = reinterpret_cast<const f32x4*>(p)[i];
+    const f32x4 f = __builtin_bit_cast(f32x4, raw.v[i]);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[4 * i + e] = h[e];
+    for (int e = 0; e < 4; ++e) v[4 * i + e] = f[e];
   }
 }
 
@@ -64,8 +65,8 @@ __device__ inline uint32_t largest_bits(const float (&v)[kMxBlock]) {
   return m;
 }
 
-// One wave per (row tile, four tiles of k): the lane's four scale bytes go out
-// as one word.
+// One wave per (row tile, four tiles of k): the loads of all four go out before
+// the first is worked on, and the lane's four scale bytes leave as one word.
 template <typename T>
 __global__ void __launch_bounds__(kMxThreads)
 mxfp4_quantize_kernel(const T* __restrict__ w, int64_t n_out, int n_in, int row_tiles, int k_tiles,
@@ -76,37 +77,39 @@ mxfp4_quantize_kernel(const T* __restrict__ w, int64_t n_out, int n_in, int row_
   if (unit >= row_tiles * groups) return;
   const int64_t tile = unit / groups, row = tile * 16 + i;
   const int kg = unit % groups;
+  // a block that does not exist (a row or run of k past the end) is zeros: the
+  // first block of the weight is read in its place
+  MxRaw<T> raw[4];
+  bool live[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const int k = (4 * kg + t) * kMxTileK + g * kMxBlock;
+    live[t] = row < n_out && k < n_in;
+    raw[t].load(w + (live[t] ? row * n_in + k : 0));
+  }
   uint32_t word = 0;
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
-    const int kt = 4 * kg + t;
-    if (kt >= k_tiles) break;
-    const int k = kt * kMxTileK + g * kMxBlock;
-    u32x4 out = {0, 0, 0, 0};
-    uint32_t s = 0;
-    if (row < n_out && k < n_in) {
-      float v[kMxBlock];
-      load_block(w + row * n_in + k, v);
-      const uint32_t m = largest_bits(v);
-      if (m >= 0x7f800000u) {
-        s = kMxNanScale;
-      } else {
-        // floor(log2 m) - 2; below 2^-125 (the field of subnormals is 0) the
-        // smallest scale.  v 2^(127 - s): exact, or far below half a code
-        s = max((int)(m >> 23) - 2, 0);
-        const float inv = float_of_bits((254u - s) << 23);
+    float v[kMxBlock];
+    values(raw[t], v);
+    uint32_t m = largest_bits(v);
+    if (!live[t]) m = 0;
+    // floor(log2 m) - 2; below 2^-125 (the field of subnormals is 0) the
+    // smallest scale.  v 2^(127 - s): exact, or far below half a code
+    const uint32_t s = m >= 0x7f800000u ? kMxNanScale : max((int)(m >> 23) - 2, 0);
+    const float inv = live[t] && s != kMxNanScale ? float_of_bits((254u - s) << 23) : 0.f;
+    u32x4 out;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t c = 0;
-          c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * q] * inv, v[8 * q + 1] * inv, 1.f, 0);
-          c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * q + 2] * inv, v[8 * q + 3] * inv, 1.f, 1);
-          c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * q + 4] * inv, v[8 * q + 5] * inv, 1.f, 2);
-          c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * q + 6] * inv, v[8 * q + 7] * inv, 1.f, 3);
-          out[q] = c;
-        }
-      }
+    for (int q = 0; q < 4; ++q) {
+      uint32_t c = 0;
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * q] * inv, v[8 * q + 1] * inv, 1.f, 0);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * q + 2] * inv, v[8 * q + 3] * inv, 1.f, 1);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * q + 4] * inv, v[8 * q + 5] * inv, 1.f, 2);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * q + 6] * inv, v[8 * q + 7] * inv, 1.f, 3);
+      out[q] = live[t] && s != kMxNanScale ? c : 0;
     }
-    codes[(tile * k_tiles + kt) * 64 + lane] = out;
+    const int kt = 4 * kg + t;
+    if (kt < k_tiles) codes[(tile * k_tiles + kt) * 64 + lane] = out;
     word |= s << (8 * t);
   }
   scales[((int64_t)kg * row_tiles + tile) * 64 + lane] = word;
@@ -209,34 +212,42 @@ __device__ inline void store8<float>(float* p, const float (&v)[8]) {
     reinterpret_cast<f32x4*>(p)[e] = f32x4{v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]};
 }
 
+// One wave per (row tile, tile of k), a lane eight values of a row at a time:
+// sixteen lanes a row of the tile, so a store is whole runs of four rows.  (A
+// lane a block, each store 16 of every 64 bytes, took 88 us for 8192 x 12288
+// and now takes MEASURED.)
 template <int BITS, typename T>
 __global__ void __launch_bounds__(kMxThreads)
-mx_dequantize_kernel(const u32x4* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t n_rows, int n_in,
+mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t n_rows, int n_in,
                      int row_tiles, int k_tiles, T* __restrict__ out) {
-  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, c = lane & 15;
   const int unit = wave_unit();
   if (unit >= row_tiles * k_tiles) return;
-  const int64_t tile = unit / k_tiles, row = tile * 16 + i;
-  const int kt = unit % k_tiles, k = kt * kMxTileK + g * kMxBlock;
-  if (row >= n_rows || k >= n_in) return;
-  const float s = scale_of(scales[((int64_t)(kt >> 2) * row_tiles + tile) * kMxScaleTile + lane * 4 + (kt & 3)]);
-  T* dst = out + row * n_in + k;
-  u32x4 c[BITS / 4];
-  if constexpr (BITS == 4) {
-    c[0] = codes[(tile * k_tiles + kt) * 64 + lane];
-  } else {
-    c[0] = codes[(tile * k_tiles + kt) * 128 + 2 * g * 16 + i];
-    c[1] = codes[(tile * k_tiles + kt) * 128 + 2 * g * 16 + i + 16];
+  const int64_t tile = unit / k_tiles;
+  const int kt = unit % k_tiles, k = kt * kMxTileK + c * 8;
+  const uint8_t* src = codes + (tile * k_tiles + kt) * (BITS == 4 ? kMxTile4 : kMxTile8);
+  const uint8_t* sc = scales + ((int64_t)(kt >> 2) * row_tiles + tile) * kMxScaleTile + (kt & 3);
+  u32x2 code[4];
+  uint32_t s[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int i = 4 * q + (lane >> 4);  // row of the tile
+    if constexpr (BITS == 4) code[q][0] = *reinterpret_cast<const uint32_t*>(src + c / 4 * 256 + i * 16 + c % 4 * 4);
+    else code[q] = *reinterpret_cast<const u32x2*>(src + c / 2 * 256 + i * 16 + c % 2 * 8);
+    s[q] = sc[(c / 4 * 16 + i) * 4];
   }
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
+    const int64_t row = tile * 16 + 4 * q + (lane >> 4);
+    if (row >= n_rows || k >= n_in) continue;
+    const float f = scale_of(s[q]);
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      if constexpr (BITS == 4) v[e] = e2m1_value(c[0][q] >> (4 * e)) * s;
-      else v[e] = e4m3_value(c[q / 2][q % 2 * 2 + e / 4] >> (8 * (e % 4))) * s;
+      if constexpr (BITS == 4) v[e] = e2m1_value(code[q][0] >> (4 * e)) * f;
+      else v[e] = e4m3_value(code[q][e / 4] >> (8 * (e % 4))) * f;
     }
-    store8(dst + 8 * q, v);
+    store8(out + row * n_in + k, v);
   }
 }
 
@@ -274,7 +285,7 @@ int dequantize(const char* who, const void* codes, const void* scales, int64_t n
   const int64_t rt = mx_row_tiles(n_rows), kt = mx_k_tiles(n_in);
   auto go = [&](auto* p) {
     hipLaunchKernelGGL((mx_dequantize_kernel<BITS, std::remove_pointer_t<decltype(p)>>), dim3(wave_grid(rt * kt)),
-                       dim3(kMxThreads), 0, as_stream(stream), static_cast<const u32x4*>(codes),
+                       dim3(kMxThreads), 0, as_stream(stream), static_cast<const uint8_t*>(codes),
                        static_cast<const uint8_t*>(scales), n_rows, (int)n_in, (int)rt, (int)kt, p);
   };
   if (dtype == NSD_DTYPE_F16) go(static_cast<f16*>(out));

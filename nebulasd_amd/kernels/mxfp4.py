@@ -19,7 +19,6 @@ quantised once with ``mxfp8_quantize`` and given instead.
 from __future__ import annotations
 
 import ctypes
-import dataclasses
 import functools
 
 import torch
@@ -40,30 +39,26 @@ def _check_blocks(codes, scales, bits: int, rows: int, n_in: int) -> None:
     _same_device(codes, scales)
 
 
-@dataclasses.dataclass(frozen=True)
 class MXFP4Weight:
     """A weight [n_out, n_in] in MXFP4: codes and scales (uint8) in the kernels' layout."""
 
-    codes: torch.Tensor
-    scales: torch.Tensor
-    n_out: int
-    n_in: int
+    __slots__ = ("codes", "scales", "n_out", "n_in")
 
-    def __post_init__(self):
-        _check_blocks(self.codes, self.scales, 4, self.n_out, self.n_in)
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, n_out: int, n_in: int, _made: bool = False):
+        if not _made:
+            _check_blocks(codes, scales, 4, n_out, n_in)
+        self.codes, self.scales, self.n_out, self.n_in = codes, scales, n_out, n_in
 
 
-@dataclasses.dataclass(frozen=True)
 class MXFP8Rows:
     """Rows [rows, n_in] in MXFP8: codes and scales (uint8) in the kernels' layout."""
 
-    codes: torch.Tensor
-    scales: torch.Tensor
-    rows: int
-    n_in: int
+    __slots__ = ("codes", "scales", "rows", "n_in")
 
-    def __post_init__(self):
-        _check_blocks(self.codes, self.scales, 8, self.rows, self.n_in)
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, n_in: int, _made: bool = False):
+        if not _made:
+            _check_blocks(codes, scales, 8, rows, n_in)
+        self.codes, self.scales, self.rows, self.n_in = codes, scales, rows, n_in
 
 
 @functools.lru_cache(maxsize=4096)
@@ -100,9 +95,9 @@ def _matrix(t: torch.Tensor, name: str) -> None:
         raise ValueError(f"{name} must be [rows, n_in] with n_in a multiple of {BLOCK}, got {tuple(t.shape)}")
 
 
-def _empty(bits: int, rows: int, n_in: int, device):
+def _empty(bits: int, rows: int, n_in: int, like: torch.Tensor):
     c, s = _bytes(bits, rows, n_in)
-    return (torch.empty(c, dtype=torch.uint8, device=device), torch.empty(s, dtype=torch.uint8, device=device))
+    return like.new_empty(c, dtype=torch.uint8), like.new_empty(s, dtype=torch.uint8)
 
 
 def mxfp4_quantize(w: torch.Tensor) -> MXFP4Weight:
@@ -113,9 +108,9 @@ def mxfp4_quantize(w: torch.Tensor) -> MXFP4Weight:
         raise TypeError(f"w must be fp16, bf16 or fp32, got {w.dtype}")
     require(w, w.dtype, "w")
     n_out, n_in = w.shape
-    codes, scales = _empty(4, n_out, n_in, w.device)
+    codes, scales = _empty(4, n_out, n_in, w)
     _call(w, "nsd_mxfp4_quantize", w.data_ptr(), _DTYPES[w.dtype], n_out, n_in, codes.data_ptr(), scales.data_ptr())
-    return MXFP4Weight(codes, scales, n_out, n_in)
+    return MXFP4Weight(codes, scales, n_out, n_in, _made=True)
 
 
 def mxfp4_pack(codes: torch.Tensor, scales: torch.Tensor) -> MXFP4Weight:
@@ -130,9 +125,9 @@ def mxfp4_pack(codes: torch.Tensor, scales: torch.Tensor) -> MXFP4Weight:
                          f"{tuple(codes.shape)} and {tuple(scales.shape)}")
     _same_device(codes, scales)
     n_out, n_in = codes.shape[0], 2 * codes.shape[1]
-    out = _empty(4, n_out, n_in, codes.device)
+    out = _empty(4, n_out, n_in, codes)
     _call(codes, "nsd_mxfp4_pack", codes.data_ptr(), scales.data_ptr(), n_out, n_in, *(t.data_ptr() for t in out))
-    return MXFP4Weight(*out, n_out, n_in)
+    return MXFP4Weight(*out, n_out, n_in, _made=True)
 
 
 def mxfp8_quantize(x: torch.Tensor) -> MXFP8Rows:
@@ -141,15 +136,15 @@ def mxfp8_quantize(x: torch.Tensor) -> MXFP8Rows:
     _matrix(x, "x")
     require(x, torch.float16, "x")
     rows, n_in = x.shape
-    codes, scales = _empty(8, rows, n_in, x.device)
+    codes, scales = _empty(8, rows, n_in, x)
     _call(x, "nsd_mxfp8_quantize", x.data_ptr(), rows, n_in, codes.data_ptr(), scales.data_ptr())
-    return MXFP8Rows(codes, scales, rows, n_in)
+    return MXFP8Rows(codes, scales, rows, n_in, _made=True)
 
 
 def _dequantize(b, rows: int, dtype: torch.dtype, name: str) -> torch.Tensor:
     if dtype not in _DTYPES:
         raise TypeError(f"dtype must be fp16, bf16 or fp32, got {dtype}")
-    out = torch.empty((rows, b.n_in), dtype=dtype, device=b.codes.device)
+    out = b.codes.new_empty((rows, b.n_in), dtype=dtype)
     _call(out, name, b.codes.data_ptr(), b.scales.data_ptr(), rows, b.n_in, out.data_ptr(), _DTYPES[dtype])
     return out
 
