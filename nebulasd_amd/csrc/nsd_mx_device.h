@@ -160,7 +160,7 @@ struct MxConfig {
 };
 
 constexpr int kMxWaves = 4;      // of a workgroup of the stream kernel
-constexpr int kMxFp16Tiles = 2;  // row tiles that it takes as fp16
+constexpr int kMxFp16Tiles = 4;  // row tiles that it takes as fp16
 
 // Up to 128 rows (nsd_mx_stream.h): y = x . W^T, and its gated form.
 int mx_stream_linear(const MxArgs& a, const MxConfig& c, hipStream_t st);

@@ -219,8 +219,11 @@ int launch_mx_stream(const MxArgs& a, hipStream_t st) {
 template <int MT, int JW, bool GATED>
 int launch_mx_stream(const MxArgs& a, const MxConfig& c, hipStream_t st) {
   if constexpr (MT <= kMxFp16Tiles)
-    if (c.fp16)
-      return c.nt ? launch_mx_stream<MT, JW, GATED, true, true>(a, st) : launch_mx_stream<MT, JW, GATED, true, false>(a, st);
+    if (c.fp16) {
+      if constexpr (MT == 1)
+        if (c.nt) return launch_mx_stream<MT, JW, GATED, true, true>(a, st);
+      return launch_mx_stream<MT, JW, GATED, true, false>(a, st);
+    }
   return c.nt ? launch_mx_stream<MT, JW, GATED, false, true>(a, st) : launch_mx_stream<MT, JW, GATED, false, false>(a, st);
 }
 
