@@ -72,9 +72,14 @@ int nsd_mxfp8_dequantize(const void* codes, const void* scales, int64_t n_rows, 
  * exp(-g))) in fp32, up and g the products with weight rows j and inter + j of
  * a [2 * inter, n_in] weight; inter a multiple of 16.
  *
- * workspace: nsd_mx_workspace bytes for the call's shape (gated: of the second;
- * quantised: x is given as codes), contents irrelevant; calls that overlap each
- * need their own.
+ * y must not overlap x (NSD_ERR_INVALID).  A row's sums may be added in another
+ * order, and end in another last place, in a batch of another size; the same
+ * call gives the same bits.  n_rows up to 2^21, n_out up to 2^27, n_in up to 2^20.
+ *
+ * workspace: nsd_mx_workspace bytes for the call's shape on the current device
+ * (n_out: the weight's rows; gated: of nsd_mxfp4_up_gate_silu_and_mul; quantised:
+ * x is given as codes), contents irrelevant; calls that overlap each need their
+ * own.
  */
 int nsd_mx_workspace(int64_t n_rows, int64_t n_out, int64_t n_in, int gated, int quantised, int64_t* bytes);
 int nsd_mxfp4_linear(const void* x, const void* x_codes, const void* x_scales, const void* w_codes,

@@ -2,6 +2,8 @@
 // operand form, shared by the quantisers and the products.
 #pragma once
 
+#include <atomic>
+
 #include "nsd_device.h"
 #include "nsd_mx.h"
 
@@ -166,12 +168,20 @@ constexpr int kMxFp16Tiles = 4;  // row tiles that it takes as fp16
 int mx_stream_linear(const MxArgs& a, const MxConfig& c, hipStream_t st);
 int mx_stream_gated(const MxArgs& a, const MxConfig& c, hipStream_t st);
 
-// Raises a kernel's dynamic-LDS limit once per process.
+// Raises a kernel's dynamic-LDS limit once per device.
 template <auto Kernel, int kLds>
 int allow_mx_lds() {
-  static const hipError_t attr =
-      hipFuncSetAttribute(reinterpret_cast<const void*>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
-  return attr == hipSuccess ? NSD_OK : fail(NSD_ERR_HIP, "mxfp4: LDS attribute: %s", hipGetErrorString(attr));
+  constexpr int kMaxDevices = 64;
+  static std::atomic<bool> done[kMaxDevices];
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  const bool known = e == hipSuccess && dev >= 0 && dev < kMaxDevices;
+  if (known && done[dev].load(std::memory_order_relaxed)) return NSD_OK;
+  if (e == hipSuccess)
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+  if (e != hipSuccess) return fail(NSD_ERR_HIP, "mxfp4: LDS attribute: %s", hipGetErrorString(e));
+  if (known) done[dev].store(true, std::memory_order_relaxed);
+  return NSD_OK;
 }
 
 // Activations to MXFP8 (arguments checked by the caller); in nsd_mx.hip.

@@ -38,6 +38,7 @@ struct MxTile {
   static constexpr bool GATED = GATED_;
   static constexpr int NW = WR * WC, XT = WR * FR * 2, WT = WC * FC * 2;  // 16-row tiles of x and of the weight
   static constexpr int TM = XT * 16, TN = WT * 16, OUT = GATED ? TN / 2 : TN;
+  static constexpr bool kSplits = !GATED && TN == 128;
   static constexpr int SK = (XT + WT) / 4;  // KB of scales of four steps
   // loads a wave, 1 KB each: a step's x and weight, four steps' scales
   static constexpr int XI = 2 * XT / NW, WI = WT / NW, SI = (SK + NW - 1) / NW;
@@ -237,7 +238,7 @@ __global__ void __launch_bounds__(S::NW* kWave, 2) mx_tile_kernel(MxArgs a, int 
   // The output goes out in whole rows of the wave's columns, by way of LDS (the
   // ring's: every wave is done with it).  Lane (l32, lg) holds columns 8 q + 4 lg
   // .. + 3 of a fragment, row l32.
-  if constexpr (!S::GATED) {
+  if constexpr (S::kSplits) {
     if (a.splits > 1) {  // fp32 sums as they lie; n a multiple of 8
 #pragma unroll
       for (int i = 0; i < FR; ++i)
@@ -298,19 +299,21 @@ __global__ void __launch_bounds__(S::NW* kWave, 2) mx_tile_kernel(MxArgs a, int 
 //   - A compute unit takes in weight and x together, however they mix, a KB in
 //     11 ns where two workgroups share it or it has one to run, in 18 where
 //     one's registers leave no room for another.
-//   - A workgroup's end, its sums through LDS, takes 155 ns a tile.
-//   - x as fp16 is more bytes to every workgroup and 40 ns of cutting a step
+//   - A workgroup's end, its sums through LDS, takes 175 ns a tile.
+//   - x as fp16 is more bytes to every workgroup and 39 ns of cutting a step
 //     and row tile, and saves the pass that cuts it once, 2.6 us.
-// The tile kernel: a step of 128 k takes a workgroup of 128 x 256 890 ns alone on
-// its compute unit, two of them 1430; of 128 x 128 430 and 780.  (One of 256 x
+// The tile kernel: a step of 128 k takes a workgroup of 128 x 256 900 ns alone on
+// its compute unit, two of them 1430; of 128 x 128 425 and 780.  (One of 256 x
 // 256, eight waves, takes as long as two of 128 x 256 and was no faster where
 // its tiles come out even, 105 us for 8192 x 4096 -> 4096 either way.)
-// Splits of k cost a pass that adds them, 1.9 us and their bytes, and serve
-// rows of whole vectors.
-constexpr double kMxSplitNs = 1900.0, kMxSplitBytesPerNs = 1900.0, kMxCutNs = 2600.0;
+// Splits of k cost a pass that adds them, 2.1 us and their bytes, at 3 TB/s the
+// stream kernel's, whose stores are runs of 64 bytes, and 4.6 the other's; they
+// serve rows of whole vectors.  (The 128 x 256 tile has none: what it serves
+// fills the device without.)
+constexpr double kMxCutNs = 2600.0;
 
-double mx_split_ns(int splits, int64_t n_rows, int64_t n) {
-  return splits == 1 ? 0.0 : kMxSplitNs + (double)splits * n_rows * n * 8 / kMxSplitBytesPerNs;
+double mx_split_ns(int splits, int64_t n_rows, int64_t n, double bytes_per_ns) {
+  return splits == 1 ? 0.0 : 2100.0 + (double)splits * n_rows * n * 8 / bytes_per_ns;
 }
 
 double choose_stream(MxConfig& best, double least, int64_t n_rows, int64_t n, int64_t T, bool gated, bool quantised,
@@ -330,9 +333,9 @@ double choose_stream(MxConfig& best, double least, int64_t n_rows, int64_t n, in
         const double rounds = wgs <= 2 * cus ? (double)((wgs + cus - 1) / cus) : (double)wgs / cus + 0.5;
         const double steps = (double)((T + splits - 1) / splits);
         const double x_kb = fp16 ? n_rows * 0.25 : 2.0 * mt;  // rows of fp16 that do not exist are not fetched
-        const double t = 2700.0 + mx_split_ns(splits, n_rows, n) + (fp16 ? 0.0 : quantised ? 0.0 : kMxCutNs) +
-                         rounds * (steps * ((jw + x_kb) * (wgs > cus && !two ? 18.0 : 11.0) + (fp16 ? 40.0 * mt : 0.0)) +
-                                   jw * mt * 155.0);
+        const double t = 2700.0 + mx_split_ns(splits, n_rows, n, 3000.0) + (fp16 || quantised ? 0.0 : kMxCutNs) +
+                         rounds * (steps * ((jw + x_kb) * (wgs > cus && !two ? 18.0 : 11.0) + (fp16 ? 39.0 * mt : 0.0)) +
+                                   jw * mt * 175.0);
         if (t < least) {
           least = t;
           best = MxConfig{};
@@ -353,13 +356,13 @@ double choose_tile(MxConfig& best, double least, int64_t n_rows, int64_t n, int6
     const int64_t columns = (wide ? 256 : 128) / (gated ? 2 : 1);
     const int64_t tiles = (n_rows + 127) / 128 * ((n + columns - 1) / columns);
     for (int splits : {1, 2, 3, 4, 6, 8}) {
-      if (splits > 1 && (gated || n % 8 || (T + 3) / 4 < splits)) break;
+      if (splits > 1 && (wide || gated || n % 8 || (T + 3) / 4 < splits)) break;
       const int64_t wgs = tiles * splits, full = wgs / (2 * cus), rest = wgs - full * 2 * cus;
-      const double one = wide ? 890.0 : 430.0, two = wide ? 1430.0 : 780.0;
+      const double one = wide ? 900.0 : 425.0, two = wide ? 1430.0 : 780.0;
       const double steps = splits == 1 ? (double)T : 4.0 * (((T + 3) / 4 + splits - 1) / splits);
-      const double t = 2800.0 + mx_split_ns(splits, n_rows, n) + (quantised ? 0.0 : kMxCutNs) +
+      const double t = 3300.0 + mx_split_ns(splits, n_rows, n, 4600.0) + (quantised ? 0.0 : kMxCutNs) +
                        steps * (full * two + (rest == 0 ? 0.0 : rest <= cus ? one : two)) +
-                       (double)(full + (rest > 0)) * (wide ? 1500.0 : 840.0);
+                       (double)(full + (rest > 0)) * (wide ? 1900.0 : 860.0);
       if (t < least) {
         least = t;
         best = MxConfig{};
@@ -413,6 +416,10 @@ int launch_mx(const MxArgs& a, const MxConfig& c, hipStream_t st) {
   }
 }
 
+bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  const uintptr_t p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b);
+  return a && b && p < q + b_bytes && q < p + a_bytes;
+}
 int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 
 int check_product(const char* who, int64_t n_rows, int64_t n, int64_t n_in) {
@@ -450,6 +457,12 @@ int product(const char* who, const void* x, const void* x_codes, const void* x_s
     return fail(NSD_ERR_INVALID, "%s: null pointer", who);
   for (const void* p : {x, x_codes, x_scales, w_codes, w_scales, (const void*)y, (const void*)workspace})
     if (!aligned16(p)) return fail(NSD_ERR_UNSUPPORTED, "%s: pointers must be 16-byte aligned", who);
+  // workgroups that are done write y while others still read x
+  int64_t codes = 0, scales = 0;
+  (void)nsd_mx_bytes(8, n_rows, n_in, &codes, &scales);
+  const int64_t y_bytes = n_rows * n * 2;
+  if (overlap(y, y_bytes, x, n_rows * n_in * 2) || (!x && (overlap(y, y_bytes, x_codes, codes) || overlap(y, y_bytes, x_scales, scales))))
+    return fail(NSD_ERR_INVALID, "%s: y overlaps x", who);
   int cus = 0;
   if (int rc = device_cus(&cus)) return rc;
   const int64_t T = mx_k_tiles(n_in);
@@ -460,10 +473,9 @@ int product(const char* who, const void* x, const void* x_codes, const void* x_s
                 (long long)need.total());
   char* ws = static_cast<char*>(workspace);
   if (x && !c.fp16) {
-    void *codes = ws, *scales = ws + align256(need.codes);
-    if (int rc = mxfp8_quantize(x, n_rows, n_in, codes, scales, stream)) return rc;
-    x_codes = codes;
-    x_scales = scales;
+    if (int rc = mxfp8_quantize(x, n_rows, n_in, ws, ws + align256(need.codes), stream)) return rc;
+    x_codes = ws;
+    x_scales = ws + align256(need.codes);
   }
   MxArgs a{};
   a.x = static_cast<const f16*>(x);

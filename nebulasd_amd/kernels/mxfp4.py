@@ -39,6 +39,10 @@ def _check_blocks(codes, scales, bits: int, rows: int, n_in: int) -> None:
     _same_device(codes, scales)
 
 
+def _fixed(self, name, value):
+    raise AttributeError(f"{type(self).__name__} is fixed once made: its sizes were checked then")
+
+
 class MXFP4Weight:
     """A weight [n_out, n_in] in MXFP4: codes and scales (uint8) in the kernels' layout."""
 
@@ -47,7 +51,10 @@ class MXFP4Weight:
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, n_out: int, n_in: int, _made: bool = False):
         if not _made:
             _check_blocks(codes, scales, 4, n_out, n_in)
-        self.codes, self.scales, self.n_out, self.n_in = codes, scales, n_out, n_in
+        for name, v in zip(self.__slots__, (codes, scales, n_out, n_in)):
+            object.__setattr__(self, name, v)
+
+    __setattr__ = _fixed
 
 
 class MXFP8Rows:
@@ -58,7 +65,10 @@ class MXFP8Rows:
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, n_in: int, _made: bool = False):
         if not _made:
             _check_blocks(codes, scales, 8, rows, n_in)
-        self.codes, self.scales, self.rows, self.n_in = codes, scales, rows, n_in
+        for name, v in zip(self.__slots__, (codes, scales, rows, n_in)):
+            object.__setattr__(self, name, v)
+
+    __setattr__ = _fixed
 
 
 @functools.lru_cache(maxsize=4096)

@@ -94,8 +94,7 @@ def mx_linear_bound(x, w_values):
     those last places; sums of blocks are fp32: another 2^-24 of the absolute sum for each of the n_in / 32 + 16
     additions (16 waves' sums and splits joined at most)."""
     xv, wv = np.abs(mx_values(*mx_quantize(x, 8), 8)), np.abs(w_values)
-    r, k = xv.shape
-    top = np.zeros((r, len(wv)))
-    for b in range(0, k, MX_BLOCK):  # the largest product is at most the product of the largest
-        top += xv[:, b:b + MX_BLOCK].max(1)[:, None] * wv[:, b:b + MX_BLOCK].max(1)[None]
-    return 32 * 2.0 ** -15 * top + (k // MX_BLOCK + 16) * 2.0 ** -24 * (xv @ wv.T)
+    k = xv.shape[1]
+    # a block's largest product is at most the product of its largest values
+    top = [v.reshape(len(v), k // MX_BLOCK, MX_BLOCK).max(2) for v in (xv, wv)]
+    return 32 * 2.0 ** -15 * (top[0] @ top[1].T) + (k // MX_BLOCK + 16) * 2.0 ** -24 * (xv @ wv.T)

@@ -143,7 +143,14 @@ SHAPES = [(1, 16, 32), (1, 1024, 1024), (3, 17, 96), (16, 33, 128), (17, 1, 160)
           (48, 250, 2080), (49, 4096, 256), (64, 6144, 1024), (65, 515, 4096), (80, 4096, 4096), (81, 96, 12288),
           (97, 2048, 2048), (112, 48, 8192), (113, 1001, 640), (128, 1024, 4096), (129, 300, 1024), (200, 1536, 608),
           (257, 255, 2048), (513, 130, 1056), (1000, 1040, 512), (16, 20001, 256),
-          (2049, 6500, 416), (1030, 13001, 96)]
+          (2049, 6500, 416), (1030, 13001, 96),
+          # every count of column tiles a workgroup, with x as fp16 and in blocks; splits of k; the tile kernel's
+          # shapes at one to five tiles of k, splits of it, and rows that start at whole vectors, at even and odd values
+          (1, 4248, 32), (1, 9104, 32), (1, 13440, 32), (1, 21320, 32), (24, 8328, 32), (23, 12680, 32),
+          (34, 18952, 64), (60, 9216, 32), (1, 16, 5472), (1, 736, 6112), (17, 704, 5248), (68, 64, 3392),
+          (66, 1368, 6528), (84, 4104, 288), (135, 5032, 576), (132, 6424, 960), (154, 8288, 1952), (122, 16, 32),
+          (81, 4464, 256), (300, 1999, 352), (300, 2002, 672), (451, 352, 5664), (917, 168, 6528), (810, 14112, 256),
+          (1500, 9216, 640)]
 
 
 @pytest.mark.parametrize("rows,n,k", SHAPES, ids=[f"{r}x{n}x{k}" for r, n, k in SHAPES])
@@ -162,7 +169,9 @@ def test_linear_matches_oracle(gpu, rows, n, k):
 
 GATED = [(1, 16, 32), (1, 2816, 1024), (5, 48, 544), (16, 12288, 256), (33, 1024, 1056), (64, 2816, 1024),
          (80, 1600, 4096), (100, 32, 8192), (128, 4096, 512), (129, 160, 1024), (300, 1040, 288), (700, 528, 2048),
-         (1100, 6416, 288)]
+         (1100, 6416, 288),
+         (1, 5344, 32), (1, 11488, 32), (22, 5520, 32), (19, 10800, 32), (35, 7888, 32), (50, 4480, 32), (49, 9360, 320),
+         (81, 12288, 320), (65, 16, 32), (158, 12832, 64)]
 
 
 @pytest.mark.parametrize("rows,inter,k", GATED, ids=[f"{r}x{n}x{k}" for r, n, k in GATED])
@@ -264,6 +273,11 @@ def test_refusals(gpu):
         K.mxfp4_pack(torch.zeros(4, 16, dtype=torch.uint8, device=gpu), torch.zeros(4, 2, dtype=torch.uint8, device=gpu))
     with pytest.raises(ValueError, match="bytes of codes"):
         K.MXFP4Weight(w.codes[:-16], w.scales, 64, 256)
+    with pytest.raises(AttributeError, match="fixed"):
+        w.codes = w.codes[:-16]
+    square, _ = _weight(gpu, 256, 256)
+    with pytest.raises(_lib.NativeLibraryError, match="overlaps"):
+        K.mxfp4_linear(x, square, out=x)
     with pytest.raises(ValueError, match="GPU tensors"):
         K.mxfp4_linear(x.cpu(), w)
     buf = torch.zeros(2 * 256 + 4, dtype=torch.float16, device=gpu)

@@ -161,6 +161,9 @@ def test_entries_refuse_before_any_launch(lib):
     refused(2, lib.nsd_mxfp4_linear(ok, None, None, ok, ok, ok, 1, 0, 32, None, 0, None), "n_out=0")
     refused(2, lib.nsd_mxfp4_linear(ok, None, None, ok, ok, ok, 2 ** 22, 16, 32, None, 0, None), "n_rows")
     refused(2, lib.nsd_mxfp4_up_gate_silu_and_mul(ok, None, None, ok, ok, ok, 1, 24, 32, None, 0, None), "inter=24")
+    refused(1, lib.nsd_mxfp4_linear(ok, None, None, ok, ok, ok + 32, 1, 32, 32, None, 0, None), "overlaps")
+    refused(1, lib.nsd_mxfp4_linear(None, ok, ok, 1 << 20, 1 << 20, ok, 1, 32, 32, None, 0, None), "overlaps")
+    refused(2, lib.nsd_mxfp4_linear(ok, None, None, ok, ok, 1 << 20, 1, 32, 2 ** 20 + 32, None, 0, None), "n_in=1048608")
     # no rows: nothing to launch
     assert lib.nsd_mxfp4_linear(None, None, None, None, None, None, 0, 16, 32, None, 0, None) == 0
     assert lib.nsd_mxfp4_quantize(None, 0, 0, 32, None, None, None) == 0
