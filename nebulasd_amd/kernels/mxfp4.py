@@ -24,7 +24,7 @@ import functools
 import torch
 
 from .. import _lib
-from ._util import require, require_cuda, stream_of
+from ._util import require, require_cuda, stream_on
 
 BLOCK = 32
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
@@ -86,13 +86,13 @@ def _workspace_bytes(device: int, rows: int, n_out: int, n_in: int, gated: bool,
     return b.value
 
 
-def _call(t: torch.Tensor, name: str, *args) -> None:
-    """``name`` on ``t``'s device and its current stream."""
-    if t.get_device() == torch.cuda.current_device():
-        _lib.call(name, *args, stream_of(t))
+def _call(device: int, name: str, *args) -> None:
+    """``name`` on a device and its current stream."""
+    if device == torch.cuda.current_device():
+        _lib.call(name, *args, stream_on(device))
     else:
-        with torch.cuda.device(t.device):
-            _lib.call(name, *args, stream_of(t))
+        with torch.cuda.device(device):
+            _lib.call(name, *args, stream_on(device))
 
 
 def _same_device(a: torch.Tensor, b: torch.Tensor) -> None:
@@ -119,7 +119,7 @@ def mxfp4_quantize(w: torch.Tensor) -> MXFP4Weight:
     require(w, w.dtype, "w")
     n_out, n_in = w.shape
     codes, scales = _empty(4, n_out, n_in, w)
-    _call(w, "nsd_mxfp4_quantize", w.data_ptr(), _DTYPES[w.dtype], n_out, n_in, codes.data_ptr(), scales.data_ptr())
+    _call(w.get_device(), "nsd_mxfp4_quantize", w.data_ptr(), _DTYPES[w.dtype], n_out, n_in, codes.data_ptr(), scales.data_ptr())
     return MXFP4Weight(codes, scales, n_out, n_in, _made=True)
 
 
@@ -136,7 +136,7 @@ def mxfp4_pack(codes: torch.Tensor, scales: torch.Tensor) -> MXFP4Weight:
     _same_device(codes, scales)
     n_out, n_in = codes.shape[0], 2 * codes.shape[1]
     out = _empty(4, n_out, n_in, codes)
-    _call(codes, "nsd_mxfp4_pack", codes.data_ptr(), scales.data_ptr(), n_out, n_in, *(t.data_ptr() for t in out))
+    _call(codes.get_device(), "nsd_mxfp4_pack", codes.data_ptr(), scales.data_ptr(), n_out, n_in, *(t.data_ptr() for t in out))
     return MXFP4Weight(*out, n_out, n_in, _made=True)
 
 
@@ -147,7 +147,7 @@ def mxfp8_quantize(x: torch.Tensor) -> MXFP8Rows:
     require(x, torch.float16, "x")
     rows, n_in = x.shape
     codes, scales = _empty(8, rows, n_in, x)
-    _call(x, "nsd_mxfp8_quantize", x.data_ptr(), rows, n_in, codes.data_ptr(), scales.data_ptr())
+    _call(x.get_device(), "nsd_mxfp8_quantize", x.data_ptr(), rows, n_in, codes.data_ptr(), scales.data_ptr())
     return MXFP8Rows(codes, scales, rows, n_in, _made=True)
 
 
@@ -155,7 +155,7 @@ def _dequantize(b, rows: int, dtype: torch.dtype, name: str) -> torch.Tensor:
     if dtype not in _DTYPES:
         raise TypeError(f"dtype must be fp16, bf16 or fp32, got {dtype}")
     out = b.codes.new_empty((rows, b.n_in), dtype=dtype)
-    _call(out, name, b.codes.data_ptr(), b.scales.data_ptr(), rows, b.n_in, out.data_ptr(), _DTYPES[dtype])
+    _call(out.get_device(), name, b.codes.data_ptr(), b.scales.data_ptr(), rows, b.n_in, out.data_ptr(), _DTYPES[dtype])
     return out
 
 
@@ -169,22 +169,28 @@ def mxfp8_dequantize(x: MXFP8Rows, dtype: torch.dtype = torch.bfloat16) -> torch
     return _dequantize(x, x.rows, dtype, "nsd_mxfp8_dequantize")
 
 
+def _check_x(x: torch.Tensor, w: MXFP4Weight) -> None:
+    require_cuda(x)
+    require(x, torch.float16, "x")
+    if x.dim() != 2:
+        raise ValueError(f"x must be [rows, n_in], got {tuple(x.shape)}")
+    _same_device(x, w.codes)
+
+
 def _product(x, w: MXFP4Weight, n: int, out, gated: bool, name: str) -> torch.Tensor:
     # the checks of a decode step's call are kept short: at one row they and
     # the launch are most of its time
     codes = w.codes
-    quantised = isinstance(x, MXFP8Rows)
+    device = codes.get_device()
+    quantised = type(x) is MXFP8Rows
     if quantised:
         rows, n_in = x.rows, x.n_in
         _same_device(x.codes, codes)
         given = (None, x.codes.data_ptr(), x.scales.data_ptr())
     else:
-        require_cuda(x)
-        require(x, torch.float16, "x")
-        if x.dim() != 2:
-            raise ValueError(f"x must be [rows, n_in], got {tuple(x.shape)}")
+        if x.dtype is not torch.float16 or x.dim() != 2 or x.get_device() != device or not x.is_contiguous():
+            _check_x(x, w)
         rows, n_in = x.shape
-        _same_device(x, codes)
         given = (x.data_ptr(), None, None)
     if n_in != w.n_in:
         raise ValueError(f"x has {n_in} columns, the weight is [{w.n_out}, {w.n_in}]")
@@ -198,10 +204,10 @@ def _product(x, w: MXFP4Weight, n: int, out, gated: bool, name: str) -> torch.Te
             raise ValueError(f"out must be [{rows}, {n}]")
     if rows == 0:
         return out
-    size = _workspace_bytes(codes.get_device(), rows, w.n_out, n_in, gated, quantised)
+    size = _workspace_bytes(device, rows, w.n_out, n_in, gated, quantised)
     # the call's own, so calls on other streams and captured ones share nothing
     ws = codes.new_empty(size) if size else None
-    _call(codes, name, *given, codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), rows, n, n_in,
+    _call(device, name, *given, codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), rows, n, n_in,
           ws.data_ptr() if size else None, size)
     return out
 
