@@ -318,6 +318,68 @@ def test_graph_replays(gpu, rows):
             assert torch.equal(y, want)
 
 
+@pytest.mark.parametrize("rows,n,k", [(3, 1424, 352), (90, 1424, 352), (500, 1424, 352)])
+def test_first_call_inside_a_capture(gpu, rows, n, k):
+    """A shape (and a kernel, where no test ran it before) first called while capturing."""
+    w, values = _weight(gpu, n, k, seed=7)
+    x = _rows(rows, k, seed=8)
+    xg = torch.from_numpy(x).to(gpu)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = K.mxfp4_linear(xg, w)
+    for _ in range(3):
+        y.fill_(7.0)
+        g.replay()
+        torch.cuda.synchronize()
+        _check(y, oracle.mx_linear(x, values), oracle.mx_linear_bound(x, values))
+
+
+def test_same_bits_every_call(gpu):
+    """No result depends on which workgroup ends first: split, gated, small and large calls repeated."""
+    w, _ = _weight(gpu, 704, 5248)
+    g, _ = _weight(gpu, 2 * 352, 1056)
+    for rows in (17, 66, 451):
+        x, z = torch.from_numpy(_rows(rows, 5248)).to(gpu), torch.from_numpy(_rows(rows, 1056)).to(gpu)
+        y, h = K.mxfp4_linear(x, w), K.mxfp4_up_gate_silu_and_mul(z, g)
+        for _ in range(10):
+            assert torch.equal(K.mxfp4_linear(x, w), y) and torch.equal(K.mxfp4_up_gate_silu_and_mul(z, g), h)
+
+
+def test_outputs_past_32_bits(gpu):
+    """2.6e9 outputs and 2.3e9 values: the last rows against the oracle."""
+    rows, n = 40003, 65528
+    w, values = _weight(gpu, n, 32, seed=3)
+    x = np.zeros((rows, 32), np.float16)
+    x[-5:] = _rows(5, 32, seed=4)
+    y = K.mxfp4_linear(torch.from_numpy(x).to(gpu), w)
+    assert y.numel() > 2 ** 31
+    _check(y[-5:], oracle.mx_linear(x[-5:], values), oracle.mx_linear_bound(x[-5:], values))
+    assert not bool(y[-200:-5].any())
+    del y
+    n, k = 70003, 32768
+    v = torch.zeros(n, k, dtype=torch.float16, device=gpu)
+    last = _rows(3, k, seed=5)
+    v[-3:] = torch.from_numpy(last).to(gpu)
+    for quantise, back, bits in ((K.mxfp4_quantize, K.mxfp4_dequantize, 4), (K.mxfp8_quantize, K.mxfp8_dequantize, 8)):
+        got = back(quantise(v))
+        want = oracle.mx_values(*oracle.mx_quantize(last, bits), bits)
+        assert np.array_equal(got[-3:].double().cpu().numpy(), want) and not bool(got[-100:-3].any())
+        del got
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_other_device(gpu):
+    """Tensors on a device that is not the current one."""
+    x = torch.from_numpy(_rows(80, 1024))
+    w = torch.randn(512, 1024)
+    want = K.mxfp4_linear(x.to(gpu), K.mxfp4_quantize(w.to(gpu)))
+    other = K.mxfp4_linear(x.to("cuda:1"), K.mxfp4_quantize(w.to("cuda:1")))
+    assert other.device.index == 1 and torch.equal(other.cpu(), want.cpu())
+    with pytest.raises(ValueError, match="one device"):
+        K.mxfp4_linear(x.to("cuda:1"), K.mxfp4_quantize(w.to(gpu)))
+
+
 def test_streams_do_not_share_scratch(gpu):
     """The same shape on two streams at once: each call's own workspace."""
     w, _ = _weight(gpu, 4096, 4096)
@@ -340,7 +402,7 @@ def test_ffn_together(gpu, rows):
     """Quantised weights from fp16 ones, then up/gate and down as a layer runs them: each step against the oracle
     on the step's own input."""
     g = torch.Generator(device=gpu).manual_seed(5)
-    hidden, inter = 1024, 1536
+    hidden, inter = 1024, 1344
     wug = torch.randn(2 * inter, hidden, device=gpu, generator=g).mul_(hidden ** -0.5).half()
     wd = torch.randn(hidden, inter, device=gpu, generator=g).mul_(inter ** -0.5).half()
     qug, qd = K.mxfp4_quantize(wug), K.mxfp4_quantize(wd)
