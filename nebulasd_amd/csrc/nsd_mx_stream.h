@@ -174,11 +174,12 @@ __global__ void __launch_bounds__(kMxWaves* kWave, 1) mx_stream_kernel(MxArgs a)
     }
     f16* y = a.y + (int64_t)m * a.n + n0;
     const f16x4 h = {(f16)v[0], (f16)v[1], (f16)v[2], (f16)v[3]};
-    if (a.n % 4 == 0) {
-      *reinterpret_cast<f16x4*>(y) = h;
+    typedef f16x4 __attribute__((aligned(2))) f16x4_any;  // rows of any n start where they do
+    if (GATED || n0 + 4 <= a.n) {
+      *reinterpret_cast<f16x4_any*>(y) = h;
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < 3; ++e)
         if (n0 + e < a.n) y[e] = h[e];
     }
   };
