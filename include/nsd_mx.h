@@ -47,8 +47,8 @@ int nsd_mx_bytes(int bits, int64_t n_rows, int64_t n_in, int64_t* codes, int64_t
  * nsd_mxfp4_quantize: w [n_out, n_in] row-major (dtype NSD_DTYPE_*) to MXFP4.
  * nsd_mxfp4_pack: the same from row-major codes [n_out, n_in / 2] (even k in
  * the low half) and scale bytes [n_out, n_in / 32], as checkpoints hold them.
- * nsd_mxfp4_dequantize: the values, row-major, in `dtype` (rounded to nearest
- * where fp16 does not hold them; bf16 and fp32 hold all but infinities).
+ * nsd_mxfp4_dequantize: the values, row-major, in `dtype`, rounded to nearest
+ * where it does not hold them (bf16 and fp32 hold all that a quantiser makes).
  */
 int nsd_mxfp4_quantize(const void* w, int dtype, int64_t n_out, int64_t n_in, void* codes, void* scales,
                        void* stream);
@@ -72,9 +72,9 @@ int nsd_mxfp8_dequantize(const void* codes, const void* scales, int64_t n_rows, 
  * exp(-g))) in fp32, up and g the products with weight rows j and inter + j of
  * a [2 * inter, n_in] weight; inter a multiple of 16.
  *
- * y must not overlap x (NSD_ERR_INVALID).  A row's sums may be added in another
- * order, and end in another last place, in a batch of another size; the same
- * call gives the same bits.  n_rows up to 2^21, n_out up to 2^27, n_in up to 2^20.
+ * y must not overlap x, the weight or the workspace (NSD_ERR_INVALID).  A row's
+ * sums may be added in another order, and end in another last place, in a batch
+ * of another size; the same call gives the same bits.  n_rows up to 2^21, n_out up to 2^27, n_in up to 2^20.
  *
  * workspace: nsd_mx_workspace bytes for the call's shape on the current device
  * (n_out: the weight's rows; gated: of nsd_mxfp4_up_gate_silu_and_mul; quantised:

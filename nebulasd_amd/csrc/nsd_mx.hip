@@ -199,14 +199,13 @@ __device__ inline void store8<f16>(f16* p, const float (&v)[8]) {
   for (int e = 0; e < 8; ++e) h[e] = (f16)v[e];
   __builtin_nontemporal_store(h, reinterpret_cast<f16x8*>(p));
 }
-// bf16: the values have at most four significant bits, so the upper half of the
-// word is the value (the smallest subnormals of E4M3 excepted: 2^-127 2^-9,
-// below bf16's; they truncate to zero)
+// bf16: exact, but for E4M3 codes below bf16's subnormals.
 template <>
 __device__ inline void store8<uint16_t>(uint16_t* p, const float (&v)[8]) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
   u32x4 h;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) h[e] = (bits_of(v[2 * e]) >> 16) | (bits_of(v[2 * e + 1]) & 0xffff0000u);
+  for (int e = 0; e < 4; ++e) h[e] = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)v[2 * e], (__bf16)v[2 * e + 1]});
   __builtin_nontemporal_store(h, reinterpret_cast<u32x4*>(p));
 }
 template <>
@@ -259,8 +258,8 @@ int check_mx(const char* who, int64_t n_rows, int64_t n_in) {
   if (n_rows < 0 || n_rows > INT32_MAX || n_in < kMxBlock || n_in % kMxBlock || n_in > INT32_MAX)
     return fail(NSD_ERR_UNSUPPORTED, "%s: %lld rows of n_in=%lld (a multiple of 32)", who, (long long)n_rows,
                 (long long)n_in);
-  // a launch has at most one unit per (row tile, tile of k), counted in 32 bits
-  if (mx_row_tiles(n_rows) * mx_k_tiles(n_in) > INT32_MAX - kMxThreads)
+  // a launch has at most one wave per (row tile, tile of k), its lanes counted in 32 bits
+  if (mx_row_tiles(n_rows) * mx_k_tiles(n_in) > (UINT32_MAX - kMxThreads) / kWave)
     return fail(NSD_ERR_UNSUPPORTED, "%s: %lld x %lld values are too many", who, (long long)n_rows, (long long)n_in);
   return NSD_OK;
 }

@@ -482,12 +482,15 @@ int product(const char* who, const void* x, const void* x_codes, const void* x_s
     return fail(NSD_ERR_INVALID, "%s: null pointer", who);
   for (const void* p : {x, x_codes, x_scales, w_codes, w_scales, (const void*)y, (const void*)workspace})
     if (!aligned16(p)) return fail(NSD_ERR_UNSUPPORTED, "%s: pointers must be 16-byte aligned", who);
-  // workgroups that are done write y while others still read x
+  // workgroups that are done write y while others still read
+  const int64_t y_bytes = n_rows * n * 2;
   int64_t codes = 0, scales = 0;
   (void)nsd_mx_bytes(8, n_rows, n_in, &codes, &scales);
-  const int64_t y_bytes = n_rows * n * 2;
   if (overlap(y, y_bytes, x, n_rows * n_in * 2) || (!x && (overlap(y, y_bytes, x_codes, codes) || overlap(y, y_bytes, x_scales, scales))))
     return fail(NSD_ERR_INVALID, "%s: y overlaps x", who);
+  (void)nsd_mx_bytes(4, GATED ? 2 * n : n, n_in, &codes, &scales);
+  if (overlap(y, y_bytes, w_codes, codes) || overlap(y, y_bytes, w_scales, scales) || overlap(y, y_bytes, workspace, workspace_bytes))
+    return fail(NSD_ERR_INVALID, "%s: y overlaps the weight or the workspace", who);
   int cus = 0;
   if (int rc = device_cus(&cus)) return rc;
   const int64_t T = mx_k_tiles(n_in);

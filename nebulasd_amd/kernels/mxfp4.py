@@ -43,6 +43,10 @@ def _fixed(self, name, value):
     raise AttributeError(f"{type(self).__name__} is fixed once made: its sizes were checked then")
 
 
+def _parts(self):
+    return type(self), tuple(getattr(self, name) for name in self.__slots__)
+
+
 class MXFP4Weight:
     """A weight [n_out, n_in] in MXFP4: codes and scales (uint8) in the kernels' layout."""
 
@@ -55,6 +59,7 @@ class MXFP4Weight:
             object.__setattr__(self, name, v)
 
     __setattr__ = _fixed
+    __reduce__ = _parts  # copy and pickle
 
 
 class MXFP8Rows:
@@ -69,6 +74,7 @@ class MXFP8Rows:
             object.__setattr__(self, name, v)
 
     __setattr__ = _fixed
+    __reduce__ = _parts  # copy and pickle
 
 
 @functools.lru_cache(maxsize=4096)

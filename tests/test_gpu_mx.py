@@ -18,6 +18,9 @@ Every case prints its name first.
 
 from __future__ import annotations
 
+import copy
+import pickle
+
 import numpy as np
 import pytest
 import torch
@@ -366,6 +369,80 @@ def test_outputs_past_32_bits(gpu):
         want = oracle.mx_values(*oracle.mx_quantize(last, bits), bits)
         assert np.array_equal(got[-3:].double().cpu().numpy(), want) and not bool(got[-100:-3].any())
         del got
+
+
+def test_operands_past_32_bits(gpu):
+    """A weight of 4.6e9 bytes, its last columns; 5.2e9 bytes of rows, the last of them."""
+    n, k, last = 70016, 131072, 37
+    codes = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, device=gpu)
+    scales = torch.randint(112, 118, (n, k // 32), dtype=torch.uint8, device=gpu)
+
+    def values(rows):
+        return oracle.mx_values(oracle.mx_unpack_nibbles(codes[rows].cpu().numpy()), scales[rows].cpu().numpy(), 4)
+
+    w = K.mxfp4_pack(codes, scales)
+    ends = np.concatenate((values(slice(n // 2 - last, n // 2)), values(slice(n - last, n))))
+    del codes, scales
+    for rows in (2, 20, 70, 130):
+        print(f"{rows} x {k} -> {n}", flush=True)
+        x = _rows(rows, k, seed=rows)
+        xg = torch.from_numpy(x).to(gpu)
+        y = K.mxfp4_linear(xg, w)
+        up, gate = np.split(oracle.mx_linear(x, ends), 2, axis=1)
+        du, dg = np.split(oracle.mx_linear_bound(x, ends), 2, axis=1)
+        _check(y[:, n // 2 - last:n // 2], up, du)
+        _check(y[:, -last:], gate, dg)
+        silu = gate / (1 + np.exp(-gate))
+        _check(K.mxfp4_up_gate_silu_and_mul(xg, w)[:, -last:], up * silu, np.abs(silu) * du + 1.1 * (np.abs(up) + du) * dg,
+               (2 * np.abs(gate) + 8) * 2.0 ** -24)
+    del w, xg, y
+    rows = 40003
+    w, v = _weight(gpu, 40, k, seed=1)
+    x = _rows(5, k, seed=2)
+    xg = torch.zeros(rows, k, dtype=torch.float16, device=gpu)
+    xg[-5:] = torch.from_numpy(x).to(gpu)
+    for given in (xg, K.mxfp8_quantize(xg)):
+        y = K.mxfp4_linear(given, w)
+        _check(y[-5:], oracle.mx_linear(x, v), oracle.mx_linear_bound(x, v))
+        assert not bool(y[:-5].any())
+
+
+def test_every_block_dequantises(gpu):
+    """Every scale byte with every code, the smallest ones too: to nearest in each type."""
+    scales = torch.arange(256, dtype=torch.uint8)
+    # 16 rows: row i of tile t has scale byte 16 t + i; both kinds' codes laid out by the product's own pack or by hand
+    codes4 = torch.arange(16, dtype=torch.uint8).repeat(256, 2)
+    w = K.mxfp4_pack(torch.from_numpy(oracle.mx_pack_nibbles(codes4.numpy())).to(gpu), scales.view(256, 1).to(gpu))
+    codes8 = torch.arange(256, dtype=torch.uint8).view(1, 256).expand(256, 256)
+    tiles = codes8.reshape(16, 16, 2, 8, 16).permute(0, 2, 3, 1, 4)  # [row tile][tile of k][run][row][16]
+    words = scales.view(16, 1, 16, 1).expand(16, 4, 16, 4)  # [row tile][block][row][tile of k]
+    x = K.MXFP8Rows(tiles.reshape(-1).contiguous().to(gpu), words.reshape(-1).contiguous().to(gpu), 256, 256)
+    for got, want in ((lambda t: K.mxfp4_dequantize(w, t), oracle.mx_values(codes4.numpy(), scales.view(256, 1).numpy(), 4)),
+                      (lambda t: K.mxfp8_dequantize(x, t),
+                       oracle.mx_values(codes8.numpy(), scales.view(256, 1).expand(256, 8).numpy(), 8))):
+        for t in (torch.float16, torch.bfloat16, torch.float32):
+            # float64 -> t by way of fp32, which holds every value (2^-149 and up) but those past its largest
+            nearest = torch.from_numpy(want).float().to(t)
+            assert np.array_equal(got(t).cpu().float().numpy(), nearest.float().numpy(), equal_nan=True), t
+
+
+def test_output_over_the_weight_is_refused(gpu):
+    w, _ = _weight(gpu, 64, 128)
+    x = torch.from_numpy(_rows(4, 128)).to(gpu)
+    for over in (w.codes[:512], w.scales[:512]):
+        before = over.clone()
+        with pytest.raises(_lib.NativeLibraryError, match="overlaps the weight"):
+            K.mxfp4_linear(x, w, out=over.view(torch.float16).view(4, 64))
+        assert torch.equal(over, before)
+
+
+def test_copies_of_weights_and_rows(gpu):
+    """copy and pickle go through the constructors' checks."""
+    w, _ = _weight(gpu, 48, 96)
+    x = K.mxfp8_quantize(torch.from_numpy(_rows(5, 96)).to(gpu))
+    want = K.mxfp4_linear(x, w)
+    for again in (copy.copy, copy.deepcopy, lambda t: pickle.loads(pickle.dumps(t))):
+        assert torch.equal(K.mxfp4_linear(again(x), again(w)), want)
 
 
 @pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
