@@ -78,8 +78,8 @@ int nsd_mxfp8_dequantize(const void* codes, const void* scales, int64_t n_rows, 
  *
  * workspace: nsd_mx_workspace bytes for the call's shape on the current device
  * (n_out: the weight's rows; gated: of nsd_mxfp4_up_gate_silu_and_mul; quantised:
- * x is given as codes), contents irrelevant; calls that overlap each need their
- * own.
+ * x is given as codes; 0 for no rows), contents irrelevant; calls that overlap
+ * each need their own.
  */
 int nsd_mx_workspace(int64_t n_rows, int64_t n_out, int64_t n_in, int gated, int quantised, int64_t* bytes);
 int nsd_mxfp4_linear(const void* x, const void* x_codes, const void* x_scales, const void* w_codes,

@@ -399,6 +399,7 @@ double choose_tile(MxConfig& best, double least, int64_t n_rows, int64_t n, int6
   return least;
 }
 
+// n_rows, n and T at least 1.
 MxConfig choose_mx(int64_t n_rows, int64_t n, int64_t T, bool gated, bool quantised, int cus) {
   // The choice of a shape, not worked out anew every call (1.5 us of a decode
   // step's 7): the last ones of this thread.
@@ -534,6 +535,10 @@ extern "C" int nsd_mx_workspace(int64_t n_rows, int64_t n_out, int64_t n_in, int
                                 int64_t* bytes) {
   if (!bytes) return fail(NSD_ERR_INVALID, "mx_workspace: null output");
   if (int rc = check_product("mx_workspace", n_rows, n_out, n_in)) return rc;
+  if (n_rows == 0) {  // no kernel to choose
+    *bytes = 0;
+    return NSD_OK;
+  }
   int cus = 0;
   if (int rc = device_cus(&cus)) return rc;
   const int64_t n = gated ? n_out / 2 : n_out;

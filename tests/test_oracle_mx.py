@@ -169,6 +169,18 @@ def test_entries_refuse_before_any_launch(lib):
     assert lib.nsd_mxfp4_quantize(None, 0, 0, 32, None, None, None) == 0
 
 
+def _workspace(lib, rows, n_out, n_in, gated=0, quantised=0):
+    b = ctypes.c_int64(-1)
+    return lib.nsd_mx_workspace(rows, n_out, n_in, gated, quantised, ctypes.byref(b)), b.value
+
+
+@pytest.mark.parametrize("gated", [0, 1])
+@pytest.mark.parametrize("quantised", [0, 1])
+def test_no_rows_need_no_workspace(lib, gated, quantised):
+    """The shape of an empty batch, which the products take: nothing is chosen for it."""
+    assert _workspace(lib, 0, 1024, 1024, gated, quantised) == (0, 0)
+
+
 def test_wrappers_refuse(lib):
     from nebulasd_amd import kernels as K
 
