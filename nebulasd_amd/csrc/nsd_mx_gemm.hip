@@ -535,6 +535,8 @@ extern "C" int nsd_mx_workspace(int64_t n_rows, int64_t n_out, int64_t n_in, int
                                 int64_t* bytes) {
   if (!bytes) return fail(NSD_ERR_INVALID, "mx_workspace: null output");
   if (int rc = check_product("mx_workspace", n_rows, n_out, n_in)) return rc;
+  if (gated && n_out % 32)
+    return fail(NSD_ERR_UNSUPPORTED, "mx_workspace: gated n_out=%lld (a multiple of 32)", (long long)n_out);
   if (n_rows == 0) {  // no kernel to choose
     *bytes = 0;
     return NSD_OK;

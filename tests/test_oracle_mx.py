@@ -181,6 +181,15 @@ def test_no_rows_need_no_workspace(lib, gated, quantised):
     assert _workspace(lib, 0, 1024, 1024, gated, quantised) == (0, 0)
 
 
+@pytest.mark.parametrize("rows", [0, 1, 300])
+@pytest.mark.parametrize("n_out", [1, 16, 33, 4080])
+def test_workspace_refuses_what_the_gated_product_refuses(lib, rows, n_out):
+    """A gated weight has 2 * inter rows, inter a multiple of 16."""
+    from nebulasd_amd import _lib
+
+    assert _workspace(lib, rows, n_out, 1024, gated=1)[0] == 2 and f"n_out={n_out} " in _lib.last_error()
+
+
 def test_wrappers_refuse(lib):
     from nebulasd_amd import kernels as K
 
