@@ -49,6 +49,7 @@ int nsd_mx_bytes(int bits, int64_t n_rows, int64_t n_in, int64_t* codes, int64_t
  * the low half) and scale bytes [n_out, n_in / 32], as checkpoints hold them.
  * nsd_mxfp4_dequantize: the values, row-major, in `dtype`, rounded to nearest
  * where it does not hold them (bf16 and fp32 hold all that a quantiser makes).
+ * None works in place: buffers that overlap are refused (NSD_ERR_INVALID).
  */
 int nsd_mxfp4_quantize(const void* w, int dtype, int64_t n_out, int64_t n_in, void* codes, void* scales,
                        void* stream);

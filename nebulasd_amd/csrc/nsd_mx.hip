@@ -9,6 +9,7 @@
 //
 // All are bound by memory.
 #include <algorithm>
+#include <initializer_list>
 
 #include "nsd_mx_device.h"
 
@@ -276,6 +277,22 @@ int check_pointers(const char* who, std::initializer_list<const void*> ps) {
   return NSD_OK;
 }
 
+// Codes and scales of n_rows x n_in values apart from each other and from the
+// conversion's other buffers: waves write while others read.
+struct MxBuffer {
+  const void* p;
+  int64_t bytes;
+};
+int check_apart(const char* who, int bits, int64_t n_rows, int64_t n_in, const void* codes, const void* scales,
+                std::initializer_list<MxBuffer> others) {
+  int64_t c = 0, s = 0;
+  (void)nsd_mx_bytes(bits, n_rows, n_in, &c, &s);
+  bool over = mx_overlap(codes, c, scales, s);
+  for (const MxBuffer& o : others) over = over || mx_overlap(codes, c, o.p, o.bytes) || mx_overlap(scales, s, o.p, o.bytes);
+  return over ? fail(NSD_ERR_INVALID, "%s: the buffers overlap", who) : NSD_OK;
+}
+int64_t dtype_bytes(int dtype) { return dtype == NSD_DTYPE_F32 ? 4 : 2; }
+
 unsigned wave_grid(int64_t units) { return (unsigned)((units + kMxThreads / kWave - 1) / (kMxThreads / kWave)); }
 
 template <int BITS>
@@ -285,6 +302,7 @@ int dequantize(const char* who, const void* codes, const void* scales, int64_t n
   if (int rc = check_dtype(who, dtype)) return rc;
   if (n_rows == 0) return NSD_OK;
   if (int rc = check_pointers(who, {codes, scales, out})) return rc;
+  if (int rc = check_apart(who, BITS, n_rows, n_in, codes, scales, {{out, n_rows * n_in * dtype_bytes(dtype)}})) return rc;
   const int64_t rt = mx_row_tiles(n_rows), kt = mx_k_tiles(n_in);
   auto go = [&](auto* p) {
     hipLaunchKernelGGL((mx_dequantize_kernel<BITS, std::remove_pointer_t<decltype(p)>>), dim3(wave_grid(rt * kt)),
@@ -327,6 +345,8 @@ extern "C" int nsd_mxfp4_quantize(const void* w, int dtype, int64_t n_out, int64
   if (int rc = check_dtype("mxfp4_quantize", dtype)) return rc;
   if (n_out == 0) return NSD_OK;
   if (int rc = check_pointers("mxfp4_quantize", {w, codes, scales})) return rc;
+  if (int rc = check_apart("mxfp4_quantize", 4, n_out, n_in, codes, scales, {{w, n_out * n_in * dtype_bytes(dtype)}}))
+    return rc;
   const int64_t rt = mx_row_tiles(n_out), kt = mx_k_tiles(n_in);
   auto go = [&](const auto* p) {
     hipLaunchKernelGGL((mxfp4_quantize_kernel<std::remove_cv_t<std::remove_pointer_t<decltype(p)>>>),
@@ -345,6 +365,9 @@ extern "C" int nsd_mxfp4_pack(const void* row_codes, const void* row_scales, int
   if (n_out == 0) return NSD_OK;
   if (!row_scales) return fail(NSD_ERR_INVALID, "mxfp4_pack: null pointer");
   if (int rc = check_pointers("mxfp4_pack", {row_codes, codes, scales})) return rc;
+  if (int rc = check_apart("mxfp4_pack", 4, n_out, n_in, codes, scales,
+                           {{row_codes, n_out * n_in / 2}, {row_scales, n_out * n_in / kMxBlock}}))
+    return rc;
   const int64_t rt = mx_row_tiles(n_out), kt = mx_k_tiles(n_in);
   hipLaunchKernelGGL(mxfp4_pack_kernel, dim3(wave_grid(rt * ((kt + 3) / 4))), dim3(kMxThreads), 0, as_stream(stream),
                      static_cast<const u32x4*>(row_codes), static_cast<const uint8_t*>(row_scales), n_out, (int)n_in,
@@ -362,6 +385,7 @@ extern "C" int nsd_mxfp8_quantize(const void* x, int64_t n_rows, int64_t n_in, v
   if (int rc = check_mx("mxfp8_quantize", n_rows, n_in)) return rc;
   if (n_rows == 0) return NSD_OK;
   if (int rc = check_pointers("mxfp8_quantize", {x, codes, scales})) return rc;
+  if (int rc = check_apart("mxfp8_quantize", 8, n_rows, n_in, codes, scales, {{x, n_rows * n_in * 2}})) return rc;
   return mxfp8_quantize(x, n_rows, n_in, codes, scales, stream);
 }
 

@@ -26,6 +26,12 @@ constexpr uint8_t kMxNanScale = 255;
 inline __host__ __device__ int64_t mx_row_tiles(int64_t rows) { return (rows + 15) / 16; }
 inline __host__ __device__ int64_t mx_k_tiles(int64_t n_in) { return (n_in + kMxTileK - 1) / kMxTileK; }
 
+// Whether two buffers share a byte.
+inline bool mx_overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  const uintptr_t p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b);
+  return a && b && p < q + b_bytes && q < p + a_bytes;
+}
+
 // Scale byte of an E4M3 block whose largest magnitude has the fp16 bits m, and
 // its power of two: m = f 2^p (1 <= f < 2) takes 2^(p-8) up to f = 1.75 = 448 /
 // 256 and 2^(p-7) above, so no value saturates.  Of a block of zeros the byte

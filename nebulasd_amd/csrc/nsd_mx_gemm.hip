@@ -442,10 +442,6 @@ int launch_mx(const MxArgs& a, const MxConfig& c, hipStream_t st) {
   }
 }
 
-bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
-  const uintptr_t p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b);
-  return a && b && p < q + b_bytes && q < p + a_bytes;
-}
 int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 
 int check_product(const char* who, int64_t n_rows, int64_t n, int64_t n_in) {
@@ -487,10 +483,10 @@ int product(const char* who, const void* x, const void* x_codes, const void* x_s
   const int64_t y_bytes = n_rows * n * 2;
   int64_t codes = 0, scales = 0;
   (void)nsd_mx_bytes(8, n_rows, n_in, &codes, &scales);
-  if (overlap(y, y_bytes, x, n_rows * n_in * 2) || (!x && (overlap(y, y_bytes, x_codes, codes) || overlap(y, y_bytes, x_scales, scales))))
+  if (mx_overlap(y, y_bytes, x, n_rows * n_in * 2) || (!x && (mx_overlap(y, y_bytes, x_codes, codes) || mx_overlap(y, y_bytes, x_scales, scales))))
     return fail(NSD_ERR_INVALID, "%s: y overlaps x", who);
   (void)nsd_mx_bytes(4, GATED ? 2 * n : n, n_in, &codes, &scales);
-  if (overlap(y, y_bytes, w_codes, codes) || overlap(y, y_bytes, w_scales, scales) || overlap(y, y_bytes, workspace, workspace_bytes))
+  if (mx_overlap(y, y_bytes, w_codes, codes) || mx_overlap(y, y_bytes, w_scales, scales) || mx_overlap(y, y_bytes, workspace, workspace_bytes))
     return fail(NSD_ERR_INVALID, "%s: y overlaps the weight or the workspace", who);
   int cus = 0;
   if (int rc = device_cus(&cus)) return rc;

@@ -190,6 +190,37 @@ def test_workspace_refuses_what_the_gated_product_refuses(lib, rows, n_out):
     assert _workspace(lib, rows, n_out, 1024, gated=1)[0] == 2 and f"n_out={n_out} " in _lib.last_error()
 
 
+def test_blocks_over_their_values_are_refused(lib):
+    """No conversion works in place: a wave's blocks are written while others still read."""
+    from nebulasd_amd import _lib
+
+    def refused(rc):
+        assert rc == 1 and "overlap" in _lib.last_error(), (rc, _lib.last_error())
+
+    # addresses that are never read
+    a, far, n, k = 1 << 20, 1 << 24, 32, 256
+    codes4, codes8, scales = _sizes(lib, 4, n, k)[1:], _sizes(lib, 8, n, k)[1:], _sizes(lib, 8, n, k)[2]
+    assert codes4[0] == 4096 and codes8[0] == 8192 and scales == 512
+    for dtype, size in ((0, 2), (1, 2), (2, 4)):
+        last = a + n * k * size - 16
+        refused(lib.nsd_mxfp4_quantize(a, dtype, n, k, a, far, None))
+        refused(lib.nsd_mxfp4_quantize(a, dtype, n, k, last, far, None))
+        refused(lib.nsd_mxfp4_quantize(a, dtype, n, k, far, last, None))
+        for back in (lib.nsd_mxfp4_dequantize, lib.nsd_mxfp8_dequantize):
+            refused(back(a, far, n, k, a, dtype, None))
+            refused(back(last, far, n, k, a, dtype, None))
+            refused(back(far, last, n, k, a, dtype, None))
+    refused(lib.nsd_mxfp8_quantize(a, n, k, a + 2 * n * k - 16, far, None))
+    refused(lib.nsd_mxfp8_quantize(a, n, k, far, a, None))
+    refused(lib.nsd_mxfp4_pack(a, far, n, k, a, 2 * far, None))
+    refused(lib.nsd_mxfp4_pack(far, a, n, k, a, 2 * far, None))
+    refused(lib.nsd_mxfp4_pack(a, far, n, k, 2 * far, far + 240, None))
+    # codes and scales over each other
+    refused(lib.nsd_mxfp4_quantize(a, 0, n, k, far, far + 4080, None))
+    refused(lib.nsd_mxfp8_quantize(a, n, k, far, far + 8176, None))
+    refused(lib.nsd_mxfp4_pack(a, 2 * a, n, k, far, far + 4080, None))
+
+
 def test_wrappers_refuse(lib):
     from nebulasd_amd import kernels as K
 
