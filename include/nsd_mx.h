@@ -73,7 +73,8 @@ int nsd_mxfp8_dequantize(const void* codes, const void* scales, int64_t n_rows, 
  * exp(-g))) in fp32, up and g the products with weight rows j and inter + j of
  * a [2 * inter, n_in] weight; inter a multiple of 16.
  *
- * y must not overlap x, the weight or the workspace (NSD_ERR_INVALID).  A row's
+ * y must not overlap x, the weight or the workspace, nor the workspace x or the
+ * weight (NSD_ERR_INVALID).  A row's
  * sums may be added in another order, and end in another last place, in a batch
  * of another size; the same call gives the same bits.  n_rows up to 2^21, n_out up to 2^27, n_in up to 2^20.
  *

@@ -479,15 +479,21 @@ int product(const char* who, const void* x, const void* x_codes, const void* x_s
     return fail(NSD_ERR_INVALID, "%s: null pointer", who);
   for (const void* p : {x, x_codes, x_scales, w_codes, w_scales, (const void*)y, (const void*)workspace})
     if (!aligned16(p)) return fail(NSD_ERR_UNSUPPORTED, "%s: pointers must be 16-byte aligned", who);
-  // workgroups that are done write y while others still read
+  // workgroups that are done write y, and the first launch the workspace, while others still read
+  int64_t xc = 0, xs = 0, wc = 0, ws_bytes = 0;
+  (void)nsd_mx_bytes(8, n_rows, n_in, &xc, &xs);
+  (void)nsd_mx_bytes(4, GATED ? 2 * n : n, n_in, &wc, &ws_bytes);
+  auto over = [&](const void* p, int64_t bytes) {
+    if (x ? mx_overlap(p, bytes, x, n_rows * n_in * 2) : mx_overlap(p, bytes, x_codes, xc) || mx_overlap(p, bytes, x_scales, xs))
+      return "x";
+    return mx_overlap(p, bytes, w_codes, wc) || mx_overlap(p, bytes, w_scales, ws_bytes) ? "the weight" : (const char*)nullptr;
+  };
   const int64_t y_bytes = n_rows * n * 2;
-  int64_t codes = 0, scales = 0;
-  (void)nsd_mx_bytes(8, n_rows, n_in, &codes, &scales);
-  if (mx_overlap(y, y_bytes, x, n_rows * n_in * 2) || (!x && (mx_overlap(y, y_bytes, x_codes, codes) || mx_overlap(y, y_bytes, x_scales, scales))))
-    return fail(NSD_ERR_INVALID, "%s: y overlaps x", who);
-  (void)nsd_mx_bytes(4, GATED ? 2 * n : n, n_in, &codes, &scales);
-  if (mx_overlap(y, y_bytes, w_codes, codes) || mx_overlap(y, y_bytes, w_scales, scales) || mx_overlap(y, y_bytes, workspace, workspace_bytes))
-    return fail(NSD_ERR_INVALID, "%s: y overlaps the weight or the workspace", who);
+  if (const char* what = over(y, y_bytes)) return fail(NSD_ERR_INVALID, "%s: y overlaps %s", who, what);
+  if (mx_overlap(y, y_bytes, workspace, workspace_bytes))
+    return fail(NSD_ERR_INVALID, "%s: y overlaps the workspace", who);
+  if (const char* what = over(workspace, workspace_bytes))
+    return fail(NSD_ERR_INVALID, "%s: the workspace overlaps %s", who, what);
   int cus = 0;
   if (int rc = device_cus(&cus)) return rc;
   const int64_t T = mx_k_tiles(n_in);

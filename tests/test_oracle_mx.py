@@ -221,6 +221,21 @@ def test_blocks_over_their_values_are_refused(lib):
     refused(lib.nsd_mxfp4_pack(a, 2 * a, n, k, far, far + 4080, None))
 
 
+def test_workspace_over_the_operands_is_refused(lib):
+    from nebulasd_amd import _lib
+
+    a, far = 1 << 20, 1 << 24
+    for entry, n, w_rows in ((lib.nsd_mxfp4_linear, 64, 64), (lib.nsd_mxfp4_up_gate_silu_and_mul, 32, 64)):
+        w_codes, w_scales = _sizes(lib, 4, w_rows, 128)[1:]
+        x_codes, x_scales = _sizes(lib, 8, 100, 128)[1:]
+        for given, at, size in (((a, None, None), a, 100 * 256), ((None, a, 2 * a), a, x_codes),
+                                ((None, a, 2 * a), 2 * a, x_scales), ((a, None, None), 3 * a, w_codes),
+                                ((a, None, None), 4 * a, w_scales)):
+            for ws in (at, at + size - 16, at - 240):
+                rc = entry(*given, 3 * a, 4 * a, far, 100, n, 128, ws, 256, None)
+                assert rc == 1 and "workspace overlaps" in _lib.last_error(), (rc, _lib.last_error())
+
+
 def test_wrappers_refuse(lib):
     from nebulasd_amd import kernels as K
 
