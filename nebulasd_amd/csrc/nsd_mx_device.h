@@ -6,6 +6,7 @@
 
 #include "nsd_device.h"
 #include "nsd_mx.h"
+#include "nsd_mx_choose.h"
 
 namespace nsd {
 
@@ -16,15 +17,7 @@ typedef short s16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kMxBlock = 32;         // values under one scale
-constexpr int kMxTileK = 128;        // k of a tile
-constexpr int kMxTile4 = 1024;       // bytes of a tile's 4-bit codes
-constexpr int kMxTile8 = 2048;       // and of its 8-bit codes
-constexpr int kMxScaleTile = 256;    // scale bytes of 16 rows x 4 tiles of k
 constexpr uint8_t kMxNanScale = 255;
-
-inline __host__ __device__ int64_t mx_row_tiles(int64_t rows) { return (rows + 15) / 16; }
-inline __host__ __device__ int64_t mx_k_tiles(int64_t n_in) { return (n_in + kMxTileK - 1) / kMxTileK; }
 
 // Whether two buffers share a byte.
 inline bool mx_overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
@@ -158,18 +151,6 @@ struct MxArgs {
   int row_tiles, w_tiles;
   int splits;
 };
-
-// Which kernel serves it, chosen in nsd_mx_gemm.hip.
-enum MxKernel { kMxStream, kMxTile128x256, kMxTile128 };
-struct MxConfig {
-  MxKernel kernel = kMxStream;  // a shape of mx_tile_kernel, or mx_stream_kernel with
-  int mt = 1, jw = 1, splits = 1;
-  bool fp16 = false;  // reads x as it is
-  bool nt = false;    // the weight past the caches
-};
-
-constexpr int kMxWaves = 4;      // of a workgroup of the stream kernel
-constexpr int kMxFp16Tiles = 4;  // row tiles that it takes as fp16
 
 // Up to 128 rows (nsd_mx_stream.h): y = x . W^T, and its gated form.
 int mx_stream_linear(const MxArgs& a, const MxConfig& c, hipStream_t st);

@@ -230,7 +230,7 @@ template <int MT, int JW, bool GATED>
 int launch_mx_stream(const MxArgs& a, const MxConfig& c, hipStream_t st) {
   if constexpr (MT <= kMxFp16Tiles)
     if (c.fp16) {
-      if constexpr (MT == 1)
+      if constexpr (mx_stream_nt(MT, JW, true))
         if (c.nt) return launch_mx_stream<MT, JW, GATED, true, true>(a, st);
       return launch_mx_stream<MT, JW, GATED, true, false>(a, st);
     }

@@ -3,11 +3,13 @@
 from __future__ import annotations
 
 import ctypes
+import subprocess
 
 import numpy as np
 import pytest
 import torch
 
+import mx_shapes
 import oracle
 from oracle import E2M1, E4M3, mx_linear, mx_pack_nibbles, mx_quantize, mx_unpack_nibbles, mx_up_gate, mx_values
 
@@ -234,6 +236,59 @@ def test_workspace_over_the_operands_is_refused(lib):
             for ws in (at, at + size - 16, at - 240):
                 rc = entry(*given, 3 * a, 4 * a, far, 100, n, 128, ws, 256, None)
                 assert rc == 1 and "workspace overlaps" in _lib.last_error(), (rc, _lib.last_error())
+
+
+# ---- the rule that chooses a product's kernel, compiled for the host -------------
+
+_CHOICE = """
+#include "nsd_mx_choose.h"
+extern "C" void choice(int64_t rows, int64_t n, int64_t n_in, int gated, int quantised, int cus, int* out) {
+  const nsd::MxConfig c = nsd::choose_mx(rows, n, nsd::mx_k_tiles(n_in), gated, quantised, cus);
+  const int v[] = {c.kernel, c.mt, c.jw, c.fp16, c.nt, c.splits};
+  for (int i = 0; i < 6; ++i) out[i] = v[i];
+}
+extern "C" int past_caches(int mt, int jw, int fp16) { return nsd::mx_stream_nt(mt, jw, fp16); }
+extern "C" int fp16_tiles() { return nsd::kMxFp16Tiles; }
+"""
+STREAM = 0
+
+
+@pytest.fixture(scope="module")
+def rule(tmp_path_factory):
+    from nebulasd_amd.build import CSRC
+
+    at = tmp_path_factory.mktemp("mx_choose")
+    (at / "choice.cpp").write_text(_CHOICE)
+    subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-Werror", "-shared", "-fPIC", f"-I{CSRC}", str(at / "choice.cpp"),
+                    "-o", str(at / "choice.so")], check=True)
+    lib = ctypes.CDLL(str(at / "choice.so"))
+    lib.choice.argtypes = [ctypes.c_int64] * 3 + [ctypes.c_int] * 3 + [ctypes.POINTER(ctypes.c_int)]
+    return lib
+
+
+def _choice(rule, rows, n, n_in, gated, quantised, cus=256):
+    """(kernel, row tiles, column tiles, x as fp16, past the caches, splits)."""
+    out = (ctypes.c_int * 6)()
+    rule.choice(rows, n, n_in, gated, quantised, cus, out)
+    return tuple(out)
+
+
+def test_shapes_take_every_kernel(rule):
+    """The GPU tests' shapes run every kernel that is compiled, and no kernel is compiled that no shape takes."""
+    for gated, shapes in ((0, mx_shapes.LINEAR + mx_shapes.LINEAR_LARGE), (1, mx_shapes.GATED + mx_shapes.GATED_LARGE)):
+        taken = {_choice(rule, r, n, k, gated, q)[:5] for r, n, k, q in shapes}
+        compiled = {(STREAM, mt, jw, fp16, nt)
+                    for mt in range(1, 9) for jw in ((2, 4, 6) if gated else (1, 2, 3, 4, 6))
+                    for fp16 in range(2 if mt <= rule.fp16_tiles() else 1)
+                    for nt in range(1 + bool(rule.past_caches(mt, jw, fp16)))}
+        stream = {c for c in taken if c[0] == STREAM}
+        assert stream == compiled, (compiled - stream, stream - compiled)
+        assert {c[0] for c in taken} == {0, 1, 2}
+
+
+def test_large_shapes_go_past_the_caches(rule):
+    for gated, shapes in ((0, mx_shapes.LINEAR_LARGE), (1, mx_shapes.GATED_LARGE)):
+        assert all(_choice(rule, r, n, k, gated, q)[4] for r, n, k, q in shapes)
 
 
 def test_wrappers_refuse(lib):
