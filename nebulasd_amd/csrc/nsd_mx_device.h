@@ -106,10 +106,12 @@ __device__ inline int mx8_operand(const f16x8 (&h)[4], int lane, i32x4& b0, i32x
 // byte BYTE of sa and sb is the scale of block g of row i and of column i.  It
 // receives C[4g .. 4g+3][i].
 //
-// The 32 products of a block are added aligned to the largest of them, with 15
-// bits kept below it (measured: beside 2688 a product of 1/8 counts, one of
-// 1/16 is lost), blocks to each other and to C in fp32.  That is 4e-6 of a
-// sum's norm, of which rounding it to fp16 takes 2.1e-4.
+// Eight products, of neighbours along k, are added at a time: each is cut toward
+// zero 13 bits below the largest sum of two operands' exponents among them
+// (measured: beside 2^8 2^2 and more, to 448 * 6, 1/8 counts and 1/16 is lost;
+// the same in both instructions).  Two eights join, and they C, in fp32, off by
+// less than a last place.  Together that is 4e-6 of a sum's norm, of which
+// rounding it to fp16 takes 2.1e-4.
 template <int BYTE>
 __device__ inline f32x4 mx_mfma(i32x4 a, i32x4 b0, i32x4 b1, f32x4 c, int sa, int sb) {
   const i32x8 av = {a[0], a[1], a[2], a[3], 0, 0, 0, 0};

@@ -494,3 +494,34 @@ def test_ffn_together(gpu, rows):
     _check(h, oracle.mx_up_gate(xn, vug), np.abs(gate / (1 + np.exp(-gate))) * du + 1.1 * (np.abs(up) + du) * dg,
            (2 * np.abs(gate) + 8) * 2.0 ** -24)
     _check(y, oracle.mx_linear(hn, vd), oracle.mx_linear_bound(hn, vd))
+
+
+@pytest.mark.parametrize("path", ["fp16", "blocks", "tile"])
+def test_products_beside_large_ones(gpu, path):
+    """One large product in every eight of a block, small ones of each magnitude beside it, and the large ones taken
+    off again by another tile of k: what is left is what the instructions keep of the small ones.  Products below
+    2^-13 of the large one's exponent are cut, at every mantissa, and the bound of the other tests covers them."""
+    rows, n = (2048, 1024) if path == "tile" else (16, 48)
+    x, w = np.zeros((16, 256)), np.zeros((16, 256))
+    for r in range(16):
+        x[r, :32] = 1.875 * 2.0 ** (r - 9)
+        x[r, :32:8] = x[r, 128:160:8] = 256.0
+    x[:, 24] = x[:, 152] = 448.0
+    tops, small = [.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, 4.0], [1.0, .5, 1.5, -1.0]
+    for c in range(16):
+        w[c, :32] = small[c // 4]
+        if c % 2:
+            w[c, 1:32:2] = -w[c, 1:32:2]
+        w[c, :32:8] = tops[c % 8]
+        w[c, 128:160:8] = -tops[c % 8]
+    values = np.tile(w, (n // 16, 1))
+    mag = np.searchsorted(oracle.E2M1, np.abs(values)).astype(np.uint8)
+    codes = torch.from_numpy(oracle.mx_pack_nibbles(mag | (np.signbit(values).astype(np.uint8) << 3))).to(gpu)
+    weight = K.mxfp4_pack(codes, torch.full((n, 8), 127, dtype=torch.uint8, device=gpu))
+    xg = torch.from_numpy(np.tile(x, (rows // 16, 1)).astype(np.float16)).to(gpu)
+    y = K.mxfp4_linear(K.mxfp8_quantize(xg) if path == "blocks" else xg, weight).double().cpu().numpy()
+    want, bound = oracle.mx_linear(x.astype(np.float16), w), oracle.mx_linear_bound(x.astype(np.float16), w)
+    off = np.abs(y.reshape(-1, 16, n // 16, 16) - want[:, None]).max((0, 2))
+    print(f"  largest share of the bound {(off / bound).max():.2f}", flush=True)
+    assert (off <= 2.0 ** -11 * (np.abs(want) + bound) + 2.0 ** -25 + bound).all()
+    assert off[:4].max() > 0.5, "the small products were meant to be cut"

@@ -110,6 +110,28 @@ def test_a_wrong_scale_is_seen():
     assert not np.allclose(mx_values(codes, scales + 1, 4), mx_values(codes, scales, 4))
 
 
+def test_bound_covers_every_eight_of_a_block():
+    """Four large products a block, one in every eight, each beside seven that just miss its last place."""
+    x = np.full((1, 32), 1.875 * 2.0 ** -4, np.float16)
+    w = np.ones((1, 32))
+    x[0, ::8], w[0, ::8] = 256.0, 4.0
+    lost = mx_linear(x, w)[0, 0] - 4 * 1024
+    assert lost == 28 * 1.875 * 2.0 ** -4 < oracle.mx_linear_bound(x, w)[0, 0]
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_bound_counts_subnormal_codes_with_their_exponent(bits):
+    """Beside a large operand on the other side an eight whose codes are all subnormal is cut as if they were not."""
+    x, w = np.full((1, 32), 256.0, np.float16), np.full((1, 32), 6.0)
+    if bits == 4:
+        w[0, 8:16] = .5   # 2^0 to the instruction
+        power = 2.0 ** 8 * 4 * 3 + 2.0 ** 8 * 1
+    else:
+        x[0, 8:16] = 2.0 ** -9  # 2^-6
+        power = 2.0 ** 8 * 4 * 3 + 2.0 ** -6 * 4
+    assert oracle.mx_linear_bound(x, w)[0, 0] >= 7 * 2.0 ** -13 * power
+
+
 # ---- the C entries, short of a GPU ------------------------------------------------
 
 
