@@ -64,10 +64,11 @@ int nsd_mxfp8_dequantize(const void* codes, const void* scales, int64_t n_rows, 
                          void* stream);
 
 /*
- * nsd_mxfp4_linear: y [n_rows, n_out] fp16 = fp16(sum over k of X[r][k] W[n][k])
- * (fp32 sums), W the MXFP4 values and X the MXFP8 values of x [n_rows, n_in]
- * fp16, quantised in the call; or, with x null, the ones given as x_codes and
- * x_scales.
+ * nsd_mxfp4_linear: y [n_rows, n_out] fp16 = fp16(sum over k of X[r][k] W[n][k]),
+ * W the MXFP4 values and X the MXFP8 values of x [n_rows, n_in] fp16, quantised
+ * in the call; or, with x null, the ones given as x_codes and x_scales.  Sums are
+ * held in fp32; among eight products that the matrix instruction adds at a time,
+ * bits 13 below the exponent of the largest are cut.
  *
  * nsd_mxfp4_up_gate_silu_and_mul: y [n_rows, inter] fp16 = fp16(up * g / (1 +
  * exp(-g))) in fp32, up and g the products with weight rows j and inter + j of

@@ -7,8 +7,10 @@ reference has only fp16 projections: swiftLLM/swiftllm/worker/kernels/linear.py:
 for any number of rows.  A row is cut into blocks of 32 values: one power of
 two and 32 codes, E2M1 for the weight (``MXFP4Weight``) and E4M3 for the rows it
 is multiplied with (``MXFP8Rows``), which gfx950's scaled matrix instructions
-multiply as they are, with fp32 sums.  ``include/nsd_mx.h`` states the formats,
-the roundings and the layouts.
+multiply as they are.  Sums are held in fp32, but of the eight products that an
+instruction adds at a time bits 13 below the largest one's exponent are cut:
+together 4e-6 of a sum's norm, where its rounding to fp16 takes 2.1e-4.
+``include/nsd_mx.h`` states the formats, the roundings and the layouts.
 
 A weight comes from ``mxfp4_quantize`` (from fp16, bf16 or fp32) or
 ``mxfp4_pack`` (from a checkpoint's codes and scales), once.  The products
@@ -220,7 +222,7 @@ def _product(x, w: MXFP4Weight, n: int, out, gated: bool, name: str) -> torch.Te
 
 def mxfp4_linear(x: torch.Tensor | MXFP8Rows, w: MXFP4Weight, out: torch.Tensor | None = None) -> torch.Tensor:
     """``linear`` with an MXFP4 weight: fp16 [rows, n_out] = fp16(X . W^T), X the MXFP8 values of x [rows, n_in]
-    (fp16, or quantised already), fp32 sums."""
+    (fp16, or quantised already), the sum held in fp32 as the module says."""
     return _product(x, w, w.n_out, out, False, "nsd_mxfp4_linear")
 
 
