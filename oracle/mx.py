@@ -12,6 +12,7 @@ How each function is pinned (``tests/test_oracle_mx.py``):
   zeros, saturation and NaN; a planted mistake (the scale one step up).
 * ``mx_values`` -- quantising the values gives the codes back.
 * ``mx_linear`` / ``mx_up_gate`` -- one-hot rows, and torch in float64.
+* ``mx_linear_cut`` -- cases worked out by hand; within ``mx_linear_bound`` of ``mx_linear``.
 """
 
 from __future__ import annotations
@@ -19,7 +20,7 @@ from __future__ import annotations
 import numpy as np
 
 __all__ = ["MX_BLOCK", "E2M1", "E4M3", "mx_quantize", "mx_values", "mx_pack_nibbles", "mx_unpack_nibbles", "mx_linear",
-           "mx_up_gate", "mx_linear_bound"]
+           "mx_up_gate", "mx_linear_bound", "mx_linear_cut"]
 
 MX_BLOCK = 32
 # The non-negative values of the codes, in code order.
@@ -84,6 +85,26 @@ def mx_up_gate(x, w_values):
     up, gate = np.split(y, 2, axis=1)
     with np.errstate(over="ignore"):
         return up * (gate / (1 + np.exp(-gate)))
+
+
+def mx_linear_cut(x, codes, scales):
+    """``mx_linear`` with each product cut as the matrix instructions cut it (see ``mx_linear_bound``), of a weight's
+    codes [n_out, n_in] and scale bytes; the sums of what is left in float64."""
+    xc, xs = mx_quantize(x, 8)
+    sides = []
+    for c, s, bits, least in ((xc, xs, 8, -6), (codes, scales, 4, 0)):
+        v = mx_values(c, s, bits)
+        e = np.repeat(s.astype(np.int64) - 127, MX_BLOCK, axis=1)
+        # an operand's exponent; a zero takes no part
+        p = np.where(v != 0, np.maximum(np.frexp(v)[1] - 1, e + least), -10 ** 4)
+        sides.append((v, p))
+    (xv, xp), (wv, wp) = sides
+    out = np.empty((len(xv), len(wv)))
+    for r in range(len(xv)):
+        last = (xp[r] + wp).reshape(len(wv), -1, 8).max(2, keepdims=True) - 13
+        at = np.ldexp((xv[r] * wv).reshape(len(wv), -1, 8), -last)
+        out[r] = np.ldexp(np.trunc(at), last).sum((1, 2))
+    return out
 
 
 def _group_powers(v, least):

@@ -525,3 +525,20 @@ def test_products_beside_large_ones(gpu, path):
     print(f"  largest share of the bound {(off / bound).max():.2f}", flush=True)
     assert (off <= 2.0 ** -11 * (np.abs(want) + bound) + 2.0 ** -25 + bound).all()
     assert off[:4].max() > 0.5, "the small products were meant to be cut"
+
+
+@pytest.mark.parametrize("rows,n,k", [(1, 96, 1024), (5, 48, 544), (40, 67, 1056), (100, 64, 4096), (300, 130, 1056)])
+def test_sums_are_what_the_instructions_keep(gpu, rows, n, k):
+    """Against the oracle that cuts each product as the instructions do, nothing is left but the fp32 joins, a last
+    place each, and the rounding."""
+    x = _rows(rows, k, seed=n)
+    codes, scales = oracle.mx_quantize(np.random.default_rng(k).standard_normal((n, k)) * k ** -0.5, 4)
+    w = K.mxfp4_pack(torch.from_numpy(oracle.mx_pack_nibbles(codes)).to(gpu), torch.from_numpy(scales).to(gpu))
+    want, values = oracle.mx_linear_cut(x, codes, scales), oracle.mx_values(codes, scales, 4)
+    joins = (k // 8 + 16) * 2.0 ** -23 * (np.abs(oracle.mx_values(*oracle.mx_quantize(x, 8), 8)) @ np.abs(values).T)
+    xg = torch.from_numpy(x).to(gpu)
+    for given in (xg, K.mxfp8_quantize(xg)):
+        y = K.mxfp4_linear(given, w)
+        _check(y, want, joins)
+        same = (y.cpu().numpy() == want.astype(np.float16)).mean()
+        print(f"  {100 * same:.2f}% equal bits", flush=True)

@@ -132,6 +132,26 @@ def test_bound_counts_subnormal_codes_with_their_exponent(bits):
     assert oracle.mx_linear_bound(x, w)[0, 0] >= 7 * 2.0 ** -13 * power
 
 
+def test_cut_products():
+    """Beside 2^(8 + 2): 1/8 stays, 1/16 goes, 3/16 becomes 1/8, either sign; another eight is not touched; beside
+    448 * 0 nothing is cut; 0.5 in the weight counts as 2^0."""
+    x, w = np.zeros((1, 32), np.float16), np.zeros((7, 32))
+    x[0, :3], x[0, 8] = (256, 2.0 ** -4, -2.0 ** -3), 2.0 ** -4
+    w[0, :2], w[1, :2], w[2, :3] = (4, 2), (4, 1), (4, 3, 0)
+    w[3, :3], w[4, 0], w[4, 8], w[5, 1], w[6, :2] = (-4, 0, 1.5), 4, 1, 1, (.5, .5)
+    mag = np.searchsorted(E2M1, np.abs(w)).astype(np.uint8) | (np.signbit(w).astype(np.uint8) << 3)
+    got = oracle.mx_linear_cut(x, mag, np.full((7, 1), 127, np.uint8))[0]
+    assert got.tolist() == [1024 + .125, 1024, 1024 + .125, -1024 - .125, 1024 + 2.0 ** -4, 2.0 ** -4, 128 + 2.0 ** -5]
+
+
+def test_cut_sums_lie_within_the_bound():
+    x = (_blocks(8, 9, 544) * np.where(np.arange(544) % 61 == 0, 24, 1)).astype(np.float16)
+    codes, scales = mx_quantize(_blocks(9, 21, 544), 4)
+    w = mx_values(codes, scales, 4)
+    off = np.abs(oracle.mx_linear_cut(x, codes, scales) - mx_linear(x, w))
+    assert off.max() > 0 and (off <= oracle.mx_linear_bound(x, w)).all()
+
+
 # ---- the C entries, short of a GPU ------------------------------------------------
 
 
