@@ -25,6 +25,7 @@ import numpy as np
 import pytest
 import torch
 
+import mx_shapes
 import oracle
 from nebulasd_amd import _lib
 from nebulasd_amd import kernels as K
@@ -542,3 +543,96 @@ def test_sums_are_what_the_instructions_keep(gpu, rows, n, k):
         _check(y, want, joins)
         same = (y.cpu().numpy() == want.astype(np.float16)).mean()
         print(f"  {100 * same:.2f}% equal bits", flush=True)
+
+
+def _random_blocks(gpu, n, k, seed):
+    """A weight of every code and several scales, drawn on the GPU."""
+    g = torch.Generator(device=gpu).manual_seed(seed)
+    codes = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, device=gpu, generator=g)
+    return codes, torch.randint(112, 118, (n, k // 32), dtype=torch.uint8, device=gpu, generator=g)
+
+
+def _ids(shapes):
+    return [f"{r}x{n}x{k}{'-blocks' if q else ''}" for r, n, k, q in shapes]
+
+
+def _run_shape(gpu, rows, n, k, blocks, gated):
+    """(x, weight's codes and scales, weight, y), y in a buffer whose end the kernel must leave alone."""
+    w_rows = 2 * n if gated else n
+    codes, scales = _random_blocks(gpu, w_rows, k, rows + n)
+    w = K.mxfp4_pack(codes, scales)
+    x = torch.from_numpy(_rows(rows, k, seed=k)).to(gpu)
+    buf = torch.full((rows * n + 512,), 7.0, dtype=torch.float16, device=gpu)
+    op = K.mxfp4_up_gate_silu_and_mul if gated else K.mxfp4_linear
+    y = op(K.mxfp8_quantize(x) if blocks else x, w, out=buf[:rows * n].view(rows, n))
+    assert bool((buf[rows * n:] == 7.0).all()), "the kernel wrote past the output"
+    return x, codes, scales, w, y
+
+
+@pytest.mark.parametrize("rows,n,k,blocks", mx_shapes.LINEAR, ids=_ids(mx_shapes.LINEAR))
+def test_linear_kernels(gpu, rows, n, k, blocks):
+    """Every kernel that serves a cached weight (the list is checked against the rule without a GPU)."""
+    print(f"mxfp4_linear {rows} x {n} x {k} blocks={blocks}", flush=True)
+    x, codes, scales, _, y = _run_shape(gpu, rows, n, k, blocks, False)
+    values = oracle.mx_values(oracle.mx_unpack_nibbles(codes.cpu().numpy()), scales.cpu().numpy(), 4)
+    xn = x.cpu().numpy()
+    _check(y, oracle.mx_linear(xn, values), oracle.mx_linear_bound(xn, values))
+
+
+@pytest.mark.parametrize("rows,n,k,blocks", mx_shapes.GATED, ids=_ids(mx_shapes.GATED))
+def test_gated_kernels(gpu, rows, n, k, blocks):
+    print(f"mxfp4_up_gate_silu_and_mul {rows} x {n} x {k} blocks={blocks}", flush=True)
+    x, codes, scales, _, y = _run_shape(gpu, rows, n, k, blocks, True)
+    values = oracle.mx_values(oracle.mx_unpack_nibbles(codes.cpu().numpy()), scales.cpu().numpy(), 4)
+    xn = x.cpu().numpy()
+    up, gate = np.split(oracle.mx_linear(xn, values), 2, axis=1)
+    du, dg = np.split(oracle.mx_linear_bound(xn, values), 2, axis=1)
+    silu = gate / (1 + np.exp(-gate))
+    _check(y, up * silu, np.abs(silu) * du + 1.1 * (np.abs(up) + du) * dg, (2 * np.abs(gate) + 8) * 2.0 ** -24)
+
+
+def _powers(v, least):
+    """``oracle.mx_linear_bound``'s powers of eights, of float64 magnitudes [n, k] on the GPU."""
+    m = v.view(v.shape[0], -1, 8).amax(2)
+    p = torch.maximum(torch.exp2(torch.frexp(m).exponent.double() - 1), least.repeat_interleave(4, 1))
+    return torch.where(m > 0, p, torch.zeros_like(p))
+
+
+def _columns(x, w, scales, at, stop):
+    """Columns at .. stop of the product and their bound, in float64 on the GPU, from the values that rows and
+    weight stand for (whose exactness has its own tests)."""
+    q = K.mxfp8_quantize(x)
+    xv = K.mxfp8_dequantize(q, torch.float32).double()
+    top = x.double().abs().view(x.shape[0], -1, 32).amax(2)
+    f, p = torch.frexp(top)
+    least_x = torch.where(top > 0, torch.exp2((p - 9 + (f > 0.875).to(p.dtype)).double() - 6), torch.zeros_like(top))
+    wv = w[at:stop].double()
+    least_w = torch.exp2(scales[at:stop].double() - 127)
+    px, pw = _powers(xv.abs(), least_x), _powers(wv.abs(), least_w)
+    bound = 7 * 2.0 ** -13 * (px @ pw.t().contiguous())
+    bound += (x.shape[1] // 8 + 16) * 2.0 ** -23 * (xv.abs() @ wv.abs().t().contiguous())
+    return (xv @ wv.t().contiguous()).cpu().numpy(), bound.cpu().numpy()
+
+
+LARGE = [(False, *s) for s in mx_shapes.LINEAR_LARGE] + [(True, *s) for s in mx_shapes.GATED_LARGE]
+
+
+@pytest.mark.parametrize("gated,rows,n,k,blocks", LARGE,
+                         ids=_ids(mx_shapes.LINEAR_LARGE) + ["gated-" + i for i in _ids(mx_shapes.GATED_LARGE)])
+def test_kernels_past_the_caches(gpu, gated, rows, n, k, blocks):
+    """Every kernel that streams a large weight past the caches: the first and last columns and some between."""
+    print(f"past the caches: gated={gated} {rows} x {n} x {k} blocks={blocks}", flush=True)
+    x, _, scales, w, y = _run_shape(gpu, rows, n, k, blocks, gated)
+    assert bool(y.isfinite().all())
+    values = K.mxfp4_dequantize(w, torch.float32)
+    for at in (0, n // 2 // 16 * 16 + 5, n - 203):
+        cols = slice(at, at + 203)
+        got = y[:, cols]
+        want, bound = _columns(x, values, scales, at, at + 203)
+        extra = 0.0
+        if gated:
+            (up, du), (gate, dg) = (want, bound), _columns(x, values, scales, n + at, n + at + 203)
+            silu = gate / (1 + np.exp(-gate))
+            want, bound = up * silu, np.abs(silu) * du + 1.1 * (np.abs(up) + du) * dg
+            extra = (2 * np.abs(gate) + 8) * 2.0 ** -24
+        _check(got, want, bound, extra)
