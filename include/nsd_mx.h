@@ -75,9 +75,10 @@ int nsd_mxfp8_dequantize(const void* codes, const void* scales, int64_t n_rows, 
  * a [2 * inter, n_in] weight; inter a multiple of 16.
  *
  * y must not overlap x, the weight or the workspace, nor the workspace x or the
- * weight (NSD_ERR_INVALID).  A row's
- * sums may be added in another order, and end in another last place, in a batch
- * of another size; the same call gives the same bits.  n_rows up to 2^21, n_out up to 2^27, n_in up to 2^20.
+ * weight (NSD_ERR_INVALID).  The same call gives the same bits; in a batch of
+ * another size, or given as codes instead of fp16, a row's sums may be added in
+ * another order (another kernel or split of k serves them) and end in another
+ * last place.  n_rows up to 2^21, n_out up to 2^27, n_in up to 2^20.
  *
  * workspace: nsd_mx_workspace bytes for the call's shape on the current device
  * (n_out: the weight's rows; gated: of nsd_mxfp4_up_gate_silu_and_mul; quantised:

@@ -15,7 +15,9 @@ together 2e-5 of the sums' norm, where their rounding to fp16 takes 2.1e-4.
 A weight comes from ``mxfp4_quantize`` (from fp16, bf16 or fp32) or
 ``mxfp4_pack`` (from a checkpoint's codes and scales), once.  The products
 quantise fp16 rows themselves; rows that several projections read are
-quantised once with ``mxfp8_quantize`` and given instead.
+quantised once with ``mxfp8_quantize`` and given instead.  The same call gives the
+same bits; in a batch of another size, or given in blocks instead of fp16, a row
+may be added up in another order and end in another last place.
 """
 
 from __future__ import annotations

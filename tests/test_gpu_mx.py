@@ -636,3 +636,14 @@ def test_kernels_past_the_caches(gpu, gated, rows, n, k, blocks):
             want, bound = up * silu, np.abs(silu) * du + 1.1 * (np.abs(up) + du) * dg
             extra = (2 * np.abs(gate) + 8) * 2.0 ** -24
         _check(got, want, bound, extra)
+
+
+def test_saved_weights_load_on_the_gpu(gpu, tmp_path):
+    """torch.save and back onto the GPU; what is made or loaded elsewhere is refused before any kernel sees it."""
+    w, _ = _weight(gpu, 48, 96)
+    x = K.mxfp8_quantize(torch.from_numpy(_rows(5, 96)).to(gpu))
+    torch.save({"w": w, "x": x}, tmp_path / "w.pt")
+    got = torch.load(tmp_path / "w.pt", map_location=gpu, weights_only=False)
+    assert torch.equal(K.mxfp4_linear(got["x"], got["w"]), K.mxfp4_linear(x, w))
+    with pytest.raises(ValueError, match="GPU tensors"):
+        torch.load(tmp_path / "w.pt", map_location="cpu", weights_only=False)
