@@ -36,17 +36,26 @@ struct MxConfig {
 constexpr bool mx_stream_nt(int mt, int jw, bool fp16) { return !fp16 || (mt == 1 && jw == 6); }
 
 // Which kernel serves a product, and how: the cheapest by a model of each one's
-// time in ns, whose constants are fitted to every choice at 222 shapes (1 to
-// 8192 rows, weights of 500 x 2048 to 151936 x 4096); the chosen one is within 1%
-// of the best on the average and 14% at worst.
+// time in ns.  Its constants are fitted to sweeps and order the choices; they are
+// no rates of one unit, and nothing in it stands for the memory (16 x 4096 ->
+// 151936 takes 59 us, 31 by the model).  Against every choice at 134 shapes (1 to
+// 8192 rows, ten weights from 1024 x 1024 to 151936 x 4096), GPU time with the
+// weight called again and again and among others together: rows given in blocks
+// 0.3% off the best on the average and 14% at worst, fp16 rows 1.4% and 38%.
 //
 // The stream kernel:
 //   - A compute unit takes in weight and x together, however they mix, a KB in
 //     11 ns where two workgroups share it or it has one to run, in 18 where
-//     one's registers leave no room for another.
-//   - A workgroup's end, its sums through LDS, takes 175 ns a tile.
+//     one's registers leave no room for another.  (Measured 9 out of the L2, 16
+//     with the weight out of the last-level cache, 24 among other weights.)
+//   - A workgroup's end, its sums through LDS and its stores, takes 175 ns a
+//     tile (measured 140 to 200).
 //   - x as fp16 is more bytes to every workgroup and 39 ns of cutting a step
-//     and row tile, and saves the pass that cuts it once, 2.6 us.
+//     and row tile, and saves the pass that cuts it once, 2.6 us.  That is the
+//     host's price of a launch too, and from 33 rows on the better part of it:
+//     33, 48 and 64 x 1024 -> 1024 take 6.9, 7.6 and 9.1 us a call against 9.7,
+//     9.8 and 9.9 with the pass, but in a graph 6.9, 7.8 and 9.3 against 6.3,
+//     6.2 and 6.7.  (33 x 2080 -> 18993: 12.4 against 10.0, and 13 against 10.)
 // The tile kernel: a step of 128 k takes a workgroup of 128 x 256 900 ns alone on
 // its compute unit, two of them 1430; of 128 x 128 425 and 780.  (One of 256 x
 // 256, eight waves, takes as long as two of 128 x 256 and was no faster where
@@ -61,8 +70,8 @@ inline double mx_split_ns(int splits, int64_t n_rows, int64_t n, double bytes_pe
   return splits == 1 ? 0.0 : 2100.0 + (double)splits * n_rows * n * 8 / bytes_per_ns;
 }
 
-inline double choose_stream(MxConfig& best, double least, int64_t n_rows, int64_t n, int64_t T, bool gated, bool quantised,
-                     int cus) {
+inline double choose_stream(MxConfig& best, double least, int64_t n_rows, int64_t n, int64_t T, bool gated,
+                            bool quantised, int cus) {
   const int64_t row_tiles = mx_row_tiles(n_rows), chunks = (row_tiles + 7) / 8;
   const int mt = (int)((row_tiles + chunks - 1) / chunks);
   const int64_t out_tiles = (n + 15) / 16;
@@ -94,8 +103,8 @@ inline double choose_stream(MxConfig& best, double least, int64_t n_rows, int64_
   return least;
 }
 
-inline double choose_tile(MxConfig& best, double least, int64_t n_rows, int64_t n, int64_t T, bool gated, bool quantised,
-                   int cus) {
+inline double choose_tile(MxConfig& best, double least, int64_t n_rows, int64_t n, int64_t T, bool gated,
+                          bool quantised, int cus) {
   for (MxKernel kernel : {kMxTile128x256, kMxTile128}) {
     const bool wide = kernel == kMxTile128x256;
     const int64_t columns = (wide ? 256 : 128) / (gated ? 2 : 1);
@@ -136,9 +145,10 @@ inline MxConfig choose_mx(int64_t n_rows, int64_t n, int64_t T, bool gated, bool
   double least = choose_stream(best, 1e300, n_rows, n, T, gated, quantised, cus);
   choose_tile(best, least, n_rows, n, T, gated, quantised, cus);
   // A weight that the 256 MB last-level cache cannot keep from call to call
-  // streams faster past it: 330 MB, 16 rows 64.9 -> 59.7 us; one that it keeps
-  // (13 to 53 MB, called again and again) slower, 3.7 -> 5.5 and 15.1 -> 16.9,
-  // and neither way among other weights.
+  // streams faster past it: 311 MB, one, 16 and 80 rows 57 -> 53, 61 -> 57 and
+  // 112 -> 106 us.  One that it keeps, called again and again, slower: 7.0 -> 9.4 (34
+  // MB, 16 rows), 24 -> 25 (134), 39 -> 42 (235).  Among other weights past the
+  // caches is faster from 34 MB on, 11.0 -> 10.5, 29 -> 27 and 48 -> 43.
   best.nt = best.kernel == kMxStream && mx_stream_nt(best.mt, best.jw, best.fp16) &&
             (double)((n + 15) / 16) * (gated ? 2 : 1) * T * kMxTile4 > 192e6;
   c = Chosen{n_rows, n, T, kind, cus, best};

@@ -1,5 +1,6 @@
-// Products of up to 128 rows with an MXFP4 weight: the stream kernel, which
-// nsd_mx_stream_linear.hip and nsd_mx_stream_gated.hip compile.
+// Products of few rows with an MXFP4 weight, up to 128 of them a workgroup: the
+// stream kernel, which nsd_mx_stream_linear.hip and nsd_mx_stream_gated.hip
+// compile.
 #pragma once
 
 #include "nsd_mx_device.h"
@@ -27,14 +28,17 @@ constexpr int kMxNowhere = 0x40000000;  // an offset past every buffer's end
 // FP16: x as it is, cut into blocks between load and product.  NT: the weight
 // past the caches.
 //
-// Bound by what a compute unit takes in, weight and x through the same queue:
-// 22 bytes a cycle for 80 rows x 4096 -> 2 x 12288 (14.9 us with the weight in the
-// last-level cache, 17.5 from memory), where rows that hit the L2 alone come in
-// at 57.  One row tile streams 330 MB of weight at 6.0 TB/s (55 us).  The sums
-// through LDS take 1.2 us of the 14.9, the output's stores 1.5.  Branches around
-// the loads instead of bounds made every step wait for all of them (17.0 ->
-// 19.0); eight waves, three or four steps ahead, and the x of an XCD read by its
-// workgroups beforehand were no faster over the shapes.
+// Bound by a fixed part and the weight's stream.  80 rows x 4096 -> 2 x 12288 (5 x
+// 6 tiles, 16 KB into each compute unit a step) takes 7 us and 32 steps of 0.25
+// us, 6.3 TB/s of weight out of the last-level cache: 15 us.  Among other weights
+// a step is 0.38 us, 4.1 TB/s from memory, and the whole 18; while the weight
+// lies in the L2, 0.14 us.  Of the 7 us 3.4 are there with one row tile, too
+// (launch, the first loads); the rest are the sums through LDS and the stores,
+// 140 to 200 ns a tile.  One row tile's steps take 0.23 us, 6.9 TB/s, and 0.29,
+// 5.4 TB/s, among others; past the caches it streams 330 MB at 6.0 TB/s (55 us).
+// Branches around the loads instead of bounds made every step wait for all of
+// them (17.0 -> 19.0); eight waves, three or four steps ahead, and the x of an XCD
+// read by its workgroups beforehand were no faster over the shapes.
 template <int MT, int JW, bool GATED>
 struct MxStream {
   static constexpr int P = GATED ? JW / 2 : JW, PER = GATED ? 2 : 1;  // column tiles of y, sums of one
