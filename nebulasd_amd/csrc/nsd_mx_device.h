@@ -22,7 +22,7 @@ constexpr uint8_t kMxNanScale = 255;
 // Whether two buffers share a byte.
 inline bool mx_overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
   const uintptr_t p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b);
-  return a && b && p < q + b_bytes && q < p + a_bytes;
+  return a && b && a_bytes > 0 && b_bytes > 0 && p < q + b_bytes && q < p + a_bytes;
 }
 
 // Scale byte of an E4M3 block whose largest magnitude has the fp16 bits m, and

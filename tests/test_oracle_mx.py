@@ -280,6 +280,13 @@ def test_workspace_over_the_operands_is_refused(lib):
                 assert rc == 1 and "workspace overlaps" in _lib.last_error(), (rc, _lib.last_error())
 
 
+def test_a_workspace_of_no_bytes_overlaps_nothing(lib):
+    """It is too small for this shape, which is what the call is refused for (without a GPU: for that)."""
+    a, far = 1 << 20, 1 << 24
+    for at in (a + 16, 3 * a + 16, far + 16):
+        assert lib.nsd_mxfp4_linear(a, None, None, 3 * a, 4 * a, far, 100, 64, 128, at, 0, None) in (3, 4)
+
+
 # ---- the rule that chooses a product's kernel, compiled for the host -------------
 
 _CHOICE = """
