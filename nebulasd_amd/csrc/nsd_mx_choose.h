@@ -51,11 +51,12 @@ constexpr bool mx_stream_nt(int mt, int jw, bool fp16) { return !fp16 || (mt == 
 //   - A workgroup's end, its sums through LDS and its stores, takes 175 ns a
 //     tile (measured 140 to 200).
 //   - x as fp16 is more bytes to every workgroup and 39 ns of cutting a step
-//     and row tile, and saves the pass that cuts it once, 2.6 us.  That is the
-//     host's price of a launch too, and from 33 rows on the better part of it:
+//     and row tile, and saves the pass that cuts it once, 2.6 us.  From 33 rows
+//     on that is what the host takes to launch it, more than the device does:
 //     33, 48 and 64 x 1024 -> 1024 take 6.9, 7.6 and 9.1 us a call against 9.7,
 //     9.8 and 9.9 with the pass, but in a graph 6.9, 7.8 and 9.3 against 6.3,
-//     6.2 and 6.7.  (33 x 2080 -> 18993: 12.4 against 10.0, and 13 against 10.)
+//     6.2 and 6.7.  (33 x 2080 -> 18993 loses either way: 12.4 against 10.0 us a
+//     call, 13 against 10 in a graph.)
 // The tile kernel: a step of 128 k takes a workgroup of 128 x 256 900 ns alone on
 // its compute unit, two of them 1430; of 128 x 128 425 and 780.  (One of 256 x
 // 256, eight waves, takes as long as two of 128 x 256 and was no faster where

@@ -154,7 +154,7 @@ struct MxArgs {
   int splits;
 };
 
-// Up to 128 rows (nsd_mx_stream.h): y = x . W^T, and its gated form.
+// Up to 128 rows a workgroup (nsd_mx_stream.h): y = x . W^T, and its gated form.
 int mx_stream_linear(const MxArgs& a, const MxConfig& c, hipStream_t st);
 int mx_stream_gated(const MxArgs& a, const MxConfig& c, hipStream_t st);
 

@@ -1,7 +1,8 @@
 // Products of microscaled weights (MXFP4) and activations (MXFP8) for gfx950:
 // y[r][n] = sum_k X[r][k] W[n][k], and the up/gate pair with its SiLU-and-mul.
-// Here the tile kernel for many rows, the choice of kernel and the C entries;
-// the kernel for decode and verify batches is in nsd_mx_stream.h.
+// Here the tile kernel for many rows and the C entries; the kernel for decode and
+// verify batches is in nsd_mx_stream.h, the choice between them in
+// nsd_mx_choose.h.
 #include <algorithm>
 
 #include "nsd_mx_device.h"
