@@ -191,9 +191,9 @@ __device__ inline float e4m3_value(uint32_t c) {
 // what they were made from and are written back later all the same.  The way
 // back alone: 8192 x 12288 E4M3 55 -> 47 us, 4096 x 4096 E2M1 10.8 -> 8.7, 24576 x
 // 4096 41.7 -> 40.1; there and back 119 -> 92, 19 -> 17 and 99 -> 82.  A kernel
-// that reads the values next gives about as much back: with a copy after it the
-// two take 24.4 -> 24.9, 133 -> 124 (24576 x 4096) and 133 -> 134 (8192 x 12288),
-// with a product 33.5 -> 33.8, 76 -> 84 and 100 -> 101.  (The quantisers' loads the
+// that reads the values next loses about as much: the way back and a copy take
+// 24.4 -> 24.9 us (4096 x 4096), 133 -> 124 (24576 x 4096) and 133 -> 134 (8192 x
+// 12288), the way back and a product 33.5 -> 33.8, 76 -> 84 and 100 -> 101.  (The quantisers' loads the
 // same way: 92 -> 120 there and back.)
 template <typename T>
 __device__ inline void store8(T* p, const float (&v)[8]);
