@@ -49,43 +49,20 @@
 // Layouts (reference swiftLLM/swiftllm/worker/kernels/paged_attn.py):
 //   k/v cache [N, L, Hkv, 16, 128] fp16, block (blk, layer, head) = 4 KB
 //   contiguous at ((blk*L + layer)*Hkv + head)*16*128 (:49-50, :70-71).
-#include <algorithm>
 #include <mutex>
 
-#include "nsd_device.h"
+#include "nsd_paged.h"
 
 namespace nsd {
 namespace {
 
-constexpr int D = kHeadDim;           // 128
-constexpr int BS = kBlockTokens;      // 16
 constexpr int kRowBytes = D * 2;      // one fp16 row of K or V
 constexpr int kTile = BS * kRowBytes; // one (block, layer, head) tile: 4 KB
 constexpr int kSlot = 2 * kTile;      // a buffer slot: the block's K tile, then its V tile
 constexpr int kSlots = 2;             // each wave's double buffer
-constexpr int kWaves = 4;             // waves per workgroup (per piece)
-constexpr int kThreads = kWaves * kWave;
 constexpr int kWaveLds = kSlots * kSlot;
 constexpr int kLdsBytes = kWaves * kWaveLds;  // 64 KB: two workgroups per CU
-// End-of-piece merge of the waves' softmax states, per 16-row tile: each
-// wave's accumulators (8 dim tiles x f32x4 per lane), then its row max and
-// row sum (16 floats each); it reuses the buffer's LDS.
-constexpr int kMergeAcc = 8 * kWave * 16;
-constexpr int kMergeWave = kMergeAcc + 2 * 16 * 4;
 static_assert(kWaves * kMergeWave <= kLdsBytes, "merge fits in the buffer's LDS");
-constexpr float kLn2 = 0.69314718055994531f;
-constexpr float kLazyMax = 8.f;       // the running max moves only when exceeded by 2^8
-constexpr int kWaitVmcnt0 = (0x7 << 4) | (0xF << 8);  // s_waitcnt vmcnt(0), other counters open
-#ifndef NSD_ATTN_COMBINE_TABLE
-#define NSD_ATTN_COMBINE_TABLE 1
-#endif
-constexpr bool kUseCombineTable = NSD_ATTN_COMBINE_TABLE != 0;
-#ifndef NSD_ATTN_PIECE_TABLE
-#define NSD_ATTN_PIECE_TABLE 1
-#endif
-constexpr bool kUsePieceTable = NSD_ATTN_PIECE_TABLE != 0;
-static_assert(kMaxGroupRows <= 48, "at most three 16-row tiles per wave");
-static_assert(kMaxPieceBlocks <= kWaves * kWave, "one block id per lane of its wave");
 
 // 16-byte chunk x of row t of a K tile sits at chunk x ^ swz_k(t): the score
 // operand reads 16 rows x one chunk, and any 8 consecutive rows land on 8
@@ -94,30 +71,6 @@ static_assert(kMaxPieceBlocks <= kWaves * kWave, "one block id per lane of its w
 // the 4 rows 4 distinct pairs.
 __device__ inline int swz_k(int t) { return t & 7; }
 __device__ inline int swz_v(int t) { return 2 * (t & 3); }
-
-struct AttnArgs {
-  const f16* q;            // [R, Hq, D]
-  f16* o;                  // [R, Hq, D]
-  float* lse;              // [R, Hq] natural log, optional
-  const f16* k_cache;
-  const f16* v_cache;
-  const int32_t* bt;
-  int64_t bt_stride;
-  const int32_t* pieces;   // plan: piece records, one per workgroup
-  f16* part_o;             // [slots, rows_max, D]  normalised O
-  float* part_lse;         // [slots, rows_max]  (log2 domain)
-  const int32_t* combines; // plan: combine records of the segments cut into pieces
-  int32_t* claim;          // claim counter of the claimed records (zero between calls)
-  int n_static;            // workgroups below this stream the record of their index
-  int n_claimed;           // records after those, claimed in order by the later workgroups
-  int n_claim_wgs;         // the later workgroups (each claims once)
-  int piece_table;         // 1: the static pieces' block-table positions are in the PieceTable argument
-  int32_t* status;
-  int64_t num_blocks;
-  int64_t blk_stride;      // elements per cache block: L*Hkv*16*128
-  int num_layers, layer, hq, hkv, gqa, rows_max;
-  float scale_log2;        // softmax_scale * log2(e)
-};
 
 // The buffer's loads and waits are inline asm: the compiler does not see
 // them, so it neither drains the loads in flight before every LDS read of
@@ -137,220 +90,11 @@ __device__ inline void wait_vm() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-// Max and sum over the four 16-lane rows of a wave (lanes l, l^16, l^32,
-// l^48) with gfx950's row-swap moves: v_permlane16_swap pairs rows 0-1 and
-// 2-3, v_permlane32_swap pairs rows 0-2 and 1-3; every lane ends with the
-// same value.
-__device__ inline float rows_max(float x) {
-  const uint32_t u = __float_as_uint(x);
-  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-  const float y = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const uint32_t v = __float_as_uint(y);
-  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ inline float rows_sum(float x) {
-  const uint32_t u = __float_as_uint(x);
-  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-  const float y = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-  const uint32_t v = __float_as_uint(y);
-  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
-// Second launch: merge the partials of the segments cut into pieces, the
-// same exp2-domain combine as phase 2 of the reference
-// (paged_attn.py:128-149).  The kernel boundary orders it after every partial
-// store of the attention launch.
-//
-// Threads per (row, 8 dims) of the merge: one while a segment's slots are one
-// round of a thread's loads (8), else four (up to 32 slots) or sixteen.  The
-// merge is latency-bound, and a round is one more trip to memory: one request
-// of 32k tokens, 64 slots a segment, took 8.1 us with one thread in eight
-// rounds and takes 3.9 with sixteen threads in one; 9 to 17 slots (ragged
-// verify) 4.6 either way.
-constexpr int kMergeSlots = 8;
-
-// Row n (of the segment's q_len x GQA rows), dims 8 d8 .. 8 d8 + 7, of a
-// split segment of kv head `head` whose partials sit in slots [first, first
-// + n_slots), at most kMergeSlots: their loads all in flight, the slots
-// folded in slot order (log-sum-exp) and the row stored.
-__device__ inline void merge_row(const AttnArgs& a, int head, int first, int n_slots, int row_start, int n,
-                                 int d8) {
-  const f16* po = a.part_o + ((int64_t)first * a.rows_max + n) * D + 8 * d8;
-  const float* pl = a.part_lse + (int64_t)first * a.rows_max + n;
-  const int64_t sstride = (int64_t)a.rows_max * D;  // elements between slots
-  f32x4 v0[kMergeSlots], v1[kMergeSlots];
-  float ls[kMergeSlots];
-#pragma unroll
-  for (int u = 0; u < kMergeSlots; ++u) {
-    const int sidx = u < n_slots ? u : 0;
-    ls[u] = u < n_slots ? pl[(int64_t)sidx * a.rows_max] : -INFINITY;
-    f16x8 h = *reinterpret_cast<const f16x8*>(po + sidx * sstride);
-    if (u >= n_slots) h = f16x8{};  // a repeated slot may hold an infinity: 0 * inf
-    v0[u] = f32x4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
-    v1[u] = f32x4{(float)h[4], (float)h[5], (float)h[6], (float)h[7]};
-  }
-  float M = -INFINITY, W = 0.f;
-#pragma unroll
-  for (int u = 0; u < kMergeSlots; ++u) M = fmaxf(M, ls[u]);  // finite: slot 0 holds token 0, which every row attends
-  f32x4 acc0 = {0.f, 0.f, 0.f, 0.f}, acc1 = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int u = 0; u < kMergeSlots; ++u) {
-    const float wgt = exp2f(ls[u] - M);
-    acc0 += v0[u] * wgt;
-    acc1 += v1[u] * wgt;
-    W += wgt;
-  }
-  const float inv = 1.f / W;
-  const int qi = n / a.gqa, gh = n - qi * a.gqa;
-  const int64_t orow = (int64_t)(row_start + qi) * a.hq + head * a.gqa + gh;
-  f16x8 hv = {(f16)(acc0[0] * inv), (f16)(acc0[1] * inv), (f16)(acc0[2] * inv),
-              (f16)(acc0[3] * inv), (f16)(acc1[0] * inv), (f16)(acc1[1] * inv),
-              (f16)(acc1[2] * inv), (f16)(acc1[3] * inv)};
-  *reinterpret_cast<f16x8*>(a.o + orow * D + 8 * d8) = hv;
-  if (d8 == 0 && a.lse != nullptr) a.lse[orow] = (M + __log2f(W)) * kLn2;
-}
-
-// A partly merged row: running max (log2), sum of weights, 8 dims.
-struct MergeState {
-  float M, W;
-  f32x4 lo, hi;
-};
-__device__ inline void merge_states(MergeState& a, float M2, float W2, f32x4 lo2, f32x4 hi2) {
-  const float M = fmaxf(a.M, M2);
-  const float use = M == -INFINITY ? 0.f : M;  // neither holds a slot
-  const float s1 = exp2f(a.M - use), s2 = exp2f(M2 - use);
-  a.lo = a.lo * s1 + lo2 * s2;
-  a.hi = a.hi * s1 + hi2 * s2;
-  a.W = a.W * s1 + W2 * s2;
-  a.M = M;
-}
-
-// merge_row for segments of many slots: SL threads take slots sl, sl + SL,
-// ... of a (row, 8 dims) each, and their states are merged over the wave's
-// 16-lane rows and, past four threads, over the workgroup's waves in LDS, in a
-// fixed order.
-template <int SL>
-__device__ inline void merge_row_wide(const AttnArgs& a, int head, int first, int n_slots, int row_start, int n,
-                                      int n_rows, int d8, int sl) {
-  const int nr = n < n_rows ? n : 0;  // every thread takes part in the exchanges
-  const f16* po = a.part_o + ((int64_t)first * a.rows_max + nr) * D + 8 * d8;
-  const float* pl = a.part_lse + (int64_t)first * a.rows_max + nr;
-  MergeState st = {-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-  for (int s0 = sl; s0 < n_slots; s0 += 4 * SL) {
-    float ls[4];
-    f16x8 h[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int s = s0 + SL * u;
-      const int at = s < n_slots ? s : s0;
-      ls[u] = s < n_slots ? pl[(int64_t)at * a.rows_max] : -INFINITY;
-      h[u] = *reinterpret_cast<const f16x8*>(po + (int64_t)at * a.rows_max * D);
-    }
-    const float M = fmaxf(fmaxf(fmaxf(ls[0], ls[1]), fmaxf(ls[2], ls[3])), st.M);
-    const float use = M == -INFINITY ? 0.f : M;
-    const float keep = exp2f(st.M - use);
-    st.lo *= keep;
-    st.hi *= keep;
-    st.W *= keep;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const float wgt = exp2f(ls[u] - use);
-      if (s0 + SL * u >= n_slots) h[u] = f16x8{};  // a repeated slot may hold an infinity: 0 * inf
-      st.lo += f32x4{(float)h[u][0], (float)h[u][1], (float)h[u][2], (float)h[u][3]} * wgt;
-      st.hi += f32x4{(float)h[u][4], (float)h[u][5], (float)h[u][6], (float)h[u][7]} * wgt;
-      st.W += wgt;
-    }
-    st.M = M;
-  }
-#pragma unroll
-  for (int m = 16; m <= 32; m <<= 1) {  // the wave's four 16-lane rows
-    f32x4 lo, hi;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      lo[e] = __shfl_xor(st.lo[e], m, kWave);
-      hi[e] = __shfl_xor(st.hi[e], m, kWave);
-    }
-    const float M2 = __shfl_xor(st.M, m, kWave), W2 = __shfl_xor(st.W, m, kWave);
-    merge_states(st, M2, W2, lo, hi);
-  }
-  if constexpr (SL == 16) {
-    __shared__ MergeState s_wave[4][16];
-    if ((threadIdx.x & 63) < 16) s_wave[threadIdx.x >> 6][d8] = st;
-    __syncthreads();
-    if (threadIdx.x >= 16) return;
-#pragma unroll
-    for (int v = 1; v < 4; ++v) merge_states(st, s_wave[v][d8].M, s_wave[v][d8].W, s_wave[v][d8].lo, s_wave[v][d8].hi);
-  }
-  if (n >= n_rows || sl != 0) return;
-  const float inv = 1.f / st.W;
-  const int qi = n / a.gqa, gh = n - qi * a.gqa;
-  const int64_t orow = (int64_t)(row_start + qi) * a.hq + head * a.gqa + gh;
-  f16x8 hv;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    hv[e] = (f16)(st.lo[e] * inv);
-    hv[e + 4] = (f16)(st.hi[e] * inv);
-  }
-  *reinterpret_cast<f16x8*>(a.o + orow * D + 8 * d8) = hv;
-  if (d8 == 0 && a.lse != nullptr) a.lse[orow] = (st.M + __log2f(st.W)) * kLn2;
-}
-
-// Row group `group` of a segment, SL threads per (row, 8 dims): 16 / SL rows
-// a workgroup.
-template <int SL>
-__device__ inline void merge_group(const AttnArgs& a, int head, int first, int n_slots, int row_start, int n_rows,
-                                   int group) {
-  const int d8 = threadIdx.x & 15, p = threadIdx.x >> 4;
-  const int n = group * (16 / SL) + p / SL;
-  if constexpr (SL == 1) {
-    if (n < n_rows) merge_row(a, head, first, n_slots, row_start, n, d8);
-  } else {
-    if (group * (16 / SL) < n_rows) merge_row_wide<SL>(a, head, first, n_slots, row_start, n, n_rows, d8, p % SL);
-  }
-}
-
-// Workgroup (c, g) merges row group g of combine record c.
-template <int SL>
-__global__ __launch_bounds__(256) void combine_kernel(AttnArgs a, int row_groups) {
-  const int32_t* c = a.combines + kPieceWords * (blockIdx.x / row_groups);
-  merge_group<SL>(a, c[kCombHead], c[kCombFirst], c[kCombSlots], c[kCombRowStart], c[kCombQLen] * a.gqa,
-                  blockIdx.x % row_groups);
-}
-
-// The combine records of plans with at most kCombineTableMax of them, packed
-// into the launch's arguments (64 bits each: first slot 20, slots 8, kv head
-// 8, first row 20, q_len 8), so that a workgroup reads its record with the
-// arguments instead of one more dependent load.
-constexpr int kCombineTableMax = 448;
-struct CombineTable {
-  uint64_t e[kCombineTableMax];
-};
-
-// Workgroup (c, g) = (blockIdx.x, blockIdx.y): the entry's address depends on
-// the workgroup index alone, so it loads with the other arguments.
-template <int SL>
-__global__ __launch_bounds__(256) void combine_table_kernel(AttnArgs a, CombineTable tab) {
-  const uint64_t e = tab.e[blockIdx.x];
-  merge_group<SL>(a, (int)((e >> 28) & 0xff), (int)(e & 0xfffff), (int)((e >> 20) & 0xff), (int)((e >> 36) & 0xfffff),
-                  (int)(e >> 56) * a.gqa, (int)blockIdx.y);
-}
-
 // One workgroup streams one piece: blocks [blk_begin, blk_end) of a (group,
 // kv head) segment, for all of the group's query rows (NT tiles of 16 rows).
 // Block j goes to wave j % 4, which streams its blocks through its own
 // double buffer and keeps its own softmax state; the four states are merged
 // in wave order at the end.
-// Block-table positions of the static pieces (32 bits each: seq_id 16, first
-// block 16), packed into the launch's arguments when there are at most
-// kPieceTableMax of them: a workgroup's block ids then load beside its
-// record instead of after it.
-constexpr int kPieceTableMax = 920;
-struct PieceTable {
-  uint32_t e[kPieceTableMax];
-};
-
 // The fused prologue (nsd_paged_attention_fused): the rows' q, k and v as
 // the q/k/v projection left them, either fp16 rows (row strides in
 // elements) or that projection's fp32 split partials [splits][rows][(Hq +
@@ -958,12 +702,6 @@ static __device__ __align__(256) char scratch[NSD_NOALLOC_SCRATCH_BYTES];
 
 namespace {
 
-// Workspace bytes a plan needs: the claim counter (when it has claimed
-// records) and the partials.
-int64_t plan_partial_bytes(const int32_t* plan_host) {
-  return plan_workspace_bytes(plan_host[kPlanSlots], plan_host[kPlanRowsMax]);
-}
-
 // Shared body of the two attention entry points: `part` holds the partials
 // (`part_capacity` bytes).
 int paged_attention_impl(const void* q, void* o, float* lse, const void* k_cache,
@@ -973,157 +711,22 @@ int paged_attention_impl(const void* q, void* o, float* lse, const void* k_cache
                          const int32_t* plan_host, const int32_t* plan_dev, void* part,
                          int64_t part_capacity, float softmax_scale, int32_t* status,
                          void* stream, const FusedArgs* fused = nullptr) {
-  if (head_dim != D) return fail(NSD_ERR_UNSUPPORTED, "paged_attention: head_dim=%d (only 128)", head_dim);
-  if (block_size != BS)
-    return fail(NSD_ERR_UNSUPPORTED, "paged_attention: block_size=%d (only 16)", block_size);
-  if (!plan_host || !plan_dev) return fail(NSD_ERR_INVALID, "paged_attention: null plan");
-  if (plan_host[kPlanMagic] != kPlanMagicValue || plan_host[kPlanVersion] != kPlanVersionValue)
-    return fail(NSD_ERR_INVALID, "paged_attention: not a plan (bad magic/version)");
-  if (plan_host[kPlanHq] != num_q_heads || plan_host[kPlanHkv] != num_kv_heads)
-    return fail(NSD_ERR_INVALID, "paged_attention: plan built for Hq=%d Hkv=%d, called with %d/%d",
-                plan_host[kPlanHq], plan_host[kPlanHkv], num_q_heads, num_kv_heads);
-  if (num_layers <= 0 || layer < 0 || layer >= num_layers || num_blocks <= 0 || bt_stride <= 0 ||
-      bt_rows <= 0)
-    return fail(NSD_ERR_INVALID,
-                "paged_attention: layer=%d of %d, blocks=%lld, block table %lld x %lld", layer,
-                num_layers, (long long)num_blocks, (long long)bt_rows, (long long)bt_stride);
-  const int grid = plan_host[kPlanWorkers];
-  const int n_combine = plan_host[kPlanCombines];
-  const int rows_max = plan_host[kPlanRowsMax];
-  const int n_rows_plan = plan_host[kPlanRows];
-  if (n_rows_plan == 0 || grid == 0) return NSD_OK;
-  if ((!q && !fused) || !o || !k_cache || !v_cache || !block_table)
-    return fail(NSD_ERR_INVALID, "paged_attention: null pointer");
-  if ((!fused && !aligned16(q)) || !aligned16(o) || !aligned16(k_cache) || !aligned16(v_cache))
-    return fail(NSD_ERR_INVALID, "paged_attention: q/o/caches must be 16-byte aligned");
-  const int nt = (rows_max + 15) / 16;
-  const int64_t n_slots = plan_host[kPlanSlots];
-  const int n_static = plan_host[kPlanStatic], n_claimed = plan_host[kPlanClaimed];
-  const int n_records = plan_host[kPlanPieces];
-  if (rows_max < 1 || rows_max > kMaxGroupRows || n_static < 0 || n_static % kXcds != 0 || n_claimed < 0 ||
-      n_records != n_static + n_claimed || grid < n_records || (n_claimed == 0 && grid != n_static) ||
-      plan_host[kPlanMaxBlocks] < 1 || plan_host[kPlanMaxBlocks] > kMaxPieceBlocks || n_slots < 0 ||
-      n_combine < 0)
-    return fail(NSD_ERR_INVALID, "paged_attention: corrupt plan header");
-  if (plan_host[kPlanBtStride] != bt_stride || plan_host[kPlanBtRows] > bt_rows)
-    return fail(NSD_ERR_INVALID,
-                "paged_attention: plan built for a block table of %d rows x %d, called with "
-                "%lld x %lld",
-                plan_host[kPlanBtRows], plan_host[kPlanBtStride], (long long)bt_rows,
-                (long long)bt_stride);
-  // the kernel trusts the records it streams blocks from: check every one
-  // against the buffers it will touch
-  const int gqa = num_q_heads / num_kv_heads;
-  const int32_t* pr = plan_host + plan_host[kPlanOffPieces];
-  for (int i = 0; i < n_records; ++i) {
-    const int32_t* r = pr + kPieceWords * i;
-    if (r[kPieceQLen] == 0) continue;  // an empty record: its workgroup exits at once
-    const int nb = r[kPieceBlkEnd] - r[kPieceBlkBegin];
-    const bool split_ok =
-        r[kPieceSlot] < 0 ||
-        (r[kPieceComb] >= 0 && r[kPieceComb] < n_combine && r[kPieceCombFirst] >= 0 &&
-         r[kPieceCombSlots] >= 2 && r[kPieceCombFirst] + (int64_t)r[kPieceCombSlots] <= n_slots &&
-         r[kPieceSlot] >= r[kPieceCombFirst] && r[kPieceSlot] < r[kPieceCombFirst] + r[kPieceCombSlots]);
-    if (r[kPieceBlkBegin] < 0 || nb < 1 || nb > kMaxPieceBlocks || r[kPieceBlkEnd] > bt_stride ||
-        r[kPieceSeqId] < 0 || r[kPieceSeqId] >= bt_rows || r[kPieceHead] < 0 ||
-        r[kPieceHead] >= num_kv_heads || r[kPieceQLen] < 1 || (int64_t)r[kPieceQLen] * gqa > rows_max ||
-        r[kPieceRowStart] < 0 || (int64_t)r[kPieceRowStart] + r[kPieceQLen] > n_rows_plan ||
-        r[kPieceCtx] < 0 || !split_ok)
-      return fail(NSD_ERR_INVALID, "paged_attention: corrupt plan (piece %d)", i);
-  }
-  // ... and every combine record against the partials and the output rows
-  const int32_t* cr = plan_host + plan_host[kPlanOffCombines];
-  for (int c = 0; c < n_combine; ++c) {
-    const int32_t* r = cr + kPieceWords * c;
-    if (r[kCombHead] < 0 || r[kCombHead] >= num_kv_heads || r[kCombFirst] < 0 ||
-        r[kCombSlots] < 2 || (int64_t)r[kCombFirst] + r[kCombSlots] > n_slots ||
-        r[kCombQLen] < 1 || (int64_t)r[kCombQLen] * gqa > rows_max || r[kCombRowStart] < 0 ||
-        (int64_t)r[kCombRowStart] + r[kCombQLen] > n_rows_plan)
-      return fail(NSD_ERR_INVALID, "paged_attention: corrupt plan (combine %d)", c);
-  }
-  const int64_t part_bytes = plan_partial_bytes(plan_host);
-  if ((n_combine > 0 || n_claimed > 0) && (part == nullptr || part_capacity < part_bytes || !aligned16(part)))
-    return fail(NSD_ERR_WORKSPACE,
-                "paged_attention: workspace holds %lld partial bytes, the plan needs %lld",
-                (long long)part_capacity, (long long)part_bytes);
-
-  AttnArgs args;
-  args.q = static_cast<const f16*>(q);
-  args.o = static_cast<f16*>(o);
-  args.lse = lse;
-  args.k_cache = static_cast<const f16*>(k_cache);
-  args.v_cache = static_cast<const f16*>(v_cache);
-  args.bt = block_table;
-  args.bt_stride = bt_stride;
-  args.pieces = plan_dev + plan_host[kPlanOffPieces];
-  char* ws = static_cast<char*>(part);
-  args.claim = n_claimed > 0 ? reinterpret_cast<int32_t*>(ws) : nullptr;
-  args.n_static = n_static;
-  args.n_claimed = n_claimed;
-  args.n_claim_wgs = grid - n_static;
-  args.part_o = reinterpret_cast<f16*>(ws + kClaimBytes);
-  args.part_lse = reinterpret_cast<float*>(args.part_o + n_slots * rows_max * D);
-  args.combines = plan_dev + plan_host[kPlanOffCombines];
-  args.status = status;
-  args.num_blocks = num_blocks;
-  args.blk_stride = (int64_t)num_layers * num_kv_heads * BS * D;
-  args.num_layers = num_layers;
-  args.layer = layer;
-  args.hq = num_q_heads;
-  args.hkv = num_kv_heads;
-  args.gqa = gqa;
-  args.rows_max = rows_max;
-  args.scale_log2 = softmax_scale * 1.4426950408889634f;
-
+  AttnCall c;
+  const int rc = prepare_attention("paged_attention", q, fused == nullptr, o, lse, k_cache, v_cache, num_blocks,
+                                   num_layers, layer, num_q_heads, num_kv_heads, head_dim, block_size, block_table,
+                                   bt_rows, bt_stride, plan_host, plan_dev, part, part_capacity, softmax_scale,
+                                   status, &c);
+  if (rc != NSD_OK || c.grid == 0) return rc;
   hipStream_t st = as_stream(stream);
-  // the static pieces' block-table positions, when they fit the arguments
-  PieceTable pt;
-  args.piece_table = kUsePieceTable && n_static <= kPieceTableMax ? 1 : 0;
-  for (int i = 0; args.piece_table && i < n_static; ++i) {
-    const int32_t* r = pr + kPieceWords * i;
-    const bool live = r[kPieceQLen] != 0;
-    const int32_t sid = live ? r[kPieceSeqId] : 0, b0 = live ? r[kPieceBlkBegin] : 0;
-    if (sid >= (1 << 16) || b0 >= (1 << 16)) {
-      args.piece_table = 0;
-      break;
-    }
-    pt.e[i] = (uint32_t)sid | (uint32_t)b0 << 16;
-  }
-  const int rc = fused != nullptr
-                     ? (nt == 1   ? launch_nt_fused<1>(args, pt, *fused, grid, st)
-                        : nt == 2 ? launch_nt_fused<2>(args, pt, *fused, grid, st)
-                                  : launch_nt_fused<3>(args, pt, *fused, grid, st))
-                 : nt == 1 ? launch_nt<1>(args, pt, grid, st)
-                 : nt == 2 ? launch_nt<2>(args, pt, grid, st)
-                           : launch_nt<3>(args, pt, grid, st);
-  if (rc != NSD_OK || n_combine == 0) return rc;
-  const int32_t* crec = plan_host + plan_host[kPlanOffCombines];
-  bool packed = kUseCombineTable && n_combine <= kCombineTableMax;
-  int most_slots = 0;
-  for (int c = 0; c < n_combine; ++c) most_slots = std::max(most_slots, (int)crec[kPieceWords * c + kCombSlots]);
-  CombineTable tab;
-  for (int c = 0; packed && c < n_combine; ++c) {
-    const int32_t* r = crec + kPieceWords * c;
-    if (r[kCombFirst] >= (1 << 20) || r[kCombSlots] >= 256 || r[kCombHead] >= 256 || r[kCombRowStart] >= (1 << 20) ||
-        r[kCombQLen] >= 256) {
-      packed = false;
-      break;
-    }
-    tab.e[c] = (uint64_t)r[kCombFirst] | (uint64_t)r[kCombSlots] << 20 | (uint64_t)r[kCombHead] << 28 |
-               (uint64_t)r[kCombRowStart] << 36 | (uint64_t)r[kCombQLen] << 56;
-  }
-  auto merge = [&](auto slc) {
-    constexpr int SL = decltype(slc)::value;
-    const int groups = (rows_max * SL + 15) / 16;
-    if (packed)
-      hipLaunchKernelGGL(combine_table_kernel<SL>, dim3(n_combine, groups), dim3(256), 0, st, args, tab);
-    else
-      hipLaunchKernelGGL(combine_kernel<SL>, dim3(n_combine * groups), dim3(256), 0, st, args, groups);
-  };
-  if (most_slots <= kMergeSlots) merge(std::integral_constant<int, 1>{});
-  else if (most_slots <= 4 * kMergeSlots) merge(std::integral_constant<int, 4>{});
-  else merge(std::integral_constant<int, 16>{});
-  return launch_status("paged_attention: partial merge");
+  const int launched = fused != nullptr
+                     ? (c.row_tiles == 1   ? launch_nt_fused<1>(c.args, c.pieces, *fused, c.grid, st)
+                        : c.row_tiles == 2 ? launch_nt_fused<2>(c.args, c.pieces, *fused, c.grid, st)
+                                  : launch_nt_fused<3>(c.args, c.pieces, *fused, c.grid, st))
+                 : c.row_tiles == 1 ? launch_nt<1>(c.args, c.pieces, c.grid, st)
+                 : c.row_tiles == 2 ? launch_nt<2>(c.args, c.pieces, c.grid, st)
+                           : launch_nt<3>(c.args, c.pieces, c.grid, st);
+  if (launched != NSD_OK) return launched;
+  return launch_merge("paged_attention: partial merge", c, plan_host, st);
 }
 
 constexpr int64_t kScratchBytes = int64_t(NSD_NOALLOC_SCRATCH_BYTES);
