@@ -19,6 +19,7 @@ NSD_ERR_WORKSPACE = 4
 STATUS_BAD_BLOCK = 1
 STATUS_BAD_SEQ = 2
 STATUS_BAD_POSITION = 4
+STATUS_NONFINITE = 8
 PLAN_HEADER_WORDS = 24
 COPY_D2H = 0
 COPY_H2D = 1
@@ -143,6 +144,22 @@ SIGNATURES = {
     "nsd_mxfp4_up_gate_silu_and_mul": (
         c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p,
                 c_int64, c_void_p]),
+    "nsd_kv8_store": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int, c_void_p,
+                c_void_p]),
+    "nsd_kv8_store_prefill": (
+        c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
+                c_int64, c_int64, c_int, c_void_p, c_void_p]),
+    "nsd_kv8_qk_norm_rope_store": (
+        c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_float,
+                c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int,
+                c_int, c_void_p, c_void_p]),
+    "nsd_kv8_load": (
+        c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
+                c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p]),
+    "nsd_kv8_paged_attention": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int64, c_int64, _I32P, c_void_p,
+                c_void_p, c_int64, c_float, c_void_p, c_void_p]),
     "nsd_prefill_attention": (
         c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
                 c_int64, c_int, c_int, c_int, c_float, c_void_p, c_void_p]),

@@ -1,0 +1,390 @@
+// Paged verify/decode attention over the 8-bit KV cache for gfx950.
+//
+// The work is the fp16 attention's (nsd_attention.hip): a workgroup of four
+// waves streams one piece, blocks [blk_begin, blk_end) of a (verify group, kv
+// head) segment, for all of the segment's query rows, by the same plan; a
+// second launch merges the segments cut into pieces.
+//
+//   S^T[token][row] = K[token][:] . Q[row][:]            (A = K, B = Q^T)
+//   O^T[dim][row]  += V^T[dim][token] . P^T[token][row]  (A = V^T, B = P^T)
+//
+// Both in v_mfma_f32_16x16x32_f16.  A cache's values are fp16 values, so the
+// codes become operands without a rounding: E4M3 with the block's scale in the
+// one instruction that converts two, whole numbers by a byte permutation and a
+// subtraction (K's scale then multiplies the scores, V's the operand).
+//
+// Wave w takes blocks w, w + 4, ... of the piece by pairs: the 32 tokens of a
+// pair are the k of one PV product.  S^T of a block leaves lane (lr, lg) with
+// tokens 4lg .. 4lg+3 of row lr, which for the two blocks is P^T's operand as it
+// stands, with the pair's tokens in the order that V's operand is put together.
+//
+// A tile lies in the cache as its operand is held: lane l's 16 bytes of load j
+// are unit 64 j + l of the tile.  So codes go from HBM straight into the
+// registers that the conversion reads, in runs of 1 KB, with no LDS and no
+// transpose.  Lane (i, g) of K holds dims 8c .. 8c+7 and 64+8c .. of token i (c =
+// 4 j + g): the query operand has its dims in that order too.  Of V it holds
+// dims 8i .. 8i+7 of tokens 4g .. 4g+3: tile m of O^T is dims m, 8 + m, ..., and
+// a lane ends with 8 dims in a row, one 16-byte store.
+//
+// Every access to a tile goes through a buffer descriptor of the tile alone, so
+// the blocks that a wave does not have (the second of an odd pair, those past
+// the last) and ids outside the pool are descriptors of no bytes: their loads
+// return zeros without a trip to memory, and every wave issues the same loads,
+// which the compiler's in-order waits count on.
+#include "nsd_kv8_device.h"
+#include "nsd_paged.h"
+
+namespace nsd {
+namespace {
+
+struct Kv8Caches {
+  const char* k;
+  const char* v;
+  const uint8_t* ks;
+  const uint8_t* vs;
+};
+
+// Pairs of blocks in registers or on their way, a wave: as many as the
+// registers of two waves a SIMD hold beside the accumulators.
+template <int NT>
+constexpr int kv8_depth() { return NT == 1 ? 4 : NT == 2 ? 3 : 2; }
+
+// 0x80 in the bytes of four E4M3 codes that are NaN; and fp16 ones for bytes of
+// 1 (zeros for 0).
+__device__ inline uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+__device__ inline f16x4 ones_of(uint32_t w) {
+  w *= 0x3cu;  // the high byte of 1.0
+  const u32x2 h = {__builtin_amdgcn_perm(0u, w, 0x010c000cu), __builtin_amdgcn_perm(0u, w, 0x030c020cu)};
+  return __builtin_bit_cast(f16x4, h);
+}
+
+template <int T, int NT>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
+void kv8_attn_kernel(AttnArgs a, PieceTable pt, Kv8Caches cache) {
+  constexpr int DEPTH = kv8_depth<NT>();
+  __shared__ __align__(16) char smem[kWaves * kMergeWave];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+  int rec_idx = blockIdx.x;
+  if (rec_idx >= a.n_static) {
+    // claim the next record: one device-scope add per workgroup; the last
+    // workgroup to claim sets the counter back to zero for the next call
+    __shared__ int s_ticket;
+    if (threadIdx.x == 0) {
+      const int t = __hip_atomic_fetch_add(a.claim, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (t == a.n_claim_wgs - 1) __hip_atomic_store(a.claim, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      s_ticket = t;
+    }
+    __syncthreads();
+    const int t = s_ticket;
+    if (t >= a.n_claimed) return;
+    rec_idx = a.n_static + t;
+  }
+  // a static workgroup with the table reads block ids right away (lanes past
+  // the piece read a clamped, in-row column and are discarded below)
+  const bool tabled = a.piece_table != 0 && (int)blockIdx.x < a.n_static;
+  int tab_id = 0;
+  if (tabled) {
+    const uint32_t e = pt.e[blockIdx.x];
+    int64_t col = (int64_t)(e >> 16) + wave + kWaves * lane;
+    col = col < a.bt_stride ? col : a.bt_stride - 1;
+    tab_id = a.bt[(int64_t)(e & 0xffffu) * a.bt_stride + col];
+  }
+  // the whole record in one round of scalar loads
+  using const_i32p = const __attribute__((address_space(4))) int32_t*;
+  const const_i32p rec = (const_i32p)(uintptr_t)(a.pieces + (int64_t)__builtin_amdgcn_readfirstlane(rec_idx) * kPieceWords);
+  int32_t rv[kPieceWords];
+#pragma unroll
+  for (int i = 0; i < kPieceWords; ++i) rv[i] = rec[i];
+  asm volatile("" ::"s"(rv[0]), "s"(rv[1]), "s"(rv[2]), "s"(rv[3]), "s"(rv[4]), "s"(rv[5]), "s"(rv[6]),
+               "s"(rv[7]), "s"(rv[8]), "s"(rv[9]), "s"(rv[10]), "s"(rv[11]));
+  const int q_len = rv[kPieceQLen];
+  if (q_len == 0) return;  // an empty record
+  const int head = rv[kPieceHead], blk0 = rv[kPieceBlkBegin];
+  const int nb = rv[kPieceBlkEnd] - blk0;  // 1 .. kMaxPieceBlocks (host-checked)
+  const int my_n = nb > wave ? (nb - wave + kWaves - 1) / kWaves : 0;  // this wave's blocks
+  const int pairs = (my_n + 1) / 2;
+  const int row_start = rv[kPieceRowStart], ctx = rv[kPieceCtx];
+  const int lr = lane & 15;
+  const int lg = lane >> 4;
+  const int n_rows = q_len * a.gqa;
+
+  // Block ids of this wave's blocks (block wave + 4i on lane i).
+  int blk_id = tab_id;
+  if (!tabled && lane < my_n) blk_id = a.bt[(int64_t)rv[kPieceSeqId] * a.bt_stride + blk0 + wave + kWaves * lane];
+  const bool bad = lane < my_n && (blk_id < 0 || blk_id >= a.num_blocks);
+  const bool good = lane < my_n && !bad;
+  const uint64_t bad_mask = __builtin_amdgcn_ballot_w64(bad);
+  if (bad_mask != 0 && lane == 0) flag_status(a.status, NSD_STATUS_BAD_BLOCK);
+  const int64_t tile = good ? ((int64_t)blk_id * a.num_layers + a.layer) * a.hkv + head : 0;
+  const int scales = good ? (int)cache.ks[tile] | (int)cache.vs[tile] << 8 : 0;
+  const uint32_t good_lo = (uint32_t)__builtin_amdgcn_ballot_w64(good);
+  const uint32_t good_hi = (uint32_t)(__builtin_amdgcn_ballot_w64(good) >> 32);
+
+  // Query rows of each row tile as the B operand of the score product; rows
+  // past the group read its row 0 and are never stored.
+  f16x8 qf[NT][4];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int n = 16 * t + lr;
+    const int nr = n < n_rows ? n : 0;
+    const int qi = nr / a.gqa, gh = nr - qi * a.gqa;
+    const f16* qrow = a.q + ((int64_t)(row_start + qi) * a.hq + head * a.gqa + gh) * D;
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+      qf[t][kk] = *reinterpret_cast<const f16x8*>(qrow + 64 * (kk & 1) + 8 * (4 * (kk >> 1) + lg));
+  }
+
+  // Block jj of the wave (any jj): its tile's bytes, two units a lane.
+  auto load = [&](const char* base, int jj, u32x4 (&w)[2]) __attribute__((always_inline)) {
+    const int at = jj < 64 ? jj : 63;
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)tile, at);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)tile >> 32), at);
+    const bool has = jj < my_n && ((jj < 32 ? good_lo >> jj : good_hi >> (jj - 32)) & 1);
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<char*>(base + (int64_t)(((uint64_t)hi << 32 | lo) * kKv8Tile)), 0, has ? kKv8Tile : 0, 0x00027000);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      w[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, lane * 16, 1024 * j, 2));
+  };
+  u32x4 kb[DEPTH][2][2], vb[DEPTH][2][2];  // [pair][block][load]
+#pragma unroll
+  for (int d = 0; d < DEPTH; ++d) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) load(cache.k, 2 * d + b, kb[d][b]);
+#pragma unroll
+    for (int b = 0; b < 2; ++b) load(cache.v, 2 * d + b, vb[d][b]);
+  }
+
+  int row_len[NT];  // causal bound of this lane's row in each tile
+  float m[NT], l[NT];
+  f32x4 acc[NT][8];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int n = 16 * t + lr;
+    row_len[t] = n < n_rows ? ctx + n / a.gqa + 1 : ctx + q_len;
+    m[t] = -INFINITY;
+    l[t] = 0.f;
+#pragma unroll
+    for (int mt = 0; mt < 8; ++mt) acc[t][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  for (int p0 = 0; p0 < pairs; p0 += DEPTH) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      const int p = p0 + d;
+      if (p >= pairs) break;
+      const int sc0 = __builtin_amdgcn_readlane(scales, 2 * p), sc1 = __builtin_amdgcn_readlane(scales, (2 * p + 1) & 63);
+      // S^T of both blocks
+      f32x4 s[2][NT];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const float power = kv8_power((b ? sc1 : sc0) & 0xff);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) s[b][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          const u32x4 w = kb[d][b][kk >> 1];
+          f16x8 ka;
+          if constexpr (T == NSD_KV8_E4M3) {
+            ka = kv8_values<T>(u32x2{w[2 * (kk & 1)], w[2 * (kk & 1) + 1]}, power);
+          } else {
+            f16x2 x[4];
+            kv8_whole(w[2 * (kk & 1)], x[0], x[1]);
+            kv8_whole(w[2 * (kk & 1) + 1], x[2], x[3]);
+            ka = f16x8{x[0][0], x[0][1], x[1][0], x[1][1], x[2][0], x[2][1], x[3][0], x[3][1]};
+          }
+#pragma unroll
+          for (int t = 0; t < NT; ++t) s[b][t] = mfma_k32(ka, qf[t][kk], s[b][t]);
+        }
+        if constexpr (T == NSD_KV8_INT8) {
+#pragma unroll
+          for (int t = 0; t < NT; ++t) s[b][t] *= power;
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < 2; ++b) load(cache.k, 2 * (p + DEPTH) + b, kb[d][b]);
+
+      const int first[2] = {(blk0 + wave + kWaves * 2 * p) * BS, (blk0 + wave + kWaves * (2 * p + 1)) * BS};
+      const bool masked[2] = {((bad_mask >> (2 * p)) & 1) != 0,
+                              2 * p + 1 >= my_n || ((bad_mask >> ((2 * p + 1) & 63)) & 1) != 0};
+      const bool edge = masked[0] || masked[1] || first[1] + BS > ctx + 1;  // a token may lie past a row's length
+      f16x8 pb[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float sv[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sv[e] = s[e / 4][t][e % 4];
+        if (edge) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (masked[e / 4] || first[e / 4] + 4 * lg + e % 4 >= row_len[t]) sv[e] = -INFINITY;
+        }
+        float mx = fmaxf(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])), fmaxf(fmaxf(sv[4], sv[5]), fmaxf(sv[6], sv[7])));
+        mx = rows_max(mx) * a.scale_log2;  // -inf stays -inf (scale > 0)
+        // lazy running max: one decision per wave and tile
+        if (__builtin_amdgcn_ballot_w64(mx > m[t] + kLazyMax) != 0) {
+          const float m_new = fmaxf(m[t], mx);
+          const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[t] - m_new);
+          l[t] *= alpha;
+#pragma unroll
+          for (int mt = 0; mt < 8; ++mt) acc[t][mt] *= alpha;
+          m[t] = m_new;
+        }
+        const float m_use = m[t] == -INFINITY ? 0.f : m[t];
+        float psum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          // weights of at most 2^8 in fp16: 2^-11 of each, as the fp16
+          // attention rounds them; their sum is of the unrounded ones
+          const float pj = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e], a.scale_log2, -m_use));
+          psum += pj;
+          pb[t][e] = (f16)pj;
+        }
+        l[t] += psum;
+      }
+
+      const float vp0 = kv8_power(sc0 >> 8), vp1 = kv8_power(sc1 >> 8);
+      if constexpr (T == NSD_KV8_E4M3) {
+        // 0 times a NaN is a NaN: where a row masks tokens, NaN codes leave the
+        // operand, and the dims that have them end as NaN for the rows that
+        // attend them
+        if (edge) {
+          uint32_t found = 0;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) found |= nan_bytes(vb[d][e / 8][e / 4 % 2][e % 4]);
+          if (__builtin_amdgcn_ballot_w64(found != 0) != 0) {
+#pragma unroll
+            for (int mt = 0; mt < 8; ++mt) {
+              uint32_t has[2];
+#pragma unroll
+              for (int b = 0; b < 2; ++b) {
+                has[b] = nan_bytes(vb[d][b][mt / 4][mt % 4]) >> 7;
+                vb[d][b][mt / 4][mt % 4] &= ~(has[b] * 0xffu);
+              }
+              const f16x8 is_nan = kv8_join(ones_of(has[0]), ones_of(has[1]));
+#pragma unroll
+              for (int t = 0; t < NT; ++t) {
+                f16x8 attended = {};
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                  if (!masked[e / 4] && first[e / 4] + 4 * lg + e % 4 < row_len[t]) attended[e] = (f16)1.f;
+                const f32x4 hit = mfma_k32(is_nan, attended, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[t][mt][e] = hit[e] > 0.f ? __builtin_nanf("") : acc[t][mt][e];
+              }
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int mt = 0; mt < 8; ++mt) {
+        const f16x8 va = kv8_join(kv8_values4<T>(vb[d][0][mt / 4][mt % 4], vp0), kv8_values4<T>(vb[d][1][mt / 4][mt % 4], vp1));
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[t][mt] = mfma_k32(va, pb[t], acc[t][mt]);
+      }
+#pragma unroll
+      for (int b = 0; b < 2; ++b) load(cache.v, 2 * (p + DEPTH) + b, vb[d][b]);
+    }
+  }
+
+  // Merge the four waves' states, one row tile at a time, in wave order.  Lane
+  // (lr, lg) of tile m holds dims 8 (4lg + r) + m of row lr in element r: wave w
+  // takes the elements r = w, the dims 32lg + 8w .. +7.
+  const int slot = rv[kPieceSlot];
+  float* mrg = (float*)smem;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const float lt = rows_sum(l[t]);
+    if (t > 0) __syncthreads();  // the previous tile's merge is read
+    float* mine = mrg + wave * (kMergeWave / 4);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<f32x4*>(mine + ((2 * r + h) * kWave + lane) * 4) =
+            f32x4{acc[t][4 * h][r], acc[t][4 * h + 1][r], acc[t][4 * h + 2][r], acc[t][4 * h + 3][r]};
+    if (lg == 0) {
+      mine[kMergeAcc / 4 + lr] = m[t];
+      mine[kMergeAcc / 4 + 16 + lr] = lt;
+    }
+    __syncthreads();
+    float mw[kWaves], lw[kWaves];
+    float M = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) {
+      mw[v] = mrg[v * (kMergeWave / 4) + kMergeAcc / 4 + lr];
+      lw[v] = mrg[v * (kMergeWave / 4) + kMergeAcc / 4 + 16 + lr];
+      M = fmaxf(M, mw[v]);
+    }
+    float L = 0.f, sc[kWaves];
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) {
+      sc[v] = mw[v] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw[v] - M);
+      L += lw[v] * sc[v];
+    }
+    const int n = 16 * t + lr;
+    if (n < n_rows) {
+      const float inv = L > 0.f ? 1.f / L : L != L ? L : 0.f;
+      const int qi = n / a.gqa, gh = n - qi * a.gqa;
+      const int64_t orow = (int64_t)(row_start + qi) * a.hq + head * a.gqa + gh;
+      f16* dst = slot < 0 ? a.o + orow * D : a.part_o + ((int64_t)slot * a.rows_max + n) * D;
+      f16x8 out;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        f32x4 o4 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int v = 0; v < kWaves; ++v)
+          o4 += *reinterpret_cast<const f32x4*>(mrg + v * (kMergeWave / 4) + ((2 * wave + h) * kWave + lane) * 4) * sc[v];
+        o4 *= inv;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[4 * h + e] = (f16)o4[e];
+      }
+      *reinterpret_cast<f16x8*>(dst + 32 * lg + 8 * wave) = out;
+      if (wave == 0 && lg == 0) {
+        const float lse2 = L > 0.f ? M + __log2f(L) : L != L ? L : -INFINITY;
+        if (slot >= 0) a.part_lse[(int64_t)slot * a.rows_max + n] = lse2;
+        else if (a.lse != nullptr) a.lse[orow] = lse2 * kLn2;
+      }
+    }
+  }
+}
+
+template <int T>
+void launch_rows(const AttnCall& c, const Kv8Caches& caches, hipStream_t st) {
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(c.grid), dim3(kThreads), 0, st, c.args, c.pieces, caches);
+  };
+  if (c.row_tiles == 1) go(kv8_attn_kernel<T, 1>);
+  else if (c.row_tiles == 2) go(kv8_attn_kernel<T, 2>);
+  else go(kv8_attn_kernel<T, 3>);
+}
+
+}  // namespace
+}  // namespace nsd
+
+using namespace nsd;
+
+extern "C" int nsd_kv8_paged_attention(const void* q, void* o, float* lse, const nsd_kv8_cache* cache, int layer,
+                                       int num_q_heads, const int32_t* block_table, int64_t bt_rows,
+                                       int64_t bt_stride, const int32_t* plan_host, const int32_t* plan_dev,
+                                       void* workspace, int64_t workspace_bytes, float softmax_scale,
+                                       int32_t* status, void* stream) {
+  const char* who = "kv8_paged_attention";
+  int rc = check_kv8_cache(who, cache, layer);
+  if (rc) return rc;
+  AttnCall c;
+  rc = prepare_attention(who, q, true, o, lse, cache->k, cache->v, cache->num_blocks, cache->num_layers, layer,
+                         num_q_heads, cache->num_kv_heads, D, BS, block_table, bt_rows, bt_stride, plan_host,
+                         plan_dev, workspace, workspace_bytes, softmax_scale, status, &c);
+  if (rc != NSD_OK || c.grid == 0) return rc;
+  const Kv8Caches caches = {static_cast<const char*>(cache->k), static_cast<const char*>(cache->v),
+                            static_cast<const uint8_t*>(cache->k_scales), static_cast<const uint8_t*>(cache->v_scales)};
+  hipStream_t st = as_stream(stream);
+  if (cache->codes == NSD_KV8_E4M3) launch_rows<NSD_KV8_E4M3>(c, caches, st);
+  else launch_rows<NSD_KV8_INT8>(c, caches, st);
+  rc = launch_status(who);
+  if (rc != NSD_OK) return rc;
+  return launch_merge("kv8_paged_attention: partial merge", c, plan_host, st);
+}

@@ -65,7 +65,7 @@ class StatusWord:
     """Optional device status word; ``check()`` synchronises and raises on flags."""
 
     NAMES = {1: "block id outside the pool", 2: "seq_id/position outside the block table",
-             4: "position outside the RoPE table"}
+             4: "position outside the RoPE table", 8: "values that are not finite"}
 
     def __init__(self, device):
         self.t = torch.zeros(1, dtype=torch.int32, device=device)
@@ -74,4 +74,4 @@ class StatusWord:
         v = int(self.t.item())
         if v:
             bad = [n for b, n in self.NAMES.items() if v & b]
-            raise RuntimeError(f"{what}: invalid metadata ({', '.join(bad)})")
+            raise RuntimeError(f"{what}: invalid {'metadata' if v & 7 else 'values'} ({', '.join(bad)})")
