@@ -158,7 +158,7 @@ SIGNATURES = {
         c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
                 c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p]),
     "nsd_kv8_paged_attention": (
-        c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int64, c_int64, _I32P, c_void_p,
+        c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
                 c_void_p, c_int64, c_float, c_void_p, c_void_p]),
     "nsd_prefill_attention": (
         c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,

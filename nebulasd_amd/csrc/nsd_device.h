@@ -60,6 +60,7 @@ inline int launch_status(const char* what) {
 inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
 typedef __attribute__((address_space(3))) char lds_char;
+typedef __attribute__((address_space(3))) uint32_t lds_u32;
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 typedef __attribute__((address_space(3))) f16x8 lds_f16x8;
 typedef __fp16 fp16x4_t __attribute__((ext_vector_type(4)));

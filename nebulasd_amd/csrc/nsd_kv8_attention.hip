@@ -19,18 +19,18 @@
 // stands, with the pair's tokens in the order that V's operand is put together.
 //
 // A tile lies in the cache as its operand is held: lane l's 16 bytes of load j
-// are unit 64 j + l of the tile.  So codes go from HBM straight into the
-// registers that the conversion reads, in runs of 1 KB, with no LDS and no
-// transpose.  Lane (i, g) of K holds dims 8c .. 8c+7 and 64+8c .. of token i (c =
-// 4 j + g): the query operand has its dims in that order too.  Of V it holds
-// dims 8i .. 8i+7 of tokens 4g .. 4g+3: tile m of O^T is dims m, 8 + m, ..., and
-// a lane ends with 8 dims in a row, one 16-byte store.
+// are unit 64 j + l of the tile.  A wave streams its pairs through a ring of its
+// own in LDS, two slots of 8 KB filled by global_load_lds_dwordx4 in runs of 1
+// KB; it reads a pair into registers, in runs again (no bank conflict, no
+// transpose), and refills the slot before it computes, so a pair and a half is
+// in flight at all times.  Lane (i, g) of K holds dims 8c .. 8c+7 and 64+8c ..
+// of token i (c = 4 j + g): the query operand has its dims in that order too.
+// Of V it holds dims 8i .. 8i+7 of tokens 4g .. 4g+3: tile m of O^T is dims m,
+// 8 + m, ..., and a lane ends with 8 dims in a row, one 16-byte store.
 //
-// Every access to a tile goes through a buffer descriptor of the tile alone, so
-// the blocks that a wave does not have (the second of an odd pair, those past
-// the last) and ids outside the pool are descriptors of no bytes: their loads
-// return zeros without a trip to memory, and every wave issues the same loads,
-// which the compiler's in-order waits count on.
+// Everything that follows the block ids comes through LDS (query rows and
+// scales too) and is waited for by count, in the order of issue, so that no
+// wait of the compiler's drains the tiles behind it.
 #include "nsd_kv8_device.h"
 #include "nsd_paged.h"
 
@@ -42,12 +42,30 @@ struct Kv8Caches {
   const char* v;
   const uint8_t* ks;
   const uint8_t* vs;
+  uint32_t ks_low, vs_low;  // the scales' addresses modulo 4
 };
 
-// Pairs of blocks in registers or on their way, a wave: as many as the
-// registers of two waves a SIMD hold beside the accumulators.
-template <int NT>
-constexpr int kv8_depth() { return NT == 1 ? 4 : NT == 2 ? 3 : 2; }
+constexpr int kSlot = 4 * kKv8Tile;  // a pair's K tiles, then its V tiles
+constexpr int kSlots = 2;
+constexpr int kRing = kWaves * kSlots * kSlot;  // 64 KB: two workgroups a CU
+constexpr int kScales = 2 * kWave * 4;          // a wave's words with the K and V scales of its blocks
+static_assert(kWaves * kMergeWave <= kRing, "the merge reuses the ring");
+
+// 1 KB from base + off (a lane's 16 bytes), or 64 dwords, into LDS; the compiler
+// sees neither the load nor its wait.
+__device__ inline void dma16(uint32_t lds, const char* base, uint32_t off) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2 nt" : : "s"(lds), "v"(off), "s"(base) : "memory", "m0");
+}
+__device__ inline void dma16_rows(uint32_t lds, const void* at) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(at) : "memory", "m0");
+}
+__device__ inline void dma4(uint32_t lds, const void* at) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" : : "s"(lds), "v"(at) : "memory", "m0");
+}
+template <int N>
+__device__ inline void wait_vm() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
 
 // 0x80 in the bytes of four E4M3 codes that are NaN; and fp16 ones for bytes of
 // 1 (zeros for 0).
@@ -61,10 +79,13 @@ __device__ inline f16x4 ones_of(uint32_t w) {
 template <int T, int NT>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
 void kv8_attn_kernel(AttnArgs a, PieceTable pt, Kv8Caches cache) {
-  constexpr int DEPTH = kv8_depth<NT>();
-  __shared__ __align__(16) char smem[kWaves * kMergeWave];
+  __shared__ __align__(16) char smem[kRing + NT * 16 * D * 2 + kWaves * kScales];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  lds_char* lds = (lds_char*)smem;
+  lds_char* ring = lds + wave * (kSlots * kSlot);
+  const lds_char* q_lds = lds + kRing;
+  const lds_char* scale_lds = q_lds + NT * 16 * D * 2 + wave * kScales;
 
   int rec_idx = blockIdx.x;
   if (rec_idx >= a.n_static) {
@@ -113,49 +134,59 @@ void kv8_attn_kernel(AttnArgs a, PieceTable pt, Kv8Caches cache) {
   // Block ids of this wave's blocks (block wave + 4i on lane i).
   int blk_id = tab_id;
   if (!tabled && lane < my_n) blk_id = a.bt[(int64_t)rv[kPieceSeqId] * a.bt_stride + blk0 + wave + kWaves * lane];
-  const bool bad = lane < my_n && (blk_id < 0 || blk_id >= a.num_blocks);
-  const bool good = lane < my_n && !bad;
-  const uint64_t bad_mask = __builtin_amdgcn_ballot_w64(bad);
-  if (bad_mask != 0 && lane == 0) flag_status(a.status, NSD_STATUS_BAD_BLOCK);
-  const int64_t tile = good ? ((int64_t)blk_id * a.num_layers + a.layer) * a.hkv + head : 0;
-  const int scales = good ? (int)cache.ks[tile] | (int)cache.vs[tile] << 8 : 0;
-  const uint32_t good_lo = (uint32_t)__builtin_amdgcn_ballot_w64(good);
-  const uint32_t good_hi = (uint32_t)(__builtin_amdgcn_ballot_w64(good) >> 32);
-
-  // Query rows of each row tile as the B operand of the score product; rows
-  // past the group read its row 0 and are never stored.
-  f16x8 qf[NT][4];
+  // The query rows of 16-row tiles as the B operand of the score product, shared
+  // by the waves: lane (lr, lg) of fragment kk holds dims 64 (kk % 2) + 8 (4 (kk /
+  // 2) + lg) .. +7 of row lr; wave w brings fragment w of every tile.  Rows past
+  // the group read its row 0 and are never stored.
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int n = 16 * t + lr;
     const int nr = n < n_rows ? n : 0;
     const int qi = nr / a.gqa, gh = nr - qi * a.gqa;
     const f16* qrow = a.q + ((int64_t)(row_start + qi) * a.hq + head * a.gqa + gh) * D;
-#pragma unroll
-    for (int kk = 0; kk < 4; ++kk)
-      qf[t][kk] = *reinterpret_cast<const f16x8*>(qrow + 64 * (kk & 1) + 8 * (4 * (kk >> 1) + lg));
+    dma16_rows((uint32_t)(uintptr_t)q_lds + (4 * t + wave) * 1024, qrow + 64 * (wave & 1) + 8 * (4 * (wave >> 1) + lg));
   }
+  const bool bad = lane < my_n && (blk_id < 0 || blk_id >= a.num_blocks);
+  const uint64_t bad_mask = __builtin_amdgcn_ballot_w64(bad);
+  // the block's tile, of fewer than 2^31 (host-checked); tile 0, masked, for
+  // ids outside the pool
+  const int tile = lane < my_n && !bad ? (blk_id * a.num_layers + a.layer) * a.hkv + head : 0;
+  // the aligned words with its scales
+  dma4((uint32_t)(uintptr_t)scale_lds, cache.ks + (((uint32_t)tile + cache.ks_low) & ~3u) - cache.ks_low);
+  dma4((uint32_t)(uintptr_t)scale_lds + 256, cache.vs + (((uint32_t)tile + cache.vs_low) & ~3u) - cache.vs_low);
 
-  // Block jj of the wave (any jj): its tile's bytes, two units a lane.
-  auto load = [&](const char* base, int jj, u32x4 (&w)[2]) __attribute__((always_inline)) {
-    const int at = jj < 64 ? jj : 63;
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)tile, at);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)tile >> 32), at);
-    const bool has = jj < my_n && ((jj < 32 ? good_lo >> jj : good_hi >> (jj - 32)) & 1);
-    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<char*>(base + (int64_t)(((uint64_t)hi << 32 | lo) * kKv8Tile)), 0, has ? kKv8Tile : 0, 0x00027000);
+  // pair p's tiles into its slot, 8 loads (4 if it has one block)
+  auto issue = [&](int p) __attribute__((always_inline)) {
+    const uint32_t slot = (uint32_t)(uintptr_t)ring + (p & 1) * kSlot;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-      w[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, lane * 16, 1024 * j, 2));
+    for (int b = 0; b < 2; ++b) {
+      if (b == 1 && 2 * p + 1 >= my_n) break;
+      const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(tile, 2 * p + b) * kKv8Tile;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        dma16(slot + b * kKv8Tile + 1024 * j, cache.k + at + 1024 * j, lane * 16);
+        dma16(slot + (2 + b) * kKv8Tile + 1024 * j, cache.v + at + 1024 * j, lane * 16);
+      }
+    }
   };
-  u32x4 kb[DEPTH][2][2], vb[DEPTH][2][2];  // [pair][block][load]
+  if (pairs > 0) issue(0);
+  if (pairs > 1) issue(1);
+  // the query rows and scales have landed; behind them up to 16 loads
+  if (my_n >= 4) wait_vm<16>();
+  else if (my_n == 3) wait_vm<12>();
+  else if (my_n == 2) wait_vm<8>();
+  else if (my_n == 1) wait_vm<4>();
+  else wait_vm<0>();
+  asm volatile("s_barrier" ::: "memory");  // the other waves' query rows
+  f16x8 qf[NT][4];
 #pragma unroll
-  for (int d = 0; d < DEPTH; ++d) {
+  for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int b = 0; b < 2; ++b) load(cache.k, 2 * d + b, kb[d][b]);
-#pragma unroll
-    for (int b = 0; b < 2; ++b) load(cache.v, 2 * d + b, vb[d][b]);
-  }
+    for (int kk = 0; kk < 4; ++kk) qf[t][kk] = *(const lds_f16x8*)(q_lds + ((4 * t + kk) * kWave + lane) * 16);
+  const uint32_t k_word = *(const lds_u32*)(scale_lds + 4 * lane), v_word = *(const lds_u32*)(scale_lds + 256 + 4 * lane);
+  const int k_scale = k_word >> (8 * (((uint32_t)tile + cache.ks_low) & 3)) & 0xff;
+  const int v_scale = v_word >> (8 * (((uint32_t)tile + cache.vs_low) & 3)) & 0xff;
+  if (bad_mask != 0 && lane == 0) flag_status(a.status, NSD_STATUS_BAD_BLOCK);
 
   int row_len[NT];  // causal bound of this lane's row in each tile
   float m[NT], l[NT];
@@ -170,122 +201,127 @@ void kv8_attn_kernel(AttnArgs a, PieceTable pt, Kv8Caches cache) {
     for (int mt = 0; mt < 8; ++mt) acc[t][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  for (int p0 = 0; p0 < pairs; p0 += DEPTH) {
+  for (int p = 0; p < pairs; ++p) {
+    // this pair has landed: behind it are the loads of the next
+    if (2 * p + 3 < my_n) wait_vm<8>();
+    else if (2 * p + 2 < my_n) wait_vm<4>();
+    else wait_vm<0>();
+    const lds_char* slot = ring + (p & 1) * kSlot + lane * 16;
+    u32x4 kb[2][2], vb[2][2];  // [block][load]
 #pragma unroll
-    for (int d = 0; d < DEPTH; ++d) {
-      const int p = p0 + d;
-      if (p >= pairs) break;
-      const int sc0 = __builtin_amdgcn_readlane(scales, 2 * p), sc1 = __builtin_amdgcn_readlane(scales, (2 * p + 1) & 63);
-      // S^T of both blocks
-      f32x4 s[2][NT];
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const float power = kv8_power((b ? sc1 : sc0) & 0xff);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) s[b][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          const u32x4 w = kb[d][b][kk >> 1];
-          f16x8 ka;
-          if constexpr (T == NSD_KV8_E4M3) {
-            ka = kv8_values<T>(u32x2{w[2 * (kk & 1)], w[2 * (kk & 1) + 1]}, power);
-          } else {
-            f16x2 x[4];
-            kv8_whole(w[2 * (kk & 1)], x[0], x[1]);
-            kv8_whole(w[2 * (kk & 1) + 1], x[2], x[3]);
-            ka = f16x8{x[0][0], x[0][1], x[1][0], x[1][1], x[2][0], x[2][1], x[3][0], x[3][1]};
-          }
-#pragma unroll
-          for (int t = 0; t < NT; ++t) s[b][t] = mfma_k32(ka, qf[t][kk], s[b][t]);
-        }
-        if constexpr (T == NSD_KV8_INT8) {
-#pragma unroll
-          for (int t = 0; t < NT; ++t) s[b][t] *= power;
-        }
+      for (int j = 0; j < 2; ++j) {
+        kb[b][j] = *(const lds_u32x4*)(slot + b * kKv8Tile + 1024 * j);
+        vb[b][j] = *(const lds_u32x4*)(slot + (2 + b) * kKv8Tile + 1024 * j);
       }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot is read
+    if (p + 2 < pairs) issue(p + 2);
+    // S^T of both blocks
+    f32x4 s[2][NT];
 #pragma unroll
-      for (int b = 0; b < 2; ++b) load(cache.k, 2 * (p + DEPTH) + b, kb[d][b]);
-
-      const int first[2] = {(blk0 + wave + kWaves * 2 * p) * BS, (blk0 + wave + kWaves * (2 * p + 1)) * BS};
-      const bool masked[2] = {((bad_mask >> (2 * p)) & 1) != 0,
-                              2 * p + 1 >= my_n || ((bad_mask >> ((2 * p + 1) & 63)) & 1) != 0};
-      const bool edge = masked[0] || masked[1] || first[1] + BS > ctx + 1;  // a token may lie past a row's length
-      f16x8 pb[NT];
+    for (int b = 0; b < 2; ++b) {
+      const float power = kv8_power(__builtin_amdgcn_readlane(k_scale, 2 * p + b));
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        float sv[8];
+      for (int t = 0; t < NT; ++t) s[b][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sv[e] = s[e / 4][t][e % 4];
-        if (edge) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (masked[e / 4] || first[e / 4] + 4 * lg + e % 4 >= row_len[t]) sv[e] = -INFINITY;
+      for (int kk = 0; kk < 4; ++kk) {
+        const u32x4 w = kb[b][kk >> 1];
+        f16x8 ka;
+        if constexpr (T == NSD_KV8_E4M3) {
+          ka = kv8_values<T>(u32x2{w[2 * (kk & 1)], w[2 * (kk & 1) + 1]}, power);
+        } else {
+          f16x2 x[4];
+          kv8_whole(w[2 * (kk & 1)], x[0], x[1]);
+          kv8_whole(w[2 * (kk & 1) + 1], x[2], x[3]);
+          ka = f16x8{x[0][0], x[0][1], x[1][0], x[1][1], x[2][0], x[2][1], x[3][0], x[3][1]};
         }
-        float mx = fmaxf(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])), fmaxf(fmaxf(sv[4], sv[5]), fmaxf(sv[6], sv[7])));
-        mx = rows_max(mx) * a.scale_log2;  // -inf stays -inf (scale > 0)
-        // lazy running max: one decision per wave and tile
-        if (__builtin_amdgcn_ballot_w64(mx > m[t] + kLazyMax) != 0) {
-          const float m_new = fmaxf(m[t], mx);
-          const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[t] - m_new);
-          l[t] *= alpha;
 #pragma unroll
-          for (int mt = 0; mt < 8; ++mt) acc[t][mt] *= alpha;
-          m[t] = m_new;
-        }
-        const float m_use = m[t] == -INFINITY ? 0.f : m[t];
-        float psum = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          // weights of at most 2^8 in fp16: 2^-11 of each, as the fp16
-          // attention rounds them; their sum is of the unrounded ones
-          const float pj = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e], a.scale_log2, -m_use));
-          psum += pj;
-          pb[t][e] = (f16)pj;
-        }
-        l[t] += psum;
+        for (int t = 0; t < NT; ++t) s[b][t] = mfma_k32(ka, qf[t][kk], s[b][t]);
       }
+      if constexpr (T == NSD_KV8_INT8) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) s[b][t] *= power;
+      }
+    }
 
-      const float vp0 = kv8_power(sc0 >> 8), vp1 = kv8_power(sc1 >> 8);
-      if constexpr (T == NSD_KV8_E4M3) {
-        // 0 times a NaN is a NaN: where a row masks tokens, NaN codes leave the
-        // operand, and the dims that have them end as NaN for the rows that
-        // attend them
-        if (edge) {
-          uint32_t found = 0;
+    const int first[2] = {(blk0 + wave + kWaves * 2 * p) * BS, (blk0 + wave + kWaves * (2 * p + 1)) * BS};
+    const bool masked[2] = {((bad_mask >> (2 * p)) & 1) != 0,
+                            2 * p + 1 >= my_n || ((bad_mask >> ((2 * p + 1) & 63)) & 1) != 0};
+    const bool edge = masked[0] || masked[1] || first[1] + BS > ctx + 1;  // a token may lie past a row's length
+    f16x8 pb[NT];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) found |= nan_bytes(vb[d][e / 8][e / 4 % 2][e % 4]);
-          if (__builtin_amdgcn_ballot_w64(found != 0) != 0) {
+    for (int t = 0; t < NT; ++t) {
+      float sv[8];
 #pragma unroll
-            for (int mt = 0; mt < 8; ++mt) {
-              uint32_t has[2];
+      for (int e = 0; e < 8; ++e) sv[e] = s[e / 4][t][e % 4];
+      if (edge) {
 #pragma unroll
-              for (int b = 0; b < 2; ++b) {
-                has[b] = nan_bytes(vb[d][b][mt / 4][mt % 4]) >> 7;
-                vb[d][b][mt / 4][mt % 4] &= ~(has[b] * 0xffu);
-              }
-              const f16x8 is_nan = kv8_join(ones_of(has[0]), ones_of(has[1]));
+        for (int e = 0; e < 8; ++e)
+          if (masked[e / 4] || first[e / 4] + 4 * lg + e % 4 >= row_len[t]) sv[e] = -INFINITY;
+      }
+      float mx = fmaxf(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])), fmaxf(fmaxf(sv[4], sv[5]), fmaxf(sv[6], sv[7])));
+      mx = rows_max(mx) * a.scale_log2;  // -inf stays -inf (scale > 0)
+      // lazy running max: one decision per wave and tile
+      if (__builtin_amdgcn_ballot_w64(mx > m[t] + kLazyMax) != 0) {
+        const float m_new = fmaxf(m[t], mx);
+        const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[t] - m_new);
+        l[t] *= alpha;
 #pragma unroll
-              for (int t = 0; t < NT; ++t) {
-                f16x8 attended = {};
+        for (int mt = 0; mt < 8; ++mt) acc[t][mt] *= alpha;
+        m[t] = m_new;
+      }
+      const float m_use = m[t] == -INFINITY ? 0.f : m[t];
+      float psum = 0.f;
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                  if (!masked[e / 4] && first[e / 4] + 4 * lg + e % 4 < row_len[t]) attended[e] = (f16)1.f;
-                const f32x4 hit = mfma_k32(is_nan, attended, f32x4{0.f, 0.f, 0.f, 0.f});
+      for (int e = 0; e < 8; ++e) {
+        // weights of at most 2^8 in fp16: 2^-11 of each, as the fp16
+        // attention rounds them; their sum is of the unrounded ones
+        const float pj = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e], a.scale_log2, -m_use));
+        psum += pj;
+        pb[t][e] = (f16)pj;
+      }
+      l[t] += psum;
+    }
+
+    const float vp0 = kv8_power(__builtin_amdgcn_readlane(v_scale, 2 * p)), vp1 = kv8_power(__builtin_amdgcn_readlane(v_scale, 2 * p + 1));
+    if constexpr (T == NSD_KV8_E4M3) {
+      // 0 times a NaN is a NaN: where a row masks tokens, NaN codes leave the
+      // operand, and the dims that have them end as NaN for the rows that
+      // attend them
+      if (edge) {
+        uint32_t found = 0;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[t][mt][e] = hit[e] > 0.f ? __builtin_nanf("") : acc[t][mt][e];
-              }
+        for (int e = 0; e < 16; ++e) found |= nan_bytes(vb[e / 8][e / 4 % 2][e % 4]);
+        if (__builtin_amdgcn_ballot_w64(found != 0) != 0) {
+#pragma unroll
+          for (int mt = 0; mt < 8; ++mt) {
+            uint32_t has[2];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              has[b] = nan_bytes(vb[b][mt / 4][mt % 4]) >> 7;
+              vb[b][mt / 4][mt % 4] &= ~(has[b] * 0xffu);
+            }
+            const f16x8 is_nan = kv8_join(ones_of(has[0]), ones_of(has[1]));
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              f16x8 attended = {};
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                if (!masked[e / 4] && first[e / 4] + 4 * lg + e % 4 < row_len[t]) attended[e] = (f16)1.f;
+              const f32x4 hit = mfma_k32(is_nan, attended, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[t][mt][e] = hit[e] > 0.f ? __builtin_nanf("") : acc[t][mt][e];
             }
           }
         }
       }
+    }
 #pragma unroll
-      for (int mt = 0; mt < 8; ++mt) {
-        const f16x8 va = kv8_join(kv8_values4<T>(vb[d][0][mt / 4][mt % 4], vp0), kv8_values4<T>(vb[d][1][mt / 4][mt % 4], vp1));
+    for (int mt = 0; mt < 8; ++mt) {
+      const f16x8 va = kv8_join(kv8_values4<T>(vb[0][mt / 4][mt % 4], vp0), kv8_values4<T>(vb[1][mt / 4][mt % 4], vp1));
 #pragma unroll
-        for (int t = 0; t < NT; ++t) acc[t][mt] = mfma_k32(va, pb[t], acc[t][mt]);
-      }
-#pragma unroll
-      for (int b = 0; b < 2; ++b) load(cache.v, 2 * (p + DEPTH) + b, vb[d][b]);
+      for (int t = 0; t < NT; ++t) acc[t][mt] = mfma_k32(va, pb[t], acc[t][mt]);
     }
   }
 
@@ -297,7 +333,7 @@ void kv8_attn_kernel(AttnArgs a, PieceTable pt, Kv8Caches cache) {
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const float lt = rows_sum(l[t]);
-    if (t > 0) __syncthreads();  // the previous tile's merge is read
+    __syncthreads();  // the ring, or the previous tile's merge, is read
     float* mine = mrg + wave * (kMergeWave / 4);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -374,13 +410,17 @@ extern "C" int nsd_kv8_paged_attention(const void* q, void* o, float* lse, const
   const char* who = "kv8_paged_attention";
   int rc = check_kv8_cache(who, cache, layer);
   if (rc) return rc;
+  if (cache->num_blocks > INT32_MAX / cache->num_layers / cache->num_kv_heads)
+    return fail(NSD_ERR_UNSUPPORTED, "%s: %lld blocks (at most 2^31 tiles)", who, (long long)cache->num_blocks);
   AttnCall c;
   rc = prepare_attention(who, q, true, o, lse, cache->k, cache->v, cache->num_blocks, cache->num_layers, layer,
                          num_q_heads, cache->num_kv_heads, D, BS, block_table, bt_rows, bt_stride, plan_host,
                          plan_dev, workspace, workspace_bytes, softmax_scale, status, &c);
   if (rc != NSD_OK || c.grid == 0) return rc;
   const Kv8Caches caches = {static_cast<const char*>(cache->k), static_cast<const char*>(cache->v),
-                            static_cast<const uint8_t*>(cache->k_scales), static_cast<const uint8_t*>(cache->v_scales)};
+                            static_cast<const uint8_t*>(cache->k_scales), static_cast<const uint8_t*>(cache->v_scales),
+                            (uint32_t)(reinterpret_cast<uintptr_t>(cache->k_scales) & 3),
+                            (uint32_t)(reinterpret_cast<uintptr_t>(cache->v_scales) & 3)};
   hipStream_t st = as_stream(stream);
   if (cache->codes == NSD_KV8_E4M3) launch_rows<NSD_KV8_E4M3>(c, caches, st);
   else launch_rows<NSD_KV8_INT8>(c, caches, st);

@@ -43,7 +43,8 @@ class KV8Cache:
     caches and the scales as another.
     """
 
-    __slots__ = ("k", "v", "k_scales", "v_scales", "dtype", "device", "_c", "_ref")
+    __slots__ = ("k", "v", "k_scales", "v_scales", "dtype", "device", "num_blocks", "num_layers", "num_kv_heads", "_c",
+                 "_ref")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
                  dtype: torch.dtype):
@@ -61,7 +62,8 @@ class KV8Cache:
         if k.data_ptr() % 16 or v.data_ptr() % 16:
             raise ValueError("codes must be 16-byte aligned")
         c = _Cache(k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), *k.shape[:3], _CODES[dtype])
-        for name, x in zip(self.__slots__, (k, v, k_scales, v_scales, dtype, k.get_device(), c, ctypes.addressof(c))):
+        for name, x in zip(self.__slots__, (k, v, k_scales, v_scales, dtype, k.get_device(), *k.shape[:3], c,
+                                            ctypes.addressof(c))):
             object.__setattr__(self, name, x)
 
     def __setattr__(self, name, value):
@@ -69,18 +71,6 @@ class KV8Cache:
 
     def __reduce__(self):  # copy and pickle
         return type(self), (self.k, self.v, self.k_scales, self.v_scales, self.dtype)
-
-    @property
-    def num_blocks(self) -> int:
-        return self.k.shape[0]
-
-    @property
-    def num_layers(self) -> int:
-        return self.k.shape[1]
-
-    @property
-    def num_kv_heads(self) -> int:
-        return self.k.shape[2]
 
     @classmethod
     def allocate(cls, num_blocks: int, model_config, dtype: torch.dtype = torch.float8_e4m3fn,
@@ -134,31 +124,55 @@ def _on(cache: KV8Cache, *tensors) -> None:
             raise ValueError(f"all tensors must be on the cache's device, cuda:{cache.device}, got {t.device}")
 
 
-def _index(cache: KV8Cache, t: torch.Tensor, name: str, n: int) -> None:
-    require(t, torch.int32, name)
-    if t.dim() != 1 or t.shape[0] < n:
-        raise ValueError(f"{name} must hold {n} entries, got {tuple(t.shape)}")
+# The checks of a call are a good part of a small one's time, so each begins with
+# one test of everything and names the fault only where that fails.
+_F16, _I32 = torch.float16, torch.int32
+
+
+def _packed(cache: KV8Cache, t: torch.Tensor, name: str, heads: int, rows: int = -1) -> None:
+    """t: contiguous fp16 [rows, heads, 128] (any rows: -1) on the cache's device."""
+    shape = t.shape
+    if t.dtype is _F16 and t.is_contiguous() and t.get_device() == cache.device and len(shape) == 3 and \
+            shape[1] == heads and shape[2] == HEAD_DIM and (rows < 0 or shape[0] == rows):
+        return
     _on(cache, t)
+    require(t, _F16, name)
+    raise ValueError(f"{name} must be [{rows if rows >= 0 else 'rows'}, {heads}, {HEAD_DIM}], got {tuple(shape)}")
 
 
-def _rows(t: torch.Tensor, name: str, shape: tuple) -> None:
-    if t.dtype != torch.float16:
+def _index(cache: KV8Cache, t: torch.Tensor, name: str, n: int) -> None:
+    """t: contiguous int32 of at least n entries on the cache's device."""
+    if t.dtype is _I32 and t.is_contiguous() and t.get_device() == cache.device and t.dim() == 1 and t.numel() >= n:
+        return
+    require(t, _I32, name)
+    _on(cache, t)
+    raise ValueError(f"{name} must hold {n} entries, got {tuple(t.shape)}")
+
+
+def _rows(cache: KV8Cache, t: torch.Tensor, name: str, rows: int, heads: int) -> int:
+    """t: fp16 [rows, heads, 128] of contiguous heads, aligned, on the cache's device; its row stride."""
+    stride, shape = t.stride(), t.shape
+    if t.dtype is _F16 and t.get_device() == cache.device and len(shape) == 3 and shape[0] == rows and \
+            shape[1] == heads and shape[2] == HEAD_DIM and stride[2] == 1 and stride[1] == HEAD_DIM and \
+            stride[0] % 8 == 0 and stride[0] >= heads * HEAD_DIM and t.data_ptr() % 16 == 0:
+        return stride[0]
+    _on(cache, t)
+    if t.dtype != _F16:
         raise TypeError(f"{name} must be torch.float16, got {t.dtype}")
-    if tuple(t.shape) != shape or t.stride(2) != 1 or t.stride(1) != shape[2] or t.stride(0) % 8 or \
-            t.stride(0) < shape[1] * shape[2]:
-        raise ValueError(f"{name} must be {list(shape)} with contiguous heads (rows may be strided by a multiple of 8 "
-                         f"elements), got {tuple(t.shape)}, strides {t.stride()}")
-    if t.data_ptr() % 16:
-        raise ValueError(f"{name} must be 16-byte aligned")
+    raise ValueError(f"{name} must be [{rows}, {heads}, {HEAD_DIM}] with contiguous heads (rows may be strided by a "
+                     f"multiple of 8 elements), 16-byte aligned; got {tuple(shape)}, strides {stride}")
 
 
 def _table(cache: KV8Cache, block_table: torch.Tensor, engine_config) -> tuple:
-    _on(cache, block_table)
-    check_block_table(block_table, engine_config)
-    if int(engine_config.block_size) != BLOCK_TOKENS:
+    shape = block_table.shape
+    if not (block_table.dtype is _I32 and block_table.is_contiguous() and block_table.get_device() == cache.device and
+            len(shape) == 2 and shape[1] == engine_config.max_blocks_per_seq):
+        _on(cache, block_table)
+        check_block_table(block_table, engine_config)
+    if engine_config.block_size != BLOCK_TOKENS:
         raise ValueError(f"engine_config.block_size is {engine_config.block_size}, the cache's blocks hold "
                          f"{BLOCK_TOKENS} tokens")
-    return block_table.data_ptr(), *block_table.shape
+    return block_table.data_ptr(), shape[0], shape[1]
 
 
 def _decode_rows(cache: KV8Cache, infer_state) -> tuple:
@@ -176,24 +190,21 @@ def kv8_store(k: torch.Tensor, v: torch.Tensor, cache: KV8Cache, block_table: to
     ``k``/``v``: [num_tokens, Hkv, d] fp16, prompts first, then one row per decode/verify row.  A prompt's blocks are
     written whole; a decode/verify row joins the tokens that its block holds below it.
     """
-    _on(cache, k, v)
     table = _table(cache, block_table, engine_config)
     hkv = cache.num_kv_heads
     npf, nd = infer_state.num_prefill_seqs, infer_state.num_decoding_seqs
     npt = infer_state.num_prefill_tokens
-    for t, n in ((k, "k"), (v, "v")):
-        require(t, torch.float16, n)
-        if t.dim() != 3 or tuple(t.shape[1:]) != (hkv, HEAD_DIM) or t.shape[0] != npt + nd:
-            raise ValueError(f"{n} must be [{npt + nd}, {hkv}, {HEAD_DIM}], got {tuple(t.shape)}")
+    _packed(cache, k, "k", hkv, npt + nd)
+    _packed(cache, v, "v", hkv, npt + nd)
     status = StatusWord(k.device) if validate else None
     flags = ptr(status.t) if status else None
     if npf > 0:
-        for name in ("prefill_seq_start_locs", "prefill_seq_lens"):
-            _index(cache, getattr(infer_state, name), f"infer_state.{name}", npf)
-        _index(cache, infer_state.seq_ids, "infer_state.seq_ids", npf)
+        ids, starts, lens = infer_state.seq_ids, infer_state.prefill_seq_start_locs, infer_state.prefill_seq_lens
+        _index(cache, ids, "infer_state.seq_ids", npf)
+        _index(cache, starts, "infer_state.prefill_seq_start_locs", npf)
+        _index(cache, lens, "infer_state.prefill_seq_lens", npf)
         _call(cache.device, "nsd_kv8_store_prefill", k.data_ptr(), v.data_ptr(), npt, cache._ref, *table,
-              infer_state.seq_ids.data_ptr(), infer_state.prefill_seq_start_locs.data_ptr(),
-              infer_state.prefill_seq_lens.data_ptr(), npf, infer_state.max_prefill_len, int(cur_layer), flags)
+              ids.data_ptr(), starts.data_ptr(), lens.data_ptr(), npf, infer_state.max_prefill_len, int(cur_layer), flags)
     if nd > 0:
         at = 2 * npt * hkv * HEAD_DIM  # bytes of the prompts' rows
         _call(cache.device, "nsd_kv8_store", k.data_ptr() + at, v.data_ptr() + at, cache._ref, *table,
@@ -213,38 +224,41 @@ def kv8_qk_norm_rope_store(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ca
     multiple of 8 elements apart); the normalised, rotated q goes to ``q_out``, or, with contiguous q and no ``q_out``,
     into q.  k and v are only read.  ``cos_cache``/``sin_cache``: the full [max_positions, d/2] fp16 tables.
     """
-    _on(cache, q, k, v, cos_cache, sin_cache, q_norm, k_norm, q_out)
     table = _table(cache, block_table, engine_config)
-    rows, hq, hkv = infer_state.num_decoding_seqs, int(model_config.num_q_heads), cache.num_kv_heads
-    for t, n, heads in ((q, "q", hq), (k, "k", hkv), (v, "v", hkv)):
-        _rows(t, n, (rows, heads, HEAD_DIM))
+    rows, hq, hkv = infer_state.num_decoding_seqs, model_config.num_q_heads, cache.num_kv_heads
+    q_stride = _rows(cache, q, "q", rows, hq)
+    k_stride = _rows(cache, k, "k", rows, hkv)
+    v_stride = _rows(cache, v, "v", rows, hkv)
     if q_out is None:
         if not q.is_contiguous():
             raise ValueError("strided q needs q_out (a contiguous [rows, Hq, d] buffer)")
         q_out = q
     else:
-        require(q_out, torch.float16, "q_out")
-        if q_out.shape != q.shape:
-            raise ValueError("q_out must have q's shape")
+        _packed(cache, q_out, "q_out", hq, rows)
     if (q_norm is None) != (k_norm is None):
         raise ValueError("pass both q_norm and k_norm, or neither")
-    for t, n in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        if t is not None:
-            require(t, torch.float16, n)
-            if tuple(t.shape) != (HEAD_DIM,):
-                raise ValueError(f"{n} must be [{HEAD_DIM}]")
+    if q_norm is not None:
+        for t, n in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+            if t.dtype is not _F16 or t.dim() != 1 or t.numel() != HEAD_DIM or not t.is_contiguous() or \
+                    t.get_device() != cache.device:
+                _on(cache, t)
+                require(t, _F16, n)
+                raise ValueError(f"{n} must be [{HEAD_DIM}], got {tuple(t.shape)}")
+    angles = cos_cache.shape
+    if len(angles) != 2 or angles[1] != HEAD_DIM // 2 or sin_cache.shape != angles:
+        raise ValueError("cos/sin caches must be [max_positions, head_dim/2]")
     for t, n in ((cos_cache, "cos_cache"), (sin_cache, "sin_cache")):
-        require(t, torch.float16, n)
-        if t.dim() != 2 or t.shape[1] != HEAD_DIM // 2 or t.shape != cos_cache.shape:
-            raise ValueError("cos/sin caches must be [max_positions, head_dim/2]")
+        if t.dtype is not _F16 or not t.is_contiguous() or t.get_device() != cache.device:
+            _on(cache, t)
+            require(t, _F16, n)
     if rows == 0:
         return
     if getattr(infer_state, "ignore_kvcache", False):
         raise ValueError("infer_state.ignore_kvcache is set but the forward has decode rows")
     status = StatusWord(q.device) if validate else None
-    _call(cache.device, "nsd_kv8_qk_norm_rope_store", q.data_ptr(), q.stride(0), q_out.data_ptr(), k.data_ptr(),
-          k.stride(0), v.data_ptr(), v.stride(0), ptr(q_norm), ptr(k_norm), float(model_config.rms_norm_eps),
-          cos_cache.data_ptr(), sin_cache.data_ptr(), cos_cache.shape[0], cache._ref, *table,
+    _call(cache.device, "nsd_kv8_qk_norm_rope_store", q.data_ptr(), q_stride, q_out.data_ptr(), k.data_ptr(), k_stride,
+          v.data_ptr(), v_stride, ptr(q_norm), ptr(k_norm), model_config.rms_norm_eps, cos_cache.data_ptr(),
+          sin_cache.data_ptr(), angles[0], cache._ref, *table,
           *_decode_rows(cache, infer_state), int(cur_layer), hq, ptr(status.t) if status else None)
     if status is not None:
         status.check("kv8_qk_norm_rope_store")
@@ -259,24 +273,24 @@ def kv8_load(k: torch.Tensor, v: torch.Tensor, cache: KV8Cache, block_table: tor
     to row ``start_locs[s] + i`` of ``k`` and ``v`` [rows, Hkv, d]; other rows are left as they are.  The index tensors
     are int32, one entry a sequence.
     """
-    _on(cache, k, v, block_table)
-    require(block_table, torch.int32, "block_table")
-    if block_table.dim() != 2:
+    if block_table.dtype is not _I32 or not block_table.is_contiguous() or block_table.dim() != 2 or \
+            block_table.get_device() != cache.device:
+        _on(cache, block_table)
+        require(block_table, _I32, "block_table")
         raise ValueError("block_table must be [rows, max_blocks_per_seq]")
-    for t, n in ((k, "k"), (v, "v")):
-        require(t, torch.float16, n)
-        if t.dim() != 3 or tuple(t.shape[1:]) != (cache.num_kv_heads, HEAD_DIM) or t.shape != k.shape:
-            raise ValueError(f"k and v must be [rows, {cache.num_kv_heads}, {HEAD_DIM}], got {tuple(t.shape)}")
-    n = seq_ids.shape[0] if seq_ids.dim() == 1 else -1
+    rows = k.shape[0] if k.dim() else 0
+    _packed(cache, k, "k", cache.num_kv_heads)
+    _packed(cache, v, "v", cache.num_kv_heads, rows)
+    n = seq_ids.numel()
     for t, name in ((seq_ids, "seq_ids"), (start_locs, "start_locs"), (seq_lens, "seq_lens"), (first, "first")):
         if t is not None:
-            _index(cache, t, name, max(n, 0))
-            if t.shape[0] != n:
+            _index(cache, t, name, n)
+            if t.numel() != n:
                 raise ValueError(f"{name} must be [{n}], one entry a sequence")
-    if n == 0 or k.shape[0] == 0:
+    if n == 0 or rows == 0:
         return
     status = StatusWord(k.device) if validate else None
-    _call(cache.device, "nsd_kv8_load", k.data_ptr(), v.data_ptr(), k.shape[0], cache._ref, block_table.data_ptr(),
+    _call(cache.device, "nsd_kv8_load", k.data_ptr(), v.data_ptr(), rows, cache._ref, block_table.data_ptr(),
           *block_table.shape, seq_ids.data_ptr(), ptr(first), start_locs.data_ptr(), seq_lens.data_ptr(), n,
           int(max_len), int(cur_layer), ptr(status.t) if status else None)
     if status is not None:
@@ -292,18 +306,19 @@ def kv8_paged_attention(q: torch.Tensor, cache: KV8Cache, block_table: torch.Ten
     natural-log sum of exp(score).  Scratch is the call's own (from the caching allocator), so calls on several
     streams and in several captured graphs share nothing.
     """
-    _on(cache, q, o, lse)
     table = _table(cache, block_table, engine_config)
-    rows, hq = infer_state.num_decoding_seqs, int(model_config.num_q_heads)
-    require(q, torch.float16, "q")
-    require(o, torch.float16, "o")
-    if tuple(q.shape) != (rows, hq, HEAD_DIM) or o.numel() != q.numel():
-        raise ValueError(f"q must be [{rows}, {hq}, {HEAD_DIM}] and o hold as many elements")
-    if lse is not None:
+    rows, hq = infer_state.num_decoding_seqs, model_config.num_q_heads
+    _packed(cache, q, "q", hq, rows)
+    if o.dtype is not _F16 or not o.is_contiguous() or o.get_device() != cache.device or o.numel() != rows * hq * HEAD_DIM:
+        _on(cache, o)
+        require(o, _F16, "o")
+        raise ValueError(f"o must hold as many elements as q, {rows} x {hq} x {HEAD_DIM}")
+    if lse is not None and (lse.dtype is not torch.float32 or not lse.is_contiguous() or
+                            lse.get_device() != cache.device or lse.numel() != rows * hq):
+        _on(cache, lse)
         require(lse, torch.float32, "lse")
-        if lse.numel() != rows * hq:
-            raise ValueError("lse must hold num_decoding_seqs * num_q_heads floats")
-    if int(model_config.num_kv_heads) != cache.num_kv_heads:
+        raise ValueError("lse must hold num_decoding_seqs * num_q_heads floats")
+    if model_config.num_kv_heads != cache.num_kv_heads:
         raise ValueError(f"model_config has {model_config.num_kv_heads} kv heads, the cache {cache.num_kv_heads}")
     if rows == 0:
         return
@@ -313,11 +328,10 @@ def kv8_paged_attention(q: torch.Tensor, cache: KV8Cache, block_table: torch.Ten
     size, ws = plan.workspace_bytes, None
     if size:
         # the claim counter of plans with more pieces than workgroup slots starts at zero
-        claims = int(plan.host[_lib.PLAN_CLAIMED]) > 0
-        ws = (torch.zeros if claims else torch.empty)(size, dtype=torch.uint8, device=q.device)
+        ws = (q.new_zeros if plan.claims else q.new_empty)(size, dtype=torch.uint8)
     status = StatusWord(q.device) if validate else None
     _call(cache.device, "nsd_kv8_paged_attention", q.data_ptr(), o.data_ptr(), ptr(lse), cache._ref, int(cur_layer),
-          hq, *table, plan.host_ptr(), plan.dev.data_ptr(), ptr(ws), size, float(infer_state.softmax_scale),
+          hq, *table, plan.host_address, plan.dev.data_ptr(), ptr(ws), size, infer_state.softmax_scale,
           ptr(status.t) if status else None)
     if status is not None:
         status.check("kv8_paged_attention")

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
+from functools import cached_property
 
 import numpy as np
 
@@ -164,6 +165,15 @@ class AttnPlan:
         return (self.num_q_heads == num_q_heads and self.num_kv_heads == num_kv_heads
                 and int(self.host[_lib.PLAN_BT_STRIDE]) == block_table.shape[1]
                 and int(self.host[_lib.PLAN_BT_ROWS]) <= block_table.shape[0])
+
+    @cached_property
+    def host_address(self) -> int:
+        return self.host.ctypes.data
+
+    @cached_property
+    def claims(self) -> bool:
+        """Whether some pieces are claimed at run time (their counter, at the workspace's start, begins at zero)."""
+        return int(self.host[_lib.PLAN_CLAIMED]) > 0
 
     def host_ptr(self):
         return self.host.ctypes.data_as(ctypes.POINTER(ctypes.c_int32))
