@@ -113,11 +113,21 @@ int nsd_kv8_load(void* k, void* v, int64_t n_tokens, const nsd_kv8_cache* cache,
                  int32_t* status, void* stream);
 
 /*
- * nsd_paged_attention over an 8-bit cache: the same plan, workspace and
- * contract, and the attention over the values that the cache holds, in the same
- * arithmetic (fp16 products, fp32 sums and softmax).  A NaN in the cache reaches
- * the rows that attend its token and no others.
+ * nsd_paged_attention over an 8-bit cache: the same contract, and the attention
+ * over the values that the cache holds, in fp16 products and fp32 sums and
+ * softmax.  A NaN in the cache reaches the rows that attend its token and no
+ * others.
+ *
+ * nsd_kv8_plan_build: its plan (nsd_attn_plan_build's words and checks) for a
+ * device of `compute_units`; nsd_attn_plan_bound gives the words for n_workers =
+ * 2 * compute_units.  Plans of nsd_attn_plan_build serve too, not as fast.  Parts
+ * of a segment are merged in fp32: the workspace is nsd_kv8_attn_workspace bytes,
+ * not those of nsd_attn_plan_build.
  */
+int nsd_kv8_plan_build(const int32_t* seq_ids, const int32_t* seq_lens, int64_t n_rows, int num_q_heads,
+                       int num_kv_heads, int64_t bt_rows, int64_t bt_stride, int compute_units, int max_group_rows,
+                       int32_t* plan, int64_t plan_capacity, int64_t* plan_words);
+int nsd_kv8_attn_workspace(const int32_t* plan_host, int64_t* bytes);
 int nsd_kv8_paged_attention(const void* q, void* o, float* lse, const nsd_kv8_cache* cache, int layer,
                             int num_q_heads, const int32_t* block_table, int64_t bt_rows, int64_t bt_stride,
                             const int32_t* plan_host, const int32_t* plan_dev, void* workspace,

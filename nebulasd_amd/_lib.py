@@ -157,6 +157,10 @@ SIGNATURES = {
     "nsd_kv8_load": (
         c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
                 c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p]),
+    "nsd_kv8_plan_build": (
+        c_int, [_I32P, _I32P, c_int64, c_int, c_int, c_int64, c_int64, c_int, c_int, _I32P, c_int64,
+                POINTER(c_int64)]),
+    "nsd_kv8_attn_workspace": (c_int, [c_void_p, POINTER(c_int64)]),
     "nsd_kv8_paged_attention": (
         c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
                 c_void_p, c_int64, c_float, c_void_p, c_void_p]),

@@ -624,7 +624,7 @@ void paged_attn_kernel(AttnArgs a, PieceTable pt, Extra fx) {
       const float inv = L > 0.f ? 1.f / L : 0.f;
       const int qi = n / a.gqa, gh = n - qi * a.gqa;
       const int64_t orow = (int64_t)(row_start + qi) * a.hq + head * a.gqa + gh;
-      f16* dst = slot < 0 ? a.o + orow * D : a.part_o + ((int64_t)slot * a.rows_max + n) * D;
+      f16* dst = slot < 0 ? a.o + orow * D : static_cast<f16*>(a.part_o) + ((int64_t)slot * a.rows_max + n) * D;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int mt = 2 * wave + h;
@@ -714,8 +714,8 @@ int paged_attention_impl(const void* q, void* o, float* lse, const void* k_cache
   AttnCall c;
   const int rc = prepare_attention("paged_attention", q, fused == nullptr, o, lse, k_cache, v_cache, num_blocks,
                                    num_layers, layer, num_q_heads, num_kv_heads, head_dim, block_size, block_table,
-                                   bt_rows, bt_stride, plan_host, plan_dev, part, part_capacity, softmax_scale,
-                                   status, &c);
+                                   bt_rows, bt_stride, plan_host, plan_dev, part, part_capacity, sizeof(f16),
+                                   softmax_scale, status, &c);
   if (rc != NSD_OK || c.grid == 0) return rc;
   hipStream_t st = as_stream(stream);
   const int launched = fused != nullptr
@@ -726,7 +726,7 @@ int paged_attention_impl(const void* q, void* o, float* lse, const void* k_cache
                  : c.row_tiles == 2 ? launch_nt<2>(c.args, c.pieces, c.grid, st)
                            : launch_nt<3>(c.args, c.pieces, c.grid, st);
   if (launched != NSD_OK) return launched;
-  return launch_merge("paged_attention: partial merge", c, plan_host, st);
+  return launch_merge<f16>("paged_attention: partial merge", c, plan_host, st);
 }
 
 constexpr int64_t kScratchBytes = int64_t(NSD_NOALLOC_SCRATCH_BYTES);

@@ -45,7 +45,7 @@ enum PlanHeader {
   kPlanClaimed,        // records kPlanStatic .. +kPlanClaimed-1, claimed at run time by the
                        // later workgroups in order (kPlanWorkers - kPlanStatic of them)
 };
-static_assert(kPlanMaxBlocks < NSD_PLAN_HEADER_WORDS, "plan header size");
+static_assert(kPlanClaimed < NSD_PLAN_HEADER_WORDS, "plan header size");
 
 // A piece: blocks [blk_begin, blk_end) of one (group, kv head) segment, with
 // the group's description inlined so a workgroup needs one record.  A record
@@ -79,6 +79,11 @@ constexpr int kMaxPieceBlocks = 256;    // blocks of one piece (four waves, one 
 // flight from the piece's start, so a shorter cut saves no latency and only
 // adds the merge of the segment's pieces.
 constexpr int kMinPieceBlocks = 8;
+// ... and over an 8-bit cache, whose block is half the bytes: the merge launch
+// (3 us) costs more than a wave's six blocks.  16 / 24 / 32, us a call: 16 rows of
+// 500 tokens 9.6 / 8.0 / 8.0, 1 of 500 7.9 / 6.7 / 6.8, but 1 of 1500 9.0 / 9.4 /
+// 10.6 and 1 x 5 of 4000 12.6 / 13.4 / 13.7.
+constexpr int kKv8MinPieceBlocks = 24;
 constexpr int kWavesPerPiece = 4;       // waves of an attention workgroup (wave w: blocks w, w + 4, ...)
 constexpr int kXcds = 8;                // workgroup i of a launch runs on XCD i % 8
 
@@ -91,10 +96,11 @@ bool plan_keeps_sequences_whole(const int32_t* plan_host);
 // Attention workspace: the claim counter of plans with claimed records
 // (zero between calls; its 256 bytes are reserved in every layout, so no
 // other plan's partials land there), then the partials of the split
-// segments, normalised O (fp16) and log2-sum-exp (fp32) per slot and row.
+// segments, normalised O (fp16; elem = 4: fp32) and log2-sum-exp (fp32) per
+// slot and row.
 constexpr int64_t kClaimBytes = 256;
-inline int64_t plan_workspace_bytes(int64_t n_slots, int64_t rows_max) {
-  return kClaimBytes + (n_slots * rows_max * (int64_t)(kHeadDim * 2 + 4) + 255) / 256 * 256;
+inline int64_t plan_workspace_bytes(int64_t n_slots, int64_t rows_max, int elem = 2) {
+  return kClaimBytes + (n_slots * rows_max * (int64_t)(kHeadDim * elem + 4) + 255) / 256 * 256;
 }
 
 }  // namespace nsd

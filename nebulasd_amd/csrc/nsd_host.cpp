@@ -55,21 +55,17 @@ extern "C" int64_t nsd_attn_plan_bound(int64_t n_rows, int num_kv_heads, int n_w
   return NSD_PLAN_HEADER_WORDS + 4 * n_rows + kPieceWords * pieces + kPieceWords * segs;
 }
 
-extern "C" int nsd_attn_plan_build(const int32_t* seq_ids, const int32_t* seq_lens, int64_t n_rows,
-                                   int num_q_heads, int num_kv_heads, int head_dim, int block_size,
-                                   int64_t bt_rows, int64_t bt_stride, int n_workers,
-                                   int max_group_rows, int32_t* plan, int64_t plan_capacity,
-                                   int64_t* plan_words, int64_t* workspace_bytes) {
-  return nsd_attn_plan_build_claimed(seq_ids, seq_lens, n_rows, num_q_heads, num_kv_heads, head_dim, block_size,
-                                     bt_rows, bt_stride, n_workers, 0, max_group_rows, plan, plan_capacity,
-                                     plan_words, workspace_bytes);
-}
+// How a plan is cut: into n_workers pieces, of which those beyond static_slots
+// are claimed at run time; no piece shorter than min_blocks.  few > 0: into that
+// many, where the segments, each in the fewest pieces that hold it, are no more.
+struct PlanCut {
+  int n_workers, static_slots, min_blocks, few;
+};
 
-extern "C" int nsd_attn_plan_build_claimed(const int32_t* seq_ids, const int32_t* seq_lens, int64_t n_rows,
-                                           int num_q_heads, int num_kv_heads, int head_dim, int block_size,
-                                           int64_t bt_rows, int64_t bt_stride, int n_workers, int static_slots,
-                                           int max_group_rows, int32_t* plan, int64_t plan_capacity,
-                                           int64_t* plan_words, int64_t* workspace_bytes) {
+static int build_plan(const int32_t* seq_ids, const int32_t* seq_lens, int64_t n_rows, int num_q_heads,
+                      int num_kv_heads, int head_dim, int block_size, int64_t bt_rows, int64_t bt_stride, PlanCut cut,
+                      int max_group_rows, int32_t* plan, int64_t plan_capacity, int64_t* plan_words,
+                      int64_t* workspace_bytes) {
   if (n_rows < 0) return fail(NSD_ERR_INVALID, "plan: n_rows=%lld < 0", (long long)n_rows);
   if (n_rows > 0 && (seq_ids == nullptr || seq_lens == nullptr))
     return fail(NSD_ERR_INVALID, "plan: null seq_ids/seq_lens");
@@ -81,8 +77,8 @@ extern "C" int nsd_attn_plan_build_claimed(const int32_t* seq_ids, const int32_t
   if (head_dim != kHeadDim) return fail(NSD_ERR_UNSUPPORTED, "plan: head_dim=%d (only 128)", head_dim);
   if (block_size != kBlockTokens)
     return fail(NSD_ERR_UNSUPPORTED, "plan: block_size=%d (only 16)", block_size);
-  if (n_workers <= 0) return fail(NSD_ERR_INVALID, "plan: n_workers=%d", n_workers);
-  if (static_slots < 0) return fail(NSD_ERR_INVALID, "plan: static_slots=%d", static_slots);
+  if (cut.n_workers <= 0) return fail(NSD_ERR_INVALID, "plan: n_workers=%d", cut.n_workers);
+  if (cut.static_slots < 0) return fail(NSD_ERR_INVALID, "plan: static_slots=%d", cut.static_slots);
   if (bt_rows <= 0 || bt_stride <= 0)
     return fail(NSD_ERR_INVALID, "plan: block table shape [%lld, %lld]", (long long)bt_rows,
                 (long long)bt_stride);
@@ -123,12 +119,13 @@ extern "C" int nsd_attn_plan_build_claimed(const int32_t* seq_ids, const int32_t
     seg_start[s + 1] = seg_start[s] + (tokens + kBlockTokens - 1) / kBlockTokens;
   }
   const int64_t total = seg_start[n_segs];
+  const int static_slots = cut.static_slots;
 
   // 3. pieces per segment.  Every segment starts with the fewest pieces of
   //    at most kMaxPieceBlocks blocks; then, while the plan has fewer than
   //    n_workers pieces, one more piece goes to the segment whose pieces are
   //    the longest (ties: the lower segment), as long as its pieces stay at
-  //    least kMinPieceBlocks long and it stays within kMaxSlotsPerSegment.
+  //    least cut.min_blocks long and it stays within kMaxSlotsPerSegment.
   //    No cut into that many pieces has a shorter longest piece, and with
   //    n_workers = the device's workgroup slots every piece starts at once.
   std::vector<int64_t> seg_pieces(n_segs);
@@ -141,6 +138,7 @@ extern "C" int nsd_attn_plan_build_claimed(const int32_t* seq_ids, const int32_t
                   (long long)nb, kMaxSlotsPerSegment, kMaxPieceBlocks);
     n_pieces += seg_pieces[s];
   }
+  const int n_workers = n_pieces <= cut.few ? cut.few : cut.n_workers;
   {
     // max-heap on blocks per piece, nb_s / n_s, compared without division
     auto shorter = [&](int64_t x, int64_t y) {
@@ -156,7 +154,7 @@ extern "C" int nsd_attn_plan_build_claimed(const int32_t* seq_ids, const int32_t
       const int64_t s = heap.back();
       heap.pop_back();
       const int64_t nb = seg_start[s + 1] - seg_start[s], n = seg_pieces[s] + 1;
-      if (n > kMaxSlotsPerSegment || nb < n * kMinPieceBlocks) continue;  // cut as far as it goes
+      if (n > kMaxSlotsPerSegment || nb < n * cut.min_blocks) continue;  // cut as far as it goes
       seg_pieces[s] = n;
       ++n_pieces;
       heap.push_back(s);
@@ -336,4 +334,39 @@ extern "C" int nsd_attn_plan_build_claimed(const int32_t* seq_ids, const int32_t
   *plan_words = words;
   *workspace_bytes = n_combines > 0 || n_claimed > 0 ? plan_workspace_bytes(n_slots, rows_max) : 0;
   return NSD_OK;
+}
+
+extern "C" int nsd_attn_plan_build(const int32_t* seq_ids, const int32_t* seq_lens, int64_t n_rows,
+                                   int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+                                   int64_t bt_rows, int64_t bt_stride, int n_workers,
+                                   int max_group_rows, int32_t* plan, int64_t plan_capacity,
+                                   int64_t* plan_words, int64_t* workspace_bytes) {
+  return nsd_attn_plan_build_claimed(seq_ids, seq_lens, n_rows, num_q_heads, num_kv_heads, head_dim, block_size,
+                                     bt_rows, bt_stride, n_workers, 0, max_group_rows, plan, plan_capacity,
+                                     plan_words, workspace_bytes);
+}
+
+extern "C" int nsd_attn_plan_build_claimed(const int32_t* seq_ids, const int32_t* seq_lens, int64_t n_rows,
+                                           int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+                                           int64_t bt_rows, int64_t bt_stride, int n_workers, int static_slots,
+                                           int max_group_rows, int32_t* plan, int64_t plan_capacity,
+                                           int64_t* plan_words, int64_t* workspace_bytes) {
+  const PlanCut cut = {n_workers, static_slots, kMinPieceBlocks, 0};
+  return build_plan(seq_ids, seq_lens, n_rows, num_q_heads, num_kv_heads, head_dim, block_size, bt_rows, bt_stride, cut,
+                    max_group_rows, plan, plan_capacity, plan_words, workspace_bytes);
+}
+
+extern "C" int nsd_kv8_plan_build(const int32_t* seq_ids, const int32_t* seq_lens, int64_t n_rows, int num_q_heads,
+                                  int num_kv_heads, int64_t bt_rows, int64_t bt_stride, int compute_units,
+                                  int max_group_rows, int32_t* plan, int64_t plan_capacity, int64_t* plan_words) {
+  if (compute_units < 1 || compute_units > (1 << 16))
+    return fail(NSD_ERR_INVALID, "kv8 plan: %d compute units", compute_units);
+  int64_t fp16_workspace = 0;
+  // One piece a compute unit where the segments allow it, two where there are
+  // more segments, or blocks for more.  One / two: 16 x 5 rows of 256 to 4096
+  // tokens 16.9 / 18.9 us, 8 x 9 of 1000 to 3000 18.6 / 22.6, 32 x 1 of 300 to 900
+  // 10.7 / 13.0 (whole segments), 1 x 1 of 32768 18.4 / 18.1.
+  const PlanCut cut = {2 * compute_units, 2 * compute_units, kKv8MinPieceBlocks, compute_units};
+  return build_plan(seq_ids, seq_lens, n_rows, num_q_heads, num_kv_heads, kHeadDim, kBlockTokens, bt_rows, bt_stride,
+                    cut, max_group_rows, plan, plan_capacity, plan_words, &fp16_workspace);
 }

@@ -47,9 +47,12 @@ struct Kv8Caches {
 
 constexpr int kSlot = 4 * kKv8Tile;  // a pair's K tiles, then its V tiles
 constexpr int kSlots = 2;
-constexpr int kRing = kWaves * kSlots * kSlot;  // 64 KB: two workgroups a CU
+constexpr int kRing = kSlots * kSlot;           // a wave's
 constexpr int kScales = 2 * kWave * 4;          // a wave's words with the K and V scales of its blocks
-static_assert(kWaves * kMergeWave <= kRing, "the merge reuses the ring");
+// The waves' rings, the query rows and scales.
+constexpr int lds_bytes(int nt) { return kWaves * (kRing + kScales) + nt * 16 * D * 2; }
+static_assert(kMergeWave <= kRing, "the merge reuses the rings");
+static_assert(2 * lds_bytes(3) <= 160 * 1024, "two workgroups a CU");
 
 // 1 KB from base + off (a lane's 16 bytes), or 64 dwords, into LDS; the compiler
 // sees neither the load nor its wait.
@@ -79,12 +82,12 @@ __device__ inline f16x4 ones_of(uint32_t w) {
 template <int T, int NT>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
 void kv8_attn_kernel(AttnArgs a, PieceTable pt, Kv8Caches cache) {
-  __shared__ __align__(16) char smem[kRing + NT * 16 * D * 2 + kWaves * kScales];
+  __shared__ __align__(16) char smem[lds_bytes(NT)];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   lds_char* lds = (lds_char*)smem;
-  lds_char* ring = lds + wave * (kSlots * kSlot);
-  const lds_char* q_lds = lds + kRing;
+  lds_char* ring = lds + wave * kRing;
+  const lds_char* q_lds = lds + kWaves * kRing;
   const lds_char* scale_lds = q_lds + NT * 16 * D * 2 + wave * kScales;
 
   int rec_idx = blockIdx.x;
@@ -325,9 +328,10 @@ void kv8_attn_kernel(AttnArgs a, PieceTable pt, Kv8Caches cache) {
     }
   }
 
-  // Merge the four waves' states, one row tile at a time, in wave order.  Lane
-  // (lr, lg) of tile m holds dims 8 (4lg + r) + m of row lr in element r: wave w
-  // takes the elements r = w, the dims 32lg + 8w .. +7.
+  // Merge the waves' states, one row tile at a time, in wave order.  Lane (lr, lg)
+  // of tile m holds dims 8 (4lg + r) + m of row lr in element r: wave w takes the
+  // elements r = w, the dims 32lg + 8w .. +7.  (All tiles in one exchange: no
+  // faster.)
   const int slot = rv[kPieceSlot];
   float* mrg = (float*)smem;
 #pragma unroll
@@ -365,19 +369,26 @@ void kv8_attn_kernel(AttnArgs a, PieceTable pt, Kv8Caches cache) {
       const float inv = L > 0.f ? 1.f / L : L != L ? L : 0.f;
       const int qi = n / a.gqa, gh = n - qi * a.gqa;
       const int64_t orow = (int64_t)(row_start + qi) * a.hq + head * a.gqa + gh;
-      f16* dst = slot < 0 ? a.o + orow * D : a.part_o + ((int64_t)slot * a.rows_max + n) * D;
-      f16x8 out;
+      f32x4 out[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        f32x4 o4 = {0.f, 0.f, 0.f, 0.f};
+        out[h] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int v = 0; v < kWaves; ++v)
-          o4 += *reinterpret_cast<const f32x4*>(mrg + v * (kMergeWave / 4) + ((2 * wave + h) * kWave + lane) * 4) * sc[v];
-        o4 *= inv;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) out[4 * h + e] = (f16)o4[e];
+          out[h] += *reinterpret_cast<const f32x4*>(mrg + v * (kMergeWave / 4) + ((2 * wave + h) * kWave + lane) * 4) * sc[v];
+        out[h] *= inv;
       }
-      *reinterpret_cast<f16x8*>(dst + 32 * lg + 8 * wave) = out;
+      const int at = 32 * lg + 8 * wave;
+      if (slot < 0) {
+        f16x8 half;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) half[e] = (f16)out[e / 4][e % 4];
+        *reinterpret_cast<f16x8*>(a.o + orow * D + at) = half;
+      } else {  // fp32: a row is rounded once, after the merge
+        float* dst = static_cast<float*>(a.part_o) + ((int64_t)slot * a.rows_max + n) * D + at;
+        *reinterpret_cast<f32x4*>(dst) = out[0];
+        *reinterpret_cast<f32x4*>(dst + 4) = out[1];
+      }
       if (wave == 0 && lg == 0) {
         const float lse2 = L > 0.f ? M + __log2f(L) : L != L ? L : -INFINITY;
         if (slot >= 0) a.part_lse[(int64_t)slot * a.rows_max + n] = lse2;
@@ -402,6 +413,15 @@ void launch_rows(const AttnCall& c, const Kv8Caches& caches, hipStream_t st) {
 
 using namespace nsd;
 
+extern "C" int nsd_kv8_attn_workspace(const int32_t* plan_host, int64_t* bytes) {
+  if (plan_host == nullptr || bytes == nullptr) return fail(NSD_ERR_INVALID, "kv8_attn_workspace: null pointer");
+  if (plan_host[kPlanMagic] != kPlanMagicValue || plan_host[kPlanVersion] != kPlanVersionValue)
+    return fail(NSD_ERR_INVALID, "kv8_attn_workspace: not a plan (bad magic/version)");
+  const bool none = plan_host[kPlanCombines] == 0 && plan_host[kPlanClaimed] == 0;
+  *bytes = none ? 0 : plan_partial_bytes(plan_host, sizeof(float));
+  return NSD_OK;
+}
+
 extern "C" int nsd_kv8_paged_attention(const void* q, void* o, float* lse, const nsd_kv8_cache* cache, int layer,
                                        int num_q_heads, const int32_t* block_table, int64_t bt_rows,
                                        int64_t bt_stride, const int32_t* plan_host, const int32_t* plan_dev,
@@ -415,7 +435,7 @@ extern "C" int nsd_kv8_paged_attention(const void* q, void* o, float* lse, const
   AttnCall c;
   rc = prepare_attention(who, q, true, o, lse, cache->k, cache->v, cache->num_blocks, cache->num_layers, layer,
                          num_q_heads, cache->num_kv_heads, D, BS, block_table, bt_rows, bt_stride, plan_host,
-                         plan_dev, workspace, workspace_bytes, softmax_scale, status, &c);
+                         plan_dev, workspace, workspace_bytes, sizeof(float), softmax_scale, status, &c);
   if (rc != NSD_OK || c.grid == 0) return rc;
   const Kv8Caches caches = {static_cast<const char*>(cache->k), static_cast<const char*>(cache->v),
                             static_cast<const uint8_t*>(cache->k_scales), static_cast<const uint8_t*>(cache->v_scales),
@@ -426,5 +446,5 @@ extern "C" int nsd_kv8_paged_attention(const void* q, void* o, float* lse, const
   else launch_rows<NSD_KV8_INT8>(c, caches, st);
   rc = launch_status(who);
   if (rc != NSD_OK) return rc;
-  return launch_merge("kv8_paged_attention: partial merge", c, plan_host, st);
+  return launch_merge<float>("kv8_paged_attention: partial merge", c, plan_host, st);
 }

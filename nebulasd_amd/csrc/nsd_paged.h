@@ -42,7 +42,7 @@ struct AttnArgs {
   const int32_t* bt;
   int64_t bt_stride;
   const int32_t* pieces;   // plan: piece records, one per workgroup
-  f16* part_o;             // [slots, rows_max, D]  normalised O
+  void* part_o;            // [slots, rows_max, D]  normalised O, f16 or float
   float* part_lse;         // [slots, rows_max]  (log2 domain)
   const int32_t* combines; // plan: combine records of the segments cut into pieces
   int32_t* claim;          // claim counter of the claimed records (zero between calls)
@@ -100,13 +100,31 @@ __device__ inline float rows_sum(float x) {
 // verify) 4.6 either way.
 constexpr int kMergeSlots = 8;
 
+// Eight dims of a partial, f16 or float; zeros if it is a repeated slot's, which
+// may hold an infinity (0 * inf).
+struct Part {
+  f32x4 lo, hi;
+};
+__device__ inline Part part_of(const f16* p, bool use) {
+  f16x8 h = *reinterpret_cast<const f16x8*>(p);
+  if (!use) h = f16x8{};
+  return {f32x4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]}, f32x4{(float)h[4], (float)h[5], (float)h[6], (float)h[7]}};
+}
+__device__ inline Part part_of(const float* p, bool use) {
+  const Part v = {*reinterpret_cast<const f32x4*>(p), *reinterpret_cast<const f32x4*>(p + 4)};
+  return use ? v : Part{f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+}
+// A merged row's 1 / W; 0 where no slot attends a token (ids outside the pool).
+__device__ inline float merge_inv(float W) { return W == 0.f ? 0.f : 1.f / W; }
+
 // Row n (of the segment's q_len x GQA rows), dims 8 d8 .. 8 d8 + 7, of a
 // split segment of kv head `head` whose partials sit in slots [first, first
 // + n_slots), at most kMergeSlots: their loads all in flight, the slots
 // folded in slot order (log-sum-exp) and the row stored.
+template <class P>
 __device__ inline void merge_row(const AttnArgs& a, int head, int first, int n_slots, int row_start, int n,
                                  int d8) {
-  const f16* po = a.part_o + ((int64_t)first * a.rows_max + n) * D + 8 * d8;
+  const P* po = static_cast<const P*>(a.part_o) + ((int64_t)first * a.rows_max + n) * D + 8 * d8;
   const float* pl = a.part_lse + (int64_t)first * a.rows_max + n;
   const int64_t sstride = (int64_t)a.rows_max * D;  // elements between slots
   f32x4 v0[kMergeSlots], v1[kMergeSlots];
@@ -115,23 +133,25 @@ __device__ inline void merge_row(const AttnArgs& a, int head, int first, int n_s
   for (int u = 0; u < kMergeSlots; ++u) {
     const int sidx = u < n_slots ? u : 0;
     ls[u] = u < n_slots ? pl[(int64_t)sidx * a.rows_max] : -INFINITY;
-    f16x8 h = *reinterpret_cast<const f16x8*>(po + sidx * sstride);
-    if (u >= n_slots) h = f16x8{};  // a repeated slot may hold an infinity: 0 * inf
-    v0[u] = f32x4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
-    v1[u] = f32x4{(float)h[4], (float)h[5], (float)h[6], (float)h[7]};
+    const Part v = part_of(po + sidx * sstride, u < n_slots);
+    v0[u] = v.lo;
+    v1[u] = v.hi;
   }
   float M = -INFINITY, W = 0.f;
 #pragma unroll
-  for (int u = 0; u < kMergeSlots; ++u) M = fmaxf(M, ls[u]);  // finite: slot 0 holds token 0, which every row attends
+  for (int u = 0; u < kMergeSlots; ++u) M = fmaxf(M, ls[u]);
+  // slot 0 holds token 0, which every row attends: -inf only where its block's
+  // id is outside the pool, as all the others' are
+  const float use = M == -INFINITY ? 0.f : M;
   f32x4 acc0 = {0.f, 0.f, 0.f, 0.f}, acc1 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int u = 0; u < kMergeSlots; ++u) {
-    const float wgt = exp2f(ls[u] - M);
+    const float wgt = exp2f(ls[u] - use);
     acc0 += v0[u] * wgt;
     acc1 += v1[u] * wgt;
     W += wgt;
   }
-  const float inv = 1.f / W;
+  const float inv = merge_inv(W);
   const int qi = n / a.gqa, gh = n - qi * a.gqa;
   const int64_t orow = (int64_t)(row_start + qi) * a.hq + head * a.gqa + gh;
   f16x8 hv = {(f16)(acc0[0] * inv), (f16)(acc0[1] * inv), (f16)(acc0[2] * inv),
@@ -160,22 +180,22 @@ __device__ inline void merge_states(MergeState& a, float M2, float W2, f32x4 lo2
 // ... of a (row, 8 dims) each, and their states are merged over the wave's
 // 16-lane rows and, past four threads, over the workgroup's waves in LDS, in a
 // fixed order.
-template <int SL>
+template <int SL, class P>
 __device__ inline void merge_row_wide(const AttnArgs& a, int head, int first, int n_slots, int row_start, int n,
                                       int n_rows, int d8, int sl) {
   const int nr = n < n_rows ? n : 0;  // every thread takes part in the exchanges
-  const f16* po = a.part_o + ((int64_t)first * a.rows_max + nr) * D + 8 * d8;
+  const P* po = static_cast<const P*>(a.part_o) + ((int64_t)first * a.rows_max + nr) * D + 8 * d8;
   const float* pl = a.part_lse + (int64_t)first * a.rows_max + nr;
   MergeState st = {-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
   for (int s0 = sl; s0 < n_slots; s0 += 4 * SL) {
     float ls[4];
-    f16x8 h[4];
+    Part h[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int s = s0 + SL * u;
       const int at = s < n_slots ? s : s0;
       ls[u] = s < n_slots ? pl[(int64_t)at * a.rows_max] : -INFINITY;
-      h[u] = *reinterpret_cast<const f16x8*>(po + (int64_t)at * a.rows_max * D);
+      h[u] = part_of(po + (int64_t)at * a.rows_max * D, s < n_slots);
     }
     const float M = fmaxf(fmaxf(fmaxf(ls[0], ls[1]), fmaxf(ls[2], ls[3])), st.M);
     const float use = M == -INFINITY ? 0.f : M;
@@ -186,9 +206,8 @@ __device__ inline void merge_row_wide(const AttnArgs& a, int head, int first, in
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const float wgt = exp2f(ls[u] - use);
-      if (s0 + SL * u >= n_slots) h[u] = f16x8{};  // a repeated slot may hold an infinity: 0 * inf
-      st.lo += f32x4{(float)h[u][0], (float)h[u][1], (float)h[u][2], (float)h[u][3]} * wgt;
-      st.hi += f32x4{(float)h[u][4], (float)h[u][5], (float)h[u][6], (float)h[u][7]} * wgt;
+      st.lo += h[u].lo * wgt;
+      st.hi += h[u].hi * wgt;
       st.W += wgt;
     }
     st.M = M;
@@ -213,7 +232,7 @@ __device__ inline void merge_row_wide(const AttnArgs& a, int head, int first, in
     for (int v = 1; v < 4; ++v) merge_states(st, s_wave[v][d8].M, s_wave[v][d8].W, s_wave[v][d8].lo, s_wave[v][d8].hi);
   }
   if (n >= n_rows || sl != 0) return;
-  const float inv = 1.f / st.W;
+  const float inv = merge_inv(st.W);
   const int qi = n / a.gqa, gh = n - qi * a.gqa;
   const int64_t orow = (int64_t)(row_start + qi) * a.hq + head * a.gqa + gh;
   f16x8 hv;
@@ -228,23 +247,23 @@ __device__ inline void merge_row_wide(const AttnArgs& a, int head, int first, in
 
 // Row group `group` of a segment, SL threads per (row, 8 dims): 16 / SL rows
 // a workgroup.
-template <int SL>
+template <int SL, class P>
 __device__ inline void merge_group(const AttnArgs& a, int head, int first, int n_slots, int row_start, int n_rows,
                                    int group) {
   const int d8 = threadIdx.x & 15, p = threadIdx.x >> 4;
   const int n = group * (16 / SL) + p / SL;
   if constexpr (SL == 1) {
-    if (n < n_rows) merge_row(a, head, first, n_slots, row_start, n, d8);
+    if (n < n_rows) merge_row<P>(a, head, first, n_slots, row_start, n, d8);
   } else {
-    if (group * (16 / SL) < n_rows) merge_row_wide<SL>(a, head, first, n_slots, row_start, n, n_rows, d8, p % SL);
+    if (group * (16 / SL) < n_rows) merge_row_wide<SL, P>(a, head, first, n_slots, row_start, n, n_rows, d8, p % SL);
   }
 }
 
 // Workgroup (c, g) merges row group g of combine record c.
-template <int SL>
+template <int SL, class P>
 __global__ __launch_bounds__(256) void combine_kernel(AttnArgs a, int row_groups) {
   const int32_t* c = a.combines + kPieceWords * (blockIdx.x / row_groups);
-  merge_group<SL>(a, c[kCombHead], c[kCombFirst], c[kCombSlots], c[kCombRowStart], c[kCombQLen] * a.gqa,
+  merge_group<SL, P>(a, c[kCombHead], c[kCombFirst], c[kCombSlots], c[kCombRowStart], c[kCombQLen] * a.gqa,
                   blockIdx.x % row_groups);
 }
 
@@ -259,17 +278,17 @@ struct CombineTable {
 
 // Workgroup (c, g) = (blockIdx.x, blockIdx.y): the entry's address depends on
 // the workgroup index alone, so it loads with the other arguments.
-template <int SL>
+template <int SL, class P>
 __global__ __launch_bounds__(256) void combine_table_kernel(AttnArgs a, CombineTable tab) {
   const uint64_t e = tab.e[blockIdx.x];
-  merge_group<SL>(a, (int)((e >> 28) & 0xff), (int)(e & 0xfffff), (int)((e >> 20) & 0xff), (int)((e >> 36) & 0xfffff),
+  merge_group<SL, P>(a, (int)((e >> 28) & 0xff), (int)(e & 0xfffff), (int)((e >> 20) & 0xff), (int)((e >> 36) & 0xfffff),
                   (int)(e >> 56) * a.gqa, (int)blockIdx.y);
 }
 
 // Workspace bytes a plan needs: the claim counter (when it has claimed
 // records) and the partials.
-inline int64_t plan_partial_bytes(const int32_t* plan_host) {
-  return plan_workspace_bytes(plan_host[kPlanSlots], plan_host[kPlanRowsMax]);
+inline int64_t plan_partial_bytes(const int32_t* plan_host, int elem = 2) {
+  return plan_workspace_bytes(plan_host[kPlanSlots], plan_host[kPlanRowsMax], elem);
 }
 
 // A checked call: what its launch is given.
@@ -282,12 +301,13 @@ struct AttnCall {
 };
 
 // Checks the arguments and the plan of an attention call (`part` holds the
-// partials, `part_capacity` bytes) and fills *c.
+// partials, `part_capacity` bytes, of values of `part_elem` bytes) and fills *c.
 inline int prepare_attention(const char* who, const void* q, bool needs_q, void* o, float* lse, const void* k_cache,
                              const void* v_cache, int64_t num_blocks, int num_layers, int layer, int num_q_heads,
                              int num_kv_heads, int head_dim, int block_size, const int32_t* block_table,
                              int64_t bt_rows, int64_t bt_stride, const int32_t* plan_host, const int32_t* plan_dev,
-                             void* part, int64_t part_capacity, float softmax_scale, int32_t* status, AttnCall* c) {
+                             void* part, int64_t part_capacity, int part_elem, float softmax_scale, int32_t* status,
+                             AttnCall* c) {
   if (head_dim != D) return fail(NSD_ERR_UNSUPPORTED, "%s: head_dim=%d (only 128)", who, head_dim);
   if (block_size != BS)
     return fail(NSD_ERR_UNSUPPORTED, "%s: block_size=%d (only 16)", who, block_size);
@@ -356,7 +376,7 @@ inline int prepare_attention(const char* who, const void* q, bool needs_q, void*
         (int64_t)r[kCombRowStart] + r[kCombQLen] > n_rows_plan)
       return fail(NSD_ERR_INVALID, "%s: corrupt plan (combine %d)", who, c);
   }
-  const int64_t part_bytes = plan_partial_bytes(plan_host);
+  const int64_t part_bytes = plan_partial_bytes(plan_host, part_elem);
   if ((n_combine > 0 || n_claimed > 0) && (part == nullptr || part_capacity < part_bytes || !aligned16(part)))
     return fail(NSD_ERR_WORKSPACE,
                 "%s: workspace holds %lld partial bytes, the plan needs %lld", who,
@@ -376,8 +396,8 @@ inline int prepare_attention(const char* who, const void* q, bool needs_q, void*
   args.n_static = n_static;
   args.n_claimed = n_claimed;
   args.n_claim_wgs = grid - n_static;
-  args.part_o = reinterpret_cast<f16*>(ws + kClaimBytes);
-  args.part_lse = reinterpret_cast<float*>(args.part_o + n_slots * rows_max * D);
+  args.part_o = ws + kClaimBytes;
+  args.part_lse = reinterpret_cast<float*>(ws + kClaimBytes + n_slots * rows_max * D * part_elem);
   args.combines = plan_dev + plan_host[kPlanOffCombines];
   args.status = status;
   args.num_blocks = num_blocks;
@@ -410,7 +430,9 @@ inline int prepare_attention(const char* who, const void* q, bool needs_q, void*
 }
 
 // The second launch: every segment cut into pieces is merged (none: nothing).
-inline int launch_merge(const char* who, const AttnCall& call, const int32_t* plan_host, hipStream_t st) {
+// P: the partials' type.
+template <class P>
+int launch_merge(const char* who, const AttnCall& call, const int32_t* plan_host, hipStream_t st) {
   const int n_combine = call.n_combine;
   if (n_combine == 0) return NSD_OK;
   const AttnArgs& args = call.args;
@@ -433,9 +455,9 @@ inline int launch_merge(const char* who, const AttnCall& call, const int32_t* pl
     constexpr int SL = decltype(slc)::value;
     const int groups = (args.rows_max * SL + 15) / 16;
     if (packed)
-      hipLaunchKernelGGL(combine_table_kernel<SL>, dim3(n_combine, groups), dim3(256), 0, st, args, tab);
+      hipLaunchKernelGGL((combine_table_kernel<SL, P>), dim3(n_combine, groups), dim3(256), 0, st, args, tab);
     else
-      hipLaunchKernelGGL(combine_kernel<SL>, dim3(n_combine * groups), dim3(256), 0, st, args, groups);
+      hipLaunchKernelGGL((combine_kernel<SL, P>), dim3(n_combine * groups), dim3(256), 0, st, args, groups);
   };
   if (most_slots <= kMergeSlots) merge(std::integral_constant<int, 1>{});
   else if (most_slots <= 4 * kMergeSlots) merge(std::integral_constant<int, 4>{});

@@ -52,6 +52,7 @@ class LlamaInferState:
     # verify grouping: 0 = pack up to 48 rows per (group, kv head); 1 = row-wise
     max_group_rows: int = 0
     attn_plan: AttnPlan | None = None
+    kv8_plan: AttnPlan | None = None  # of the attention over an 8-bit cache
 
     def decode_rows_host(self):
         """(seq_ids, seq_lens) of the decode rows as host lists (one D2H copy if absent)."""

@@ -21,7 +21,7 @@ import ctypes
 import torch
 
 from .. import _lib
-from ..plan import plan_for
+from ..plan import kv8_plan_for
 from ._util import StatusWord, check_block_table, ptr, require, require_cuda, stream_on
 
 HEAD_DIM, BLOCK_TOKENS = 128, 16
@@ -322,7 +322,7 @@ def kv8_paged_attention(q: torch.Tensor, cache: KV8Cache, block_table: torch.Ten
         raise ValueError(f"model_config has {model_config.num_kv_heads} kv heads, the cache {cache.num_kv_heads}")
     if rows == 0:
         return
-    plan = plan_for(infer_state, model_config, engine_config, block_table)
+    plan = kv8_plan_for(infer_state, model_config, engine_config, block_table)
     if plan.n_rows != rows:
         raise ValueError(f"the forward's attention plan covers {plan.n_rows} rows, q has {rows}")
     size, ws = plan.workspace_bytes, None

@@ -68,6 +68,27 @@ def plan_words(seq_ids, seq_lens, num_q_heads: int, num_kv_heads: int, head_dim:
                max_group_rows: int = 0, static_slots: int = 0) -> tuple[np.ndarray, int]:
     """Run the native planner on host lists; returns (plan words int32, workspace bytes).
     ``static_slots`` > 0: pieces beyond that many are claimed at run time."""
+    out = ctypes.c_int64(0)
+    words = _planned(seq_ids, seq_lens, num_kv_heads, n_workers, lambda lib, rows, words, buf, cap: (
+        lib.nsd_attn_plan_build_claimed(
+            *rows, num_q_heads, num_kv_heads, head_dim, block_size, bt_rows, bt_stride, n_workers, static_slots,
+            max_group_rows, buf, cap, words, ctypes.byref(out))))
+    return words, int(out.value)
+
+
+def kv8_plan_words(seq_ids, seq_lens, num_q_heads: int, num_kv_heads: int, bt_rows: int, bt_stride: int,
+                   compute_units: int, max_group_rows: int = 0) -> tuple[np.ndarray, int]:
+    """``plan_words`` for the attention over an 8-bit cache on a device of ``compute_units``."""
+    words = _planned(seq_ids, seq_lens, num_kv_heads, 2 * compute_units, lambda lib, rows, words, buf, cap: (
+        lib.nsd_kv8_plan_build(*rows, num_q_heads, num_kv_heads, bt_rows, bt_stride, compute_units, max_group_rows,
+                               buf, cap, words)))
+    out = ctypes.c_int64(0)
+    _lib.call("nsd_kv8_attn_workspace", words.ctypes.data, ctypes.byref(out))
+    return words, int(out.value)
+
+
+def _planned(seq_ids, seq_lens, num_kv_heads: int, n_workers: int, build) -> np.ndarray:
+    """The plan words that ``build(lib, rows, words, buffer, capacity)`` writes."""
     sid = np.ascontiguousarray(np.asarray(seq_ids, dtype=np.int32))
     sl = np.ascontiguousarray(np.asarray(seq_lens, dtype=np.int32))
     if sid.shape != sl.shape or sid.ndim != 1:
@@ -81,16 +102,13 @@ def plan_words(seq_ids, seq_lens, num_q_heads: int, num_kv_heads: int, head_dim:
     for _ in range(2):  # the bound assumes n_workers; a plan that needs more reports its size
         buf = np.zeros(cap, dtype=np.int32)
         words = ctypes.c_int64(0)
-        ws = ctypes.c_int64(0)
-        rc = lib.nsd_attn_plan_build_claimed(
-            sid.ctypes.data_as(i32p), sl.ctypes.data_as(i32p), len(sid), num_q_heads,
-            num_kv_heads, head_dim, block_size, bt_rows, bt_stride, n_workers, static_slots,
-            max_group_rows, buf.ctypes.data_as(i32p), cap, ctypes.byref(words), ctypes.byref(ws))
+        rc = build(lib, (sid.ctypes.data_as(i32p), sl.ctypes.data_as(i32p), len(sid)), ctypes.byref(words),
+                   buf.ctypes.data_as(i32p), cap)
         if rc == _lib.NSD_ERR_WORKSPACE and words.value > cap:
             cap = words.value
             continue
         _lib.check(rc, "nsd_attn_plan_build")
-        return buf[: words.value].copy(), int(ws.value)
+        return buf[: words.value].copy()
     raise _lib.NativeLibraryError("nsd_attn_plan_build: plan size did not converge")
 
 
@@ -207,15 +225,51 @@ def build_attn_plan(seq_ids, seq_lens, num_q_heads: int, num_kv_heads: int, head
         words, ws = plan_words(seq_ids, seq_lens, num_q_heads, num_kv_heads, head_dim,
                                block_size, bt_rows, bt_stride, pieces_for(slots, rows_max), max_group_rows,
                                slots)
-    # pinned and non-blocking: the upload does not wait for the stream
-    # (the caching host allocator keeps the pinned block until the copy ran)
-    src = torch.from_numpy(words)
-    dev = (src.pin_memory().to(device, non_blocking=True) if device.type == "cuda"
-           else src.to(device))
     # the claim counter (zero before the first call; every call leaves it
     # zero) and the split segments' partials
     workspace = torch.zeros(max(ws, 256), dtype=torch.uint8, device=device)
-    return AttnPlan(words, dev, workspace, ws, num_q_heads, num_kv_heads)
+    return AttnPlan(words, _upload(words, device), workspace, ws, num_q_heads, num_kv_heads)
+
+
+def _upload(words: np.ndarray, device):
+    """Plan words on the device: pinned and non-blocking, so the upload does not wait for the stream (the caching host
+    allocator keeps the pinned block until the copy ran)."""
+    import torch
+
+    src = torch.from_numpy(words)
+    return src.pin_memory().to(device, non_blocking=True) if device.type == "cuda" else src.to(device)
+
+
+def _decode_rows(infer_state):
+    """(seq_ids, seq_lens) of an infer state's decode rows as host lists (copied from the device where it has none)."""
+    getter = getattr(infer_state, "decode_rows_host", None)
+    if getter is not None:
+        return getter()
+    sids = getattr(infer_state, "seq_ids_list", None)
+    slens = getattr(infer_state, "decoding_seq_lens_list", None)
+    if sids is None:
+        sids = infer_state.seq_ids[int(infer_state.num_prefill_seqs):].cpu().tolist()
+    if slens is None:
+        slens = infer_state.decoding_seq_lens.cpu().tolist()
+    return sids, slens
+
+
+def kv8_plan_for(infer_state, model_config, engine_config, block_table) -> AttnPlan:
+    """``plan_for`` for the attention over an 8-bit cache: cut for half the bytes a block, kept on the infer state as
+    ``kv8_plan``.  It has no workspace: a call brings its own of ``workspace_bytes``."""
+    import torch
+
+    plan = getattr(infer_state, "kv8_plan", None)
+    if plan is None or not plan.fits(model_config.num_q_heads, model_config.num_kv_heads, block_table):
+        sids, slens = _decode_rows(infer_state)
+        device = block_table.device
+        words, ws = kv8_plan_words(sids, slens, model_config.num_q_heads, model_config.num_kv_heads,
+                                   block_table.shape[0], block_table.shape[1],
+                                   torch.cuda.get_device_properties(device).multi_processor_count,
+                                   int(getattr(infer_state, "max_group_rows", 0)))
+        plan = AttnPlan(words, _upload(words, device), None, ws, model_config.num_q_heads, model_config.num_kv_heads)
+        infer_state.kv8_plan = plan
+    return plan
 
 
 def plan_for(infer_state, model_config, engine_config, block_table) -> AttnPlan:
@@ -235,13 +289,7 @@ def plan_for(infer_state, model_config, engine_config, block_table) -> AttnPlan:
     if plan is not None and plan.fits(model_config.num_q_heads, model_config.num_kv_heads,
                                       block_table):
         return plan
-    npf = int(infer_state.num_prefill_seqs)
-    sids = getattr(infer_state, "seq_ids_list", None)
-    slens = getattr(infer_state, "decoding_seq_lens_list", None)
-    if sids is None:
-        sids = infer_state.seq_ids[npf:].cpu().tolist()
-    if slens is None:
-        slens = infer_state.decoding_seq_lens.cpu().tolist()
+    sids, slens = _decode_rows(infer_state)
     plan = build_attn_plan(sids, slens, model_config.num_q_heads, model_config.num_kv_heads,
                            model_config.head_dim, engine_config.block_size, block_table.shape[0],
                            block_table.shape[1], block_table.device,

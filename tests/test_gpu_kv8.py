@@ -17,6 +17,7 @@ from nebulasd_amd import _lib
 from nebulasd_amd.config import QWEN3_0_6B, QWEN3_8B, EngineConfig, ModelConfig
 from nebulasd_amd.hostkv import swap_blocks
 from nebulasd_amd.infer_state import build_infer_state, rope_cache
+from nebulasd_amd.plan import kv8_plan_for
 from nebulasd_amd.kernels import (KV8Cache, kv8_load, kv8_paged_attention, kv8_qk_norm_rope_store, kv8_store,
                                   paged_attention, prefill_attention, qk_norm_rope_store)
 
@@ -504,7 +505,7 @@ def test_attention_block_and_pair_edges(gpu, codes, hq, hkv, q_len):
 def test_attention_segments_in_pieces(gpu, codes, hq, hkv, q_len, ctxs):
     mc, ec, table, bt, cache, ids, lens, q = filled(codes, gpu, hq, hkv, ctxs, q_len, seed=1)
     o, lse, st = attend(cache, bt, mc, ec, ids, lens, q)
-    assert int(st.attn_plan.host[_lib.PLAN_COMBINES]) > 0
+    assert int(st.kv8_plan.host[_lib.PLAN_COMBINES]) > 0
     check_attention(cache, table, 1, q, ids, lens, o, lse)
 
 
@@ -514,7 +515,7 @@ def test_attention_of_more_segments_than_slots(gpu, codes):
     ctxs = [3 * i % 97 for i in range(80)]
     mc, ec, table, bt, cache, ids, lens, q = filled(codes, gpu, 16, 8, ctxs, 1, seed=2)
     o, lse, st = attend(cache, bt, mc, ec, ids, lens, q)
-    assert int(st.attn_plan.host[_lib.PLAN_CLAIMED]) > 0
+    assert int(st.kv8_plan.host[_lib.PLAN_CLAIMED]) > 0
     check_attention(cache, table, 1, q, ids, lens, o, lse)
     for _ in range(3):
         o2, lse2, _ = attend(cache, bt, mc, ec, ids, lens, q, st=st)
@@ -645,7 +646,7 @@ def _step_state(codes, gpu, seed, q_len=5, ctxs=(700, 33, 2000), hq=16, hkv=8):
     i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=gpu)  # noqa: E731
     cos, sin = rope_cache(128, 1e6, 4096, gpu)
     st = state(mc, ids, lens)
-    st.get_attn_plan(mc, ec, bt)
+    kv8_plan_for(st, mc, ec, bt)
     return dict(mc=mc, ec=ec, table=table, bt=bt, cache=cache, st=st, q=half(n, hq, 128), k=half(n, hkv, 128),
                 v=half(n, hkv, 128), w=1 + half(128) / 8, cos=cos, sin=sin, q_out=half(n, hq, 128), o=half(n, hq, 128),
                 lse=torch.empty(n, hq, device=gpu), k_out=half(total, hkv, 128), v_out=half(total, hkv, 128),

@@ -216,10 +216,48 @@ def test_c_refusals_of_arguments():
         _lib.call(*args)
 
 
+def test_plans():
+    """Every block of every segment in one piece, parts in fp32, and few pieces where they do."""
+    from nebulasd_amd.plan import decode_plan, kv8_plan_words
+    rng = np.random.default_rng(6)
+    for n, hq, hkv, longest, rows in ((1, 32, 8, 60000, 1), (4, 16, 8, 300, 1), (16, 32, 8, 4000, 5), (80, 16, 8, 900, 1),
+                                      (40, 8, 1, 3000, 9), (3, 48, 1, 20, 2)):
+        ctx = rng.integers(0, longest, n)
+        ids = [s for s in range(n) for _ in range(rows)]
+        lens = [int(c) + i + 1 for c in ctx for i in range(rows)]
+        words, ws = kv8_plan_words(ids, lens, hq, hkv, n, longest // 16 + 2, 256)
+        p = decode_plan(words)
+        seen = {}
+        for rec in p["pieces"]:
+            seen.setdefault((int(rec[4]), int(rec[0])), []).append((int(rec[1]), int(rec[2])))
+        assert len(seen) == len(p["groups"]) * hkv
+        for (row, head), parts in seen.items():
+            parts.sort()
+            group = next(g for g in p["groups"] if g[0] == row)
+            assert parts[0][0] == 0 and parts[-1][1] == -(-int(group[3] + group[1]) // 16)
+            assert all(a[1] == b[0] for a, b in zip(parts, parts[1:]))
+            assert all(b - a <= 256 for a, b in parts)
+            assert len(parts) == 1 or min(b - a for a, b in parts) >= 20  # 24, less the rounding of starts
+        fewest = sum(-(-sum(b - a for a, b in parts) // 256) for parts in seen.values())
+        assert len(p["pieces"]) <= (256 if fewest <= 256 else max(512, fewest))
+        split = p["slots"]
+        assert ws == (0 if split == 0 and p["claimed"] == 0 else 256 + -(-split * p["rows_max"] * (4 * 128 + 4) // 256) * 256)
+    with pytest.raises(ValueError, match="workers=0"):
+        kv8_plan_words([0], [1], 4, 2, 1, 1, 0)
+    with pytest.raises(_lib.NativeLibraryError, match="compute units"):
+        kv8_plan_words([0], [1], 4, 2, 1, 1, 1 << 17)
+    for bad in (dict(seq_ids=[1], seq_lens=[1]), dict(seq_ids=[0], seq_lens=[0]), dict(seq_ids=[0], seq_lens=[17]),
+                dict(seq_ids=[-1], seq_lens=[1])):
+        with pytest.raises(_lib.NativeLibraryError):
+            kv8_plan_words(*bad.values(), 4, 2, 1, 1, 256)
+    with pytest.raises(_lib.NativeLibraryError, match="not a plan"):
+        _lib.call("nsd_kv8_attn_workspace", np.zeros(64, np.int32).ctypes.data, ctypes.byref(ctypes.c_int64()))
+
+
 def test_attention_refusals():
-    from nebulasd_amd.plan import plan_words
-    words, ws = plan_words([0, 1], [40, 900], 4, 2, 128, 16, 2, 64, 64)
-    buf = words.ctypes.data_as(ctypes.POINTER(ctypes.c_int32))
+    from nebulasd_amd.plan import kv8_plan_words
+    words, ws = kv8_plan_words([0, 1], [40, 900], 4, 2, 2, 64, 64)
+    buf = words.ctypes.data
     c = _c()
 
     def args(cache=c, layer=0, q=16, o=16, hq=4, bt=16, bt_rows=2, stride=64, plan=buf, dev=16, work=16, size=ws):
