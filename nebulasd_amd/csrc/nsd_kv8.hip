@@ -309,18 +309,38 @@ __global__ __launch_bounds__(kThreads) void kv8_append_kernel(Cache c, AppendArg
   }
 }
 
-// Whole prompts: grid (block of the prompt, prompt, four units of 2 Hkv).
-template <int T>
+// Sixteen bytes of a row, and of codes; FAR: past the caches.
+template <bool FAR>
+__device__ inline f16x8 row16(const f16* p) {
+  const f16x8* q = reinterpret_cast<const f16x8*>(p);
+  return FAR ? __builtin_nontemporal_load(q) : *q;
+}
+template <bool FAR>
+__device__ inline void put16(u32x4* at, u32x4 v) {
+  if (FAR) __builtin_nontemporal_store(v, at);
+  else *at = v;
+}
+
+// Workgroups run over the units of a block first, so that a block's rows, one
+// run in memory, are read or written at one time (units last: prompts of 32k
+// tokens x 8 heads stored in 84.2 us with the kernel that makes the rows, 78.5
+// so; read back by 92.7 and 86.3 with their reader).
+
+// Whole prompts: grid (block of the prompt x four units of 2 Hkv, prompt).  FAR:
+// 1 codes are written past the caches, 2 rows are read past them too.
+template <int T, int FAR>
 __global__ __launch_bounds__(kThreads) void kv8_prefill_kernel(
     Cache c, const f16* __restrict__ k, const f16* __restrict__ v, int64_t n_tokens, const int32_t* __restrict__ bt,
     int64_t bt_rows, int64_t bt_stride, const int32_t* __restrict__ seq_ids, const int32_t* __restrict__ start_locs,
     const int32_t* __restrict__ lens, int64_t max_len, int32_t* status) {
-  const int64_t b = blockIdx.x, s = blockIdx.y;
+  const int groups = (2 * c.hkv + kWaves - 1) / kWaves;
+  const int64_t b = blockIdx.x / groups, s = blockIdx.y;
+  const int group = blockIdx.x % groups;
   const int64_t len = lens[s], start = start_locs[s], sid = seq_ids[s];
   if (b * BS >= len) return;
   const int lane = threadIdx.x & 63;
-  const int unit = blockIdx.z * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const bool first = blockIdx.z == 0 && threadIdx.x == 0;
+  const int unit = group * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool first = group == 0 && threadIdx.x == 0;
   if (sid < 0 || sid >= bt_rows || len > bt_stride * BS || len > max_len || start < 0 || start + len > n_tokens) {
     if (first) flag_status(status, NSD_STATUS_BAD_SEQ);
     return;
@@ -345,22 +365,22 @@ __global__ __launch_bounds__(kThreads) void kv8_prefill_kernel(
       h[2 * j] = h[2 * j + 1] = f16x8{};
       if (t0 + 8 * j < n) {
         const f16* src = rows + (t0 + 8 * j) * rs + 8 * cc;
-        h[2 * j] = *reinterpret_cast<const f16x8*>(src);
-        h[2 * j + 1] = *reinterpret_cast<const f16x8*>(src + D / 2);
+        h[2 * j] = row16<FAR == 2>(src);
+        h[2 * j + 1] = row16<FAR == 2>(src + D / 2);
       }
     }
     const Scale sc = tile_scale<T>(h, status);
 #pragma unroll
     for (int j = 0; j < 2; ++j)
-      u.codes[16 * cc + t0 + 8 * j] =
-          k_unit(kv8_codes<T>(h[2 * j], sc.e, sc.careful), kv8_codes<T>(h[2 * j + 1], sc.e, sc.careful));
+      put16<FAR != 0>(u.codes + 16 * cc + t0 + 8 * j,
+              k_unit(kv8_codes<T>(h[2 * j], sc.e, sc.careful), kv8_codes<T>(h[2 * j + 1], sc.e, sc.careful)));
     if (lane == 0) *u.scale = (uint8_t)(sc.e + 127);
   } else {
     const int i = lane & 15, t0 = 4 * (lane >> 4);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       h[j] = f16x8{};
-      if (t0 + j < n) h[j] = *reinterpret_cast<const f16x8*>(rows + (t0 + j) * rs + 8 * i);
+      if (t0 + j < n) h[j] = row16<FAR == 2>(rows + (t0 + j) * rs + 8 * i);
     }
     const Scale sc = tile_scale<T>(h, status);
     u32x4 b0, b1;
@@ -370,37 +390,42 @@ __global__ __launch_bounds__(kThreads) void kv8_prefill_kernel(
       b0[j] = w[0];
       b1[j] = w[1];
     }
-    u.codes[lane] = kv8_transpose(b0);
-    u.codes[64 + lane] = kv8_transpose(b1);
+    put16<FAR != 0>(u.codes + lane, kv8_transpose(b0));
+    put16<FAR != 0>(u.codes + 64 + lane, kv8_transpose(b1));
     if (lane == 0) *u.scale = (uint8_t)(sc.e + 127);
   }
 }
 
-// Reading back: grid (block from the first token's on, sequence, four units).
+// Reading back: grid (block from the first token's on x four units, sequence).
+// Bound by memory, as a copy is.  Stores that pass the caches make it faster (16
+// sequences of 256 to 4096 tokens 31 -> 24 us) and its reader slower by more
+// (24k tokens, then the prefill attention over them: 175.4 -> 182.7).
 template <int T>
 __global__ __launch_bounds__(kThreads) void kv8_load_kernel(
     Cache c, f16* __restrict__ k, f16* __restrict__ v, int64_t n_tokens, const int32_t* __restrict__ bt,
     int64_t bt_rows, int64_t bt_stride, const int32_t* __restrict__ seq_ids, const int32_t* __restrict__ firsts,
     const int32_t* __restrict__ start_locs, const int32_t* __restrict__ lens, int64_t max_len, int32_t* status) {
-  const int64_t s = blockIdx.y;
+  const int groups = (2 * c.hkv + kWaves - 1) / kWaves;
+  const int64_t s = blockIdx.y, from = blockIdx.x / groups;
+  const int group = blockIdx.x % groups;
   const int64_t first = firsts != nullptr ? firsts[s] : 0, len = lens[s], start = start_locs[s], sid = seq_ids[s];
   const int64_t end = first + len;
   if (len <= 0) return;
-  const bool says = blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0;
+  const bool says = blockIdx.x == 0 && threadIdx.x == 0;
   if (sid < 0 || sid >= bt_rows || first < 0 || end > bt_stride * BS || len > max_len || start < 0 ||
       start + len > n_tokens) {
     if (says) flag_status(status, NSD_STATUS_BAD_SEQ);
     return;
   }
-  const int64_t b = first / BS + blockIdx.x;
+  const int64_t b = first / BS + from;
   if (b * BS >= end) return;
   const int64_t blk = bt[sid * bt_stride + b];
   if (blk < 0 || blk >= c.num_blocks) {
-    if (blockIdx.z == 0 && threadIdx.x == 0) flag_status(status, NSD_STATUS_BAD_BLOCK);
+    if (group == 0 && threadIdx.x == 0) flag_status(status, NSD_STATUS_BAD_BLOCK);
     return;
   }
   const int lane = threadIdx.x & 63;
-  const int unit = blockIdx.z * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int unit = group * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (unit >= 2 * c.hkv) return;
   const bool isv = unit >= c.hkv;
   const int head = isv ? unit - c.hkv : unit;
@@ -564,13 +589,25 @@ extern "C" int nsd_kv8_store_prefill(const void* k, const void* v, int64_t n_tok
     return fail(NSD_ERR_INVALID, "%s: null pointer", who);
   if (!aligned16(k) || !aligned16(v)) return fail(NSD_ERR_INVALID, "%s: k and v must be 16-byte aligned", who);
   const int64_t nb = std::min((max_prefill_len + BS - 1) / BS, bt_stride);
-  if (nb > kMaxGrid || n_seqs > 65535) return fail(NSD_ERR_UNSUPPORTED, "%s: grid too large", who);
+  const int64_t grid = nb * unit_groups(cache);
+  if (grid > kMaxGrid || n_seqs > 65535) return fail(NSD_ERR_UNSUPPORTED, "%s: grid too large", who);
+  // Many rows do not stay in the 256 MB memory-side cache beside what follows.
+  // Their codes are read next by a decode step, layers later: written past the
+  // caches, 16k tokens x 8 heads (67 MB of rows) with the kernel that makes the
+  // rows 42.2 -> 39.5 us, 9k 25.4 -> 25.0, but 9k read back at once 18.4 -> 21.4.
+  // The rows themselves, read past them: 32k 38.9 -> 36.6, but 16k, still there
+  // when their maker has just ended, 17.7 -> 19.2.
+  const int64_t row_bytes = n_tokens * cache->num_kv_heads * (int64_t)(2 * D * sizeof(f16));
   with_codes(cache, [&](auto t) {
-    hipLaunchKernelGGL(kv8_prefill_kernel<decltype(t)::value>,
-                       dim3((unsigned)nb, (unsigned)n_seqs, (unsigned)unit_groups(cache)), dim3(kThreads), 0,
-                       as_stream(stream), cache_of(cache, layer), static_cast<const f16*>(k),
-                       static_cast<const f16*>(v), n_tokens, block_table, bt_rows, bt_stride, seq_ids, start_locs,
-                       prefill_lens, max_prefill_len, status);
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)grid, (unsigned)n_seqs), dim3(kThreads), 0, as_stream(stream),
+                         cache_of(cache, layer), static_cast<const f16*>(k), static_cast<const f16*>(v), n_tokens,
+                         block_table, bt_rows, bt_stride, seq_ids, start_locs, prefill_lens, max_prefill_len, status);
+    };
+    constexpr int T = decltype(t)::value;
+    if (row_bytes >= 128000000) go(kv8_prefill_kernel<T, 2>);
+    else if (row_bytes >= 64000000) go(kv8_prefill_kernel<T, 1>);
+    else go(kv8_prefill_kernel<T, 0>);
   });
   return launch_status(who);
 }
@@ -590,10 +627,10 @@ extern "C" int nsd_kv8_load(void* k, void* v, int64_t n_tokens, const nsd_kv8_ca
   if (!aligned16(k) || !aligned16(v)) return fail(NSD_ERR_INVALID, "%s: k and v must be 16-byte aligned", who);
   // a range that starts inside a block touches one more
   const int64_t nb = std::min((max_len + BS - 1) / BS + (first != nullptr ? 1 : 0), bt_stride);
-  if (nb > kMaxGrid || n_seqs > 65535) return fail(NSD_ERR_UNSUPPORTED, "%s: grid too large", who);
+  const int64_t grid = nb * unit_groups(cache);
+  if (grid > kMaxGrid || n_seqs > 65535) return fail(NSD_ERR_UNSUPPORTED, "%s: grid too large", who);
   with_codes(cache, [&](auto t) {
-    hipLaunchKernelGGL(kv8_load_kernel<decltype(t)::value>,
-                       dim3((unsigned)nb, (unsigned)n_seqs, (unsigned)unit_groups(cache)), dim3(kThreads), 0,
+    hipLaunchKernelGGL(kv8_load_kernel<decltype(t)::value>, dim3((unsigned)grid, (unsigned)n_seqs), dim3(kThreads), 0,
                        as_stream(stream), cache_of(cache, layer), static_cast<f16*>(k), static_cast<f16*>(v),
                        n_tokens, block_table, bt_rows, bt_stride, seq_ids, first, start_locs, lens, max_len, status);
   });
