@@ -98,6 +98,22 @@ __device__ inline Unit unit_of(const Cache& c, int64_t blk, int head, bool isv) 
 
 __device__ inline u32x4 k_unit(u32x2 lo, u32x2 hi) { return u32x4{lo[0], lo[1], hi[0], hi[1]}; }
 
+// v + v of lane ^ 4, ^ 2 or ^ 1, of eight lanes a row, by DPP: shifts by four
+// into the lanes that have a partner there, or permutations of four.  (Through
+// LDS, __shfl_xor: 64 rows 4.6 us, 4.4 so.)
+template <int M>
+__device__ inline float add_lane(float v) {
+  const int u = __float_as_int(v);
+  int t;
+  if constexpr (M == 4) {
+    t = __builtin_amdgcn_update_dpp(0, u, 0x104, 0xf, 0x5, false);  // lanes 0 .. 3 of 8: from lane + 4
+    t = __builtin_amdgcn_update_dpp(t, u, 0x114, 0xf, 0xa, false);  // lanes 4 .. 7: from lane - 4
+  } else {
+    t = __builtin_amdgcn_mov_dpp(u, M == 2 ? 0x4E : 0xB1, 0xf, 0xf, true);  // quad_perm [2,3,0,1], [1,0,3,2]
+  }
+  return v + __int_as_float(t);
+}
+
 // What the decode/verify writer reads.  With the prologue (`PRO`) k is
 // normalised and rotated before it is stored, and q into q_out.
 struct AppendArgs {
@@ -124,19 +140,28 @@ struct AppendArgs {
   int hq;
 };
 
-// Where row r goes: its block, or -1 and the flag that says why not.
+// Where row r goes: its block, or -1 and the flag that says why not.  In two
+// parts, both without a branch, so that a caller has several rows' loads in
+// flight: the row's numbers, then its entry of the block table (any entry, where
+// the numbers are not good).
+struct RowNumbers {
+  int64_t sid, pos;
+};
 struct Place {
   int64_t blk, pos;
   int32_t flag;
 };
+__device__ inline RowNumbers numbers_of(const AppendArgs& a, int64_t r) {
+  return {a.seq_ids[r], (int64_t)a.seq_lens[r] - 1};
+}
 template <bool PRO>
-__device__ inline Place place_of(const Cache& c, const AppendArgs& a, int64_t r) {
-  const int64_t sid = a.seq_ids[r], pos = (int64_t)a.seq_lens[r] - 1;
-  if (sid < 0 || sid >= a.bt_rows || pos < 0 || pos >= a.bt_stride * BS) return {-1, pos, NSD_STATUS_BAD_SEQ};
-  if (PRO && pos >= a.n_pos) return {-1, pos, NSD_STATUS_BAD_POSITION};
-  const int64_t blk = a.bt[sid * a.bt_stride + pos / BS];
-  if (blk < 0 || blk >= c.num_blocks) return {-1, pos, NSD_STATUS_BAD_BLOCK};
-  return {blk, pos, 0};
+__device__ inline Place place_of(const Cache& c, const AppendArgs& a, const RowNumbers& n) {
+  const bool in = n.sid >= 0 && n.sid < a.bt_rows && n.pos >= 0 && n.pos < a.bt_stride * BS;
+  const bool turned = !PRO || n.pos < a.n_pos;
+  const int64_t blk = a.bt[in ? n.sid * a.bt_stride + n.pos / BS : 0];
+  const bool held = blk >= 0 && blk < c.num_blocks;
+  return {in && turned && held ? blk : -1, n.pos,
+          !in ? NSD_STATUS_BAD_SEQ : !turned ? NSD_STATUS_BAD_POSITION : NSD_STATUS_BAD_BLOCK};
 }
 
 // Dims 8c .. 8c+7 (lo) and 64+8c .. (hi) of a row, eight lanes a row: RMS-
@@ -161,9 +186,7 @@ __device__ inline void norm_rope(f16x8& lo, f16x8& hi, const f16* w, float eps, 
 #pragma unroll
     for (int j = 0; j < 8; ++j) u[j] = sq_pair(x0[j], x1[j]);
 #pragma unroll
-    for (int m = 4; m >= 1; m >>= 1)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) u[j] += __shfl_xor(u[j], m, kWave);
+    for (int j = 0; j < 8; ++j) u[j] = add_lane<1>(add_lane<2>(add_lane<4>(u[j])));
     const float ss = ((u[0] + u[4]) + (u[2] + u[6])) + ((u[1] + u[5]) + (u[3] + u[7]));
     const float rstd = 1.f / sqrtf(ss / (float)D + eps);
 #pragma unroll
@@ -185,8 +208,9 @@ __device__ inline void norm_rope(f16x8& lo, f16x8& hi, const f16* w, float eps, 
 // the rows, 256 at a time, and keeps for each of the block's slots the last row
 // that goes there.
 //
-// Bound by latency: row numbers, then the block table, then the tile and the
-// rows.
+// Bound by latency, one trip to memory after another: row numbers, the block
+// table, the tile and then the rows.  64 rows of 16 + 2 x 8 heads with the prologue
+// 4.4 us, 16 x 5 of 32 + 2 x 8 5.6.
 template <int T, bool PRO>
 __global__ __launch_bounds__(kThreads) void kv8_append_kernel(Cache c, AppendArgs a) {
   const int lane = threadIdx.x & 63;
@@ -215,7 +239,11 @@ __global__ __launch_bounds__(kThreads) void kv8_append_kernel(Cache c, AppendArg
   __shared__ unsigned long long s_slot[BS];  // (row + 1) << 32 | position, 0: none
   __shared__ int s_earlier;
   const int r = (int)blockIdx.x / a.kv_groups, group = (int)blockIdx.x - r * a.kv_groups;
-  const Place own = place_of<PRO>(c, a, r);
+  // this row's place and, beside it, the places of the first 256
+  const RowNumbers own_numbers = numbers_of(a, r);
+  const RowNumbers numbers = numbers_of(a, min((int)threadIdx.x, a.n_rows - 1));
+  const Place own = place_of<PRO>(c, a, own_numbers);
+  Place p = place_of<PRO>(c, a, numbers);
   if (own.blk < 0) {
     if (group == 0 && threadIdx.x == 0) flag_status(a.status, own.flag);
     return;
@@ -235,7 +263,7 @@ __global__ __launch_bounds__(kThreads) void kv8_append_kernel(Cache c, AppendArg
   if (threadIdx.x == 0) s_earlier = 0;
   __syncthreads();
   for (int rr = threadIdx.x; rr < a.n_rows; rr += kThreads) {
-    const Place p = place_of<PRO>(c, a, rr);
+    if (rr != (int)threadIdx.x) p = place_of<PRO>(c, a, numbers_of(a, rr));
     if (p.blk != own.blk) continue;
     atomicMax(&s_slot[p.pos % BS], (unsigned long long)(rr + 1) << 32 | (unsigned long long)p.pos);
     if (rr < r) s_earlier = 1;
