@@ -18,7 +18,8 @@
  * than fp16's own steps.
  *
  * A value that is not finite has the NaN code in E4M3 and 0 in whole numbers,
- * counts for no scale, and raises NSD_STATUS_NONFINITE.
+ * counts for no scale, and raises NSD_STATUS_NONFINITE; an E4M3 NaN raises it
+ * again whenever its block is written and its token stays.
  *
  * Rows stored at position p go to slot p % 16 of their block.  A prompt's blocks
  * are written whole, slots behind its last token as zeros.  Decode/verify rows
@@ -26,7 +27,9 @@
  * below the highest one written: the block's scale is that of these tokens'
  * values and the new rows together, and the tokens' codes are rounded again
  * where it changes.  Slots above hold no token (rows of a rejected draft, or of
- * the block's earlier owner), count for nothing and keep their codes.  A scale
+ * the block's earlier owner), count for nothing and keep their codes (V's end as
+ * zeros under the largest scale, where a code past the largest value would be an
+ * infinity).  A scale
  * that grows at least doubles, so however often a token is rounded again it
  * ends less than one of the last scale's steps (E4M3: of the value's own steps)
  * from its value; one that shrinks loses nothing.  Free scales would let every

@@ -60,6 +60,7 @@ __device__ inline uint32_t wave_max(uint32_t v) {
 // has none): the exponent, and whether the conversion has to be careful.
 struct Scale {
   int e;
+  bool top;  // the largest
   bool careful;
 };
 template <int T, int R>
@@ -83,7 +84,8 @@ __device__ inline Scale tile_scale(const f16x8 (&h)[R], int32_t* status) {
     m = wave_max(m);
   }
   const int e = kv8_exponent<T>(m);
-  return {e, careful || e == (T == NSD_KV8_E4M3 ? 8 : 9)};
+  const bool top = e == (T == NSD_KV8_E4M3 ? 8 : 9);
+  return {e, top, careful || top};
 }
 
 // The unit's tile: its codes and its scale byte.
@@ -321,7 +323,10 @@ __global__ __launch_bounds__(kThreads) void kv8_append_kernel(Cache c, AppendArg
       else if (old >> (t0 + j) & 1) h[j] = kv8_values<T>(u32x2{a0[j], a1[j]}, power);
     }
     const Scale s = tile_scale<T>(h, a.status);
-    const uint32_t put = fresh | (s.e + 127 != old_byte ? old : 0u);
+    // under the largest scale codes that no writer makes there would be
+    // infinities, which the attention multiplies by masked tokens' zeros: slots
+    // that hold no token become zeros
+    const uint32_t put = s.top ? 0xffffu : fresh | (s.e + 127 != old_byte ? old : 0u);
     u32x4 b0 = a0, b1 = a1;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {

@@ -188,7 +188,8 @@ void kv8_attn_kernel(AttnArgs a, PieceTable pt, Kv8Caches cache) {
     for (int kk = 0; kk < 4; ++kk) qf[t][kk] = *(const lds_f16x8*)(q_lds + ((4 * t + kk) * kWave + lane) * 16);
   const uint32_t k_word = *(const lds_u32*)(scale_lds + 4 * lane), v_word = *(const lds_u32*)(scale_lds + 256 + 4 * lane);
   const int k_scale = k_word >> (8 * (((uint32_t)tile + cache.ks_low) & 3)) & 0xff;
-  const int v_scale = v_word >> (8 * (((uint32_t)tile + cache.vs_low) & 3)) & 0xff;
+  // a masked block's bytes may be anything, infinities under its scale too: its values are zeros
+  const int v_scale = lane < my_n && !bad ? v_word >> (8 * (((uint32_t)tile + cache.vs_low) & 3)) & 0xff : 0;
   if (bad_mask != 0 && lane == 0) flag_status(a.status, NSD_STATUS_BAD_BLOCK);
 
   int row_len[NT];  // causal bound of this lane's row in each tile

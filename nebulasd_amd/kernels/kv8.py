@@ -304,7 +304,8 @@ def kv8_paged_attention(q: torch.Tensor, cache: KV8Cache, block_table: torch.Ten
 
     ``q``: [num_decoding_seqs, Hq, d] fp16; ``o``: as many elements, written in place; ``lse``: fp32 [rows, Hq], the
     natural-log sum of exp(score).  Scratch is the call's own (from the caching allocator), so calls on several
-    streams and in several captured graphs share nothing.
+    streams and in several captured graphs share nothing but the forward's plan, which the first call uploads on its
+    stream (``infer_state.kv8_plan``; a capture needs it built before).
     """
     table = _table(cache, block_table, engine_config)
     rows, hq = infer_state.num_decoding_seqs, model_config.num_q_heads

@@ -256,11 +256,16 @@ def _decode_rows(infer_state):
 
 def kv8_plan_for(infer_state, model_config, engine_config, block_table) -> AttnPlan:
     """``plan_for`` for the attention over an 8-bit cache: cut for half the bytes a block, kept on the infer state as
-    ``kv8_plan``.  It has no workspace: a call brings its own of ``workspace_bytes``."""
+    ``kv8_plan``.  It has no workspace: a call brings its own of ``workspace_bytes``.
+
+    A plan is made of host data, so it is refused inside a stream capture: the capture would replay the upload from
+    memory that is long another's.  Build it (this function, or one eager call) before."""
     import torch
 
     plan = getattr(infer_state, "kv8_plan", None)
     if plan is None or not plan.fits(model_config.num_q_heads, model_config.num_kv_heads, block_table):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the attention plan has to be built before the capture (kv8_plan_for, or an eager call)")
         sids, slens = _decode_rows(infer_state)
         device = block_table.device
         words, ws = kv8_plan_words(sids, slens, model_config.num_q_heads, model_config.num_kv_heads,

@@ -582,6 +582,40 @@ def test_attention_bad_blocks(gpu, codes):
 
 
 @pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("n", [1, 3, 17, 40])
+def test_slots_without_tokens_hold_any_code(gpu, codes, n):
+    """Codes that the largest scale makes infinite, in slots above the rows and in blocks that no piece streams."""
+    mc, ec, rng, table, bt, cache = make(codes, gpu, layers=1, seqs=1, blocks_per_seq=4, seed=12)
+    cache.k.fill_(0x7E if codes == "e4m3" else 0)  # 448, or -128
+    cache.v.fill_(0x7E if codes == "e4m3" else 0)
+    cache.k_scales.fill_(255), cache.v_scales.fill_(255)
+    m = Mirror(cache, 0, codes)
+    q = gpu_of(rows_of(rng, 1, 4, sizes=0.0))
+    for t in range(n):
+        k, v = rows_of(rng, 1, 2, sizes=0.0), rows_of(rng, 1, 2, sizes=0.0)
+        if t % 16 == 0:
+            v[0, :, 7] = 65504
+        kv8_store(gpu_of(k), gpu_of(v), cache, bt, mc, ec, state(mc, [0], [t + 1]), 0, validate=True)
+        m.append(table, [0], [t + 1], k, v)
+    m.check(cache)
+    o, lse, _ = attend(cache, bt, mc, ec, [0], [n], q, layer=0)
+    check_attention(cache, table, 0, q, [0], [n], o, lse)
+
+
+@pytest.mark.parametrize("codes", CODES)
+def test_attention_bad_blocks_among_pieces(gpu, codes):
+    """A piece whose blocks are all outside the pool counts for nothing in the merge; a row whose every piece is so is
+    zero, its lse -inf."""
+    mc, ec, table, bt, cache, ids, lens, q = filled(codes, gpu, 4, 2, [9000, 9000], 2, seed=13)
+    bad = table.copy()
+    bad[0, 100:], bad[1, :] = cache.num_blocks, -1
+    o, lse, st = attend(cache, gpu_of(bad), mc, ec, ids, lens, q, validate=False)
+    assert int(st.kv8_plan.host[_lib.PLAN_COMBINES]) > 0
+    assert (o[2:] == 0).all() and (lse[2:] == -np.inf).all()
+    check_attention(cache, table, 1, q[:2], [0, 0], [1600, 1600], o[:2], lse[:2])
+
+
+@pytest.mark.parametrize("codes", CODES)
 def test_attention_writes_its_rows_alone(gpu, codes):
     mc, ec, table, bt, cache, ids, lens, q = filled(codes, gpu, 8, 2, [33, 700], 2, seed=7)
     room = torch.full((q.numel() + 4096,), 7.0, dtype=torch.float16, device=gpu)
@@ -623,6 +657,37 @@ def test_tiles_past_32_bits(gpu):
     q = gpu_of(rows_of(rng, 2, 16, sizes=0.0))
     o, lse, _ = attend(cache, bt, mc, ec, [0, 1], [101, 101], q, layer=27)
     check_attention(small, near, 0, q, [0, 1], [101, 101], o, lse)
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("seqs,n,hkv", [(4, 3000, 16), (3, 10900, 8)])
+def test_large_prompts_are_small_ones(gpu, codes, seqs, n, hkv):
+    """Rows enough to be read, and codes to be written, past the caches: the bytes of the same prompts one by one."""
+    mc, ec = config(hkv, hkv, 1, -(-n // 16))
+    cache, one = (KV8Cache.allocate(seqs * ec.max_blocks_per_seq, mc, DTYPE[codes], gpu) for _ in range(2))
+    bt = torch.randperm(cache.num_blocks, device=gpu).to(torch.int32).view(seqs, -1)
+    g = torch.Generator(device=gpu).manual_seed(14)
+    lens = [n - 7 * s for s in range(seqs)]
+    k, v = (torch.randn(sum(lens), hkv, 128, device=gpu, generator=g).half() for _ in range(2))
+    assert k.numel() * 4 >= (128000000 if n > 10000 else 64000000)
+    kv8_store(k, v, cache, bt, mc, ec, state(mc, [], [], lens, range(seqs)), 0, validate=True)
+    at = 0
+    for s, m in enumerate(lens):
+        for lo in range(0, m, 4000):  # a prompt's blocks from another row of a table on
+            part = slice(at + lo, at + min(lo + 4000, m))
+            row = torch.zeros_like(bt[:1])
+            ids = bt[s, lo // 16:]
+            row[0, : len(ids)] = ids
+            kv8_store(k[part], v[part], one, row, mc, ec, state(mc, [], [], [part.stop - part.start], [0]), 0, validate=True)
+        at += m
+    for a, b in zip((cache.k, cache.v, cache.k_scales, cache.v_scales), (one.k, one.v, one.k_scales, one.v_scales)):
+        assert torch.equal(a, b)
+    out = [torch.empty_like(k) for _ in range(2)]
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=gpu)  # noqa: E731
+    kv8_load(*out, cache, bt, i32(range(seqs)), i32([sum(lens[:s]) for s in range(seqs)]), i32(lens), n, 0, validate=True)
+    for x, y in zip((k, v), out):  # half a step: 2^-4 of the value (below normal codes 2^-9 of the scale), or a scale
+        off = x.abs().float() / 16 + 2.0 ** -14 if codes == "e4m3" else x.abs().float().max() / 127
+        assert ((x.float() - y.float()).abs() <= off).all()
 
 
 # ---------------------------------------------------------------- streams, graphs, together
@@ -693,6 +758,44 @@ def test_graph_replays(gpu, codes):
             for n, w in zip(("q_out", "o", "lse", "k_out", "v_out"), want):
                 assert torch.equal(s[n], w), f"replay {seed}: {n}"
             assert torch.equal(s["cache"].k, eager["cache"].k) and torch.equal(s["cache"].v_scales, eager["cache"].v_scales)
+
+
+def test_a_plan_is_not_made_in_a_capture(gpu):
+    """Refused while capturing: the upload's source is host memory that a replay would find changed."""
+    a = _step_state("e4m3", gpu, 3, ctxs=(40,))
+    a["st"] = state(a["mc"], a["seq_ids"], a["lens"])
+    x = torch.zeros(4, device=gpu)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        x.add_(1)
+        with pytest.raises(RuntimeError, match="before the capture"):
+            kv8_paged_attention(a["q"], a["cache"], a["bt"], a["mc"], a["ec"], a["st"], 1, a["o"])
+    for _ in range(2):
+        g.replay()
+    torch.cuda.synchronize()
+    assert (x == 2).all() and a["st"].kv8_plan is None
+
+
+def test_two_streams_claim_pieces(gpu):
+    """More segments than slots, two calls of one plan at once: each claims by a counter of its own."""
+    ctxs = [5 * i % 301 for i in range(90)]
+    mc, ec, table, bt, cache, ids, lens, q = filled("int8", gpu, 16, 8, ctxs, 1, seed=15)
+    q2 = q.flip(0).contiguous()
+    want, _, st = attend(cache, bt, mc, ec, ids, lens, q)
+    want2, _, _ = attend(cache, bt, mc, ec, ids, lens, q2, st=st)
+    assert st.kv8_plan.claims
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(8):
+        for s, x in zip(streams, (q, q2)):
+            with torch.cuda.stream(s):
+                o = torch.empty_like(x)
+                kv8_paged_attention(x, cache, bt, mc, ec, st, 1, o)
+                outs.append(o)
+    torch.cuda.synchronize()
+    for i, o in enumerate(outs):
+        assert torch.equal(o, (want, want2)[i % 2])
 
 
 def test_two_streams_share_a_plan(gpu):
