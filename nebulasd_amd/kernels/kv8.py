@@ -110,11 +110,14 @@ class KV8Cache:
 
 def _call(device: int, name: str, *args) -> None:
     """``name`` on a device and its current stream."""
+    f = getattr(_lib.load(), name)
     if device == torch.cuda.current_device():
-        _lib.call(name, *args, stream_on(device))
+        rc = f(*args, stream_on(device))
     else:
         with torch.cuda.device(device):
-            _lib.call(name, *args, stream_on(device))
+            rc = f(*args, stream_on(device))
+    if rc:
+        _lib.check(rc, name)
 
 
 def _on(cache: KV8Cache, *tensors) -> None:
@@ -125,24 +128,23 @@ def _on(cache: KV8Cache, *tensors) -> None:
 
 
 # The checks of a call are a good part of a small one's time, so each begins with
-# one test of everything and names the fault only where that fails.
+# one test of everything, over as few of a tensor's attributes as tell it (each is
+# a tenth of a microsecond), and names the fault only where that fails.
 _F16, _I32 = torch.float16, torch.int32
 
 
-def _packed(cache: KV8Cache, t: torch.Tensor, name: str, heads: int, rows: int = -1) -> None:
-    """t: contiguous fp16 [rows, heads, 128] (any rows: -1) on the cache's device."""
-    shape = t.shape
-    if t.dtype is _F16 and t.is_contiguous() and t.get_device() == cache.device and len(shape) == 3 and \
-            shape[1] == heads and shape[2] == HEAD_DIM and (rows < 0 or shape[0] == rows):
+def _packed(cache: KV8Cache, t: torch.Tensor, name: str, heads: int, rows: int) -> None:
+    """t: contiguous fp16 [rows, heads, 128] on the cache's device."""
+    if t.dtype is _F16 and t.shape == (rows, heads, HEAD_DIM) and t.is_contiguous() and t.get_device() == cache.device:
         return
     _on(cache, t)
     require(t, _F16, name)
-    raise ValueError(f"{name} must be [{rows if rows >= 0 else 'rows'}, {heads}, {HEAD_DIM}], got {tuple(shape)}")
+    raise ValueError(f"{name} must be [{rows}, {heads}, {HEAD_DIM}], got {tuple(t.shape)}")
 
 
 def _index(cache: KV8Cache, t: torch.Tensor, name: str, n: int) -> None:
     """t: contiguous int32 of at least n entries on the cache's device."""
-    if t.dtype is _I32 and t.is_contiguous() and t.get_device() == cache.device and t.dim() == 1 and t.numel() >= n:
+    if t.dtype is _I32 and t.ndim == 1 and t.numel() >= n and t.is_contiguous() and t.get_device() == cache.device:
         return
     require(t, _I32, name)
     _on(cache, t)
@@ -151,16 +153,16 @@ def _index(cache: KV8Cache, t: torch.Tensor, name: str, n: int) -> None:
 
 def _rows(cache: KV8Cache, t: torch.Tensor, name: str, rows: int, heads: int) -> int:
     """t: fp16 [rows, heads, 128] of contiguous heads, aligned, on the cache's device; its row stride."""
-    stride, shape = t.stride(), t.shape
-    if t.dtype is _F16 and t.get_device() == cache.device and len(shape) == 3 and shape[0] == rows and \
-            shape[1] == heads and shape[2] == HEAD_DIM and stride[2] == 1 and stride[1] == HEAD_DIM and \
-            stride[0] % 8 == 0 and stride[0] >= heads * HEAD_DIM and t.data_ptr() % 16 == 0:
-        return stride[0]
+    if t.dtype is _F16 and t.shape == (rows, heads, HEAD_DIM) and t.get_device() == cache.device:
+        apart, per_head, per_dim = t.stride()
+        if per_dim == 1 and per_head == HEAD_DIM and apart % 8 == 0 and apart >= heads * HEAD_DIM and \
+                t.data_ptr() % 16 == 0:
+            return apart
     _on(cache, t)
     if t.dtype != _F16:
         raise TypeError(f"{name} must be torch.float16, got {t.dtype}")
     raise ValueError(f"{name} must be [{rows}, {heads}, {HEAD_DIM}] with contiguous heads (rows may be strided by a "
-                     f"multiple of 8 elements), 16-byte aligned; got {tuple(shape)}, strides {stride}")
+                     f"multiple of 8 elements), 16-byte aligned; got {tuple(t.shape)}, strides {t.stride()}")
 
 
 def _table(cache: KV8Cache, block_table: torch.Tensor, engine_config) -> tuple:
@@ -239,8 +241,7 @@ def kv8_qk_norm_rope_store(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ca
         raise ValueError("pass both q_norm and k_norm, or neither")
     if q_norm is not None:
         for t, n in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-            if t.dtype is not _F16 or t.dim() != 1 or t.numel() != HEAD_DIM or not t.is_contiguous() or \
-                    t.get_device() != cache.device:
+            if t.dtype is not _F16 or t.shape != (HEAD_DIM,) or not t.is_contiguous() or t.get_device() != cache.device:
                 _on(cache, t)
                 require(t, _F16, n)
                 raise ValueError(f"{n} must be [{HEAD_DIM}], got {tuple(t.shape)}")
@@ -273,20 +274,20 @@ def kv8_load(k: torch.Tensor, v: torch.Tensor, cache: KV8Cache, block_table: tor
     to row ``start_locs[s] + i`` of ``k`` and ``v`` [rows, Hkv, d]; other rows are left as they are.  The index tensors
     are int32, one entry a sequence.
     """
-    if block_table.dtype is not _I32 or not block_table.is_contiguous() or block_table.dim() != 2 or \
+    if block_table.dtype is not _I32 or block_table.ndim != 2 or not block_table.is_contiguous() or \
             block_table.get_device() != cache.device:
         _on(cache, block_table)
         require(block_table, _I32, "block_table")
         raise ValueError("block_table must be [rows, max_blocks_per_seq]")
-    rows = k.shape[0] if k.dim() else 0
-    _packed(cache, k, "k", cache.num_kv_heads)
+    rows = k.shape[0] if k.ndim else 0
+    _packed(cache, k, "k", cache.num_kv_heads, rows)
     _packed(cache, v, "v", cache.num_kv_heads, rows)
     n = seq_ids.numel()
     for t, name in ((seq_ids, "seq_ids"), (start_locs, "start_locs"), (seq_lens, "seq_lens"), (first, "first")):
-        if t is not None:
+        if t is not None and not (t.dtype is _I32 and t.shape == (n,) and t.is_contiguous() and
+                                  t.get_device() == cache.device):
             _index(cache, t, name, n)
-            if t.numel() != n:
-                raise ValueError(f"{name} must be [{n}], one entry a sequence")
+            raise ValueError(f"{name} must be [{n}], one entry a sequence")
     if n == 0 or rows == 0:
         return
     status = StatusWord(k.device) if validate else None
