@@ -38,6 +38,8 @@
 
 #include <stdint.h>
 
+#include "nsd_kv8.h"
+
 #ifdef __cplusplus
 extern "C" {
 #endif
@@ -89,6 +91,22 @@ int nsd_decoder_forward(nsd_decoder* dec, void* x, void* residual, int64_t n_row
                         int64_t attn_workspace_bytes, float softmax_scale, int probe_layer,
                         void* probe_q, void* probe_o, float* probe_lse, int32_t* status,
                         void* stream);
+
+/*
+ * nsd_decoder_forward over an 8-bit cache (nsd_kv8.h) of the model's layers and
+ * kv heads: the plan is nsd_kv8_plan_build's (or nsd_attn_plan_build's), the
+ * workspace nsd_kv8_attn_workspace bytes, its first 256 zero if the plan has
+ * claimed pieces.  The q/k/v projection's splits are summed by a launch of their
+ * own, before nsd_kv8_qk_norm_rope_store and nsd_kv8_paged_attention.
+ */
+int nsd_decoder_forward_kv8(nsd_decoder* dec, void* x, void* residual, int64_t n_rows,
+                            const nsd_kv8_cache* cache, const int32_t* block_table, int64_t bt_rows,
+                            int64_t bt_stride, const int32_t* seq_ids, const int32_t* seq_lens,
+                            const void* cos_cache, const void* sin_cache, int64_t n_positions,
+                            const int32_t* plan_host, const int32_t* plan_dev, void* attn_workspace,
+                            int64_t attn_workspace_bytes, float softmax_scale, int probe_layer,
+                            void* probe_q, void* probe_o, float* probe_lse, int32_t* status,
+                            void* stream);
 
 #ifdef __cplusplus
 }

@@ -115,6 +115,10 @@ SIGNATURES = {
         c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64,
                 c_void_p, c_void_p, c_void_p, c_void_p, c_int64, _I32P, c_void_p, c_void_p, c_int64, c_float,
                 c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "nsd_decoder_forward_kv8": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
+                c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_float, c_int, c_void_p, c_void_p,
+                c_void_p, c_void_p, c_void_p]),
     "nsd_lm_head_argmax": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
     "nsd_argmax_rows": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p]),
     "nsd_probe_stream_read": (c_int, [c_void_p, c_int64, c_void_p, c_int, c_void_p]),

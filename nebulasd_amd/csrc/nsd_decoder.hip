@@ -22,6 +22,7 @@
 
 #include "nsd_common.h"
 #include "nsd_decoder.h"
+#include "nsd_kv8.h"
 
 using namespace nsd;
 
@@ -36,13 +37,14 @@ struct nsd_decoder {
   std::vector<nsd_decoder_layer> w;
   // activations for max_rows rows
   float* part = nullptr;  // split partials of the projection in flight
+  void* qkv = nullptr;    // [rows, (hq + 2 hkv) d], over an 8-bit cache
   void* q = nullptr;      // [rows, hq, d]
   void* o = nullptr;      // [rows, hq d]
   void* oo = nullptr;     // [rows, hidden]
   void* h = nullptr;      // [rows, inter]
 
   ~nsd_decoder() {
-    for (void* p : {(void*)part, q, o, oo, h})
+    for (void* p : {(void*)part, qkv, q, o, oo, h})
       if (p) (void)hipFree(p);
   }
 };
@@ -89,6 +91,7 @@ extern "C" int nsd_decoder_create(int num_layers, int hidden, int inter, int num
   const int64_t part_elems = r * std::max({dec->s_qkv * qkv_w, (int64_t)dec->s_o * hidden,
                                            (int64_t)dec->s_down * hidden});
   hipError_t e = hipMalloc(reinterpret_cast<void**>(&dec->part), part_elems * 4);
+  if (e == hipSuccess) e = hipMalloc(&dec->qkv, r * qkv_w * 2);
   if (e == hipSuccess) e = hipMalloc(&dec->q, r * num_q_heads * head_dim * 2);
   if (e == hipSuccess) e = hipMalloc(&dec->o, r * num_q_heads * head_dim * 2);
   if (e == hipSuccess) e = hipMalloc(&dec->oo, r * hidden * 2);
@@ -106,35 +109,31 @@ extern "C" int nsd_decoder_destroy(nsd_decoder* dec) {
   return NSD_OK;
 }
 
-extern "C" int nsd_decoder_forward(nsd_decoder* dec, void* x, void* residual, int64_t n_rows, void* k_cache,
-                                   void* v_cache, int64_t num_blocks, const int32_t* block_table, int64_t bt_rows,
-                                   int64_t bt_stride, const int32_t* seq_ids, const int32_t* seq_lens,
-                                   const void* cos_cache, const void* sin_cache, int64_t n_positions,
-                                   const int32_t* plan_host, const int32_t* plan_dev, void* attn_workspace,
-                                   int64_t attn_workspace_bytes, float softmax_scale, int probe_layer,
-                                   void* probe_q, void* probe_o, float* probe_lse, int32_t* status, void* stream) {
-  if (dec == nullptr || x == nullptr || residual == nullptr)
-    return fail(NSD_ERR_INVALID, "decoder_forward: null pointer");
+namespace {
+// The layer that a check reads: -1, or its q, o and lse go here.
+struct Probe {
+  int layer;
+  void* q;
+  void* o;
+  float* lse;
+};
+
+// Every layer of a forward; attend(layer, its weights, whether it is probed)
+// takes the q/k/v projection's partials (dec->part) to the attention's output
+// (dec->o).
+template <typename Attend>
+int forward_layers(const char* who, nsd_decoder* dec, void* x, void* residual, int64_t n_rows, const Probe& probe,
+                   void* stream, Attend&& attend) {
+  if (dec == nullptr || x == nullptr || residual == nullptr) return fail(NSD_ERR_INVALID, "%s: null pointer", who);
   if (n_rows < 1 || n_rows > dec->max_rows)
-    return fail(NSD_ERR_INVALID, "decoder_forward: n_rows=%lld outside [1, %d]", (long long)n_rows, dec->max_rows);
+    return fail(NSD_ERR_INVALID, "%s: n_rows=%lld outside [1, %d]", who, (long long)n_rows, dec->max_rows);
   if (!aligned16(x) || !aligned16(residual))
-    return fail(NSD_ERR_UNSUPPORTED, "decoder_forward: x and residual must be 16-byte aligned");
-  if (probe_layer >= dec->layers || (probe_layer >= 0 && (!probe_q || !probe_o || !probe_lse)))
-    return fail(NSD_ERR_INVALID, "decoder_forward: probe layer %d of %d (or a null probe buffer)", probe_layer,
-                dec->layers);
+    return fail(NSD_ERR_UNSUPPORTED, "%s: x and residual must be 16-byte aligned", who);
+  if (probe.layer >= dec->layers || (probe.layer >= 0 && (!probe.q || !probe.o || !probe.lse)))
+    return fail(NSD_ERR_INVALID, "%s: probe layer %d of %d (or a null probe buffer)", who, probe.layer, dec->layers);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const int64_t H = dec->hidden, I = dec->inter, hq = dec->hq, hkv = dec->hkv, d = dec->d;
   const int64_t qkv_w = (hq + 2 * hkv) * d;
-  // The prologue runs inside the attention's launch (one launch instead of
-  // two, the same bits) where the plan keeps every sequence's rows in one
-  // verify group and a group's query rows per kv head fit one 16-row tile
-  // (decode batches: the Qwen3-0.6B draft layer 91.5 us against 93.8 us).
-  // Past one tile every piece builds its group's query rows from the q/k/v
-  // projection's five split partials, which gains nothing over the
-  // prologue's own launch (the Qwen3-8B verify layer, 16 x 5 rows: 154.9 us
-  // fused against 155.0 us), so verify batches keep two launches.  The
-  // probe layer keeps the two calls, whose q it copies out.
-  const bool fused = plan_host != nullptr && plan_host[kPlanRowsMax] <= 16 && plan_keeps_sequences_whole(plan_host);
   int rc = NSD_OK;
   for (int li = 0; li < dec->layers && rc == NSD_OK; ++li) {
     const nsd_decoder_layer& lw = dec->w[li];
@@ -144,28 +143,12 @@ extern "C" int nsd_decoder_forward(nsd_decoder* dec, void* x, void* residual, in
                  : nsd_fused_add_rmsnorm_partials(dec->part, dec->s_down, x, residual, lw.norm_in, n_rows, H,
                                                   dec->eps, stream);
     if (rc == NSD_OK) rc = nsd_linear_partials(x, lw.w_qkv, dec->part, n_rows, qkv_w, H, stream);
-    const bool one_launch = fused && li != probe_layer;
-    if (rc == NSD_OK && one_launch)
-      rc = nsd_paged_attention_fused(nullptr, 0, nullptr, 0, nullptr, 0, dec->part, dec->s_qkv, lw.q_norm, lw.k_norm,
-                                     dec->eps, cos_cache, sin_cache, n_positions, dec->o, nullptr, k_cache, v_cache,
-                                     num_blocks, dec->layers, li, (int)hq, (int)hkv, (int)d, 16, block_table, bt_rows,
-                                     bt_stride, plan_host, plan_dev, attn_workspace, attn_workspace_bytes,
-                                     softmax_scale, status, stream);
-    if (rc == NSD_OK && !one_launch)
-      rc = nsd_qk_norm_rope_store_partials(dec->part, dec->s_qkv, dec->q, lw.q_norm, lw.k_norm, dec->eps, cos_cache,
-                                           sin_cache, n_positions, k_cache, v_cache, block_table, bt_rows, bt_stride,
-                                           seq_ids, seq_lens, n_rows, num_blocks, dec->layers, li, (int)hq, (int)hkv,
-                                           (int)d, 16, status, stream);
-    if (rc == NSD_OK && !one_launch)
-      rc = nsd_paged_attention(dec->q, dec->o, li == probe_layer ? probe_lse : nullptr, k_cache, v_cache, num_blocks,
-                               dec->layers, li, (int)hq, (int)hkv, (int)d, 16, block_table, bt_rows, bt_stride,
-                               plan_host, plan_dev, attn_workspace, attn_workspace_bytes, softmax_scale, status,
-                               stream);
-    if (rc == NSD_OK && li == probe_layer) {
+    if (rc == NSD_OK) rc = attend(li, lw, li == probe.layer);
+    if (rc == NSD_OK && li == probe.layer) {
       const size_t bytes = (size_t)(n_rows * hq * d * 2);
-      hipError_t e = hipMemcpyAsync(probe_q, dec->q, bytes, hipMemcpyDeviceToDevice, s);
-      if (e == hipSuccess) e = hipMemcpyAsync(probe_o, dec->o, bytes, hipMemcpyDeviceToDevice, s);
-      if (e != hipSuccess) rc = fail(NSD_ERR_HIP, "decoder_forward: probe copy: %s", hipGetErrorString(e));
+      hipError_t e = hipMemcpyAsync(probe.q, dec->q, bytes, hipMemcpyDeviceToDevice, s);
+      if (e == hipSuccess) e = hipMemcpyAsync(probe.o, dec->o, bytes, hipMemcpyDeviceToDevice, s);
+      if (e != hipSuccess) rc = fail(NSD_ERR_HIP, "%s: probe copy: %s", who, hipGetErrorString(e));
     }
     if (rc == NSD_OK) rc = nsd_linear_partials(dec->o, lw.w_o, dec->part, n_rows, H, hq * d, stream);
     if (rc == NSD_OK)
@@ -176,4 +159,73 @@ extern "C" int nsd_decoder_forward(nsd_decoder* dec, void* x, void* residual, in
   }
   if (rc == NSD_OK) rc = nsd_sum_partials(dec->part, dec->s_down, x, n_rows, H, stream);
   return rc;
+}
+}  // namespace
+
+extern "C" int nsd_decoder_forward(nsd_decoder* dec, void* x, void* residual, int64_t n_rows, void* k_cache,
+                                   void* v_cache, int64_t num_blocks, const int32_t* block_table, int64_t bt_rows,
+                                   int64_t bt_stride, const int32_t* seq_ids, const int32_t* seq_lens,
+                                   const void* cos_cache, const void* sin_cache, int64_t n_positions,
+                                   const int32_t* plan_host, const int32_t* plan_dev, void* attn_workspace,
+                                   int64_t attn_workspace_bytes, float softmax_scale, int probe_layer,
+                                   void* probe_q, void* probe_o, float* probe_lse, int32_t* status, void* stream) {
+  // The prologue runs inside the attention's launch (one launch instead of
+  // two, the same bits) where the plan keeps every sequence's rows in one
+  // verify group and a group's query rows per kv head fit one 16-row tile
+  // (decode batches: the Qwen3-0.6B draft layer 91.5 us against 93.8 us).
+  // Past one tile every piece builds its group's query rows from the q/k/v
+  // projection's five split partials, which gains nothing over the
+  // prologue's own launch (the Qwen3-8B verify layer, 16 x 5 rows: 154.9 us
+  // fused against 155.0 us), so verify batches keep two launches.  The
+  // probe layer keeps the two calls, whose q it copies out.
+  const bool fused = plan_host != nullptr && plan_host[kPlanRowsMax] <= 16 && plan_keeps_sequences_whole(plan_host);
+  const Probe probe = {probe_layer, probe_q, probe_o, probe_lse};
+  return forward_layers("decoder_forward", dec, x, residual, n_rows, probe, stream,
+                        [&](int li, const nsd_decoder_layer& lw, bool probed) {
+    const int hq = dec->hq, hkv = dec->hkv, d = dec->d;
+    if (fused && !probed)
+      return nsd_paged_attention_fused(nullptr, 0, nullptr, 0, nullptr, 0, dec->part, dec->s_qkv, lw.q_norm, lw.k_norm,
+                                       dec->eps, cos_cache, sin_cache, n_positions, dec->o, nullptr, k_cache, v_cache,
+                                       num_blocks, dec->layers, li, hq, hkv, d, 16, block_table, bt_rows, bt_stride,
+                                       plan_host, plan_dev, attn_workspace, attn_workspace_bytes, softmax_scale,
+                                       status, stream);
+    const int rc = nsd_qk_norm_rope_store_partials(dec->part, dec->s_qkv, dec->q, lw.q_norm, lw.k_norm, dec->eps,
+                                                   cos_cache, sin_cache, n_positions, k_cache, v_cache, block_table,
+                                                   bt_rows, bt_stride, seq_ids, seq_lens, n_rows, num_blocks,
+                                                   dec->layers, li, hq, hkv, d, 16, status, stream);
+    if (rc != NSD_OK) return rc;
+    return nsd_paged_attention(dec->q, dec->o, probed ? probe_lse : nullptr, k_cache, v_cache, num_blocks, dec->layers,
+                               li, hq, hkv, d, 16, block_table, bt_rows, bt_stride, plan_host, plan_dev,
+                               attn_workspace, attn_workspace_bytes, softmax_scale, status, stream);
+  });
+}
+
+extern "C" int nsd_decoder_forward_kv8(nsd_decoder* dec, void* x, void* residual, int64_t n_rows,
+                                       const nsd_kv8_cache* cache, const int32_t* block_table, int64_t bt_rows,
+                                       int64_t bt_stride, const int32_t* seq_ids, const int32_t* seq_lens,
+                                       const void* cos_cache, const void* sin_cache, int64_t n_positions,
+                                       const int32_t* plan_host, const int32_t* plan_dev, void* attn_workspace,
+                                       int64_t attn_workspace_bytes, float softmax_scale, int probe_layer,
+                                       void* probe_q, void* probe_o, float* probe_lse, int32_t* status, void* stream) {
+  if (dec == nullptr || cache == nullptr) return fail(NSD_ERR_INVALID, "decoder_forward_kv8: null pointer");
+  if (cache->num_layers != dec->layers || cache->num_kv_heads != dec->hkv)
+    return fail(NSD_ERR_INVALID, "decoder_forward_kv8: a cache of %d layers and %d kv heads, a model of %d and %d",
+                (int)cache->num_layers, (int)cache->num_kv_heads, dec->layers, dec->hkv);
+  const Probe probe = {probe_layer, probe_q, probe_o, probe_lse};
+  return forward_layers("decoder_forward_kv8", dec, x, residual, n_rows, probe, stream,
+                        [&](int li, const nsd_decoder_layer& lw, bool probed) {
+    const int64_t hq = dec->hq, hkv = dec->hkv, d = dec->d, qkv_w = (hq + 2 * hkv) * d;
+    const char* q = static_cast<const char*>(dec->qkv);
+    const char *k = q + 2 * hq * d, *v = k + 2 * hkv * d;
+    int rc = nsd_sum_partials(dec->part, dec->s_qkv, dec->qkv, n_rows, qkv_w, stream);
+    if (rc == NSD_OK)
+      rc = nsd_kv8_qk_norm_rope_store(q, qkv_w, dec->q, k, qkv_w, v, qkv_w, lw.q_norm, lw.k_norm, dec->eps, cos_cache,
+                                      sin_cache, n_positions, cache, block_table, bt_rows, bt_stride, seq_ids,
+                                      seq_lens, n_rows, li, dec->hq, status, stream);
+    if (rc == NSD_OK)
+      rc = nsd_kv8_paged_attention(dec->q, dec->o, probed ? probe_lse : nullptr, cache, li, dec->hq, block_table,
+                                   bt_rows, bt_stride, plan_host, plan_dev, attn_workspace, attn_workspace_bytes,
+                                   softmax_scale, status, stream);
+    return rc;
+  });
 }

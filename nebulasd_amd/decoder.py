@@ -12,6 +12,7 @@ projection, fused add-RMSNorm, the fused
 up/gate + SiLU-and-mul, the down projection (the projections are this
 library's split-k GEMM, whose fp32 split partials the next kernel sums where
 it reads them).  The embedding lookup and the post-layer stay in Python.
+``DecoderStack.forward_kv8`` runs it over an 8-bit cache.
 """
 
 from __future__ import annotations
@@ -23,7 +24,8 @@ import torch
 
 from . import _lib
 from .kernels._util import cache_dims, check_block_table, ptr, require, require_cuda, stream_of
-from .plan import plan_for
+from .kernels.kv8 import KV8Cache
+from .plan import kv8_plan_for, plan_for
 
 __all__ = ["DecoderStack", "MAX_ROWS"]
 
@@ -97,36 +99,15 @@ class DecoderStack:
         ``probe_layer`` >= 0 returns that layer's attention (q, o, lse), else
         None."""
         mc = self.mc
-        if self._handle is None:
-            raise RuntimeError("the decoder stack was closed")
-        require_cuda(x, residual, k_cache, v_cache, block_table, cos_cache, sin_cache)
-        require(x, torch.float16, "x")
-        require(residual, torch.float16, "residual")
+        require_cuda(k_cache, v_cache)
         require(k_cache, torch.float16, "k_cache")
         require(v_cache, torch.float16, "v_cache")
-        check_block_table(block_table, engine_config)
-        rows = int(infer_state.num_decoding_seqs)
-        if infer_state.num_prefill_seqs:
-            raise ValueError("the decoder stack serves forwards of decode/verify rows only")
-        if rows < 1 or rows > self.max_rows:
-            raise ValueError(f"{rows} rows: the decoder stack serves 1..{self.max_rows}")
-        if tuple(x.shape) != (rows, mc.hidden_size) or residual.shape != x.shape:
-            raise ValueError(f"x and residual must be [{rows}, {mc.hidden_size}]")
+        rows = self._check(x, residual, block_table, engine_config, infer_state, cos_cache, sin_cache)
         n_blocks, n_layers, hkv, bs, d = cache_dims(k_cache)
         if v_cache.shape != k_cache.shape or n_layers != mc.num_layers or hkv != mc.num_kv_heads or bs != 16:
             raise ValueError("KV caches do not match the model ([blocks, layers, kv heads, 16, head_dim])")
-        if cos_cache.dim() != 2 or cos_cache.shape[1] != d // 2 or sin_cache.shape != cos_cache.shape:
-            raise ValueError("cos/sin caches must be [max_positions, head_dim/2]")
-        if getattr(infer_state, "ignore_kvcache", False):
-            raise ValueError("infer_state.ignore_kvcache is set but the forward has decode rows")
-        plan = plan_for(infer_state, mc, engine_config, block_table)
-        if plan.n_rows != rows:
-            raise ValueError(f"the forward's attention plan covers {plan.n_rows} rows, not {rows}")
-        probe = None
-        if probe_layer >= 0:
-            probe = (torch.empty((rows, mc.num_q_heads, d), dtype=torch.float16, device=x.device),
-                     torch.empty((rows, mc.num_q_heads, d), dtype=torch.float16, device=x.device),
-                     torch.empty((rows, mc.num_q_heads), dtype=torch.float32, device=x.device))
+        plan = self._plan(plan_for, rows, infer_state, engine_config, block_table)
+        probe = self._probe(rows, probe_layer, x.device)
         _lib.call("nsd_decoder_forward", self._handle, x.data_ptr(), residual.data_ptr(), rows,
                   k_cache.data_ptr(), v_cache.data_ptr(), n_blocks, block_table.data_ptr(), block_table.shape[0],
                   block_table.shape[1], infer_state.seq_ids.data_ptr(), infer_state.decoding_seq_lens.data_ptr(),
@@ -135,3 +116,58 @@ class DecoderStack:
                   float(infer_state.softmax_scale), int(probe_layer),
                   *(t.data_ptr() for t in probe) if probe else (None, None, None), None, stream_of(x))
         return probe
+
+    def forward_kv8(self, x: torch.Tensor, residual: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor,
+                    engine_config, infer_state, cos_cache: torch.Tensor, sin_cache: torch.Tensor,
+                    probe_layer: int = -1):
+        """``forward`` over an 8-bit cache, the same arguments and result."""
+        rows = self._check(x, residual, block_table, engine_config, infer_state, cos_cache, sin_cache)
+        if x.get_device() != cache.device:
+            raise ValueError(f"x is on {x.device}, the cache on cuda:{cache.device}")
+        plan = self._plan(kv8_plan_for, rows, infer_state, engine_config, block_table)
+        size, ws = plan.workspace_bytes, None
+        if size:  # the layers' in turn; the claim counter at its start is zero between them
+            ws = (x.new_zeros if plan.claims else x.new_empty)(size, dtype=torch.uint8)
+        probe = self._probe(rows, probe_layer, x.device)
+        _lib.call("nsd_decoder_forward_kv8", self._handle, x.data_ptr(), residual.data_ptr(), rows, cache._ref,
+                  block_table.data_ptr(), block_table.shape[0], block_table.shape[1], infer_state.seq_ids.data_ptr(),
+                  infer_state.decoding_seq_lens.data_ptr(), cos_cache.data_ptr(), sin_cache.data_ptr(),
+                  cos_cache.shape[0], plan.host_address, plan.dev.data_ptr(), ptr(ws), size,
+                  float(infer_state.softmax_scale), int(probe_layer),
+                  *(t.data_ptr() for t in probe) if probe else (None, None, None), None, stream_of(x))
+        return probe
+
+    def _check(self, x, residual, block_table, engine_config, infer_state, cos_cache, sin_cache) -> int:
+        """The rows of a forward whose arguments, but for the cache, the stack can take."""
+        mc = self.mc
+        if self._handle is None:
+            raise RuntimeError("the decoder stack was closed")
+        require_cuda(x, residual, block_table, cos_cache, sin_cache)
+        require(x, torch.float16, "x")
+        require(residual, torch.float16, "residual")
+        check_block_table(block_table, engine_config)
+        rows = int(infer_state.num_decoding_seqs)
+        if infer_state.num_prefill_seqs:
+            raise ValueError("the decoder stack serves forwards of decode/verify rows only")
+        if rows < 1 or rows > self.max_rows:
+            raise ValueError(f"{rows} rows: the decoder stack serves 1..{self.max_rows}")
+        if tuple(x.shape) != (rows, mc.hidden_size) or residual.shape != x.shape:
+            raise ValueError(f"x and residual must be [{rows}, {mc.hidden_size}]")
+        if cos_cache.dim() != 2 or cos_cache.shape[1] != mc.head_dim // 2 or sin_cache.shape != cos_cache.shape:
+            raise ValueError("cos/sin caches must be [max_positions, head_dim/2]")
+        if getattr(infer_state, "ignore_kvcache", False):
+            raise ValueError("infer_state.ignore_kvcache is set but the forward has decode rows")
+        return rows
+
+    def _plan(self, of, rows: int, infer_state, engine_config, block_table):
+        plan = of(infer_state, self.mc, engine_config, block_table)
+        if plan.n_rows != rows:
+            raise ValueError(f"the forward's attention plan covers {plan.n_rows} rows, not {rows}")
+        return plan
+
+    def _probe(self, rows: int, probe_layer: int, device):
+        """A probed layer's (q, o, lse), or None."""
+        if probe_layer < 0:
+            return None
+        q = torch.empty((rows, self.mc.num_q_heads, self.mc.head_dim), dtype=torch.float16, device=device)
+        return q, torch.empty_like(q), torch.empty(q.shape[:2], dtype=torch.float32, device=device)

@@ -13,6 +13,9 @@ this package's gfx950 kernels:
   prefill ``store_kvcache`` and the prompts' causal attention in one launch
   (``flash_attn_varlen_func``, the entry point of transformer_layer.py:7-32
   and :151-164);
+* over an 8-bit cache (``kv_codes``): ``kv8_store`` for prompts,
+  ``kv8_qk_norm_rope_store`` and ``kv8_paged_attention`` for decode / verify
+  rows;
 * the rest of the layer in the reference's order
   (transformer_layer.py:83-201, model.py:266-301): the residual buffer with
   ``fused_add_rmsnorm_inplace`` before attention and before the FFN, the
@@ -54,7 +57,8 @@ import torch.nn.functional as F
 
 from .config import QWEN3_0_6B, QWEN3_8B, EngineConfig, ModelConfig
 from .infer_state import build_infer_state, host_to_device, model_rope_cache
-from .kernels import (FUSED_UP_GATE_MAX_ROWS, flash_attn_varlen_func, fused_add_rmsnorm_inplace, paged_attention,
+from .kernels import (FUSED_UP_GATE_MAX_ROWS, KV8Cache, flash_attn_varlen_func, fused_add_rmsnorm_inplace,
+                      kv8_paged_attention, kv8_qk_norm_rope_store, kv8_store, paged_attention,
                       paged_attention_fused, post_layer_forward, qk_norm_rope_store, rmsnorm_inplace,
                       rotary_embedding_inplace, silu_and_mul_inplace, store_kvcache, up_gate_silu_and_mul)
 from .decoder import MAX_ROWS as DECODER_MAX_ROWS
@@ -71,9 +75,12 @@ class RandomQwen3:
     ``native``: decode/verify forwards of up to 128 rows run their layers in
     one call of the native decoder stack (``DecoderStack``), the same kernels
     and GEMMs enqueued from C++; otherwise (and always for prompts, or with
-    the forward-phase ranges on) the layers run from Python as below."""
+    the forward-phase ranges on) the layers run from Python as below.
+    ``kv_codes`` (``torch.float8_e4m3fn`` or ``torch.int8``): the cache holds
+    8 bits a value (``kv8``) instead of fp16 (``k_cache``, ``v_cache``)."""
 
-    def __init__(self, cfg: dict, seq_blocks: list, device, seed: int, std: float = 0.02, native: bool = True):
+    def __init__(self, cfg: dict, seq_blocks: list, device, seed: int, std: float = 0.02, native: bool = True,
+                 kv_codes: torch.dtype | None = None):
         self.mc = mc = ModelConfig(cfg)
         self.dev = dev = torch.device(device)
         g = torch.Generator(device=dev).manual_seed(seed)
@@ -106,9 +113,13 @@ class RandomQwen3:
             pos += nb
         self.block_table = bt.to(dev)
         self.ec = EngineConfig(block_size=16, max_blocks_per_seq=width, num_gpu_blocks=n_blocks)
-        shape = (n_blocks, mc.num_layers, hkv, 16, d)
-        self.k_cache = torch.zeros(shape, dtype=torch.float16, device=dev)
-        self.v_cache = torch.zeros(shape, dtype=torch.float16, device=dev)
+        self.kv8 = None
+        if kv_codes is not None:
+            self.kv8 = KV8Cache.allocate(n_blocks, mc, kv_codes, dev)
+        else:
+            shape = (n_blocks, mc.num_layers, hkv, 16, d)
+            self.k_cache = torch.zeros(shape, dtype=torch.float16, device=dev)
+            self.v_cache = torch.zeros(shape, dtype=torch.float16, device=dev)
         self.cos, self.sin = model_rope_cache(mc, width * 16 + 1, dev)
         self.check = None  # (layer, callback) of a sampled attention check
         self.native = native
@@ -173,7 +184,10 @@ class RandomQwen3:
             rotary_embedding_inplace(q, k, st)
             if not st.ignore_kvcache:
                 with forward_phase_range(f"layer_{li}_store_kvcache"):
-                    store_kvcache(k, v, self.k_cache, self.v_cache, self.block_table, mc, self.ec, st, li)
+                    if self.kv8 is not None:
+                        kv8_store(k, v, self.kv8, self.block_table, mc, self.ec, st, li)
+                    else:
+                        store_kvcache(k, v, self.k_cache, self.v_cache, self.block_table, mc, self.ec, st, li)
             return flash_attn_varlen_func(q, k, v, st.prefill_seq_start_locs_with_end,
                                           st.prefill_seq_start_locs_with_end, st.max_prefill_len,
                                           st.max_prefill_len, softmax_scale=st.softmax_scale)
@@ -194,28 +208,29 @@ class RandomQwen3:
 
         def attention(li, lw, q_rows, k, v):
             checked = self.check is not None and self.check[0] == li
-            if not checked and not PHASE_RANGES and plan_for(st, mc, self.ec, self.block_table).keeps_sequences_whole:
+            if self.kv8 is None and not checked and not PHASE_RANGES and \
+                    plan_for(st, mc, self.ec, self.block_table).keeps_sequences_whole:
                 # the prologue inside the attention's launch: the two calls' results, one launch
                 o = torch.empty(q_rows.shape, dtype=q_rows.dtype, device=dev)
                 paged_attention_fused(q_rows, k, v, self.k_cache, self.v_cache, self.block_table, lw["q_norm"],
                                       lw["k_norm"], mc, self.ec, st, li, self.cos, self.sin, o)
                 return o
             q = torch.empty(q_rows.shape, dtype=q_rows.dtype, device=dev)  # the prologue's contiguous q
+            cache = (self.kv8,) if self.kv8 is not None else (self.k_cache, self.v_cache)
+            store, attend = (kv8_qk_norm_rope_store, kv8_paged_attention) if self.kv8 is not None else \
+                (qk_norm_rope_store, paged_attention)
             with forward_phase_range(f"layer_{li}_store_kvcache"):  # QK-norm + RoPE + store, one launch
-                qk_norm_rope_store(q_rows, k, v, self.k_cache, self.v_cache, self.block_table,
-                                   lw["q_norm"], lw["k_norm"], mc, self.ec, st, li, self.cos, self.sin,
-                                   q_out=q)
+                store(q_rows, k, v, *cache, self.block_table, lw["q_norm"], lw["k_norm"], mc, self.ec, st, li, self.cos,
+                      self.sin, q_out=q)
             o = torch.empty_like(q)
             if self.check is not None and self.check[0] == li:
                 lse = torch.empty((q.shape[0], hq), dtype=torch.float32, device=dev)
-                paged_attention(q, self.k_cache, self.v_cache, self.block_table, mc, self.ec, st,
-                                li, o, lse)
+                attend(q, *cache, self.block_table, mc, self.ec, st, li, o, lse)
                 self.check[1](self, li, q, o, lse, seq_ids, seq_lens)
                 self.check = None
             else:
                 with forward_phase_range(f"layer_{li}_paged_attention"):
-                    paged_attention(q, self.k_cache, self.v_cache, self.block_table, mc, self.ec, st,
-                                    li, o)
+                    attend(q, *cache, self.block_table, mc, self.ec, st, li, o)
             return o
         return self._forward(st, tokens, attention, as_tensor)
 
@@ -230,8 +245,11 @@ class RandomQwen3:
         x = self.embed[self._token_tensor(tokens)]
         res = torch.zeros_like(x)
         probe_layer = self.check[0] if self.check is not None else -1
-        probe = stack.forward(x, res, self.k_cache, self.v_cache, self.block_table, self.ec, st, self.cos,
-                                   self.sin, probe_layer)
+        where = (self.block_table, self.ec, st, self.cos, self.sin, probe_layer)
+        if self.kv8 is not None:
+            probe = stack.forward_kv8(x, res, self.kv8, *where)
+        else:
+            probe = stack.forward(x, res, self.k_cache, self.v_cache, *where)
         if probe is not None:
             q, o, lse = probe
             self.check[1](self, probe_layer, q, o, lse, seq_ids, seq_lens)
@@ -250,7 +268,8 @@ def _sync(dev: torch.device) -> None:
 def run(n_requests=512, prompt_lo=128, prompt_hi=1024, new_tokens=128, draft_batch=64,
         target_batch=16, depth=4, seed=0, check_every=0, make_check=None, device="cuda:0",
         draft_cfg=QWEN3_0_6B, target_cfg=QWEN3_8B, share_weights=False, return_outputs=False,
-        log=None, native=True, sync_each_forward=False, overlap=True, target_streams=2) -> dict:
+        log=None, native=True, sync_each_forward=False, overlap=True, target_streams=2,
+        kv_codes=None) -> dict:
     """The speculative loop over `n_requests` synthetic requests; returns a summary.
 
     With ``check_every`` > 0, every check_every-th forward calls
@@ -279,6 +298,8 @@ def run(n_requests=512, prompt_lo=128, prompt_hi=1024, new_tokens=128, draft_bat
     over ``target_streams`` streams (each with its own decoder-stack lane),
     so verifies of different batches run side by side too.  Results are the
     same either way.
+
+    ``kv_codes``: both models' caches in 8 bits (``RandomQwen3``).
     """
     dev = torch.device(device)
     rng = np.random.default_rng(seed)
@@ -287,11 +308,12 @@ def run(n_requests=512, prompt_lo=128, prompt_hi=1024, new_tokens=128, draft_bat
     prompts = [rng.integers(0, vocab, n).tolist() for n in plens]
     # room for the prompt, the output and one proposal beyond it
     blocks = [math.ceil((p + new_tokens + depth + 2) / 16) for p in plens]
-    target = RandomQwen3(target_cfg, blocks, dev, seed + 1, native=native)
+    how = {"native": native} if kv_codes is None else {"native": native, "kv_codes": kv_codes}
+    target = RandomQwen3(target_cfg, blocks, dev, seed + 1, **how)
     if share_weights:
-        draft = RandomQwen3(target_cfg, blocks, dev, seed + 1, native=native)
+        draft = RandomQwen3(target_cfg, blocks, dev, seed + 1, **how)
     else:
-        draft = RandomQwen3(draft_cfg, blocks, dev, seed + 2, native=native)
+        draft = RandomQwen3(draft_cfg, blocks, dev, seed + 2, **how)
     n_checks = 0
     t0 = time.perf_counter()
 
@@ -496,11 +518,13 @@ def main():
                    help="draft and target forwards on one stream (no draft/verify overlap)")
     p.add_argument("--target-streams", type=int, default=2,
                    help="streams a draft group's target batches alternate over")
+    p.add_argument("--kv", choices=["fp16", "e4m3", "int8"], default="fp16", help="what the KV caches hold")
     a = p.parse_args()
     res = run(a.requests, a.prompt_lo, a.prompt_hi, a.new_tokens, a.draft_batch, a.target_batch,
               a.depth, a.seed, share_weights=a.share_weights, log=lambda m: print(m, flush=True),
               native=not a.python_layers, overlap=not a.no_overlap,
-              target_streams=a.target_streams)
+              target_streams=a.target_streams,
+              kv_codes={"fp16": None, "e4m3": torch.float8_e4m3fn, "int8": torch.int8}[a.kv])
     print(json.dumps(res), flush=True)
 
 
