@@ -96,8 +96,8 @@ int nsd_decoder_forward(nsd_decoder* dec, void* x, void* residual, int64_t n_row
  * nsd_decoder_forward over an 8-bit cache (nsd_kv8.h) of the model's layers and
  * kv heads: the plan is nsd_kv8_plan_build's (or nsd_attn_plan_build's), the
  * workspace nsd_kv8_attn_workspace bytes, its first 256 zero if the plan has
- * claimed pieces.  The q/k/v projection's splits are summed by a launch of their
- * own, before nsd_kv8_qk_norm_rope_store and nsd_kv8_paged_attention.
+ * claimed pieces.  Prologue and attention are two launches
+ * (nsd_kv8_qk_norm_rope_store_partials, nsd_kv8_paged_attention).
  */
 int nsd_decoder_forward_kv8(nsd_decoder* dec, void* x, void* residual, int64_t n_rows,
                             const nsd_kv8_cache* cache, const int32_t* block_table, int64_t bt_rows,

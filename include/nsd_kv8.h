@@ -106,6 +106,18 @@ int nsd_kv8_qk_norm_rope_store(const void* q, int64_t q_row_stride, void* q_out,
                                int64_t n_rows, int layer, int num_q_heads, int32_t* status, void* stream);
 
 /*
+ * nsd_qk_norm_rope_store_partials into an 8-bit cache: q, k and v as the split
+ * partials [splits][n_rows][(Hq + 2 Hkv) 128] (1 to 8 splits) of their one
+ * projection, each value their sum rounded once to fp16.
+ */
+int nsd_kv8_qk_norm_rope_store_partials(const float* partials, int splits, void* q_out, const void* q_norm_w,
+                                        const void* k_norm_w, float eps, const void* cos_cache,
+                                        const void* sin_cache, int64_t n_positions, const nsd_kv8_cache* cache,
+                                        const int32_t* block_table, int64_t bt_rows, int64_t bt_stride,
+                                        const int32_t* seq_ids, const int32_t* seq_lens, int64_t n_rows, int layer,
+                                        int num_q_heads, int32_t* status, void* stream);
+
+/*
  * The values of cached tokens: token first[s] + i of block_table[seq_ids[s]]
  * (i < lens[s] <= max_len; first NULL: 0) to row start_locs[s] + i of k, v fp16
  * [n_tokens, Hkv, 128].  Other rows are left as they are.

@@ -158,6 +158,9 @@ SIGNATURES = {
         c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_float,
                 c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int,
                 c_int, c_void_p, c_void_p]),
+    "nsd_kv8_qk_norm_rope_store_partials": (
+        c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_int64, c_void_p, c_void_p,
+                c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p]),
     "nsd_kv8_load": (
         c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
                 c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p]),

@@ -37,14 +37,13 @@ struct nsd_decoder {
   std::vector<nsd_decoder_layer> w;
   // activations for max_rows rows
   float* part = nullptr;  // split partials of the projection in flight
-  void* qkv = nullptr;    // [rows, (hq + 2 hkv) d], over an 8-bit cache
   void* q = nullptr;      // [rows, hq, d]
   void* o = nullptr;      // [rows, hq d]
   void* oo = nullptr;     // [rows, hidden]
   void* h = nullptr;      // [rows, inter]
 
   ~nsd_decoder() {
-    for (void* p : {(void*)part, qkv, q, o, oo, h})
+    for (void* p : {(void*)part, q, o, oo, h})
       if (p) (void)hipFree(p);
   }
 };
@@ -91,7 +90,6 @@ extern "C" int nsd_decoder_create(int num_layers, int hidden, int inter, int num
   const int64_t part_elems = r * std::max({dec->s_qkv * qkv_w, (int64_t)dec->s_o * hidden,
                                            (int64_t)dec->s_down * hidden});
   hipError_t e = hipMalloc(reinterpret_cast<void**>(&dec->part), part_elems * 4);
-  if (e == hipSuccess) e = hipMalloc(&dec->qkv, r * qkv_w * 2);
   if (e == hipSuccess) e = hipMalloc(&dec->q, r * num_q_heads * head_dim * 2);
   if (e == hipSuccess) e = hipMalloc(&dec->o, r * num_q_heads * head_dim * 2);
   if (e == hipSuccess) e = hipMalloc(&dec->oo, r * hidden * 2);
@@ -214,14 +212,9 @@ extern "C" int nsd_decoder_forward_kv8(nsd_decoder* dec, void* x, void* residual
   const Probe probe = {probe_layer, probe_q, probe_o, probe_lse};
   return forward_layers("decoder_forward_kv8", dec, x, residual, n_rows, probe, stream,
                         [&](int li, const nsd_decoder_layer& lw, bool probed) {
-    const int64_t hq = dec->hq, hkv = dec->hkv, d = dec->d, qkv_w = (hq + 2 * hkv) * d;
-    const char* q = static_cast<const char*>(dec->qkv);
-    const char *k = q + 2 * hq * d, *v = k + 2 * hkv * d;
-    int rc = nsd_sum_partials(dec->part, dec->s_qkv, dec->qkv, n_rows, qkv_w, stream);
-    if (rc == NSD_OK)
-      rc = nsd_kv8_qk_norm_rope_store(q, qkv_w, dec->q, k, qkv_w, v, qkv_w, lw.q_norm, lw.k_norm, dec->eps, cos_cache,
-                                      sin_cache, n_positions, cache, block_table, bt_rows, bt_stride, seq_ids,
-                                      seq_lens, n_rows, li, dec->hq, status, stream);
+    int rc = nsd_kv8_qk_norm_rope_store_partials(dec->part, dec->s_qkv, dec->q, lw.q_norm, lw.k_norm, dec->eps,
+                                                 cos_cache, sin_cache, n_positions, cache, block_table, bt_rows,
+                                                 bt_stride, seq_ids, seq_lens, n_rows, li, dec->hq, status, stream);
     if (rc == NSD_OK)
       rc = nsd_kv8_paged_attention(dec->q, dec->o, probed ? probe_lse : nullptr, cache, li, dec->hq, block_table,
                                    bt_rows, bt_stride, plan_host, plan_dev, attn_workspace, attn_workspace_bytes,

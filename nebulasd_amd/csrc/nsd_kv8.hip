@@ -129,7 +129,9 @@ struct AppendArgs {
   int n_rows;
   int kv_groups;  // workgroups of a row's units
   int32_t* status;
-  // the prologue's
+  // the prologue's; part: q, k and v are a projection's split partials, fp32
+  // [splits, n_rows, (hq + 2 Hkv) 128], and q_rs is its width
+  const float* part;
   const f16* q;
   int64_t q_rs;
   f16* q_out;
@@ -141,6 +143,32 @@ struct AppendArgs {
   int64_t n_pos;
   int hq;
 };
+
+// Eight values of a row: fp16, or the sum of S split partials `per_split`
+// elements apart, in their order, as the projection's fp16 output (the rounding
+// is the output's).
+template <int S>
+__device__ inline f16x8 eight_of(const f16* rows, const float* part, int64_t per_split) {
+  if constexpr (S == 0) {
+    return *reinterpret_cast<const f16x8*>(rows);
+  } else {
+    f32x4 lo[S], hi[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      lo[s] = *reinterpret_cast<const f32x4*>(part + s * per_split);
+      hi[s] = *reinterpret_cast<const f32x4*>(part + s * per_split + 4);
+    }
+    f16x8 h;
+#pragma unroll
+    for (int s = 1; s < S; ++s) {
+      lo[0] += lo[s];
+      hi[0] += hi[s];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = (f16)(e < 4 ? lo[0][e % 4] : hi[0][e % 4]);
+    return h;
+  }
+}
 
 // Where row r goes: its block, or -1 and the flag that says why not.  In two
 // parts, both without a branch, so that a caller has several rows' loads in
@@ -213,8 +241,13 @@ __device__ inline void norm_rope(f16x8& lo, f16x8& hi, const f16* w, float eps, 
 // Bound by latency, one trip to memory after another: row numbers, the block
 // table, the tile and then the rows.  64 rows of 16 + 2 x 8 heads with the prologue
 // 4.4 us, 16 x 5 of 32 + 2 x 8 5.6.
-template <int T, bool PRO>
+//
+// S: 0 for fp16 rows, else the split partials of the projection that makes them
+// (a decoder layer's: their sum in a launch of its own costs 3 us more).
+template <int T, bool PRO, int S>
 __global__ __launch_bounds__(kThreads) void kv8_append_kernel(Cache c, AppendArgs a) {
+  static_assert(PRO || S == 0, "only the prologue reads partials");
+  const int64_t per_split = a.n_rows * a.q_rs;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kv_wgs = a.n_rows * a.kv_groups;
@@ -227,8 +260,9 @@ __global__ __launch_bounds__(kThreads) void kv8_append_kernel(Cache c, AppendArg
     const int64_t pos = (int64_t)a.seq_lens[r] - 1;
     const bool in = pos >= 0 && pos < a.n_pos;
     if (any && !in && cc == 0) flag_status(a.status, NSD_STATUS_BAD_POSITION);
-    const f16* src = a.q + r * a.q_rs + (int64_t)h * D + 8 * cc;
-    f16x8 lo = *reinterpret_cast<const f16x8*>(src), hi = *reinterpret_cast<const f16x8*>(src + D / 2);
+    const int64_t from = r * a.q_rs + (int64_t)h * D + 8 * cc;
+    f16x8 lo = eight_of<S>(a.q + from, a.part + from, per_split);
+    f16x8 hi = eight_of<S>(a.q + from + D / 2, a.part + from + D / 2, per_split);
     norm_rope(lo, hi, a.qw, a.eps, a.cos_c, a.sin_c, in ? pos : 0, cc);  // a head's eight lanes agree on any and in
     if (any && in) {
       f16* dst = a.q_out + at * D + 8 * cc;
@@ -289,7 +323,8 @@ __global__ __launch_bounds__(kThreads) void kv8_append_kernel(Cache c, AppendArg
       if (fresh >> (8 * j) & 0xff) {  // a new row among these eight slots
         const int64_t row = key ? (int64_t)(key >> 32) - 1 : r;
         const f16* src = a.k + row * a.k_rs + (int64_t)head * D + 8 * cc;
-        f16x8 lo = *reinterpret_cast<const f16x8*>(src), hi = *reinterpret_cast<const f16x8*>(src + D / 2);
+        const float* part = a.part + row * a.q_rs + (int64_t)(a.hq + head) * D + 8 * cc;
+        f16x8 lo = eight_of<S>(src, part, per_split), hi = eight_of<S>(src + D / 2, part + D / 2, per_split);
         if constexpr (PRO)
           norm_rope(lo, hi, a.kw, a.eps, a.cos_c, a.sin_c, key ? (int64_t)(key & 0xffffffffu) : 0, cc);
         if (key) {
@@ -319,7 +354,10 @@ __global__ __launch_bounds__(kThreads) void kv8_append_kernel(Cache c, AppendArg
     for (int j = 0; j < 4; ++j) {
       const unsigned long long key = s_slot[t0 + j];
       h[j] = f16x8{};
-      if (key) h[j] = *reinterpret_cast<const f16x8*>(a.v + ((int64_t)(key >> 32) - 1) * a.v_rs + (int64_t)head * D + 8 * i);
+      const int64_t row = (int64_t)(key >> 32) - 1;
+      if (key)
+        h[j] = eight_of<S>(a.v + row * a.v_rs + (int64_t)head * D + 8 * i,
+                           a.part + row * a.q_rs + (int64_t)(a.hq + c.hkv + head) * D + 8 * i, per_split);
       else if (old >> (t0 + j) & 1) h[j] = kv8_values<T>(u32x2{a0[j], a1[j]}, power);
     }
     const Scale s = tile_scale<T>(h, a.status);
@@ -514,7 +552,8 @@ int check_append(const char* who, const AppendArgs& a, const nsd_kv8_cache* cach
   if (rc) return rc;
   if (n_rows < 0 || a.bt_rows <= 0 || a.bt_stride <= 0) return fail(NSD_ERR_INVALID, "%s: bad sizes", who);
   if (n_rows == 0) return NSD_OK;
-  if (!a.k || !a.v || !a.bt || !a.seq_ids || !a.seq_lens) return fail(NSD_ERR_INVALID, "%s: null pointer", who);
+  if (!a.bt || !a.seq_ids || !a.seq_lens || (!a.part && (!a.k || !a.v)))
+    return fail(NSD_ERR_INVALID, "%s: null pointer", who);
   if (!aligned16(a.k) || !aligned16(a.v)) return fail(NSD_ERR_INVALID, "%s: k and v must be 16-byte aligned", who);
   if (n_rows > (1 << 20)) return fail(NSD_ERR_UNSUPPORTED, "%s: n_rows=%lld (at most 2^20)", who, (long long)n_rows);
   return NSD_OK;
@@ -545,34 +584,25 @@ extern "C" int nsd_kv8_store(const void* k, const void* v, const nsd_kv8_cache* 
   const int64_t grid = n_rows * a.kv_groups;
   if (grid > kMaxGrid) return fail(NSD_ERR_UNSUPPORTED, "kv8_store: grid too large");
   with_codes(cache, [&](auto t) {
-    hipLaunchKernelGGL((kv8_append_kernel<decltype(t)::value, false>), dim3((unsigned)grid), dim3(kThreads), 0,
+    hipLaunchKernelGGL((kv8_append_kernel<decltype(t)::value, false, 0>), dim3((unsigned)grid), dim3(kThreads), 0,
                        as_stream(stream), cache_of(cache, layer), a);
   });
   return launch_status("kv8_store");
 }
 
-extern "C" int nsd_kv8_qk_norm_rope_store(const void* q, int64_t q_row_stride, void* q_out, const void* k,
-                                          int64_t k_row_stride, const void* v, int64_t v_row_stride,
-                                          const void* q_norm_w, const void* k_norm_w, float eps,
-                                          const void* cos_cache, const void* sin_cache, int64_t n_positions,
-                                          const nsd_kv8_cache* cache, const int32_t* block_table, int64_t bt_rows,
-                                          int64_t bt_stride, const int32_t* seq_ids, const int32_t* seq_lens,
-                                          int64_t n_rows, int layer, int num_q_heads, int32_t* status,
-                                          void* stream) {
-  const char* who = "kv8_qk_norm_rope_store";
-  AppendArgs a{};
-  a.k = static_cast<const f16*>(k);
-  a.v = static_cast<const f16*>(v);
-  a.k_rs = k_row_stride;
-  a.v_rs = v_row_stride;
+// The prologue over fp16 rows (splits 0) or partials; `a` has what the entries
+// differ in: the rows, or `part`, and q_rs.
+static int prologue(const char* who, AppendArgs a, int splits, void* q_out, const void* q_norm_w, const void* k_norm_w,
+                    float eps, const void* cos_cache, const void* sin_cache, int64_t n_positions,
+                    const nsd_kv8_cache* cache, const int32_t* block_table, int64_t bt_rows, int64_t bt_stride,
+                    const int32_t* seq_ids, const int32_t* seq_lens, int64_t n_rows, int layer, int num_q_heads,
+                    int32_t* status, void* stream) {
   a.bt = block_table;
   a.bt_rows = bt_rows;
   a.bt_stride = bt_stride;
   a.seq_ids = seq_ids;
   a.seq_lens = seq_lens;
   a.status = status;
-  a.q = static_cast<const f16*>(q);
-  a.q_rs = q_row_stride;
   a.q_out = static_cast<f16*>(q_out);
   a.qw = static_cast<const f16*>(q_norm_w);
   a.kw = static_cast<const f16*>(k_norm_w);
@@ -587,24 +617,68 @@ extern "C" int nsd_kv8_qk_norm_rope_store(const void* q, int64_t q_row_stride, v
   if ((q_norm_w == nullptr) != (k_norm_w == nullptr))
     return fail(NSD_ERR_INVALID, "%s: pass both norm weights or neither", who);
   if (n_rows == 0) return NSD_OK;
-  if (!q || !q_out || !cos_cache || !sin_cache) return fail(NSD_ERR_INVALID, "%s: null pointer", who);
-  for (const void* p : {q, (const void*)q_out, cos_cache, sin_cache, q_norm_w, k_norm_w})
+  if ((!a.q && !a.part) || !q_out || !cos_cache || !sin_cache) return fail(NSD_ERR_INVALID, "%s: null pointer", who);
+  for (const void* p : {(const void*)a.q, (const void*)a.part, (const void*)q_out, cos_cache, sin_cache, q_norm_w, k_norm_w})
     if (!aligned16(p)) return fail(NSD_ERR_INVALID, "%s: rows, tables and norm weights must be 16-byte aligned", who);
-  const int64_t hkv = cache->num_kv_heads;
-  if (q_row_stride < (int64_t)num_q_heads * D || k_row_stride < hkv * D || v_row_stride < hkv * D ||
-      (q_row_stride | k_row_stride | v_row_stride) & 7)
-    return fail(NSD_ERR_INVALID, "%s: row strides must be multiples of 8 that cover the heads", who);
-  if (q == q_out && q_row_stride != (int64_t)num_q_heads * D)
-    return fail(NSD_ERR_INVALID, "%s: q in place has to be contiguous", who);
   a.n_rows = (int)n_rows;
   a.kv_groups = unit_groups(cache);
   const int64_t grid = n_rows * a.kv_groups + (n_rows * num_q_heads + kThreads / 8 - 1) / (kThreads / 8);
   if (grid > kMaxGrid) return fail(NSD_ERR_UNSUPPORTED, "%s: grid too large", who);
   with_codes(cache, [&](auto t) {
-    hipLaunchKernelGGL((kv8_append_kernel<decltype(t)::value, true>), dim3((unsigned)grid), dim3(kThreads), 0,
-                       as_stream(stream), cache_of(cache, layer), a);
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(kThreads), 0, as_stream(stream), cache_of(cache, layer), a);
+    };
+    constexpr int T = decltype(t)::value;
+    if (splits == 0) go(kv8_append_kernel<T, true, 0>);
+    else with_splits(splits, [&](auto count) { go(kv8_append_kernel<T, true, decltype(count)::value>); });
   });
   return launch_status(who);
+}
+
+extern "C" int nsd_kv8_qk_norm_rope_store(const void* q, int64_t q_row_stride, void* q_out, const void* k,
+                                          int64_t k_row_stride, const void* v, int64_t v_row_stride,
+                                          const void* q_norm_w, const void* k_norm_w, float eps,
+                                          const void* cos_cache, const void* sin_cache, int64_t n_positions,
+                                          const nsd_kv8_cache* cache, const int32_t* block_table, int64_t bt_rows,
+                                          int64_t bt_stride, const int32_t* seq_ids, const int32_t* seq_lens,
+                                          int64_t n_rows, int layer, int num_q_heads, int32_t* status,
+                                          void* stream) {
+  const char* who = "kv8_qk_norm_rope_store";
+  if (cache != nullptr) {
+    const int64_t hkv = cache->num_kv_heads;
+    if (q_row_stride < (int64_t)num_q_heads * D || k_row_stride < hkv * D || v_row_stride < hkv * D ||
+        (q_row_stride | k_row_stride | v_row_stride) & 7)
+      return fail(NSD_ERR_INVALID, "%s: row strides must be multiples of 8 that cover the heads", who);
+  }
+  if (q != nullptr && q == q_out && q_row_stride != (int64_t)num_q_heads * D)
+    return fail(NSD_ERR_INVALID, "%s: q in place has to be contiguous", who);
+  AppendArgs a{};
+  a.k = static_cast<const f16*>(k);
+  a.v = static_cast<const f16*>(v);
+  a.k_rs = k_row_stride;
+  a.v_rs = v_row_stride;
+  a.q = static_cast<const f16*>(q);
+  a.q_rs = q_row_stride;
+  return prologue(who, a, 0, q_out, q_norm_w, k_norm_w, eps, cos_cache, sin_cache, n_positions, cache, block_table,
+                  bt_rows, bt_stride, seq_ids, seq_lens, n_rows, layer, num_q_heads, status, stream);
+}
+
+extern "C" int nsd_kv8_qk_norm_rope_store_partials(const float* partials, int splits, void* q_out,
+                                                   const void* q_norm_w, const void* k_norm_w, float eps,
+                                                   const void* cos_cache, const void* sin_cache, int64_t n_positions,
+                                                   const nsd_kv8_cache* cache, const int32_t* block_table,
+                                                   int64_t bt_rows, int64_t bt_stride, const int32_t* seq_ids,
+                                                   const int32_t* seq_lens, int64_t n_rows, int layer,
+                                                   int num_q_heads, int32_t* status, void* stream) {
+  const char* who = "kv8_qk_norm_rope_store_partials";
+  if (cache == nullptr) return fail(NSD_ERR_INVALID, "%s: null cache", who);
+  if (splits < 1 || splits > 8) return fail(NSD_ERR_INVALID, "%s: %d splits (1..8)", who, splits);
+  if (n_rows > 0 && partials == nullptr) return fail(NSD_ERR_INVALID, "%s: null pointer", who);
+  AppendArgs a{};
+  a.part = partials;
+  a.q_rs = ((int64_t)num_q_heads + 2 * (int64_t)cache->num_kv_heads) * D;
+  return prologue(who, a, splits, q_out, q_norm_w, k_norm_w, eps, cos_cache, sin_cache, n_positions, cache, block_table,
+                  bt_rows, bt_stride, seq_ids, seq_lens, n_rows, layer, num_q_heads, status, stream);
 }
 
 extern "C" int nsd_kv8_store_prefill(const void* k, const void* v, int64_t n_tokens, const nsd_kv8_cache* cache,

@@ -2,7 +2,8 @@
 
 from .block_mgmt import (gather_allocated_blocks_and_unset, set_block_table_and_num_seq_alloc_blocks,
                          unset_block_table_and_num_seq_alloc_blocks, write_block_table_ranges)
-from .kv8 import KV8Cache, kv8_load, kv8_paged_attention, kv8_qk_norm_rope_store, kv8_store
+from .kv8 import (KV8Cache, kv8_load, kv8_paged_attention, kv8_qk_norm_rope_store, kv8_qk_norm_rope_store_partials,
+                  kv8_store)
 from .kvcache_mgmt import store_kvcache
 from .linear import fused_add_rmsnorm_partials, linear, linear_partials, linear_splits, sum_partials
 from .mxfp4 import (MXFP4Weight, MXFP8Rows, mxfp4_dequantize, mxfp4_linear, mxfp4_pack, mxfp4_quantize,
@@ -23,4 +24,5 @@ __all__ = ["paged_attention", "paged_attention_fused", "store_kvcache", "rotary_
            "argmax_rows", "post_layer_forward", "linear", "linear_partials", "linear_splits", "sum_partials",
            "fused_add_rmsnorm_partials", "qk_norm_rope_store_partials", "MXFP4Weight", "MXFP8Rows", "mxfp4_quantize",
            "mxfp4_pack", "mxfp4_dequantize", "mxfp4_linear", "mxfp4_up_gate_silu_and_mul", "mxfp8_quantize",
-           "mxfp8_dequantize", "KV8Cache", "kv8_store", "kv8_qk_norm_rope_store", "kv8_load", "kv8_paged_attention"]
+           "mxfp8_dequantize", "KV8Cache", "kv8_store", "kv8_qk_norm_rope_store",
+           "kv8_qk_norm_rope_store_partials", "kv8_load", "kv8_paged_attention"]

@@ -185,6 +185,26 @@ def _decode_rows(cache: KV8Cache, infer_state) -> tuple:
     return infer_state.seq_ids.data_ptr() + 4 * npf, infer_state.decoding_seq_lens.data_ptr(), nd
 
 
+def _prologue_tables(cache: KV8Cache, q_norm, k_norm, cos_cache, sin_cache) -> int:
+    """Checks the prologue's norm weights and RoPE tables; the positions that these hold."""
+    if (q_norm is None) != (k_norm is None):
+        raise ValueError("pass both q_norm and k_norm, or neither")
+    if q_norm is not None:
+        for t, n in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+            if t.dtype is not _F16 or t.shape != (HEAD_DIM,) or not t.is_contiguous() or t.get_device() != cache.device:
+                _on(cache, t)
+                require(t, _F16, n)
+                raise ValueError(f"{n} must be [{HEAD_DIM}], got {tuple(t.shape)}")
+    angles = cos_cache.shape
+    if len(angles) != 2 or angles[1] != HEAD_DIM // 2 or sin_cache.shape != angles:
+        raise ValueError("cos/sin caches must be [max_positions, head_dim/2]")
+    for t, n in ((cos_cache, "cos_cache"), (sin_cache, "sin_cache")):
+        if t.dtype is not _F16 or not t.is_contiguous() or t.get_device() != cache.device:
+            _on(cache, t)
+            require(t, _F16, n)
+    return angles[0]
+
+
 def kv8_store(k: torch.Tensor, v: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor, model_config,
               engine_config, infer_state, cur_layer: int, validate: bool = False) -> None:
     """``store_kvcache`` into an 8-bit cache: every token's K/V of the forward at layer ``cur_layer``.
@@ -237,21 +257,7 @@ def kv8_qk_norm_rope_store(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ca
         q_out = q
     else:
         _packed(cache, q_out, "q_out", hq, rows)
-    if (q_norm is None) != (k_norm is None):
-        raise ValueError("pass both q_norm and k_norm, or neither")
-    if q_norm is not None:
-        for t, n in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-            if t.dtype is not _F16 or t.shape != (HEAD_DIM,) or not t.is_contiguous() or t.get_device() != cache.device:
-                _on(cache, t)
-                require(t, _F16, n)
-                raise ValueError(f"{n} must be [{HEAD_DIM}], got {tuple(t.shape)}")
-    angles = cos_cache.shape
-    if len(angles) != 2 or angles[1] != HEAD_DIM // 2 or sin_cache.shape != angles:
-        raise ValueError("cos/sin caches must be [max_positions, head_dim/2]")
-    for t, n in ((cos_cache, "cos_cache"), (sin_cache, "sin_cache")):
-        if t.dtype is not _F16 or not t.is_contiguous() or t.get_device() != cache.device:
-            _on(cache, t)
-            require(t, _F16, n)
+    positions = _prologue_tables(cache, q_norm, k_norm, cos_cache, sin_cache)
     if rows == 0:
         return
     if getattr(infer_state, "ignore_kvcache", False):
@@ -259,10 +265,39 @@ def kv8_qk_norm_rope_store(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ca
     status = StatusWord(q.device) if validate else None
     _call(cache.device, "nsd_kv8_qk_norm_rope_store", q.data_ptr(), q_stride, q_out.data_ptr(), k.data_ptr(), k_stride,
           v.data_ptr(), v_stride, ptr(q_norm), ptr(k_norm), model_config.rms_norm_eps, cos_cache.data_ptr(),
-          sin_cache.data_ptr(), angles[0], cache._ref, *table,
+          sin_cache.data_ptr(), positions, cache._ref, *table,
           *_decode_rows(cache, infer_state), int(cur_layer), hq, ptr(status.t) if status else None)
     if status is not None:
         status.check("kv8_qk_norm_rope_store")
+
+
+def kv8_qk_norm_rope_store_partials(partials: torch.Tensor, q_out: torch.Tensor, cache: KV8Cache,
+                                    block_table: torch.Tensor, q_norm: torch.Tensor | None,
+                                    k_norm: torch.Tensor | None, model_config, engine_config, infer_state,
+                                    cur_layer: int, cos_cache: torch.Tensor, sin_cache: torch.Tensor,
+                                    validate: bool = False) -> None:
+    """``kv8_qk_norm_rope_store`` over the rows' fused q/k/v projection as split partials, fp32 [splits, rows, (Hq + 2
+    Hkv) d] (``linear_partials``); q goes to ``q_out`` [rows, Hq, d]."""
+    table = _table(cache, block_table, engine_config)
+    rows, hq = infer_state.num_decoding_seqs, model_config.num_q_heads
+    width = (hq + 2 * cache.num_kv_heads) * HEAD_DIM
+    _on(cache, partials)
+    require(partials, torch.float32, "partials")
+    if partials.ndim != 3 or partials.shape[1:] != (rows, width):
+        raise ValueError(f"partials must be [splits, {rows}, {width}], got {tuple(partials.shape)}")
+    _packed(cache, q_out, "q_out", hq, rows)
+    positions = _prologue_tables(cache, q_norm, k_norm, cos_cache, sin_cache)
+    if rows == 0:
+        return
+    if getattr(infer_state, "ignore_kvcache", False):
+        raise ValueError("infer_state.ignore_kvcache is set but the forward has decode rows")
+    status = StatusWord(q_out.device) if validate else None
+    _call(cache.device, "nsd_kv8_qk_norm_rope_store_partials", partials.data_ptr(), partials.shape[0],
+          q_out.data_ptr(), ptr(q_norm), ptr(k_norm), model_config.rms_norm_eps, cos_cache.data_ptr(),
+          sin_cache.data_ptr(), positions, cache._ref, *table, *_decode_rows(cache, infer_state), int(cur_layer), hq,
+          ptr(status.t) if status else None)
+    if status is not None:
+        status.check("kv8_qk_norm_rope_store_partials")
 
 
 def kv8_load(k: torch.Tensor, v: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor, seq_ids: torch.Tensor,

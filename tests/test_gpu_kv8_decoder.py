@@ -19,7 +19,7 @@ from nebulasd_amd.config import QWEN3_0_6B, QWEN3_8B
 from nebulasd_amd.decoder import DecoderStack
 from nebulasd_amd.infer_state import build_infer_state
 from nebulasd_amd.kernels import (KV8Cache, fused_add_rmsnorm_inplace, kv8_paged_attention, kv8_qk_norm_rope_store,
-                                  linear, up_gate_silu_and_mul)
+                                  kv8_qk_norm_rope_store_partials, linear, sum_partials, up_gate_silu_and_mul)
 from nebulasd_amd.spec_loop import RandomQwen3, run
 
 pytestmark = pytest.mark.gpu
@@ -109,6 +109,48 @@ def test_stack_is_its_kernels_from_python(gpu, codes, cfg, n_layers, n_req, dept
             worst = oracle_excess(m, probe_layer, *got, sids, slens)
             print(f"layer {probe_layer}: worst {worst:.2f} of the bound", flush=True)
             assert worst <= 1
+
+
+@pytest.mark.parametrize("codes", ["e4m3", "int8"])
+@pytest.mark.parametrize("splits", range(1, 9))
+def test_prologue_over_partials(gpu, codes, splits):
+    """A projection's split partials: the prologue over their sum, bit for bit; a NaN among them ends in its row alone."""
+    m, sids, slens, _ = model_and_rows(codes, QWEN3_0_6B, 1, 9, splits - 1, gpu)
+    st = build_infer_state(sids, slens, [], m.mc, m.cos, m.sin, gpu)
+    mc, n = m.mc, len(sids)
+    hq, hkv = mc.num_q_heads, mc.num_kv_heads
+    g = torch.Generator(device=gpu).manual_seed(splits)
+    part = torch.randn((splits, n, (hq + 2 * hkv) * 128), device=gpu, generator=g)
+    if splits == 3:
+        part[1, 4, -1] = float("nan")
+    mine = copy.deepcopy(m.kv8)
+    q, k, v = sum_partials(part).view(n, hq + 2 * hkv, 128).split((hq, hkv, hkv), 1)
+    outs = [torch.full((n, hq, 128), 7.0, dtype=torch.float16, device=gpu) for _ in range(2)]
+    for w in ((None, None), (m.layers[0]["q_norm"], m.layers[0]["k_norm"])):
+        rest = (m.block_table, *w, mc, m.ec, st, 0, m.cos, m.sin)
+        kv8_qk_norm_rope_store_partials(part, outs[0], m.kv8, *rest, validate=splits != 3)
+        kv8_qk_norm_rope_store(q, k, v, mine, *rest, q_out=outs[1])
+        assert torch.equal(*outs)
+        assert all(torch.equal(a, b) for a, b in zip(bytes_of(m.kv8), bytes_of(mine)))
+
+
+def test_prologue_over_partials_refusals(gpu):
+    m, sids, slens, _ = model_and_rows("int8", QWEN3_0_6B, 1, 3, 0, gpu)
+    st = build_infer_state(sids, slens, [], m.mc, m.cos, m.sin, gpu)
+    hq, hkv = m.mc.num_q_heads, m.mc.num_kv_heads
+    part = torch.zeros((2, 3, (hq + 2 * hkv) * 128), device=gpu)
+    q = torch.zeros((3, hq, 128), dtype=torch.float16, device=gpu)
+    call = lambda part=part, q=q, **kw: kv8_qk_norm_rope_store_partials(  # noqa: E731
+        part, q, m.kv8, m.block_table, kw.get("w"), None, m.mc, m.ec, st, kw.get("layer", 0), m.cos, m.sin)
+    for bad, error in ((dict(part=part.half()), TypeError), (dict(part=part[:, :2].contiguous()), ValueError),
+                       (dict(part=part[0]), ValueError), (dict(part=part[:, :, 1:]), ValueError),
+                       (dict(part=part.cpu()), ValueError), (dict(q=q[:2]), ValueError),
+                       (dict(q=q.float()), TypeError), (dict(w=m.layers[0]["q_norm"]), ValueError),
+                       (dict(layer=1), _lib.NativeLibraryError), (dict(part=part[:0]), _lib.NativeLibraryError),
+                       (dict(part=torch.cat([part] * 5)), _lib.NativeLibraryError)):
+        with pytest.raises(error):
+            call(**bad)
+    call()
 
 
 @pytest.mark.parametrize("codes", ["e4m3", "int8"])
