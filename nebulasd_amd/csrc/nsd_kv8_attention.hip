@@ -31,6 +31,25 @@
 // Everything that follows the block ids comes through LDS (query rows and
 // scales too) and is waited for by count, in the order of issue, so that no
 // wait of the compiler's drains the tiles behind it.
+//
+// Bound by the tiles' intake, us a call with the merge's launch (the bytes at the
+// 7.0 TB/s of a contiguous read): 64 rows of 512 to 2048 tokens 26.8 (19.1), 16 x
+// 5 of 256 to 4096 18.6 (7.5), 16 x 9 of 1024 to 32768 57.7 (36.8), one row of
+// 32768 18.9 (9.6).  The loads and waits alone, without arithmetic, took 24.6,
+// 18.0, 52.7 and 18.6 where the kernel took 27.2, 20.5, 59.7 and 20.0.  A piece
+// begins with 3 us of latency (ids, then tiles), or 8 to 9 in a compute unit's
+// second workgroup, whose first tiles come behind the burst of everyone's, and
+// ends with 1 to 2.6 of merge; the merge launch takes 3 to 4.
+//
+// Other forms, us in that order unless said:
+//   tiles straight into registers, a pair ahead: spills, and a wait for every
+//     load at the loop's head: 28, 22, 81, 20 (4 short rows 16, now 6.2)
+//   three slots a wave: slower at each
+//   without nt (a block is read once): 30.9 against 27.7 (64 rows)
+//   one workgroup of eight waves a compute unit: 18.7 against 16.9 (16 x 5)
+//   the refill behind the products: 16 x 9 -2.7%, 16 x 5 +2%
+//   K tiles before V tiles, both in one 4 KB run, scores scaled before the
+//     maximum: no difference
 #include "nsd_kv8_device.h"
 #include "nsd_paged.h"
 
@@ -433,6 +452,8 @@ extern "C" int nsd_kv8_paged_attention(const void* q, void* o, float* lse, const
   if (rc) return rc;
   if (cache->num_blocks > INT32_MAX / cache->num_layers / cache->num_kv_heads)
     return fail(NSD_ERR_UNSUPPORTED, "%s: %lld blocks (at most 2^31 tiles)", who, (long long)cache->num_blocks);
+  if (!(softmax_scale > 0.f) || softmax_scale == INFINITY)  // masked scores, -inf, have to stay that
+    return fail(NSD_ERR_INVALID, "%s: softmax_scale=%g (a positive number)", who, (double)softmax_scale);
   AttnCall c;
   rc = prepare_attention(who, q, true, o, lse, cache->k, cache->v, cache->num_blocks, cache->num_layers, layer,
                          num_q_heads, cache->num_kv_heads, D, BS, block_table, bt_rows, bt_stride, plan_host,

@@ -216,6 +216,24 @@ def test_c_refusals_of_arguments():
         _lib.call(*args)
 
 
+def test_c_refusals_of_partials():
+    c = _c()
+
+    def args(part=16, splits=2, q_out=16, qn=None, kn=None, cos=16, pos=8, cache=c, bt=16, rows=1, layer=0, hq=4):
+        return ("nsd_kv8_qk_norm_rope_store_partials", part, splits, q_out, qn, kn, 1e-6, cos, 16, pos,
+                cache and ctypes.byref(cache), bt, 2, 4, 16, 16, rows, layer, hq, None, None)
+
+    for bad in BAD_CACHES:
+        _refused(*args(cache=_c(**bad)))
+    for kw in (dict(part=None), dict(part=8), dict(splits=0), dict(splits=9), dict(q_out=None), dict(q_out=8), dict(qn=16),
+               dict(cos=None), dict(cos=24), dict(pos=0), dict(cache=None), dict(bt=None), dict(rows=-1),
+               dict(rows=(1 << 20) + 1), dict(layer=2), dict(hq=0)):
+        _refused(*args(**kw))
+    _lib.call(*args(rows=0))
+    _refused("nsd_decoder_forward_kv8", None, 16, 16, 1, ctypes.byref(c), *[16, 1, 1, 16, 16, 16, 16, 8, None, None, None],
+             0, 0.1, -1, None, None, None, None, None)
+
+
 def test_plans():
     """Every block of every segment in one piece, parts in fp32, and few pieces where they do."""
     from nebulasd_amd.plan import decode_plan, kv8_plan_words
@@ -260,9 +278,10 @@ def test_attention_refusals():
     buf = words.ctypes.data
     c = _c()
 
-    def args(cache=c, layer=0, q=16, o=16, hq=4, bt=16, bt_rows=2, stride=64, plan=buf, dev=16, work=16, size=ws):
+    def args(cache=c, layer=0, q=16, o=16, hq=4, bt=16, bt_rows=2, stride=64, plan=buf, dev=16, work=16, size=ws,
+             scale=0.1):
         return ("nsd_kv8_paged_attention", q, o, None, cache and ctypes.byref(cache), layer, hq, bt, bt_rows, stride,
-                plan, dev, work, size, 0.1, None, None)
+                plan, dev, work, size, scale, None, None)
 
     assert ws > 0
     for bad in BAD_CACHES:
@@ -270,6 +289,8 @@ def test_attention_refusals():
     for kw in (dict(cache=None), dict(layer=2), dict(q=None), dict(q=8), dict(o=None), dict(hq=8), dict(bt=None),
                dict(bt_rows=1), dict(stride=65), dict(dev=None), dict(cache=_c(num_kv_heads=4))):
         _refused(*args(**kw))
+    for scale in (0.0, -1.0, float("nan"), float("inf")):
+        assert "softmax_scale" in _refused(*args(scale=scale))
     for kw in (dict(work=None), dict(size=ws - 1), dict(work=8)):
         with pytest.raises(_lib.NativeLibraryError, match="status 4"):
             _lib.call(*args(**kw))
