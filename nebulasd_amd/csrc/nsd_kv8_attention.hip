@@ -42,8 +42,9 @@
 // ends with 1 to 2.6 of merge; the merge launch takes 3 to 4.
 //
 // Other forms, us in that order unless said:
-//   tiles straight into registers, a pair ahead: spills, and a wait for every
-//     load at the loop's head: 28, 22, 81, 20 (4 short rows 16, now 6.2)
+//   tiles straight into registers, a pair ahead (spills, and a wait for every
+//     load at the loop's head): 30.3, 23.3, 85.3 and 22.4 against 28.5, 20.1, 59.4
+//     and 19.9
 //   three slots a wave: slower at each
 //   without nt (a block is read once): 30.9 against 27.7 (64 rows)
 //   one workgroup of eight waves a compute unit: 18.7 against 16.9 (16 x 5)
