@@ -7,6 +7,7 @@ inputs (``oracle.kv8_attention``).
 from __future__ import annotations
 
 import copy
+import ctypes
 
 import numpy as np
 import pytest
@@ -17,7 +18,7 @@ from nebulasd_amd import _lib
 from nebulasd_amd.config import QWEN3_0_6B, QWEN3_8B, EngineConfig, ModelConfig
 from nebulasd_amd.hostkv import swap_blocks
 from nebulasd_amd.infer_state import build_infer_state, rope_cache
-from nebulasd_amd.plan import kv8_plan_for
+from nebulasd_amd.plan import AttnPlan, kv8_plan_for, plan_for
 from nebulasd_amd.kernels import (KV8Cache, kv8_load, kv8_paged_attention, kv8_qk_norm_rope_store, kv8_store,
                                   paged_attention, prefill_attention, qk_norm_rope_store)
 
@@ -520,6 +521,54 @@ def test_attention_of_more_segments_than_slots(gpu, codes):
     for _ in range(3):
         o2, lse2, _ = attend(cache, bt, mc, ec, ids, lens, q, st=st)
         assert torch.equal(o, o2) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("rows", ["fp16 plan", "one by one", "any order"])
+def test_attention_by_other_plans(gpu, codes, rows):
+    """The fp16 attention's plan, rows each a group of its own, and rows repeated and in any order."""
+    q_len = 5
+    mc, ec, table, bt, cache, ids, lens, q = filled(codes, gpu, 16, 8, [3000, 250, 31, 90], q_len, seed=16)
+    if rows == "any order":
+        order = np.random.default_rng(17).permutation(len(ids) * 2) % len(ids)  # every row twice
+        ids, lens, q = [ids[r] for r in order], [lens[r] for r in order], q[torch.from_numpy(order).to(gpu)].contiguous()
+    st = state(mc, ids, lens)
+    if rows == "one by one":
+        st.max_group_rows = 1
+    if rows == "fp16 plan":
+        plan, size = plan_for(st, mc, ec, bt), ctypes.c_int64()
+        assert int(plan.host[_lib.PLAN_COMBINES]) > 0
+        _lib.call("nsd_kv8_attn_workspace", plan.host_address, ctypes.byref(size))
+        st.kv8_plan = AttnPlan(plan.host, plan.dev, None, size.value, 16, 8)
+    o, lse, _ = attend(cache, bt, mc, ec, ids, lens, q, st=st)
+    check_attention(cache, table, 1, q, ids, lens, o, lse)
+
+
+@pytest.mark.parametrize("codes", CODES)
+def test_attention_over_half_a_million_tokens(gpu, codes):
+    """The longest segment that a plan takes, 128 pieces of 256 blocks, of seven blocks again and again."""
+    n = 1 << 19
+    mc, ec, _, _, cache, _, _, q = filled(codes, gpu, 4, 1, [7 * 16 - 1], 1, layers=1, seed=18)
+    ec = EngineConfig(max_blocks_per_seq=n // 16)
+    table = np.arange(n // 16, dtype=np.int32)[None] % 7
+    o, lse, st = attend(cache, gpu_of(table), mc, ec, [0], [n], q, layer=0)
+    assert st.kv8_plan.host[_lib.PLAN_SLOTS] == 128
+    with pytest.raises(_lib.NativeLibraryError, match="pieces"):
+        attend(cache, gpu_of(np.zeros((1, n // 16 + 1), np.int32)), mc, EngineConfig(max_blocks_per_seq=n // 16 + 1), [0],
+               [n + 1], q, layer=0)
+    k, v = (x[:7, 0, 0].reshape(-1, 128) for x in values_of(cache))
+    times = np.repeat(np.bincount(table[0], minlength=7), 16).astype(np.float64)
+    for h in range(4):
+        s = k @ q[0, h].double().cpu().numpy() * 128 ** -0.5
+        p = times * np.exp(s - s.max())
+        want, total = p @ v / p.sum(), p.sum()
+        # as oracle.kv8_attention; sums of a lane's 256 weights, four waves and 128 parts in fp32
+        ds = 130 * 2.0 ** -24 * (np.abs(k) @ np.abs(q[0, h].double().cpu().numpy())).max() * 128 ** -0.5 + \
+            (np.abs(s).max() + np.abs(s - s.max()).max()) * 2.0 ** -22
+        off = ((3 * 2.0 ** -11 + 2 * ds + 400 * 2.0 ** -24) * p + times * 2.0 ** -25) @ np.abs(v) / total + 2.0 ** -24
+        assert (np.abs(o[0, h].double().cpu().numpy() - want) <= off).all()
+        ln = s.max() + np.log(total)
+        assert abs(float(lse[0, h]) - ln) <= ds + 400 * 2.0 ** -24 + 2.0 ** -22 * (1 + abs(ln))
 
 
 @pytest.mark.parametrize("codes", CODES)
