@@ -50,7 +50,8 @@
  * arrays need not be).  Metadata that points outside the cache, the block table
  * or the rows is skipped and flagged in *status (NULL: not flagged).  A block is
  * written for one sequence in a call, but any number of its rows, in any order;
- * of rows with the same position the last one stays.
+ * of rows with the same position the last one stays.  Calls that write the same
+ * block, or read what another writes, are ordered by the caller.
  */
 #ifndef NSD_KV8_H
 #define NSD_KV8_H

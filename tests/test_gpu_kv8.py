@@ -16,7 +16,7 @@ import torch
 import oracle
 from nebulasd_amd import _lib
 from nebulasd_amd.config import QWEN3_0_6B, QWEN3_8B, EngineConfig, ModelConfig
-from nebulasd_amd.hostkv import swap_blocks
+from nebulasd_amd.hostkv import CopyPlan, CopyRegion, HostKVArena, HostKVCopyBackend, swap_blocks
 from nebulasd_amd.infer_state import build_infer_state, rope_cache
 from nebulasd_amd.plan import AttnPlan, kv8_plan_for, plan_for
 from nebulasd_amd.kernels import (KV8Cache, kv8_load, kv8_paged_attention, kv8_qk_norm_rope_store, kv8_store,
@@ -896,6 +896,31 @@ def test_swap_out_and_in(gpu, codes):
         swap_blocks(list(range(n)), back.tolist(), True, *p)
     got, _, _ = attend(cache, gpu_of(back[None]), mc, ec, ids, lens, q)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("engine", ["dma", "kernel"])
+def test_host_copies(gpu, engine):
+    """A backend for the codes and one for the scales bring blocks to the host and back."""
+    rng = np.random.default_rng(19)
+    mc, ec = config(16, 8, 4)
+    cache = KV8Cache.allocate(20, mc, torch.int8, gpu)
+    planes = (cache.k, cache.v), (cache.k_scales, cache.v_scales)
+    want = []
+    for t in (t for pair in planes for t in pair):
+        t.copy_(torch.from_numpy(rng.integers(0, 256, tuple(t.shape), dtype=np.uint8)))
+        want.append(t.cpu())
+    for k, v in planes:
+        arena = HostKVArena.create(total_blocks=9, block_bytes=k[0].numel(), kv_block_shape=tuple(k.shape[1:]))
+        backend = HostKVCopyBackend(arena=arena, k_cache=k, v_cache=v, engine=engine)
+        extent = arena.make_extent(offset_blocks=1, capacity_blocks=7)
+        torch.cuda.synchronize()
+        backend.launch(CopyPlan("D2H", (CopyRegion(extent, 5, 0, 7),))).synchronize()
+        k.zero_(), v.zero_()
+        torch.cuda.synchronize()
+        backend.launch(CopyPlan("H2D", (CopyRegion(extent, 11, 0, 7),))).synchronize()
+        backend.close()
+    for t, w in zip((t for pair in planes for t in pair), want):
+        assert torch.equal(t[11:18].cpu(), w[5:12]) and not t[:11].any() and not t[18:].any()
 
 
 @pytest.mark.parametrize("codes", CODES)
