@@ -45,7 +45,10 @@
 //   tiles straight into registers, a pair ahead (spills, and a wait for every
 //     load at the loop's head): 30.3, 23.3, 85.3 and 22.4 against 28.5, 20.1, 59.4
 //     and 19.9
-//   three slots a wave: slower at each
+//   four slots a wave (the LDS given at launch: where a kernel's own size leaves
+//     one workgroup a compute unit, the compiler moves accumulators between two
+//     register files, 16 x 5 16.6 -> 18.9): 32.1, 18.6, 73.0 and 19.6 against 27.2,
+//     16.6, 60.6 and 18.1; issuing them all delays the first
 //   without nt (a block is read once): 30.9 against 27.7 (64 rows)
 //   one workgroup of eight waves a compute unit: 18.7 against 16.9 (16 x 5)
 //   the refill behind the products: 16 x 9 -2.7%, 16 x 5 +2%
