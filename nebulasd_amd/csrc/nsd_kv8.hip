@@ -343,7 +343,8 @@ __global__ __launch_bounds__(kThreads) void kv8_append_kernel(Cache c, AppendArg
     for (int j = 0; j < 2; ++j) {
       const int t = t0 + 8 * j;
       if ((fresh | (again ? old : 0u)) >> t & 1)
-        u.codes[at0 + 8 * j] = k_unit(kv8_codes<T>(h[2 * j], s.e, s.careful), kv8_codes<T>(h[2 * j + 1], s.e, s.careful));
+        u.codes[at0 + 8 * j] =
+            k_unit(kv8_codes<T>(h[2 * j], s.e, s.careful), kv8_codes<T>(h[2 * j + 1], s.e, s.careful));
     }
     if (lane == 0) *u.scale = (uint8_t)(s.e + 127);
   } else {
@@ -470,9 +471,10 @@ __global__ __launch_bounds__(kThreads) void kv8_prefill_kernel(
 }
 
 // Reading back: grid (block from the first token's on x four units, sequence).
-// Bound by memory, as a copy is: 32749 tokens x 8 heads 42 us, 4.8 TB/s.  Stores that pass the caches make it faster (16
-// sequences of 256 to 4096 tokens 31 -> 24 us) and its reader slower by more
-// (24k tokens, then the prefill attention over them: 175.4 -> 182.7).
+// Bound by memory, as a copy is: 32749 tokens x 8 heads 42 us, 4.8 TB/s.  Stores
+// that pass the caches make it faster (16 sequences of 256 to 4096 tokens 31 ->
+// 24 us) and its reader slower by more (24k tokens, then the prefill attention
+// over them: 175.4 -> 182.7).
 template <int T>
 __global__ __launch_bounds__(kThreads) void kv8_load_kernel(
     Cache c, f16* __restrict__ k, f16* __restrict__ v, int64_t n_tokens, const int32_t* __restrict__ bt,
@@ -620,7 +622,8 @@ static int prologue(const char* who, AppendArgs a, int splits, void* q_out, cons
     return fail(NSD_ERR_INVALID, "%s: pass both norm weights or neither", who);
   if (n_rows == 0) return NSD_OK;
   if ((!a.q && !a.part) || !q_out || !cos_cache || !sin_cache) return fail(NSD_ERR_INVALID, "%s: null pointer", who);
-  for (const void* p : {(const void*)a.q, (const void*)a.part, (const void*)q_out, cos_cache, sin_cache, q_norm_w, k_norm_w})
+  for (const void* p : {(const void*)a.q, (const void*)a.part, (const void*)q_out, cos_cache, sin_cache, q_norm_w,
+                        k_norm_w})
     if (!aligned16(p)) return fail(NSD_ERR_INVALID, "%s: rows, tables and norm weights must be 16-byte aligned", who);
   a.n_rows = (int)n_rows;
   a.kv_groups = unit_groups(cache);

@@ -80,7 +80,8 @@ static_assert(2 * lds_bytes(3) <= 160 * 1024, "two workgroups a CU");
 // 1 KB from base + off (a lane's 16 bytes), or 64 dwords, into LDS; the compiler
 // sees neither the load nor its wait.
 __device__ inline void dma16(uint32_t lds, const char* base, uint32_t off) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2 nt" : : "s"(lds), "v"(off), "s"(base) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2 nt"
+               : : "s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
 __device__ inline void dma16_rows(uint32_t lds, const void* at) {
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(at) : "memory", "m0");
@@ -140,7 +141,8 @@ void kv8_attn_kernel(AttnArgs a, PieceTable pt, Kv8Caches cache) {
   }
   // the whole record in one round of scalar loads
   using const_i32p = const __attribute__((address_space(4))) int32_t*;
-  const const_i32p rec = (const_i32p)(uintptr_t)(a.pieces + (int64_t)__builtin_amdgcn_readfirstlane(rec_idx) * kPieceWords);
+  const const_i32p rec =
+      (const_i32p)(uintptr_t)(a.pieces + (int64_t)__builtin_amdgcn_readfirstlane(rec_idx) * kPieceWords);
   int32_t rv[kPieceWords];
 #pragma unroll
   for (int i = 0; i < kPieceWords; ++i) rv[i] = rec[i];
@@ -209,7 +211,8 @@ void kv8_attn_kernel(AttnArgs a, PieceTable pt, Kv8Caches cache) {
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) qf[t][kk] = *(const lds_f16x8*)(q_lds + ((4 * t + kk) * kWave + lane) * 16);
-  const uint32_t k_word = *(const lds_u32*)(scale_lds + 4 * lane), v_word = *(const lds_u32*)(scale_lds + 256 + 4 * lane);
+  const uint32_t k_word = *(const lds_u32*)(scale_lds + 4 * lane);
+  const uint32_t v_word = *(const lds_u32*)(scale_lds + 256 + 4 * lane);
   const int k_scale = k_word >> (8 * (((uint32_t)tile + cache.ks_low) & 3)) & 0xff;
   // a masked block's bytes may be anything, infinities under its scale too: its values are zeros
   const int v_scale = lane < my_n && !bad ? v_word >> (8 * (((uint32_t)tile + cache.vs_low) & 3)) & 0xff : 0;
@@ -287,7 +290,8 @@ void kv8_attn_kernel(AttnArgs a, PieceTable pt, Kv8Caches cache) {
         for (int e = 0; e < 8; ++e)
           if (masked[e / 4] || first[e / 4] + 4 * lg + e % 4 >= row_len[t]) sv[e] = -INFINITY;
       }
-      float mx = fmaxf(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])), fmaxf(fmaxf(sv[4], sv[5]), fmaxf(sv[6], sv[7])));
+      float mx =
+          fmaxf(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])), fmaxf(fmaxf(sv[4], sv[5]), fmaxf(sv[6], sv[7])));
       mx = rows_max(mx) * a.scale_log2;  // -inf stays -inf (scale > 0)
       // lazy running max: one decision per wave and tile
       if (__builtin_amdgcn_ballot_w64(mx > m[t] + kLazyMax) != 0) {
@@ -311,7 +315,8 @@ void kv8_attn_kernel(AttnArgs a, PieceTable pt, Kv8Caches cache) {
       l[t] += psum;
     }
 
-    const float vp0 = kv8_power(__builtin_amdgcn_readlane(v_scale, 2 * p)), vp1 = kv8_power(__builtin_amdgcn_readlane(v_scale, 2 * p + 1));
+    const float vp0 = kv8_power(__builtin_amdgcn_readlane(v_scale, 2 * p));
+    const float vp1 = kv8_power(__builtin_amdgcn_readlane(v_scale, 2 * p + 1));
     if constexpr (T == NSD_KV8_E4M3) {
       // 0 times a NaN is a NaN: where a row masks tokens, NaN codes leave the
       // operand, and the dims that have them end as NaN for the rows that
@@ -399,7 +404,8 @@ void kv8_attn_kernel(AttnArgs a, PieceTable pt, Kv8Caches cache) {
         out[h] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int v = 0; v < kWaves; ++v)
-          out[h] += *reinterpret_cast<const f32x4*>(mrg + v * (kMergeWave / 4) + ((2 * wave + h) * kWave + lane) * 4) * sc[v];
+          out[h] +=
+              *reinterpret_cast<const f32x4*>(mrg + v * (kMergeWave / 4) + ((2 * wave + h) * kWave + lane) * 4) * sc[v];
         out[h] *= inv;
       }
       const int at = 32 * lg + 8 * wave;

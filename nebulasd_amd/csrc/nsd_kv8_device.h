@@ -88,10 +88,6 @@ __device__ inline u32x2 kv8_codes(f16x8 h, int e, bool careful) {
   return out;
 }
 
-// The codes that stand for zeros.
-template <int T>
-constexpr uint32_t kv8_zeros() { return T == NSD_KV8_E4M3 ? 0u : 0x80808080u; }
-
 // Four whole numbers held as code + 128: 0x6400 | byte is the fp16 number 1024
 // + byte.
 __device__ inline void kv8_whole(uint32_t c, f16x2& lo, f16x2& hi) {
