@@ -105,7 +105,7 @@ __device__ inline f16x4 ones_of(uint32_t w) {
 
 template <int T, int NT>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
-void kv8_attn_kernel(AttnArgs a, PieceTable pt, Kv8Caches cache) {
+void kv8_attn_kernel(AttnArgs a, Kv8Caches cache, PieceTable pt) {
   __shared__ __align__(16) char smem[lds_bytes(NT)];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -113,6 +113,14 @@ void kv8_attn_kernel(AttnArgs a, PieceTable pt, Kv8Caches cache) {
   lds_char* ring = lds + wave * kRing;
   const lds_char* q_lds = lds + kWaves * kRing;
   const lds_char* scale_lds = q_lds + NT * 16 * D * 2 + wave * kScales;
+
+  // every argument, and the piece's table entry, in one round of scalar loads:
+  // left to the compiler they came in four, each a trip to memory
+  const uint32_t entry = pt.e[min((int)blockIdx.x, kPieceTableMax - 1)];
+  asm volatile("" ::"s"(a.q), "s"(a.bt), "s"(a.bt_stride), "s"(a.pieces), "s"(a.n_static), "s"(a.n_claimed),
+               "s"(a.piece_table), "s"(a.num_blocks), "s"(a.num_layers), "s"(a.layer), "s"(a.hq), "s"(a.hkv),
+               "s"(a.gqa), "s"(a.scale_log2), "s"(cache.k), "s"(cache.v), "s"(cache.ks), "s"(cache.vs),
+               "s"(cache.ks_low), "s"(cache.vs_low), "s"(entry));
 
   int rec_idx = blockIdx.x;
   if (rec_idx >= a.n_static) {
@@ -134,10 +142,9 @@ void kv8_attn_kernel(AttnArgs a, PieceTable pt, Kv8Caches cache) {
   const bool tabled = a.piece_table != 0 && (int)blockIdx.x < a.n_static;
   int tab_id = 0;
   if (tabled) {
-    const uint32_t e = pt.e[blockIdx.x];
-    int64_t col = (int64_t)(e >> 16) + wave + kWaves * lane;
+    int64_t col = (int64_t)(entry >> 16) + wave + kWaves * lane;
     col = col < a.bt_stride ? col : a.bt_stride - 1;
-    tab_id = a.bt[(int64_t)(e & 0xffffu) * a.bt_stride + col];
+    tab_id = a.bt[(int64_t)(entry & 0xffffu) * a.bt_stride + col];
   }
   // the whole record in one round of scalar loads
   using const_i32p = const __attribute__((address_space(4))) int32_t*;
@@ -431,7 +438,7 @@ void kv8_attn_kernel(AttnArgs a, PieceTable pt, Kv8Caches cache) {
 template <int T>
 void launch_rows(const AttnCall& c, const Kv8Caches& caches, hipStream_t st) {
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(c.grid), dim3(kThreads), 0, st, c.args, c.pieces, caches);
+    hipLaunchKernelGGL(kernel, dim3(c.grid), dim3(kThreads), 0, st, c.args, caches, c.pieces);
   };
   if (c.row_tiles == 1) go(kv8_attn_kernel<T, 1>);
   else if (c.row_tiles == 2) go(kv8_attn_kernel<T, 2>);
