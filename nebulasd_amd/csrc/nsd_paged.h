@@ -100,18 +100,24 @@ __device__ inline float rows_sum(float x) {
 // verify) 4.6 either way.
 constexpr int kMergeSlots = 8;
 
-// Eight dims of a partial, f16 or float; zeros if it is a repeated slot's, which
-// may hold an infinity (0 * inf).
+// Eight dims of a partial, f16 or float, as they are loaded and as values; zeros
+// if it is a repeated slot's, which may hold an infinity (0 * inf).
 struct Part {
   f32x4 lo, hi;
 };
-__device__ inline Part part_of(const f16* p, bool use) {
-  f16x8 h = *reinterpret_cast<const f16x8*>(p);
-  if (!use) h = f16x8{};
-  return {f32x4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]}, f32x4{(float)h[4], (float)h[5], (float)h[6], (float)h[7]}};
+__device__ inline f16x8 loaded(const f16* p) { return *reinterpret_cast<const f16x8*>(p); }
+__device__ inline Part loaded(const float* p) {
+  return {*reinterpret_cast<const f32x4*>(p), *reinterpret_cast<const f32x4*>(p + 4)};
 }
-__device__ inline Part part_of(const float* p, bool use) {
-  const Part v = {*reinterpret_cast<const f32x4*>(p), *reinterpret_cast<const f32x4*>(p + 4)};
+// What was loaded is in registers from here on.
+__device__ inline void arrived(const f16x8& h) { asm volatile("" ::"v"(h)); }
+__device__ inline void arrived(const Part& v) { asm volatile("" ::"v"(v.lo), "v"(v.hi)); }
+__device__ inline Part part_of(f16x8 h, bool use) {
+  if (!use) h = f16x8{};
+  return {f32x4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]},
+          f32x4{(float)h[4], (float)h[5], (float)h[6], (float)h[7]}};
+}
+__device__ inline Part part_of(const Part& v, bool use) {
   return use ? v : Part{f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 }
 // A merged row's 1 / W; 0 where no slot attends a token (ids outside the pool).
@@ -129,11 +135,24 @@ __device__ inline void merge_row(const AttnArgs& a, int head, int first, int n_s
   const int64_t sstride = (int64_t)a.rows_max * D;  // elements between slots
   f32x4 v0[kMergeSlots], v1[kMergeSlots];
   float ls[kMergeSlots];
+  decltype(loaded(po)) raw[kMergeSlots];
 #pragma unroll
   for (int u = 0; u < kMergeSlots; ++u) {
     const int sidx = u < n_slots ? u : 0;
-    ls[u] = u < n_slots ? pl[(int64_t)sidx * a.rows_max] : -INFINITY;
-    const Part v = part_of(po + sidx * sstride, u < n_slots);
+    ls[u] = pl[(int64_t)sidx * a.rows_max];
+    raw[u] = loaded(po + sidx * sstride);
+  }
+  // all of them, before any is looked at: with a branch around the loads of slots
+  // that there are not, the first was waited for before the second
+#pragma unroll
+  for (int u = 0; u < kMergeSlots; ++u) {
+    asm volatile("" ::"v"(ls[u]));
+    arrived(raw[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < kMergeSlots; ++u) {
+    const Part v = part_of(raw[u], u < n_slots);
+    ls[u] = u < n_slots ? ls[u] : -INFINITY;
     v0[u] = v.lo;
     v1[u] = v.hi;
   }
@@ -195,7 +214,7 @@ __device__ inline void merge_row_wide(const AttnArgs& a, int head, int first, in
       const int s = s0 + SL * u;
       const int at = s < n_slots ? s : s0;
       ls[u] = s < n_slots ? pl[(int64_t)at * a.rows_max] : -INFINITY;
-      h[u] = part_of(po + (int64_t)at * a.rows_max * D, s < n_slots);
+      h[u] = part_of(loaded(po + (int64_t)at * a.rows_max * D), s < n_slots);
     }
     const float M = fmaxf(fmaxf(fmaxf(ls[0], ls[1]), fmaxf(ls[2], ls[3])), st.M);
     const float use = M == -INFINITY ? 0.f : M;
@@ -281,6 +300,8 @@ struct CombineTable {
 template <int SL, class P>
 __global__ __launch_bounds__(256) void combine_table_kernel(AttnArgs a, CombineTable tab) {
   const uint64_t e = tab.e[blockIdx.x];
+  // the arguments in one round of loads with it
+  asm volatile("" ::"s"(e), "s"(a.gqa), "s"(a.part_o), "s"(a.part_lse), "s"(a.rows_max), "s"(a.o), "s"(a.lse), "s"(a.hq));
   merge_group<SL, P>(a, (int)((e >> 28) & 0xff), (int)(e & 0xfffff), (int)((e >> 20) & 0xff), (int)((e >> 36) & 0xfffff),
                   (int)(e >> 56) * a.gqa, (int)blockIdx.y);
 }
