@@ -170,48 +170,63 @@ __device__ inline f16x8 eight_of(const f16* rows, const float* part, int64_t per
   }
 }
 
-// Where row r goes: its block, or -1 and the flag that says why not.  In two
-// parts, both without a branch, so that a caller has several rows' loads in
-// flight: the row's numbers, then its entry of the block table (any entry, where
-// the numbers are not good).
+// Where a row goes: its block, or -1 and the flag that says why not.  In parts
+// without a branch, so that a caller has several rows' loads in flight: the row's
+// numbers, its entry of the block table (any entry, where the numbers are not
+// good), and what they say.
 struct RowNumbers {
-  int64_t sid, pos;
+  int sid, len;
 };
 struct Place {
   int64_t blk, pos;
   int32_t flag;
 };
-__device__ inline RowNumbers numbers_of(const AppendArgs& a, int64_t r) {
-  return {a.seq_ids[r], (int64_t)a.seq_lens[r] - 1};
+__device__ inline RowNumbers numbers_of(const AppendArgs& a, int64_t r) { return {a.seq_ids[r], a.seq_lens[r]}; }
+__device__ inline bool in_table(const AppendArgs& a, const RowNumbers& n) {
+  return n.sid >= 0 && n.sid < a.bt_rows && n.len >= 1 && n.len <= a.bt_stride * BS;
+}
+__device__ inline int entry_of(const AppendArgs& a, const RowNumbers& n) {
+  return a.bt[in_table(a, n) ? n.sid * a.bt_stride + (n.len - 1) / BS : 0];
 }
 template <bool PRO>
-__device__ inline Place place_of(const Cache& c, const AppendArgs& a, const RowNumbers& n) {
-  const bool in = n.sid >= 0 && n.sid < a.bt_rows && n.pos >= 0 && n.pos < a.bt_stride * BS;
-  const bool turned = !PRO || n.pos < a.n_pos;
-  const int64_t blk = a.bt[in ? n.sid * a.bt_stride + n.pos / BS : 0];
-  const bool held = blk >= 0 && blk < c.num_blocks;
-  return {in && turned && held ? blk : -1, n.pos,
+__device__ inline Place place_of(const Cache& c, const AppendArgs& a, const RowNumbers& n, int entry) {
+  const bool in = in_table(a, n);
+  const int64_t pos = (int64_t)n.len - 1;
+  const bool turned = !PRO || pos < a.n_pos;
+  const bool held = entry >= 0 && entry < c.num_blocks;
+  return {in && turned && held ? entry : -1, pos,
           !in ? NSD_STATUS_BAD_SEQ : !turned ? NSD_STATUS_BAD_POSITION : NSD_STATUS_BAD_BLOCK};
 }
 
+// The norm's weights of a lane's 16 dims, and the angles of a position.
+struct Weights {
+  f16x8 lo, hi;
+};
+__device__ inline Weights weights_of(const f16* w, int c) {
+  if (w == nullptr) return {};
+  return {*reinterpret_cast<const f16x8*>(w + 8 * c), *reinterpret_cast<const f16x8*>(w + D / 2 + 8 * c)};
+}
+struct Angles {
+  f16x8 cos, sin;
+};
+__device__ inline Angles angles_of(const AppendArgs& a, int64_t pos, int c) {
+  return {*reinterpret_cast<const f16x8*>(a.cos_c + pos * (D / 2) + 8 * c),
+          *reinterpret_cast<const f16x8*>(a.sin_c + pos * (D / 2) + 8 * c)};
+}
+
 // Dims 8c .. 8c+7 (lo) and 64+8c .. (hi) of a row, eight lanes a row: RMS-
-// normalised with w (null: not) and rotated by the position's angles, in the
+// normalised with w (if `norm`) and rotated by the position's angles, in the
 // fp16 prologue's arithmetic bit for bit: it adds x_d^2 + x_{d+64}^2 over a
 // butterfly of lanes d ^ 32, ^ 16, ^ 8, ^ 4, ^ 2, ^ 1, which here are the lanes
 // c ^ 4, ^ 2, ^ 1 and then the eight of a lane.
-__device__ inline void norm_rope(f16x8& lo, f16x8& hi, const f16* w, float eps, const f16* cos_c, const f16* sin_c,
-                                 int64_t pos, int c) {
-  const f16x8 cs = *reinterpret_cast<const f16x8*>(cos_c + pos * (D / 2) + 8 * c);
-  const f16x8 sn = *reinterpret_cast<const f16x8*>(sin_c + pos * (D / 2) + 8 * c);
+__device__ inline void norm_rope(f16x8& lo, f16x8& hi, bool norm, const Weights& w, float eps, const Angles& at) {
   float x0[8], x1[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     x0[j] = (float)lo[j];
     x1[j] = (float)hi[j];
   }
-  if (w != nullptr) {
-    const f16x8 w0 = *reinterpret_cast<const f16x8*>(w + 8 * c);
-    const f16x8 w1 = *reinterpret_cast<const f16x8*>(w + D / 2 + 8 * c);
+  if (norm) {
     float u[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) u[j] = sq_pair(x0[j], x1[j]);
@@ -221,14 +236,14 @@ __device__ inline void norm_rope(f16x8& lo, f16x8& hi, const f16* w, float eps, 
     const float rstd = 1.f / sqrtf(ss / (float)D + eps);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      x0[j] = (float)f16_of(x0[j] * rstd * (float)w0[j]);
-      x1[j] = (float)f16_of(x1[j] * rstd * (float)w1[j]);
+      x0[j] = (float)f16_of(x0[j] * rstd * (float)w.lo[j]);
+      x1[j] = (float)f16_of(x1[j] * rstd * (float)w.hi[j]);
     }
   }
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    lo[j] = f16_of(rope_lo(x0[j], x1[j], (float)cs[j], (float)sn[j]));
-    hi[j] = f16_of(rope_hi(x0[j], x1[j], (float)cs[j], (float)sn[j]));
+    lo[j] = f16_of(rope_lo(x0[j], x1[j], (float)at.cos[j], (float)at.sin[j]));
+    hi[j] = f16_of(rope_hi(x0[j], x1[j], (float)at.cos[j], (float)at.sin[j]));
   }
 }
 
@@ -240,7 +255,9 @@ __device__ inline void norm_rope(f16x8& lo, f16x8& hi, const f16* w, float eps, 
 //
 // Bound by latency, one trip to memory after another: row numbers, the block
 // table, the tile and then the rows.  64 rows of 16 + 2 x 8 heads with the prologue
-// 4.4 us, 16 x 5 of 32 + 2 x 8 5.6.
+// 4.3 us, 16 x 5 of 32 + 2 x 8 5.2 (an empty launch 1.9).  So loads go out together
+// (asm that names them keeps them so): one trip less each for the row numbers, the
+// norm's weights and a tile's several rows, 4.4 and 5.6 before.
 //
 // S: 0 for fp16 rows, else the split partials of the projection that makes them
 // (a decoder layer's: their sum in a launch of its own costs 3 us more).
@@ -257,13 +274,15 @@ __global__ __launch_bounds__(kThreads) void kv8_append_kernel(Cache c, AppendArg
     const bool any = at < (int64_t)a.n_rows * a.hq;
     const int64_t r = any ? at / a.hq : 0;
     const int h = any ? (int)(at - r * a.hq) : 0;
-    const int64_t pos = (int64_t)a.seq_lens[r] - 1;
-    const bool in = pos >= 0 && pos < a.n_pos;
-    if (any && !in && cc == 0) flag_status(a.status, NSD_STATUS_BAD_POSITION);
     const int64_t from = r * a.q_rs + (int64_t)h * D + 8 * cc;
     f16x8 lo = eight_of<S>(a.q + from, a.part + from, per_split);
     f16x8 hi = eight_of<S>(a.q + from + D / 2, a.part + from + D / 2, per_split);
-    norm_rope(lo, hi, a.qw, a.eps, a.cos_c, a.sin_c, in ? pos : 0, cc);  // a head's eight lanes agree on any and in
+    const Weights w = weights_of(a.qw, cc);
+    const int64_t pos = (int64_t)a.seq_lens[r] - 1;
+    const bool in = pos >= 0 && pos < a.n_pos;
+    const Angles at_pos = angles_of(a, in ? pos : 0, cc);
+    if (any && !in && cc == 0) flag_status(a.status, NSD_STATUS_BAD_POSITION);
+    norm_rope(lo, hi, a.qw != nullptr, w, a.eps, at_pos);  // a head's eight lanes agree on any and in
     if (any && in) {
       f16* dst = a.q_out + at * D + 8 * cc;
       *reinterpret_cast<f16x8*>(dst) = lo;
@@ -275,11 +294,17 @@ __global__ __launch_bounds__(kThreads) void kv8_append_kernel(Cache c, AppendArg
   __shared__ unsigned long long s_slot[BS];  // (row + 1) << 32 | position, 0: none
   __shared__ int s_earlier;
   const int r = (int)blockIdx.x / a.kv_groups, group = (int)blockIdx.x - r * a.kv_groups;
-  // this row's place and, beside it, the places of the first 256
-  const RowNumbers own_numbers = numbers_of(a, r);
+  // this row's place and, beside it, the places of the first 256; by a row number
+  // in a vector register (+ 0), since a scalar's way there waits for its load
+  const RowNumbers own_numbers = numbers_of(a, r + (int)(threadIdx.x >> 16));
   const RowNumbers numbers = numbers_of(a, min((int)threadIdx.x, a.n_rows - 1));
-  const Place own = place_of<PRO>(c, a, own_numbers);
-  Place p = place_of<PRO>(c, a, numbers);
+  asm volatile("" ::"v"(own_numbers.sid), "v"(own_numbers.len), "v"(numbers.sid), "v"(numbers.len));  // in one trip
+  const int own_entry = entry_of(a, own_numbers), entry = entry_of(a, numbers);
+  const Weights kw = PRO ? weights_of(a.kw, lane & 7) : Weights{};
+  asm volatile("" ::"v"(own_entry), "v"(entry));
+  Place own = place_of<PRO>(c, a, own_numbers, own_entry);
+  own.blk = __builtin_amdgcn_readfirstlane((int)own.blk);
+  Place p = place_of<PRO>(c, a, numbers, entry);
   if (own.blk < 0) {
     if (group == 0 && threadIdx.x == 0) flag_status(a.status, own.flag);
     return;
@@ -299,7 +324,10 @@ __global__ __launch_bounds__(kThreads) void kv8_append_kernel(Cache c, AppendArg
   if (threadIdx.x == 0) s_earlier = 0;
   __syncthreads();
   for (int rr = threadIdx.x; rr < a.n_rows; rr += kThreads) {
-    if (rr != (int)threadIdx.x) p = place_of<PRO>(c, a, numbers_of(a, rr));
+    if (rr != (int)threadIdx.x) {
+      const RowNumbers n = numbers_of(a, rr);
+      p = place_of<PRO>(c, a, n, entry_of(a, n));
+    }
     if (p.blk != own.blk) continue;
     atomicMax(&s_slot[p.pos % BS], (unsigned long long)(rr + 1) << 32 | (unsigned long long)p.pos);
     if (rr < r) s_earlier = 1;
@@ -312,26 +340,31 @@ __global__ __launch_bounds__(kThreads) void kv8_append_kernel(Cache c, AppendArg
   const uint32_t old = below & ~fresh;  // slots whose tokens stay
   const float power = kv8_power(old_byte);
   const int head = isv ? unit - c.hkv : unit;
+  asm volatile("" ::"v"(was[0]), "v"(was[1]));  // the tile is here: what is waited for below are rows
   if (!isv) {
     const int cc = lane & 7, t0 = lane >> 3;
-    f16x8 h[4];
+    f16x8 h[4] = {};
+    Angles at_pos[2] = {};
+    unsigned long long key[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      key[j] = s_slot[t0 + 8 * j];
+      // a new row among these eight slots; fp16 rows are read without asking (any
+      // row will do), since the loads after a branch begin when those before it end
+      if (S == 0 || (fresh >> (8 * j) & 0xff)) {
+        const int64_t row = key[j] ? (int64_t)(key[j] >> 32) - 1 : r;
+        const f16* src = a.k + row * a.k_rs + (int64_t)head * D + 8 * cc;
+        const float* part = a.part + row * a.q_rs + (int64_t)(a.hq + head) * D + 8 * cc;
+        h[2 * j] = eight_of<S>(src, part, per_split);
+        h[2 * j + 1] = eight_of<S>(src + D / 2, part + D / 2, per_split);
+        if constexpr (PRO) at_pos[j] = angles_of(a, key[j] ? (int64_t)(key[j] & 0xffffffffu) : 0, cc);
+      }
+    }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int t = t0 + 8 * j;
-      const unsigned long long key = s_slot[t];
-      h[2 * j] = h[2 * j + 1] = f16x8{};
-      if (fresh >> (8 * j) & 0xff) {  // a new row among these eight slots
-        const int64_t row = key ? (int64_t)(key >> 32) - 1 : r;
-        const f16* src = a.k + row * a.k_rs + (int64_t)head * D + 8 * cc;
-        const float* part = a.part + row * a.q_rs + (int64_t)(a.hq + head) * D + 8 * cc;
-        f16x8 lo = eight_of<S>(src, part, per_split), hi = eight_of<S>(src + D / 2, part + D / 2, per_split);
-        if constexpr (PRO)
-          norm_rope(lo, hi, a.kw, a.eps, a.cos_c, a.sin_c, key ? (int64_t)(key & 0xffffffffu) : 0, cc);
-        if (key) {
-          h[2 * j] = lo;
-          h[2 * j + 1] = hi;
-        }
-      }
+      if (PRO && (fresh >> (8 * j) & 0xff)) norm_rope(h[2 * j], h[2 * j + 1], a.kw != nullptr, kw, a.eps, at_pos[j]);
+      if (!key[j]) h[2 * j] = h[2 * j + 1] = f16x8{};
       if (old >> t & 1) {
         h[2 * j] = kv8_values<T>(u32x2{was[j][0], was[j][1]}, power);
         h[2 * j + 1] = kv8_values<T>(u32x2{was[j][2], was[j][3]}, power);
@@ -350,16 +383,22 @@ __global__ __launch_bounds__(kThreads) void kv8_append_kernel(Cache c, AppendArg
   } else {
     const int i = lane & 15, t0 = 4 * (lane >> 4);
     const u32x4 a0 = kv8_transpose(was[0]), a1 = kv8_transpose(was[1]);  // a token a register: dims 8i .. +3, +4 .. +7
-    f16x8 h[4];
+    f16x8 h[4] = {};
+    bool news[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const unsigned long long key = s_slot[t0 + j];
-      h[j] = f16x8{};
-      const int64_t row = (int64_t)(key >> 32) - 1;
-      if (key)
+      news[j] = key != 0;
+      if (S == 0 || (fresh & (0x1111u << j))) {  // a new row among slots j, j + 4, ...
+        const int64_t row = key ? (int64_t)(key >> 32) - 1 : r;
         h[j] = eight_of<S>(a.v + row * a.v_rs + (int64_t)head * D + 8 * i,
                            a.part + row * a.q_rs + (int64_t)(a.hq + c.hkv + head) * D + 8 * i, per_split);
-      else if (old >> (t0 + j) & 1) h[j] = kv8_values<T>(u32x2{a0[j], a1[j]}, power);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f16x8 held = kv8_values<T>(u32x2{a0[j], a1[j]}, power);
+      h[j] = news[j] ? h[j] : old >> (t0 + j) & 1 ? held : f16x8{};
     }
     const Scale s = tile_scale<T>(h, a.status);
     // under the largest scale codes that no writer makes there would be
