@@ -74,7 +74,8 @@ constexpr int kRing = kSlots * kSlot;           // a wave's
 constexpr int kScales = 2 * kWave * 4;          // a wave's words with the K and V scales of its blocks
 // The waves' rings, the query rows and scales.
 constexpr int lds_bytes(int nt) { return kWaves * (kRing + kScales) + nt * 16 * D * 2; }
-static_assert(kMergeWave <= kRing, "the merge reuses the rings");
+constexpr int kMerge8 = kMergeAcc + 3 * 16 * 4;  // a wave's accumulators, maxima and both sums in the merge
+static_assert(kMerge8 <= kRing, "the merge reuses the rings");
 static_assert(2 * lds_bytes(3) <= 160 * 1024, "two workgroups a CU");
 
 // 1 KB from base + off (a lane's 16 bytes), or 64 dwords, into LDS; the compiler
@@ -106,6 +107,13 @@ __device__ inline f16x4 ones_of(uint32_t w) {
 template <int T, int NT>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
 void kv8_attn_kernel(AttnArgs a, Kv8Caches cache, PieceTable pt) {
+  // An output is divided by the sum of its weights as the product had them,
+  // rounded to fp16: where one token has most of a row's weight, the rounding
+  // cancels (a row of 32768 tokens: off by 2.0 to 2.9e-4 of the norm over 14
+  // inputs, 2.0 to 3.3e-4 by the unrounded sum, which the lse needs).  The matrix
+  // cores add them, beside the values: no time at one tile, 1% at two; three tiles
+  // have no registers left (16 x 9 60.8 -> 68 us) and keep the one sum.
+  constexpr bool kRounded = NT < 3;
   __shared__ __align__(16) char smem[lds_bytes(NT)];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -227,6 +235,7 @@ void kv8_attn_kernel(AttnArgs a, Kv8Caches cache, PieceTable pt) {
 
   int row_len[NT];  // causal bound of this lane's row in each tile
   float m[NT], l[NT];
+  f32x4 whole[kRounded ? NT : 1];  // the rounded weights' sums, a row's in every element
   f32x4 acc[NT][8];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
@@ -234,6 +243,7 @@ void kv8_attn_kernel(AttnArgs a, Kv8Caches cache, PieceTable pt) {
     row_len[t] = n < n_rows ? ctx + n / a.gqa + 1 : ctx + q_len;
     m[t] = -INFINITY;
     l[t] = 0.f;
+    if constexpr (kRounded) whole[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int mt = 0; mt < 8; ++mt) acc[t][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -305,6 +315,7 @@ void kv8_attn_kernel(AttnArgs a, Kv8Caches cache, PieceTable pt) {
         const float m_new = fmaxf(m[t], mx);
         const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[t] - m_new);
         l[t] *= alpha;
+        if constexpr (kRounded) whole[t] *= alpha;
 #pragma unroll
         for (int mt = 0; mt < 8; ++mt) acc[t][mt] *= alpha;
         m[t] = m_new;
@@ -313,8 +324,8 @@ void kv8_attn_kernel(AttnArgs a, Kv8Caches cache, PieceTable pt) {
       float psum = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        // weights of at most 2^8 in fp16: 2^-11 of each, as the fp16
-        // attention rounds them; their sum is of the unrounded ones
+        // weights of at most 2^8 in fp16: 2^-11 of each, or 2^-25 of the largest
+        // (a wave has 1024 tokens at most)
         const float pj = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e], a.scale_log2, -m_use));
         psum += pj;
         pb[t][e] = (f16)pj;
@@ -322,6 +333,12 @@ void kv8_attn_kernel(AttnArgs a, Kv8Caches cache, PieceTable pt) {
       l[t] += psum;
     }
 
+    if constexpr (kRounded) {
+      const f16 one = 1.f;
+      const f16x8 ones = {one, one, one, one, one, one, one, one};
+#pragma unroll
+      for (int t = 0; t < NT; ++t) whole[t] = mfma_k32(ones, pb[t], whole[t]);
+    }
     const float vp0 = kv8_power(__builtin_amdgcn_readlane(v_scale, 2 * p));
     const float vp1 = kv8_power(__builtin_amdgcn_readlane(v_scale, 2 * p + 1));
     if constexpr (T == NSD_KV8_E4M3) {
@@ -374,7 +391,7 @@ void kv8_attn_kernel(AttnArgs a, Kv8Caches cache, PieceTable pt) {
   for (int t = 0; t < NT; ++t) {
     const float lt = rows_sum(l[t]);
     __syncthreads();  // the ring, or the previous tile's merge, is read
-    float* mine = mrg + wave * (kMergeWave / 4);
+    float* mine = mrg + wave * (kMerge8 / 4);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -384,25 +401,28 @@ void kv8_attn_kernel(AttnArgs a, Kv8Caches cache, PieceTable pt) {
     if (lg == 0) {
       mine[kMergeAcc / 4 + lr] = m[t];
       mine[kMergeAcc / 4 + 16 + lr] = lt;
+      mine[kMergeAcc / 4 + 32 + lr] = kRounded ? whole[t][0] : lt;
     }
     __syncthreads();
-    float mw[kWaves], lw[kWaves];
+    float mw[kWaves], lw[kWaves], hw[kWaves];
     float M = -INFINITY;
 #pragma unroll
     for (int v = 0; v < kWaves; ++v) {
-      mw[v] = mrg[v * (kMergeWave / 4) + kMergeAcc / 4 + lr];
-      lw[v] = mrg[v * (kMergeWave / 4) + kMergeAcc / 4 + 16 + lr];
+      mw[v] = mrg[v * (kMerge8 / 4) + kMergeAcc / 4 + lr];
+      lw[v] = mrg[v * (kMerge8 / 4) + kMergeAcc / 4 + 16 + lr];
+      hw[v] = mrg[v * (kMerge8 / 4) + kMergeAcc / 4 + 32 + lr];
       M = fmaxf(M, mw[v]);
     }
-    float L = 0.f, sc[kWaves];
+    float L = 0.f, H = 0.f, sc[kWaves];
 #pragma unroll
     for (int v = 0; v < kWaves; ++v) {
       sc[v] = mw[v] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw[v] - M);
       L += lw[v] * sc[v];
+      H += hw[v] * sc[v];
     }
     const int n = 16 * t + lr;
     if (n < n_rows) {
-      const float inv = L > 0.f ? 1.f / L : L != L ? L : 0.f;
+      const float inv = H > 0.f ? 1.f / H : H != H ? H : 0.f;
       const int qi = n / a.gqa, gh = n - qi * a.gqa;
       const int64_t orow = (int64_t)(row_start + qi) * a.hq + head * a.gqa + gh;
       f32x4 out[2];
@@ -412,7 +432,7 @@ void kv8_attn_kernel(AttnArgs a, Kv8Caches cache, PieceTable pt) {
 #pragma unroll
         for (int v = 0; v < kWaves; ++v)
           out[h] +=
-              *reinterpret_cast<const f32x4*>(mrg + v * (kMergeWave / 4) + ((2 * wave + h) * kWave + lane) * 4) * sc[v];
+              *reinterpret_cast<const f32x4*>(mrg + v * (kMerge8 / 4) + ((2 * wave + h) * kWave + lane) * 4) * sc[v];
         out[h] *= inv;
       }
       const int at = 32 * lg + 8 * wave;
