@@ -91,7 +91,8 @@ def oracle_excess(m, layer, q, o, lse, seq_ids, seq_lens):
 @CASES
 def test_stack_is_its_kernels_from_python(gpu, codes, cfg, n_layers, n_req, depth):
     m, sids, slens, toks = model_and_rows(codes, cfg, n_layers, n_req, depth, gpu)
-    stack = DecoderStack(m.mc, m.layers, max_rows=len(sids))
+    room = 128 if depth == 2 else len(sids)
+    stack = DecoderStack(m.mc, m.layers, max_rows=room)
     mine = copy.deepcopy(m.kv8)
     st = build_infer_state(sids, slens, [], m.mc, m.cos, m.sin, gpu)
     for probe_layer in (-1, n_layers - 1, 0):  # rows stored again where they are leave the cache as it is
