@@ -74,13 +74,14 @@ __device__ inline int swz_v(int t) { return 2 * (t & 3); }
 
 // The buffer's loads and waits are inline asm: the compiler does not see
 // them, so it neither drains the loads in flight before every LDS read of
-// the buffer nor moves its own LDS reads across the asm (memory clobber).
+// the buffer nor moves its own LDS reads across the asm (memory clobber); nor
+// does it put the wait state that a load to LDS needs behind the write of m0.
 // No other vector-memory operation is issued inside the block loop.  The
 // loads are non-temporal: every K/V byte is read once per call, and keeping
 // it out of the caches' replacement made the decode and ragged-verify calls
 // 7-10% faster than the default policy on the same pieces.
 __device__ inline void dma_load(uint32_t lds_addr, const void* src) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off nt"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt"
                :
                : "s"(lds_addr), "v"(src)
                : "memory", "m0");

@@ -60,15 +60,17 @@ __device__ inline int chunk_swizzle(int row) { return row & 15; }
 // A weight small enough to stay in the MALL from call to call loses by it
 // (1024 x 3072 called alone again and again 3.8 -> 4.3 us); a forward's
 // weights do not stay.
+// s_nop: the wait state between a write of m0 and a load to LDS, which the
+// compiler does not put into asm.
 template <bool NT>
 __device__ inline void gemm_dma(uint32_t lds_addr, const void* src) {
   if constexpr (NT)
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off nt"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt"
                  :
                  : "s"(lds_addr), "v"(src)
                  : "memory", "m0");
   else
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                  :
                  : "s"(lds_addr), "v"(src)
                  : "memory", "m0");

@@ -79,16 +79,19 @@ static_assert(kMerge8 <= kRing, "the merge reuses the rings");
 static_assert(2 * lds_bytes(3) <= 160 * 1024, "two workgroups a CU");
 
 // 1 KB from base + off (a lane's 16 bytes), or 64 dwords, into LDS; the compiler
-// sees neither the load nor its wait.
+// sees neither the load nor its wait.  Nor does it put the wait states that a load
+// to LDS needs behind a write of m0 (one), or of its base by a VALU (five).
 __device__ inline void dma16(uint32_t lds, const char* base, uint32_t off) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2 nt"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2 nt"
                : : "s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
 __device__ inline void dma16_rows(uint32_t lds, const void* at) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(at) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               : : "s"(lds), "v"(at) : "memory", "m0");
 }
 __device__ inline void dma4(uint32_t lds, const void* at) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" : : "s"(lds), "v"(at) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+               : : "s"(lds), "v"(at) : "memory", "m0");
 }
 template <int N>
 __device__ inline void wait_vm() {

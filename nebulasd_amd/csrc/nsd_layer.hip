@@ -206,15 +206,19 @@ constexpr int kRgMaxRowTiles = 8;   // up to 128 rows of x per pass
 // faster: lm_head 151936 x 4096, 80 rows 236 -> 225 us.  Earlier passes of a
 // call with more than 128 rows keep the default policy: the next pass reads
 // the same weight again.
+// s_nop: the wait state between a write of m0 and a load to LDS, which the
+// compiler does not put into asm.
 template <bool NT>
 __device__ inline void rg_dma(uint32_t lds_addr, const void* src) {
   if constexpr (NT)
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off nt"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt"
                  :
                  : "s"(lds_addr), "v"(src)
                  : "memory", "m0");
   else
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds_addr), "v"(src) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                 :
+                 : "s"(lds_addr), "v"(src) : "memory", "m0");
 }
 template <int N>
 __device__ inline void rg_wait_n() {

@@ -62,8 +62,12 @@ constexpr int kGatherMaxItems = 1536;        // tile offsets a workgroup holds i
 constexpr int kGatherLds = kGatherRing * kGatherSlot + kGatherMaxItems * 8;
 static_assert(2 * kGatherLds <= 160 * 1024, "two workgroups per CU");
 
+// s_nop: the wait state between a write of m0 and a load to LDS, which the
+// compiler does not put into asm.
 __device__ inline void dma16(uint32_t lds_addr, const void* src) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds_addr), "v"(src) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :
+               : "s"(lds_addr), "v"(src) : "memory", "m0");
 }
 template <int N>
 __device__ inline void wait_vm() {
