@@ -130,9 +130,10 @@ int nsd_kv8_load(void* k, void* v, int64_t n_tokens, const nsd_kv8_cache* cache,
 
 /*
  * nsd_paged_attention over an 8-bit cache: the same contract, and the attention
- * over the values that the cache holds, in fp16 products and fp32 sums and
- * softmax; softmax_scale is a positive number.  A NaN in the cache reaches the
- * rows that attend its token and no others.
+ * over the values that the cache holds, with fp32 scores, softmax and sums; a
+ * weight meets the values as two fp16 numbers, 22 bits of it.  softmax_scale is a
+ * positive number.  A NaN in the cache reaches the rows that attend its token and
+ * no others.
  *
  * nsd_kv8_plan_build: its plan (nsd_attn_plan_build's words and checks) for a
  * device of `compute_units`; nsd_attn_plan_bound gives the words for n_workers =

@@ -33,15 +33,16 @@
 // wait of the compiler's drains the tiles behind it.
 //
 // Bound by the tiles' intake, us a call with the merge's launch (the bytes at the
-// 7.0 TB/s of a contiguous read): 64 rows of 512 to 2048 tokens 26.5 (19.1), 16 x
-// 5 of 256 to 4096 18.2 (7.5), 16 x 9 of 1024 to 32768 57.6 (36.8), one row of
-// 32768 17.8 (9.6).  The loads and waits alone, without arithmetic, took 24.6,
+// 7.0 TB/s of a contiguous read): 64 rows of 512 to 2048 tokens 26.9 (19.1), 16 x
+// 5 of 256 to 4096 19.5 (7.5), 16 x 9 of 1024 to 32768 60.5 (36.8), one row of
+// 32768 17.9 (9.6).  The loads and waits alone, without arithmetic, took 24.6,
 // 18.0, 52.7 and 18.6 where the kernel (of then) took 27.2, 20.5, 59.7 and 20.0.  A piece
 // begins with 3 us of latency (ids, then tiles), or 8 to 9 in a compute unit's
 // second workgroup, whose first tiles come behind the burst of everyone's, and
 // ends with 1 to 2.6 of merge; the merge launch takes 3 to 4.
 //
-// Other forms, us in that order unless said:
+// Other forms, us in that order unless said, of the kernel with one fp16 number a
+// weight:
 //   tiles straight into registers, a pair ahead (spills, and a wait for every
 //     load at the loop's head): 30.3, 23.3, 85.3 and 22.4 against 28.5, 20.1, 59.4
 //     and 19.9
@@ -74,15 +75,17 @@ constexpr int kRing = kSlots * kSlot;           // a wave's
 constexpr int kScales = 2 * kWave * 4;          // a wave's words with the K and V scales of its blocks
 // The waves' rings, the query rows and scales.
 constexpr int lds_bytes(int nt) { return kWaves * (kRing + kScales) + nt * 16 * D * 2; }
-constexpr int kMerge8 = kMergeAcc + 3 * 16 * 4;  // a wave's accumulators, maxima and both sums in the merge
-static_assert(kMerge8 <= kRing, "the merge reuses the rings");
+static_assert(kMergeWave <= kRing, "the merge reuses the rings");
 static_assert(2 * lds_bytes(3) <= 160 * 1024, "two workgroups a CU");
 
-// 1 KB from base + off (a lane's 16 bytes), or 64 dwords, into LDS; the compiler
-// sees neither the load nor its wait.  Nor does it put the wait states that a load
-// to LDS needs behind a write of m0 (one), or of its base by a VALU (five).
-__device__ inline void dma16(uint32_t lds, const char* base, uint32_t off) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2 nt"
+// A tile from base + off (a lane's 16 bytes), 1 KB of rows or 64 dwords into LDS;
+// the compiler sees neither the loads nor their wait.  Nor does it put the wait
+// states that a load to LDS needs behind a write of m0 (one), or of its base by a
+// VALU (five).  An offset counts in memory and in LDS: one m0 a tile (one a KB 64 x 1
+// 28.1, 27.9 so; 16 x 5 20.0 and 19.85).
+__device__ inline void dma_tile(uint32_t lds, const char* base, uint32_t off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2 nt\n\t"
+               "global_load_lds_dwordx4 %1, %2 offset:1024 nt"
                : : "s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
 __device__ inline void dma16_rows(uint32_t lds, const void* at) {
@@ -97,6 +100,18 @@ template <int N>
 __device__ inline void wait_vm() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
+
+// A weight goes into the product as two fp16 numbers, itself rounded and what that
+// left: off by 2^-22 of itself at most, or by 2^-25 under the smallest normal
+// number.  The running maximum's own weight is 2^7, so that the latter is 2^-32 of
+// it; the largest, with the lazy maximum, is 2^15.  Outputs then differ from 64 bits
+// by their own rounding alone (2.0 to 2.3e-4 of the norm, as fp32 weights'); from
+// fp32 weights' outputs by 5e-6 to 2e-5.  One fp16 number: 2.1 to 2.9e-4 and 1.6 to
+// 3.2e-4, and the second product's time less, 16 x 5 19.1 for 19.85 us and 16 x 9 59.4
+// for 62.7 in a graph, one tile 0.2 for any length.
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+constexpr float kWeightTop = 7.f;
+static_assert(kLazyMax + kWeightTop < 16.f, "fp16 holds 2^15");
 
 // 0x80 in the bytes of four E4M3 codes that are NaN; and fp16 ones for bytes of
 // 1 (zeros for 0).
@@ -118,13 +133,6 @@ static_assert(sizeof(AttnArgs) + sizeof(Kv8Caches) + sizeof(ShortTable) < 1024, 
 template <int T, int NT, class Table>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
 void kv8_attn_kernel(AttnArgs a, Kv8Caches cache, Table pt) {
-  // An output is divided by the sum of its weights as the product had them,
-  // rounded to fp16: where one token has most of a row's weight, the rounding
-  // cancels (a row of 32768 tokens: off by 2.0 to 2.9e-4 of the norm over 14
-  // inputs, 2.0 to 3.3e-4 by the unrounded sum, which the lse needs).  The matrix
-  // cores add them, beside the values: no time at one tile, 1% at two; three tiles
-  // have no registers left (16 x 9 60.8 -> 68 us) and keep the one sum.
-  constexpr bool kRounded = NT < 3;
   __shared__ __align__(16) char smem[lds_bytes(NT)];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -216,11 +224,8 @@ void kv8_attn_kernel(AttnArgs a, Kv8Caches cache, Table pt) {
     for (int b = 0; b < 2; ++b) {
       if (b == 1 && 2 * p + 1 >= my_n) break;
       const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(tile, 2 * p + b) * kKv8Tile;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        dma16(slot + b * kKv8Tile + 1024 * j, cache.k + at + 1024 * j, lane * 16);
-        dma16(slot + (2 + b) * kKv8Tile + 1024 * j, cache.v + at + 1024 * j, lane * 16);
-      }
+      dma_tile(slot + b * kKv8Tile, cache.k + at, lane * 16);
+      dma_tile(slot + (2 + b) * kKv8Tile, cache.v + at, lane * 16);
     }
   };
   if (pairs > 0) issue(0);
@@ -246,7 +251,6 @@ void kv8_attn_kernel(AttnArgs a, Kv8Caches cache, Table pt) {
 
   int row_len[NT];  // causal bound of this lane's row in each tile
   float m[NT], l[NT];
-  f32x4 whole[kRounded ? NT : 1];  // the rounded weights' sums, a row's in every element
   f32x4 acc[NT][8];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
@@ -254,11 +258,12 @@ void kv8_attn_kernel(AttnArgs a, Kv8Caches cache, Table pt) {
     row_len[t] = n < n_rows ? ctx + n / a.gqa + 1 : ctx + q_len;
     m[t] = -INFINITY;
     l[t] = 0.f;
-    if constexpr (kRounded) whole[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int mt = 0; mt < 8; ++mt) acc[t][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
+  float minus = -1.f;
+  asm("" : "+s"(minus));  // unknown to the compiler, which has conversions and differences for a known one
   for (int p = 0; p < pairs; ++p) {
     // this pair has landed: behind it are the loads of the next
     if (2 * p + 3 < my_n) wait_vm<8>();
@@ -307,7 +312,7 @@ void kv8_attn_kernel(AttnArgs a, Kv8Caches cache, Table pt) {
     const bool masked[2] = {((bad_mask >> (2 * p)) & 1) != 0,
                             2 * p + 1 >= my_n || ((bad_mask >> ((2 * p + 1) & 63)) & 1) != 0};
     const bool edge = masked[0] || masked[1] || first[1] + BS > ctx + 1;  // a token may lie past a row's length
-    f16x8 pb[NT];
+    f16x8 pb[NT], pl[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       float sv[8];
@@ -322,11 +327,10 @@ void kv8_attn_kernel(AttnArgs a, Kv8Caches cache, Table pt) {
           fmaxf(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])), fmaxf(fmaxf(sv[4], sv[5]), fmaxf(sv[6], sv[7])));
       mx = rows_max(mx) * a.scale_log2;  // -inf stays -inf (scale > 0)
       // lazy running max: one decision per wave and tile
-      if (__builtin_amdgcn_ballot_w64(mx > m[t] + kLazyMax) != 0) {
-        const float m_new = fmaxf(m[t], mx);
+      if (__builtin_amdgcn_ballot_w64(mx > m[t] + kLazyMax + kWeightTop) != 0) {
+        const float m_new = fmaxf(m[t], mx - kWeightTop);
         const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[t] - m_new);
         l[t] *= alpha;
-        if constexpr (kRounded) whole[t] *= alpha;
 #pragma unroll
         for (int mt = 0; mt < 8; ++mt) acc[t][mt] *= alpha;
         m[t] = m_new;
@@ -334,22 +338,25 @@ void kv8_attn_kernel(AttnArgs a, Kv8Caches cache, Table pt) {
       const float m_use = m[t] == -INFINITY ? 0.f : m[t];
       float psum = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        // weights of at most 2^8 in fp16: 2^-11 of each, or 2^-25 of the largest
-        // (a wave has 1024 tokens at most)
-        const float pj = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e], a.scale_log2, -m_use));
-        psum += pj;
-        pb[t][e] = (f16)pj;
+      for (int e = 0; e < 8; e += 2) {
+        f32x2 pj;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          pj[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e + i], a.scale_log2, -m_use));
+          psum += pj[i];
+        }
+        const f16x2 hi = __builtin_convertvector(pj, f16x2);  // a fused product and sum takes it as it is
+        const f16x2 lo = {(f16)__builtin_fmaf((float)hi[0], minus, pj[0]),
+                          (f16)__builtin_fmaf((float)hi[1], minus, pj[1])};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          pb[t][e + i] = hi[i];
+          pl[t][e + i] = lo[i];
+        }
       }
       l[t] += psum;
     }
 
-    if constexpr (kRounded) {
-      const f16 one = 1.f;
-      const f16x8 ones = {one, one, one, one, one, one, one, one};
-#pragma unroll
-      for (int t = 0; t < NT; ++t) whole[t] = mfma_k32(ones, pb[t], whole[t]);
-    }
     const float vp0 = kv8_power(__builtin_amdgcn_readlane(v_scale, 2 * p));
     const float vp1 = kv8_power(__builtin_amdgcn_readlane(v_scale, 2 * p + 1));
     if constexpr (T == NSD_KV8_E4M3) {
@@ -389,6 +396,8 @@ void kv8_attn_kernel(AttnArgs a, Kv8Caches cache, Table pt) {
       const f16x8 va = kv8_join(kv8_values4<T>(vb[0][mt / 4][mt % 4], vp0), kv8_values4<T>(vb[1][mt / 4][mt % 4], vp1));
 #pragma unroll
       for (int t = 0; t < NT; ++t) acc[t][mt] = mfma_k32(va, pb[t], acc[t][mt]);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) acc[t][mt] = mfma_k32(va, pl[t], acc[t][mt]);
     }
   }
 
@@ -402,7 +411,7 @@ void kv8_attn_kernel(AttnArgs a, Kv8Caches cache, Table pt) {
   for (int t = 0; t < NT; ++t) {
     const float lt = rows_sum(l[t]);
     __syncthreads();  // the ring, or the previous tile's merge, is read
-    float* mine = mrg + wave * (kMerge8 / 4);
+    float* mine = mrg + wave * (kMergeWave / 4);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -412,28 +421,25 @@ void kv8_attn_kernel(AttnArgs a, Kv8Caches cache, Table pt) {
     if (lg == 0) {
       mine[kMergeAcc / 4 + lr] = m[t];
       mine[kMergeAcc / 4 + 16 + lr] = lt;
-      mine[kMergeAcc / 4 + 32 + lr] = kRounded ? whole[t][0] : lt;
     }
     __syncthreads();
-    float mw[kWaves], lw[kWaves], hw[kWaves];
+    float mw[kWaves], lw[kWaves];
     float M = -INFINITY;
 #pragma unroll
     for (int v = 0; v < kWaves; ++v) {
-      mw[v] = mrg[v * (kMerge8 / 4) + kMergeAcc / 4 + lr];
-      lw[v] = mrg[v * (kMerge8 / 4) + kMergeAcc / 4 + 16 + lr];
-      hw[v] = mrg[v * (kMerge8 / 4) + kMergeAcc / 4 + 32 + lr];
+      mw[v] = mrg[v * (kMergeWave / 4) + kMergeAcc / 4 + lr];
+      lw[v] = mrg[v * (kMergeWave / 4) + kMergeAcc / 4 + 16 + lr];
       M = fmaxf(M, mw[v]);
     }
-    float L = 0.f, H = 0.f, sc[kWaves];
+    float L = 0.f, sc[kWaves];
 #pragma unroll
     for (int v = 0; v < kWaves; ++v) {
       sc[v] = mw[v] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw[v] - M);
       L += lw[v] * sc[v];
-      H += hw[v] * sc[v];
     }
     const int n = 16 * t + lr;
     if (n < n_rows) {
-      const float inv = H > 0.f ? 1.f / H : H != H ? H : 0.f;
+      const float inv = L > 0.f ? 1.f / L : L != L ? L : 0.f;
       const int qi = n / a.gqa, gh = n - qi * a.gqa;
       const int64_t orow = (int64_t)(row_start + qi) * a.hq + head * a.gqa + gh;
       f32x4 out[2];
@@ -443,7 +449,7 @@ void kv8_attn_kernel(AttnArgs a, Kv8Caches cache, Table pt) {
 #pragma unroll
         for (int v = 0; v < kWaves; ++v)
           out[h] +=
-              *reinterpret_cast<const f32x4*>(mrg + v * (kMerge8 / 4) + ((2 * wave + h) * kWave + lane) * 4) * sc[v];
+              *reinterpret_cast<const f32x4*>(mrg + v * (kMergeWave / 4) + ((2 * wave + h) * kWave + lane) * 4) * sc[v];
         out[h] *= inv;
       }
       const int at = 32 * lg + 8 * wave;

@@ -1,0 +1,57 @@
+"""The 8-bit KV cache where a call's answer hangs on more than its kernels' ordinary path: the attention's roundings
+counted, lengths below zero, strides of axes of one, and how many rows a call may have."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_kv8 import CODES, attend, filled, values_of
+
+pytestmark = pytest.mark.gpu
+
+
+def close_weights(cache, table, layer, q, seq_ids, lens, o, scale):
+    """The worst of the outputs' errors over their bounds, for queries of one nonzero dim.
+
+    A score is then one product of an fp16 query and a code's value, 11 x 11 bits: exact in fp32.  What is rounded:
+    the scale times log2(e), and its product with the score against the reference m (steps of the largest of them,
+    halved: 2^-24 each, and m's own cancels, since weights and sum have the same one); exp2, by a step, 2^-23; a weight
+    as a pair of fp16 numbers, 2^-22 of it or 2^-32 of the row's largest; the sums, fp32: a product instruction's by
+    2^-22 of what it has added up at most, two a pair of blocks, and ten steps of merging waves and parts; the output,
+    half a step of fp16.
+    """
+    kk, vv = (x[:, layer] for x in values_of(cache))
+    q, o = q.double().cpu().numpy(), o.double().cpu().numpy()
+    hkv, worst = kk.shape[1], 0.0
+    for r, (sid, n) in enumerate(zip(seq_ids, lens)):
+        ids = table[sid, : -(-n // 16)]
+        k, v = (x[ids].transpose(0, 2, 1, 3).reshape(-1, hkv, 128)[:n] for x in (kk, vv))
+        for h in range(q.shape[1]):
+            s = k[:, h * hkv // q.shape[1]] @ q[r, h] * scale / np.log(2)
+            p = np.exp2(s - s.max())
+            w, total = v[:, h * hkv // q.shape[1]], p.sum()
+            ds = (2 * np.abs(s).max() + np.abs(s - s.max()).max() + 16) * 2.0 ** -24
+            rel = np.log(2) * ds + 2.0 ** -23 + 2.0 ** -22
+            off = (2 * rel + (2 * -(-n // 32) + 10) * 2.0 ** -22) * (p @ np.abs(w)) / total
+            off += 2.0 ** -32 * np.abs(w).sum(0) / total
+            want = p @ w / total
+            off += 2.0 ** -11 * (np.abs(want) + off) + 2.0 ** -25
+            worst = max(worst, (np.abs(o[r, h] - want) / off).max())
+    return worst
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("hq,hkv,q_len,ctxs", [(4, 4, 1, [40, 700]), (16, 8, 1, [300, 5]), (32, 8, 5, [600, 90]),
+                                               (32, 8, 9, [500, 33]), (8, 2, 12, [2500]), (4, 1, 1, [6000])],
+                         ids=["gqa1", "one-tile", "two-tiles", "three-tiles", "pieces-of-three", "pieces-of-one"])
+def test_attention_weights_lose_nothing_that_fp16_outputs_keep(gpu, codes, hq, hkv, q_len, ctxs):
+    mc, ec, table, bt, cache, ids, lens, q = filled(codes, gpu, hq, hkv, ctxs, q_len, seed=21)
+    g = torch.Generator(device=gpu).manual_seed(22)
+    dim = torch.randint(0, 128, (*q.shape[:2], 1), device=gpu, generator=g)
+    q = torch.zeros_like(q).scatter_(2, dim, 8 * torch.randn(dim.shape, device=gpu, generator=g).half())
+    o, _, _ = attend(cache, bt, mc, ec, ids, lens, q)
+    worst = close_weights(cache, table, 1, q, ids, lens, o, mc.head_dim ** -0.5)
+    print(f"worst {worst:.2f} of the bound", flush=True)
+    assert worst <= 1
