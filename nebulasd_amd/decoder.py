@@ -104,7 +104,8 @@ class DecoderStack:
         require(v_cache, torch.float16, "v_cache")
         rows = self._check(x, residual, block_table, engine_config, infer_state, cos_cache, sin_cache)
         n_blocks, n_layers, hkv, bs, d = cache_dims(k_cache)
-        if v_cache.shape != k_cache.shape or n_layers != mc.num_layers or hkv != mc.num_kv_heads or bs != 16:
+        if v_cache.shape != k_cache.shape or n_layers != mc.num_layers or hkv != mc.num_kv_heads or bs != 16 or \
+                d != mc.head_dim:
             raise ValueError("KV caches do not match the model ([blocks, layers, kv heads, 16, head_dim])")
         plan = self._plan(plan_for, rows, infer_state, engine_config, block_table)
         probe = self._probe(rows, probe_layer, x.device)

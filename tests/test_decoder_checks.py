@@ -1,0 +1,54 @@
+"""What the decoder stack refuses before it calls native code (no GPU: the native calls are stand-ins that record)."""
+
+from __future__ import annotations
+
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from nebulasd_amd import decoder
+from nebulasd_amd.config import QWEN3_8B, EngineConfig, ModelConfig
+
+ROWS, BLOCKS = 3, 4
+
+
+@pytest.fixture
+def stack(monkeypatch):
+    """A stack of two layers whose native calls are recorded in ``calls``."""
+    s = object.__new__(decoder.DecoderStack)
+    s.mc = ModelConfig(dict(QWEN3_8B, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2, hidden_size=256))
+    s.max_rows, s._handle, s.calls = 128, SimpleNamespace(value=None), []
+    plan = SimpleNamespace(n_rows=ROWS, workspace_bytes=0, claims=False, host_address=0, host_ptr=lambda: 0,
+                           dev=torch.zeros(1, dtype=torch.int32), workspace=torch.zeros(1, dtype=torch.uint8))
+    monkeypatch.setattr(decoder, "require_cuda", lambda *t: None)
+    monkeypatch.setattr(decoder, "stream_of", lambda t: 0)
+    monkeypatch.setattr(decoder._lib, "call", lambda name, *a: s.calls.append(name))
+    monkeypatch.setattr(decoder, "plan_for", lambda *a: plan)
+    monkeypatch.setattr(decoder, "kv8_plan_for", lambda *a: plan)
+    return s
+
+
+def arguments(stack, cos_d=128):
+    mc = stack.mc
+    half = lambda *shape: torch.zeros(shape, dtype=torch.float16)  # noqa: E731
+    state = SimpleNamespace(num_prefill_seqs=0, num_decoding_seqs=ROWS, seq_ids=torch.zeros(ROWS, dtype=torch.int32),
+                            decoding_seq_lens=torch.ones(ROWS, dtype=torch.int32), softmax_scale=1.0)
+    return dict(x=half(ROWS, mc.hidden_size), residual=half(ROWS, mc.hidden_size),
+                block_table=torch.zeros((2, 5), dtype=torch.int32), engine_config=EngineConfig(max_blocks_per_seq=5),
+                infer_state=state, cos_cache=half(9, cos_d // 2), sin_cache=half(9, cos_d // 2))
+
+
+@pytest.mark.parametrize("cache_d,cos_d", [(64, 128), (64, 64), (128, 64), (256, 128)])
+def test_forward_refuses_other_head_dims(stack, cache_d, cos_d):
+    """Caches, and RoPE tables, of another head_dim than the model's: the stack addresses both by the model's."""
+    cache = torch.zeros((BLOCKS, 2, 2, 16, cache_d), dtype=torch.float16)
+    with pytest.raises(ValueError):
+        stack.forward(k_cache=cache, v_cache=cache, **arguments(stack, cos_d))
+    assert not stack.calls
+
+
+def test_forward_takes_the_models_head_dim(stack):
+    cache = torch.zeros((BLOCKS, 2, 2, 16, 128), dtype=torch.float16)
+    stack.forward(k_cache=cache, v_cache=cache, **arguments(stack))
+    assert stack.calls == ["nsd_decoder_forward"]
