@@ -52,3 +52,22 @@ def test_forward_takes_the_models_head_dim(stack):
     cache = torch.zeros((BLOCKS, 2, 2, 16, 128), dtype=torch.float16)
     stack.forward(k_cache=cache, v_cache=cache, **arguments(stack))
     assert stack.calls == ["nsd_decoder_forward"]
+
+
+def cache8(**change):
+    return SimpleNamespace(**{**dict(device=-1, num_layers=2, num_kv_heads=2, _ref=0), **change})
+
+
+def test_forward_kv8_takes_its_arguments(stack):
+    stack.forward_kv8(cache=cache8(), **arguments(stack))
+    assert stack.calls == ["nsd_decoder_forward_kv8"]
+
+
+@pytest.mark.parametrize("block_size", [8, 32])
+def test_forward_kv8_refuses_other_block_sizes(stack, block_size):
+    """A cache's blocks hold 16 tokens: with another size the table's entries would mean other tokens."""
+    args = arguments(stack)
+    args["engine_config"] = EngineConfig(block_size=block_size, max_blocks_per_seq=5)
+    with pytest.raises(ValueError, match="block_size"):
+        stack.forward_kv8(cache=cache8(), **args)
+    assert not stack.calls
