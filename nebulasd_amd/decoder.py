@@ -18,13 +18,14 @@ it reads them).  The embedding lookup and the post-layer stay in Python.
 from __future__ import annotations
 
 import ctypes
+from contextlib import nullcontext
 from ctypes import c_void_p
 
 import torch
 
 from . import _lib
 from .kernels._util import cache_dims, check_block_table, ptr, require, require_cuda, stream_of
-from .kernels.kv8 import KV8Cache, _table
+from .kernels.kv8 import KV8Cache, _decode_rows, _on, _prologue_tables, _table
 from .plan import kv8_plan_for, plan_for
 
 __all__ = ["DecoderStack", "MAX_ROWS"]
@@ -123,19 +124,23 @@ class DecoderStack:
                     probe_layer: int = -1):
         """``forward`` over an 8-bit cache, the same arguments and result."""
         rows = self._check(x, residual, block_table, engine_config, infer_state, cos_cache, sin_cache)
-        if x.get_device() != cache.device:
-            raise ValueError(f"x is on {x.device}, the cache on cuda:{cache.device}")
+        _on(cache, x, residual)
+        if self._layers[0]["wqkv"].get_device() != cache.device:
+            raise ValueError(f"the cache is on cuda:{cache.device}, the weights elsewhere")
         table = _table(cache, block_table, engine_config)
-        plan = self._plan(kv8_plan_for, rows, infer_state, engine_config, block_table)
-        size, ws = plan.workspace_bytes, None
-        if size:  # the layers' in turn; the claim counter at its start is zero between them
-            ws = (x.new_zeros if plan.claims else x.new_empty)(size, dtype=torch.uint8)
-        probe = self._probe(rows, probe_layer, x.device)
-        _lib.call("nsd_decoder_forward_kv8", self._handle, x.data_ptr(), residual.data_ptr(), rows, cache._ref,
-                  *table, infer_state.seq_ids.data_ptr(), infer_state.decoding_seq_lens.data_ptr(),
-                  cos_cache.data_ptr(), sin_cache.data_ptr(), cos_cache.shape[0], plan.host_address,
-                  plan.dev.data_ptr(), ptr(ws), size, float(infer_state.softmax_scale), int(probe_layer),
-                  *(t.data_ptr() for t in probe) if probe else (None, None, None), None, stream_of(x))
+        seq_ids, seq_lens, _ = _decode_rows(cache, infer_state)
+        positions = _prologue_tables(cache, None, None, cos_cache, sin_cache)
+        current = torch.cuda.current_device() == cache.device
+        with nullcontext() if current else torch.cuda.device(cache.device):
+            plan = self._plan(kv8_plan_for, rows, infer_state, engine_config, block_table)
+            size, ws = plan.workspace_bytes, None
+            if size:  # the layers' in turn; the claim counter at its start is zero between them
+                ws = (x.new_zeros if plan.claims else x.new_empty)(size, dtype=torch.uint8)
+            probe = self._probe(rows, probe_layer, x.device)
+            _lib.call("nsd_decoder_forward_kv8", self._handle, x.data_ptr(), residual.data_ptr(), rows, cache._ref, *table,
+                      seq_ids, seq_lens, cos_cache.data_ptr(), sin_cache.data_ptr(), positions, plan.host_address,
+                      plan.dev.data_ptr(), ptr(ws), size, float(infer_state.softmax_scale), int(probe_layer),
+                      *(t.data_ptr() for t in probe) if probe else (None, None, None), None, stream_of(x))
         return probe
 
     def _check(self, x, residual, block_table, engine_config, infer_state, cos_cache, sin_cache) -> int:
