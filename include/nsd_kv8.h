@@ -29,11 +29,16 @@
  * where it changes.  Slots above hold no token (rows of a rejected draft, or of
  * the block's earlier owner), count for nothing and keep their codes (V's end as
  * zeros under the largest scale, where a code past the largest value would be an
- * infinity).  A scale
- * that grows at least doubles, so however often a token is rounded again it
- * ends less than one of the last scale's steps (E4M3: of the value's own steps)
- * from its value; one that shrinks loses nothing.  Free scales would let every
- * append cost another half step.
+ * infinity).  A scale that grows at least doubles, so however often a token is
+ * rounded again it ends from its value by less than one step of the largest scale
+ * that its block has had since (E4M3: of the value's own steps under that scale);
+ * a scale that shrinks loses nothing, and brings nothing back.  Free scales would
+ * let every append cost another half step.
+ *
+ * So rows that are written over later, a rejected draft's, leave the tokens below
+ * them, and accepted rows of their own call, on the grid of their scale.  Where
+ * tokens must not depend on them, the bytes of the sequence's last block are copied
+ * before such a call and put back after it, and the accepted rows stored again.
  *
  * Layout: codes [num_blocks, num_layers, num_kv_heads, 2048 bytes], scales
  * uint8 [num_blocks, num_layers, num_kv_heads], each for K and for V, so that a

@@ -10,8 +10,8 @@ caches) and take a ``KV8Cache`` in place of ``k_cache, v_cache``; prompts attend
 A block of 16 tokens holds, for every layer and kv head, 16 x 128 codes and one power of two for K, and the same for
 V.  Codes are E4M3 (4 significant bits, whatever a value's size) or whole numbers from -127 to 127 (7 bits of the
 block's largest).  Every value of a cache is an fp16 value, so reading back is exact.  ``include/nsd_kv8.h`` states
-the format, what a row does to the tokens that its block holds already, and what becomes of values that are not
-finite.
+the format, what a row, rejected later or not, does to the tokens that its block holds already, and what becomes of
+values that are not finite.
 """
 
 from __future__ import annotations

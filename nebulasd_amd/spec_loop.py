@@ -299,7 +299,8 @@ def run(n_requests=512, prompt_lo=128, prompt_hi=1024, new_tokens=128, draft_bat
     so verifies of different batches run side by side too.  Results are the
     same either way.
 
-    ``kv_codes``: both models' caches in 8 bits (``RandomQwen3``).
+    ``kv_codes``: both models' caches in 8 bits (``RandomQwen3``).  Rejected rows larger than their block's tokens leave
+    these coarser (``include/nsd_kv8.h``), so outputs may differ from plain decoding's over such a cache.
     """
     dev = torch.device(device)
     rng = np.random.default_rng(seed)

@@ -3,11 +3,14 @@ counted, lengths below zero, strides of axes of one, and how many rows a call ma
 
 from __future__ import annotations
 
+import copy
+
 import numpy as np
 import pytest
 import torch
 
-from test_gpu_kv8 import CODES, attend, filled, values_of
+from nebulasd_amd.kernels import kv8_store
+from test_gpu_kv8 import CODES, Mirror, attend, filled, gpu_of, make, rows_of, state, values_of
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +58,43 @@ def test_attention_weights_lose_nothing_that_fp16_outputs_keep(gpu, codes, hq, h
     worst = close_weights(cache, table, 1, q, ids, lens, o, mc.head_dim ** -0.5)
     print(f"worst {worst:.2f} of the bound", flush=True)
     assert worst <= 1
+
+
+@pytest.mark.parametrize("codes", CODES)
+def test_a_block_put_back_has_not_seen_rejected_rows(gpu, codes):
+    """Verify steps whose rejected rows are far larger than the tokens: written over, they leave the tokens below within a
+    step of the largest scale; the block put back and the accepted rows stored again are a cache that never saw them."""
+    mc, ec, rng, table, bt, cache = make(codes, gpu, seqs=1, seed=23)
+    back, never = copy.deepcopy(cache), copy.deepcopy(cache)
+    tensors = lambda c: (c.k, c.v, c.k_scales, c.v_scales)  # noqa: E731
+    put = lambda c, x, at: kv8_store(gpu_of(x[0]), gpu_of(x[1]), c, bt, mc, ec, state(  # noqa: E731
+        mc, [0] * len(x[0]), list(range(at + 1, at + 1 + len(x[0])))), 1, validate=True)
+    m, have, kept, most = Mirror(cache, 1, codes), 0, [], np.full(128, -99)
+    rows = lambda n: [rows_of(rng, n, 2, sizes=0.0) for _ in range(2)]  # noqa: E731
+    for step in range(20):
+        good, bad = rows(1 + step % 3), [x * np.float16(2.0 ** (6 if step % 4 else 11)) for x in rows(2)]
+        n, both = len(good[0]), [np.concatenate(x) for x in zip(good, bad)]
+        blk = table[0, have // 16]
+        saved = [t[blk].clone() for t in tensors(back)]
+        for c in (cache, back):
+            put(c, both, have)
+        m.append(table, [0] * (n + 2), list(range(have + 1, have + n + 3)), *both)
+        m.check(cache)
+        for b in range(have // 16, (have + n + 1) // 16 + 1):
+            part = slice(16 * b, min(16 * b + 16, have + n))
+            most[part] = np.maximum(most[part], max(p[table[0, b]].max() for p in m.power))
+        for t, s in zip(tensors(back), saved):
+            t[blk] = s
+        for c in (back, never):
+            put(c, good, have)
+        kept.append(good)
+        have += n
+    want = [np.concatenate(x) for x in zip(*kept)]
+    live = table[0, : have // 16]  # whole blocks: behind the last token nothing counts
+    for a, b in zip(tensors(back), tensors(never)):
+        assert torch.equal(a[live.tolist()], b[live.tolist()])
+    for w, got in zip(want, m.tokens(table, 0, have)):
+        own = 2.0 ** (np.frexp(np.abs(w.astype(np.float64)))[1] - 4)
+        step = np.ldexp(1.0, most[:have])[:, None, None]
+        off = np.abs(got - w.astype(np.float64))
+        assert (off < (step if codes == "int8" else np.maximum(step * 2.0 ** -9, own))).all()

@@ -310,3 +310,28 @@ def test_python_refusals():
         KV8Cache.pack(k.view(torch.int8), k.view(torch.int8), s, s)
     for f in (kv8_load, kv8_paged_attention, kv8_qk_norm_rope_store, kv8_store):
         assert f.__doc__
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("size", [16.0, 64.0, 1024.0, 4096.0])
+def test_rejected_rows_leave_the_grid_of_their_scale(codes, size):
+    """A history of steps of two rows, the second rejected and now and then far larger: tokens that stay end less than one
+    step of the largest scale since they were written from their values (E4M3: of the value's own steps under it), not
+    of the last; a block that never saw those rows keeps them within a step of its own."""
+    rng = np.random.default_rng(8)
+    rows = rng.standard_normal((16, 128)).astype(np.float16).astype(np.float64)
+    held, alone = np.full((16, 128), np.nan), np.full((16, 128), np.nan)
+    most = np.full(16, -99)
+    for t in range(15):
+        draft = (rng.standard_normal(128) * (size if t % 4 == 1 else 0.5)).astype(np.float16).astype(np.float64)
+        held, _, e = kv8_append(held, {t: rows[t], t + 1: draft}, codes)
+        most[: t + 1] = np.maximum(most[: t + 1], e)
+        held, _, e = kv8_append(held, {t: held[t]}, codes)  # the scale without the draft
+        alone, _, e1 = kv8_append(alone, {t: rows[t]}, codes)
+    own = 2.0 ** (np.frexp(np.abs(rows[:15]))[1] - 4)
+    step = lambda e: 2.0 ** e if codes == "int8" else np.maximum(2.0 ** (e - 9), own)  # noqa: E731
+    off = np.abs(held[:15] - rows[:15])
+    assert (off < step(most[:15, None].astype(float))).all()
+    assert (np.abs(alone[:15] - rows[:15]) < step(float(e1))).all()
+    if codes == "int8" or size > 1000:
+        assert (off >= step(float(e))).any(), "these rows do not tell the two bounds apart"
