@@ -88,6 +88,8 @@ typedef struct {
  * nsd_kv8_store: nsd_store_kvcache into an 8-bit cache (row r of k, v fp16
  * [n_rows, Hkv, 128] to position seq_lens[r] - 1 of block_table[seq_ids[r]]).
  * nsd_kv8_store_prefill: nsd_store_kvcache_prefill, of k, v [n_tokens, Hkv, 128].
+ * Every decode/verify row is compared with every other: at most 65536 rows a call,
+ * here and in the prologues, and time by their square from about 500 on.
  */
 int nsd_kv8_store(const void* k, const void* v, const nsd_kv8_cache* cache, const int32_t* block_table,
                   int64_t bt_rows, int64_t bt_stride, const int32_t* seq_ids, const int32_t* seq_lens,

@@ -9,8 +9,8 @@ import numpy as np
 import pytest
 import torch
 
-from nebulasd_amd.kernels import kv8_store
-from test_gpu_kv8 import CODES, Mirror, attend, filled, gpu_of, make, rows_of, state, values_of
+from nebulasd_amd.kernels import KV8Cache, kv8_store
+from test_gpu_kv8 import CODES, Mirror, attend, config, filled, gpu_of, make, rows_of, state, values_of
 
 pytestmark = pytest.mark.gpu
 
@@ -98,3 +98,18 @@ def test_a_block_put_back_has_not_seen_rejected_rows(gpu, codes):
         step = np.ldexp(1.0, most[:have])[:, None, None]
         off = np.abs(got - w.astype(np.float64))
         assert (off < (step if codes == "int8" else np.maximum(step * 2.0 ** -9, own))).all()
+
+
+def test_as_many_rows_as_a_call_takes(gpu):
+    """65536 rows that fill 4096 blocks, in any order: the bytes of as many prompts of a block."""
+    mc, ec = config(1, 1, 1, 1)
+    rows, one = (KV8Cache.allocate(4096, mc, torch.int8, gpu) for _ in range(2))
+    g = torch.Generator(device=gpu).manual_seed(24)
+    bt = torch.randperm(4096, device=gpu, generator=g).to(torch.int32).view(4096, 1)
+    k, v = (torch.randn(1 << 16, 1, 128, device=gpu, generator=g).half() for _ in range(2))
+    kv8_store(k, v, one, bt, mc, ec, state(mc, [], [], [16] * 4096, range(4096)), 0, validate=True)
+    order = torch.randperm(1 << 16, device=gpu, generator=g)
+    ids, lens = (order // 16).tolist(), (order % 16 + 1).tolist()
+    kv8_store(k[order], v[order], rows, bt, mc, ec, state(mc, ids, lens), 0, validate=True)
+    for a, b in zip((rows.k, rows.v, rows.k_scales, rows.v_scales), (one.k, one.v, one.k_scales, one.v_scales)):
+        assert torch.equal(a, b)

@@ -335,3 +335,12 @@ def test_rejected_rows_leave_the_grid_of_their_scale(codes, size):
     assert (np.abs(alone[:15] - rows[:15]) < step(float(e1))).all()
     if codes == "int8" or size > 1000:
         assert (off >= step(float(e))).any(), "these rows do not tell the two bounds apart"
+
+
+def test_c_refuses_more_rows_than_an_append_compares():
+    """Rows are compared with each other: a count that would hold the GPU for seconds is refused, the one below taken."""
+    c = _c()
+    for args in (_store, _prologue):
+        assert "65536" in _refused(*args(c, rows=(1 << 16) + 1))
+    assert "65536" in _refused("nsd_kv8_qk_norm_rope_store_partials", 16, 2, 16, None, None, 1e-6, 16, 16, 8,
+                               ctypes.byref(c), 16, 2, 4, 16, 16, (1 << 16) + 1, 0, 4, None, None)
