@@ -454,7 +454,10 @@ __global__ __launch_bounds__(kThreads) void kv8_prefill_kernel(
   const int64_t b = blockIdx.x / groups, s = blockIdx.y;
   const int group = blockIdx.x % groups;
   const int64_t len = lens[s], start = start_locs[s], sid = seq_ids[s];
-  if (b * BS >= len) return;
+  if (b * BS >= len) {
+    if (len < 0 && blockIdx.x == 0 && threadIdx.x == 0) flag_status(status, NSD_STATUS_BAD_SEQ);
+    return;
+  }
   const int lane = threadIdx.x & 63;
   const int unit = group * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool first = group == 0 && threadIdx.x == 0;
@@ -528,9 +531,9 @@ __global__ __launch_bounds__(kThreads) void kv8_load_kernel(
   const int group = blockIdx.x % groups;
   const int64_t first = firsts != nullptr ? firsts[s] : 0, len = lens[s], start = start_locs[s], sid = seq_ids[s];
   const int64_t end = first + len;
-  if (len <= 0) return;
+  if (len == 0) return;
   const bool says = blockIdx.x == 0 && threadIdx.x == 0;
-  if (sid < 0 || sid >= bt_rows || first < 0 || end > bt_stride * BS || len > max_len || start < 0 ||
+  if (len < 0 || sid < 0 || sid >= bt_rows || first < 0 || end > bt_stride * BS || len > max_len || start < 0 ||
       start + len > n_tokens) {
     if (says) flag_status(status, NSD_STATUS_BAD_SEQ);
     return;

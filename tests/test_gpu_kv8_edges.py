@@ -9,7 +9,7 @@ import numpy as np
 import pytest
 import torch
 
-from nebulasd_amd.kernels import KV8Cache, kv8_store
+from nebulasd_amd.kernels import KV8Cache, kv8_load, kv8_store
 from test_gpu_kv8 import CODES, Mirror, attend, config, filled, gpu_of, make, rows_of, state, values_of
 
 pytestmark = pytest.mark.gpu
@@ -113,3 +113,25 @@ def test_as_many_rows_as_a_call_takes(gpu):
     kv8_store(k[order], v[order], rows, bt, mc, ec, state(mc, ids, lens), 0, validate=True)
     for a, b in zip((rows.k, rows.v, rows.k_scales, rows.v_scales), (one.k, one.v, one.k_scales, one.v_scales)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("n", [-1, -16, -(2 ** 31)])
+def test_lengths_below_zero_are_flagged(gpu, codes, n):
+    """Of three prompts, and three ranges to read, the one of a negative length is left out and flagged."""
+    mc, ec, rng, table, bt, cache = make(codes, gpu, seqs=3, seed=25)
+    k, v = gpu_of(rows_of(rng, 40, 2)), gpu_of(rows_of(rng, 40, 2))
+    want = copy.deepcopy(cache)
+    kv8_store(k, v, want, bt, mc, ec, state(mc, [], [], [17, 0, 23], range(3)), 0, validate=True)
+    st = state(mc, [], [], [17, 0, 23], range(3))
+    st.prefill_seq_lens = torch.tensor([17, n, 23], dtype=torch.int32, device=gpu)
+    with pytest.raises(RuntimeError, match="outside the block table"):
+        kv8_store(k, v, cache, bt, mc, ec, st, 0, validate=True)
+    assert all(torch.equal(a, b) for a, b in zip((cache.k, cache.v, cache.k_scales), (want.k, want.v, want.k_scales)))
+    outs = [[torch.full((40, 2, 128), 7.0, dtype=torch.float16, device=gpu) for _ in range(2)] for _ in range(2)]
+    kv8_load(*outs[0], cache, bt, st.seq_ids, st.prefill_seq_start_locs, st.prefill_seq_lens.clamp(min=0), 23, 0, validate=True)
+    for first in (None, torch.zeros(3, dtype=torch.int32, device=gpu)):
+        with pytest.raises(RuntimeError, match="outside the block table"):
+            kv8_load(*outs[1], cache, bt, st.seq_ids, st.prefill_seq_start_locs, st.prefill_seq_lens, 23, 0, first=first,
+                     validate=True)
+        assert all(torch.equal(a, b) for a, b in zip(*outs))
