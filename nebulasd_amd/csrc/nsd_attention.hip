@@ -718,6 +718,7 @@ int paged_attention_impl(const void* q, void* o, float* lse, const void* k_cache
                                    bt_rows, bt_stride, plan_host, plan_dev, part, part_capacity, sizeof(f16),
                                    softmax_scale, status, &c);
   if (rc != NSD_OK || c.grid == 0) return rc;
+  end_table(c.pieces.e, c.args.piece_table ? c.args.n_static : 0);
   hipStream_t st = as_stream(stream);
   const int launched = fused != nullptr
                      ? (c.row_tiles == 1   ? launch_nt_fused<1>(c.args, c.pieces, *fused, c.grid, st)

@@ -3,6 +3,8 @@
 
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "nsd_attn.h"
 
 namespace nsd {
@@ -101,6 +103,18 @@ bool plan_keeps_sequences_whole(const int32_t* plan_host);
 constexpr int64_t kClaimBytes = 256;
 inline int64_t plan_workspace_bytes(int64_t n_slots, int64_t rows_max, int elem = 2) {
   return kClaimBytes + (n_slots * rows_max * (int64_t)(kHeadDim * elem + 4) + 255) / 256 * 256;
+}
+
+// A launch's table with its first n entries filled: zeros behind them, as a launch
+// takes all of it; and a short table of the first n entries of a long one.
+template <typename E, size_t N>
+inline void end_table(E (&table)[N], int n) {
+  std::fill(table + n, table + N, E{});
+}
+template <typename E, size_t N>
+inline void short_table(E (&table)[N], const E* from, int n) {
+  std::copy(from, from + n, table);
+  end_table(table, n);
 }
 
 }  // namespace nsd

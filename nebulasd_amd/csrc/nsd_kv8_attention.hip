@@ -482,11 +482,15 @@ void launch_rows(const AttnCall& c, const Kv8Caches& caches, const Table& table,
   else go(kv8_attn_kernel<T, 3, Table>);
 }
 template <int T>
-void launch_codes(const AttnCall& c, const Kv8Caches& caches, hipStream_t st) {
+void launch_codes(AttnCall& c, const Kv8Caches& caches, hipStream_t st) {
   ShortTable few;
   constexpr int kFew = sizeof(few.e) / sizeof(few.e[0]);
-  if (c.args.n_static > kFew) return launch_rows<T>(c, caches, c.pieces, st);
-  std::copy_n(c.pieces.e, kFew, few.e);
+  const int filled = c.args.piece_table ? c.args.n_static : 0;
+  if (c.args.n_static > kFew) {
+    end_table(c.pieces.e, filled);
+    return launch_rows<T>(c, caches, c.pieces, st);
+  }
+  short_table(few.e, c.pieces.e, filled);
   launch_rows<T>(c, caches, few, st);
 }
 

@@ -480,10 +480,11 @@ int launch_merge(const char* who, const AttnCall& call, const int32_t* plan_host
     const int groups = (args.rows_max * SL + 15) / 16;
     if (packed && n_combine <= kCombineTableFew) {
       CombineTable<kCombineTableFew> few;
-      std::copy_n(tab.e, kCombineTableFew, few.e);
+      short_table(few.e, tab.e, n_combine);
       hipLaunchKernelGGL((combine_table_kernel<SL, P, kCombineTableFew>), dim3(n_combine, groups), dim3(256), 0, st,
                          args, few);
     } else if (packed) {
+      end_table(tab.e, n_combine);
       hipLaunchKernelGGL((combine_table_kernel<SL, P, kCombineTableMax>), dim3(n_combine, groups), dim3(256), 0, st,
                          args, tab);
     } else {
