@@ -158,6 +158,11 @@ def _rows(cache: KV8Cache, t: torch.Tensor, name: str, rows: int, heads: int) ->
         if per_dim == 1 and per_head == HEAD_DIM and apart % 8 == 0 and apart >= heads * HEAD_DIM and \
                 t.data_ptr() % 16 == 0:
             return apart
+        # the stride of an axis of one says nothing
+        apart = apart if rows > 1 else heads * HEAD_DIM
+        if per_dim == 1 and (per_head == HEAD_DIM or heads == 1) and apart % 8 == 0 and apart >= heads * HEAD_DIM and \
+                t.data_ptr() % 16 == 0:
+            return apart
     _on(cache, t)
     if t.dtype != _F16:
         raise TypeError(f"{name} must be torch.float16, got {t.dtype}")
