@@ -4,6 +4,7 @@
 #include <stdio.h>
 
 #include <algorithm>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -62,10 +63,10 @@ struct PlanCut {
   int n_workers, static_slots, min_blocks, few;
 };
 
-static int build_plan(const int32_t* seq_ids, const int32_t* seq_lens, int64_t n_rows, int num_q_heads,
-                      int num_kv_heads, int head_dim, int block_size, int64_t bt_rows, int64_t bt_stride, PlanCut cut,
-                      int max_group_rows, int32_t* plan, int64_t plan_capacity, int64_t* plan_words,
-                      int64_t* workspace_bytes) {
+static int cut_plan(const int32_t* seq_ids, const int32_t* seq_lens, int64_t n_rows, int num_q_heads,
+                    int num_kv_heads, int head_dim, int block_size, int64_t bt_rows, int64_t bt_stride, PlanCut cut,
+                    int max_group_rows, int32_t* plan, int64_t plan_capacity, int64_t* plan_words,
+                    int64_t* workspace_bytes) {
   if (n_rows < 0) return fail(NSD_ERR_INVALID, "plan: n_rows=%lld < 0", (long long)n_rows);
   if (n_rows > 0 && (seq_ids == nullptr || seq_lens == nullptr))
     return fail(NSD_ERR_INVALID, "plan: null seq_ids/seq_lens");
@@ -110,6 +111,8 @@ static int build_plan(const int32_t* seq_ids, const int32_t* seq_lens, int64_t n
   }
   const int64_t n_groups = (int64_t)groups.size() / 4;
   const int64_t n_segs = n_groups * num_kv_heads;
+  if (n_segs > INT32_MAX / kPieceWords)  // a record of its own each
+    return fail(NSD_ERR_INVALID, "plan: too large (%lld segments)", (long long)n_segs);
 
   // 2. block counts per segment (segment = group * Hkv + kv head).
   std::vector<int64_t> seg_start(n_segs + 1, 0);
@@ -334,6 +337,16 @@ static int build_plan(const int32_t* seq_ids, const int32_t* seq_lens, int64_t n
   *plan_words = words;
   *workspace_bytes = n_combines > 0 || n_claimed > 0 ? plan_workspace_bytes(n_slots, rows_max) : 0;
   return NSD_OK;
+}
+
+// What the vectors need may not be there: no exception leaves a C entry.
+template <typename... Args>
+static int build_plan(Args... args) {
+  try {
+    return cut_plan(args...);
+  } catch (const std::bad_alloc&) {
+    return fail(NSD_ERR_INVALID, "plan: out of host memory");
+  }
 }
 
 extern "C" int nsd_attn_plan_build(const int32_t* seq_ids, const int32_t* seq_lens, int64_t n_rows,

@@ -3,6 +3,8 @@
 from __future__ import annotations
 
 import ctypes
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -10,6 +12,7 @@ import torch
 
 import oracle
 from nebulasd_amd import _lib
+from nebulasd_amd.build import ROOT
 from nebulasd_amd.kernels import KV8Cache, kv8_load, kv8_paged_attention, kv8_qk_norm_rope_store, kv8_store
 from nebulasd_amd.kernels.kv8 import _Cache
 from oracle.kv8 import (KV8_E4M3, KV8_RANGES, kv8_append, kv8_attention, kv8_exponent, kv8_round, kv8_tiles,
@@ -344,3 +347,21 @@ def test_c_refuses_more_rows_than_an_append_compares():
         assert "65536" in _refused(*args(c, rows=(1 << 16) + 1))
     assert "65536" in _refused("nsd_kv8_qk_norm_rope_store_partials", 16, 2, 16, None, None, 1e-6, 16, 16, 8,
                                ctypes.byref(c), 16, 2, 4, 16, 16, (1 << 16) + 1, 0, 4, None, None)
+
+
+@pytest.mark.parametrize("rows,heads", [(4096, 2 ** 31 - 1), (1, 2 ** 31 - 1), (64, 1 << 24)])
+def test_plans_too_large_are_refused(rows, heads):
+    """More segments than a plan can hold: an error, where the planner's memory ran out and ended the process (so in a
+    process of its own)."""
+    code = f"""
+import ctypes, numpy as np
+from nebulasd_amd import _lib
+ids, lens, buf = np.arange({rows}, dtype=np.int32), np.ones({rows}, np.int32), np.zeros(64, np.int32)
+at = lambda a: a.ctypes.data_as(ctypes.POINTER(ctypes.c_int32))
+lib, words = _lib.load(), ctypes.c_int64()
+rc = lib.nsd_kv8_plan_build(at(ids), at(lens), {rows}, {heads}, {heads}, {rows}, 1, 256, 0, at(buf), 64, ctypes.byref(words))
+assert rc == 1, rc  # NSD_ERR_INVALID
+assert b"too large" in lib.nsd_last_error(), lib.nsd_last_error()
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=60)
+    assert done.returncode == 0, done.stderr
