@@ -189,6 +189,11 @@ class AttnPlan:
         return self.host.ctypes.data
 
     @cached_property
+    def device(self) -> int:
+        """The number of the GPU that the plan is on."""
+        return self.dev.get_device()
+
+    @cached_property
     def claims(self) -> bool:
         """Whether some pieces are claimed at run time (their counter, at the workspace's start, begins at zero)."""
         return int(self.host[_lib.PLAN_CLAIMED]) > 0
@@ -263,7 +268,8 @@ def kv8_plan_for(infer_state, model_config, engine_config, block_table) -> AttnP
     import torch
 
     plan = getattr(infer_state, "kv8_plan", None)
-    if plan is None or not plan.fits(model_config.num_q_heads, model_config.num_kv_heads, block_table):
+    if plan is None or plan.device != block_table.get_device() or \
+            not plan.fits(model_config.num_q_heads, model_config.num_kv_heads, block_table):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("the attention plan has to be built before the capture (kv8_plan_for, or an eager call)")
         sids, slens = _decode_rows(infer_state)

@@ -33,3 +33,25 @@ def test_rows_of_any_layout_with_contiguous_heads(t, rows, heads, apart):
 def test_rows_of_apart_heads_are_refused(t, rows, heads):
     with pytest.raises(ValueError):
         kv8._rows(HERE, t, "q", rows, heads)
+
+
+class Elsewhere(torch.Tensor):
+    """A tensor that says it is on another GPU."""
+
+    def get_device(self):
+        return 5
+
+
+def test_a_plan_on_another_gpu_is_not_used(monkeypatch):
+    """An infer state whose plan was made beside another cache's block table: the kernel would read it from that GPU."""
+    from nebulasd_amd import plan
+
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "get_device_properties", lambda d: SimpleNamespace(multi_processor_count=256))
+    mc, ec = SimpleNamespace(num_q_heads=4, num_kv_heads=2), SimpleNamespace()
+    table = torch.zeros((2, 5), dtype=torch.int32)
+    st = SimpleNamespace(seq_ids_list=[0, 1], decoding_seq_lens_list=[7, 80])
+    first = plan.kv8_plan_for(st, mc, ec, table)
+    assert plan.kv8_plan_for(st, mc, ec, table) is first  # the forward's, for every layer
+    other = plan.kv8_plan_for(st, mc, ec, table.as_subclass(Elsewhere))
+    assert other is not first and st.kv8_plan is other
