@@ -325,10 +325,13 @@ void kv8_attn_kernel(AttnArgs a, Kv8Caches cache, Table pt) {
       }
       float mx =
           fmaxf(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])), fmaxf(fmaxf(sv[4], sv[5]), fmaxf(sv[6], sv[7])));
-      mx = rows_max(mx) * a.scale_log2;  // -inf stays -inf (scale > 0)
-      // lazy running max: one decision per wave and tile
-      if (__builtin_amdgcn_ballot_w64(mx > m[t] + kLazyMax + kWeightTop) != 0) {
-        const float m_new = fmaxf(m[t], mx - kWeightTop);
+      mx = rows_max(mx);
+      // lazy running max: one decision per wave and tile, on the largest weight's own
+      // exponent (large scores' maxima and references are whole steps apart: by
+      // them, one may have 2^18 where the other says 2^15).  -inf stays -inf (scale >
+      // 0), and -inf less itself decides nothing
+      if (__builtin_amdgcn_ballot_w64(__builtin_fmaf(mx, a.scale_log2, -m[t]) > kLazyMax + kWeightTop) != 0) {
+        const float m_new = fmaxf(m[t], __builtin_fmaf(mx, a.scale_log2, -kWeightTop));
         const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[t] - m_new);
         l[t] *= alpha;
 #pragma unroll

@@ -10,7 +10,8 @@ import pytest
 import torch
 
 from nebulasd_amd.kernels import KV8Cache, kv8_load, kv8_store
-from test_gpu_kv8 import CODES, Mirror, attend, config, filled, gpu_of, make, rows_of, state, values_of
+from test_gpu_kv8 import (CODES, DTYPE, Mirror, attend, config, filled, gpu_of, make, rows_of, state,
+                          values_of)
 
 pytestmark = pytest.mark.gpu
 
@@ -135,3 +136,41 @@ def test_lengths_below_zero_are_flagged(gpu, codes, n):
             kv8_load(*outs[1], cache, bt, st.seq_ids, st.prefill_seq_start_locs, st.prefill_seq_lens, 23, 0, first=first,
                      validate=True)
         assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("q_len", [1, 5, 9])
+@pytest.mark.parametrize("more", [64.0, 96.0, 160.0])
+def test_attention_of_scores_in_the_hundred_millions(gpu, codes, q_len, more):
+    """Scores of 269 to 276 million before the scale, those of the later tokens by a few of fp32's steps (32) larger: exact
+    sums, whose softmax is that of their differences; no weight leaves fp16's range.
+
+    Twice 2^25 in powers of two, steps of 4: the reference of a row cancels in its weights' exponents (a fused product
+    and sum, rounded as the difference is), exp2 and the fp32 sums cost less than 2^-16.
+    """
+    hq, hkv, n = 8, 2, 512
+    mc, ec, table, bt, cache, ids, lens, q = filled(codes, gpu, hq, hkv, [n - q_len], q_len, seed=26)
+    k, v, ks, vs = cache.codes()
+    power = 4 if codes == "e4m3" else 6
+    code = lambda x: torch.tensor(x / 2.0 ** power).to(DTYPE[codes]).view(torch.uint8).item()  # noqa: E731
+    raw = torch.zeros_like(k.view(torch.uint8))
+    raw[..., 0] = code(4608.0)
+    for i in range(32):  # block i, of wave i % 4: larger from one pair of a wave's blocks to the next, and back
+        raw[int(table[0, i]), ..., 1 + i // 8 % 3] = code(2.0 ** power)
+    cache = KV8Cache.pack(raw.view(k.dtype), v, torch.full_like(ks, 127 + power), vs)
+    q = torch.zeros_like(q)
+    size = 60000 - 96 * (torch.arange(q_len * hq, device=gpu) % 17).view(q_len, hq)
+    q[..., 0] = size.half()
+    for i in range(3):
+        q[..., 1 + i] = i * more / 2.0 ** power
+    o, _, _ = attend(cache, bt, mc, ec, ids, lens, q)
+    vv = values_of(cache)[1][table[0], 1].transpose(0, 2, 1, 3).reshape(-1, hkv, 128)
+    c = np.float64(np.float32(np.float32(128 ** -0.5) * np.float32(1.4426950408889634)))
+    above = np.arange(n) // 128 % 3 * more * c
+    for r in range(q_len):
+        p = np.exp2(above[: lens[r]] - above[: lens[r]].max())
+        for h in range(hq):
+            w = vv[: lens[r], h * hkv // hq]
+            want = p @ w / p.sum()
+            off = 2.0 ** -11 * np.abs(want) + 2.0 ** -16 * (p @ np.abs(w)) / p.sum() + 2.0 ** -25
+            assert (np.abs(o[r, h].double().cpu().numpy() - want) <= off).all()
