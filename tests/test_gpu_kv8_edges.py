@@ -174,3 +174,31 @@ def test_attention_of_scores_in_the_hundred_millions(gpu, codes, q_len, more):
             want = p @ w / p.sum()
             off = 2.0 ** -11 * np.abs(want) + 2.0 ** -16 * (p @ np.abs(w)) / p.sum() + 2.0 ** -25
             assert (np.abs(o[r, h].double().cpu().numpy() - want) <= off).all()
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("q_len", [1, 5, 9])
+def test_attention_of_the_largest_scores(gpu, codes, q_len):
+    """Every dim of queries and keys near fp16's largest, 5e11 before the scale: finite, and the later tokens' values where
+    their scores are larger by a 64th."""
+    hq, hkv, n = 8, 2, 600
+    mc, ec, table, bt, cache, ids, lens, q = filled(codes, gpu, hq, hkv, [n - q_len], q_len, seed=27)
+    k, v, ks, vs = cache.codes()
+    top, power = (224.0, 8) if codes == "e4m3" else (126.0, 9)
+    code = lambda x: torch.tensor(x).to(DTYPE[codes]).view(torch.uint8).item()  # noqa: E731
+    raw = torch.full_like(k.view(torch.uint8), code(top))
+    late = torch.from_numpy(table[0, 20:].astype(np.int64)).to(gpu)
+    raw[late] = code(240.0 if codes == "e4m3" else 127.0)
+    cache = KV8Cache.pack(raw.view(k.dtype), v, torch.full_like(ks, 127 + power), vs)
+    for size in (65504.0, -65504.0, 1000.0):
+        q = torch.full_like(q, size)
+        o, lse, _ = attend(cache, bt, mc, ec, ids, lens, q)
+        vv = values_of(cache)[1][table[0], 1].transpose(0, 2, 1, 3).reshape(-1, hkv, 128)
+        for r in range(q_len):
+            part = slice(320, lens[r]) if size > 0 else slice(0, 320)
+            for h in range(hq):
+                w = vv[part, h * hkv // hq]  # scores apart by 1e5 and more: no other token has a weight
+                off = 2.0 ** -11 * np.abs(w.mean(0)) + 2.0 ** -16 * np.abs(w).mean(0) + 2.0 ** -25
+                assert (np.abs(o[r, h].double().cpu().numpy() - w.mean(0)) <= off).all()
+        want = size * 128 * 2.0 ** power * ((240.0 if codes == "e4m3" else 127.0) if size > 0 else top) * 128 ** -0.5
+        assert (lse.double() / want - 1).abs().max() <= 2.0 ** -21
