@@ -527,7 +527,8 @@ extern "C" int nsd_kv8_paged_attention(const void* q, void* o, float* lse, const
   if (rc) return rc;
   if (cache->num_blocks > INT32_MAX / cache->num_layers / cache->num_kv_heads)
     return fail(NSD_ERR_UNSUPPORTED, "%s: %lld blocks (at most 2^31 tiles)", who, (long long)cache->num_blocks);
-  if (!(softmax_scale > 0.f) || softmax_scale == INFINITY)  // masked scores, -inf, have to stay that
+  // masked scores, -inf, have to stay that, and a score less itself 0, in powers of two too
+  if (!(softmax_scale > 0.f) || !(softmax_scale * 1.4426950408889634f < INFINITY))
     return fail(NSD_ERR_INVALID, "%s: softmax_scale=%g (a positive number)", who, (double)softmax_scale);
   AttnCall c;
   rc = prepare_attention(who, q, true, o, lse, cache->k, cache->v, cache->num_blocks, cache->num_layers, layer,

@@ -365,3 +365,12 @@ assert b"too large" in lib.nsd_last_error(), lib.nsd_last_error()
 """
     done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=60)
     assert done.returncode == 0, done.stderr
+
+
+def test_attention_refuses_scales_that_are_infinite_in_powers_of_two():
+    from nebulasd_amd.plan import kv8_plan_words
+    words, ws = kv8_plan_words([0], [40], 4, 2, 1, 64, 64)
+    c = _c()
+    for scale in (2.4e38, 3.4e38):
+        assert "softmax_scale" in _refused("nsd_kv8_paged_attention", 16, 16, None, ctypes.byref(c), 0, 4, 16, 1, 64,
+                                           words.ctypes.data, 16, 16, ws, scale, None, None)
