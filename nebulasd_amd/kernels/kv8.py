@@ -92,7 +92,7 @@ class KV8Cache:
         if k.dim() != 5 or tuple(k.shape[3:]) != (BLOCK_TOKENS, HEAD_DIM) or v.shape != k.shape:
             raise ValueError(f"codes must be [num_blocks, num_layers, num_kv_heads, {BLOCK_TOKENS}, {HEAD_DIM}]")
         bias = 128 if k.dtype == torch.int8 else 0
-        kb, vb = (t.contiguous().view(torch.uint8) ^ bias for t in (k, v))
+        kb, vb = (t.view(torch.uint8) ^ bias for t in (k, v))
         top = k.shape[:3]
         kb = kb.view(*top, 16, 2, 8, 8).permute(0, 1, 2, 5, 3, 4, 6)  # [token, half, c, dim] -> [c, token, half, dim]
         vb = vb.view(*top, 4, 4, 16, 2, 4).permute(0, 1, 2, 6, 3, 5, 7, 4)  # [g, j, i, h, m] -> [h, g, i, m, j]

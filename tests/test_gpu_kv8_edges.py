@@ -202,16 +202,3 @@ def test_attention_of_the_largest_scores(gpu, codes, q_len):
                 assert (np.abs(o[r, h].double().cpu().numpy() - w.mean(0)) <= off).all()
         want = size * 128 * 2.0 ** power * ((240.0 if codes == "e4m3" else 127.0) if size > 0 else top) * 128 ** -0.5
         assert (lse.double() / want - 1).abs().max() <= 2.0 ** -21
-
-
-@pytest.mark.parametrize("codes", CODES)
-def test_pack_takes_codes_of_any_strides(gpu, codes):
-    rng = np.random.default_rng(28)
-    raw = gpu_of(rng.integers(0, 127, (2, 5, 16, 3, 128), dtype=np.uint8)).view(DTYPE[codes])
-    s = gpu_of(rng.integers(100, 140, (2, 3, 5), dtype=np.uint8)).transpose(1, 2)
-    for k in (raw.transpose(2, 3), raw.transpose(2, 3)[:, 1:4], raw.transpose(2, 3)[..., :, :].flip(0)):
-        scales = s[:, : k.shape[1]]
-        want = KV8Cache.pack(k.contiguous(), k.contiguous(), scales.contiguous(), scales.contiguous())
-        got = KV8Cache.pack(k, k, scales, scales)
-        for a, b in zip((got.k, got.v, got.k_scales, got.v_scales), (want.k, want.v, want.k_scales, want.v_scales)):
-            assert torch.equal(a, b)
