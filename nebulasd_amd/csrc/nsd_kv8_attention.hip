@@ -33,9 +33,9 @@
 // wait of the compiler's drains the tiles behind it.
 //
 // Bound by the tiles' intake, us a call with the merge's launch (the bytes at the
-// 7.0 TB/s of a contiguous read): 64 rows of 512 to 2048 tokens 26.9 (19.1), 16 x
-// 5 of 256 to 4096 19.5 (7.5), 16 x 9 of 1024 to 32768 60.5 (36.8), one row of
-// 32768 17.9 (9.6).  The loads and waits alone, without arithmetic, took 24.6,
+// 7.0 TB/s of a contiguous read): 64 rows of 512 to 2048 tokens 26.8 (19.1), 16 x
+// 5 of 256 to 4096 18.8 (7.5), 16 x 9 of 1024 to 32768 61.2 (36.8), one row of
+// 32768 17.7 (9.6).  The loads and waits alone, without arithmetic, took 24.6,
 // 18.0, 52.7 and 18.6 where the kernel (of then) took 27.2, 20.5, 59.7 and 20.0.  A piece
 // begins with 3 us of latency (ids, then tiles), or 8 to 9 in a compute unit's
 // second workgroup, whose first tiles come behind the burst of everyone's, and
