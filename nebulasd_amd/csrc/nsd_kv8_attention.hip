@@ -105,8 +105,8 @@ __device__ inline void wait_vm() {
 // left: off by 2^-22 of itself at most, or by 2^-25 under the smallest normal
 // number.  The running maximum's own weight is 2^7, so that the latter is 2^-32 of
 // it; the largest, with the lazy maximum, is 2^15.  Outputs then differ from 64 bits
-// by their own rounding alone (2.0 to 2.3e-4 of the norm, as fp32 weights'); from
-// fp32 weights' outputs by 5e-6 to 2e-5.  One fp16 number: 2.1 to 2.9e-4 and 1.6 to
+// by their own rounding alone (1.8 to 2.3e-4 of the norm, as fp32 weights'); from
+// fp32 weights' outputs by 2e-6 to 4e-5.  One fp16 number: 2.1 to 2.9e-4 and 1.6 to
 // 3.2e-4, and the second product's time less, 16 x 5 19.1 for 19.85 us and 16 x 9 59.4
 // for 62.7 in a graph, one tile 0.2 for any length.
 typedef float f32x2 __attribute__((ext_vector_type(2)));
