@@ -20,8 +20,8 @@ def close_weights(cache, table, layer, q, seq_ids, lens, o, scale):
     """The worst of the outputs' errors over their bounds, for queries of one nonzero dim.
 
     A score is then one product of an fp16 query and a code's value, 11 x 11 bits: exact in fp32.  What is rounded:
-    the scale times log2(e), and its product with the score against the reference m (steps of the largest of them,
-    halved: 2^-24 each, and m's own cancels, since weights and sum have the same one); exp2, by a step, 2^-23; a weight
+    the scale times log2(e), and its product with the score against the reference (half a step of the largest of them,
+    2^-24 each; less where scores are subtracted first); exp2, by a step, 2^-23; a weight
     as a pair of fp16 numbers, 2^-22 of it or 2^-32 of the row's largest; the sums, fp32: a product instruction's by
     2^-22 of what it has added up at most, two a pair of blocks, and ten steps of merging waves and parts; the output,
     half a step of fp16.
